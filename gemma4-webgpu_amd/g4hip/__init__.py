@@ -19,7 +19,6 @@ from ._lib import (  # noqa: F401
     SoftmaxParams,
     AttnOutputParams,
     AttnFusedParams,
-    Kv8Params,
     PagedAttnParams,
     PerHeadNormParams,
     NormRopeParams,
