@@ -198,7 +198,7 @@ def _workspace(ctx, nbytes):
 def _params(ctx, s, window=0):
     c = s["case"]
     n, width = s["table"].shape
-    return ctx.kv8_params(n, c["heads"], c["kv"], c["dim"], c["page"], width, c["page"] * width,
+    return ctx.kv8_params(n, c["heads"], c["kv"], c["dim"], c["page"], width, c["longest"],
                           s["k_pool"].shape[0], num_rows=s["q"].shape[-3], max_rows=c["rows"], window=window, eps=EPS)
 
 
