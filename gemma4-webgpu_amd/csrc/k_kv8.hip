@@ -1,0 +1,404 @@
+// k_kv8.hip — appending to the 8-bit paged K/V pool, and reading its values
+// (the f16 pool's prologue is attn_prologue_kernel of k_attn.hip; the
+// reference appends f32 rows, shaders/kv_cache_store.wgsl).
+//
+// A value is code * 2^e with one e per page and KV head. Powers of two: a value
+// divided by the scale is exact, so the code is the correctly rounded one, and
+// when a later row makes the scale grow, the codes already there are shifted
+// and rounded once, to at most half a step of the new scale. After the norms a
+// page's largest element stays within an octave, so growth is rare; the price
+// is up to one bit against a scale of amax / 127.
+//
+// kv8_prologue_kernel: every page of a KV head that a call touches belongs to
+// one workgroup (K and V apart), which forms its rows' largest element before
+// it stores any code; other workgroups take the query rows, one wave a row and
+// head. Norms, rotation and rounding of K and V are in f64: a value near the
+// border of two codes then gets the same code as in exact arithmetic, whatever
+// the order of the sums (the f64 units are idle otherwise). q is f32. Up to 16
+// rows of a page stay in registers between the two steps; more are formed
+// again for the second.
+#include "kv8.hpp"
+#include "mqf_core.hpp"
+
+namespace {
+
+using namespace g4kv8;
+
+constexpr int NT = 256, NW = NT / 64;
+constexpr int KEEP = 4;  // rows a wave keeps in registers
+
+struct ProArgs {
+  const float *q, *k, *v;
+  uint32_t nparts;
+  const uint16_t *q_w, *k_w;
+  const uint16_t* rope_freqs;
+  const float2* rope_cs;
+  float* q_out;
+  int8_t *kp, *vp;
+  float *ks, *vs;
+  const int32_t* page_table;
+  Rows rows;
+  uint32_t nqh, nkh, page_size, max_pages, num_pages;
+  uint32_t q_blocks, seq_pages;  // workgroups of the query rows; pages a sequence's rows may touch
+  float eps, theta;
+  uint32_t apply_divisor;
+};
+
+// A lane's share of a row: PP neighbouring pairs (i, i + HD / 2).
+template <int HD>
+struct Row {
+  static constexpr int HALF = HD / 2, PP = HALF >= 64 ? HALF / 64 : 1, ACT = HALF / PP;
+};
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ double wave_max64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// Parts added in order, in T.
+template <int HD, typename T>
+__device__ __forceinline__ void load_row(const float* p, size_t stride, uint32_t nparts, int lane, T* lo, T* hi) {
+  constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
+  typedef float vec __attribute__((ext_vector_type(PP == 1 ? 2 : PP)));  // (PP 1: the second is not used)
+#pragma unroll
+  for (int i = 0; i < PP; ++i) lo[i] = hi[i] = 0;
+  if (lane >= Row<HD>::ACT) return;
+  const float* b = p + PP * lane;
+#pragma unroll 4
+  for (uint32_t c = 0; c < nparts; ++c, b += stride) {
+    if constexpr (PP == 1) {
+      lo[0] += (T)b[0];
+      hi[0] += (T)b[HALF];
+    } else {
+      const vec x = *(const vec*)b, y = *(const vec*)(b + HALF);
+#pragma unroll
+      for (int i = 0; i < PP; ++i) {
+        lo[i] += (T)x[i];
+        hi[i] += (T)y[i];
+      }
+    }
+  }
+}
+
+template <int HD, typename T>
+__device__ __forceinline__ void rotate(const ProArgs& a, const uint16_t* w, uint32_t pos, int lane, T* lo, T* hi) {
+  constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
+  if (lane >= Row<HD>::ACT) return;
+#pragma unroll
+  for (int i = 0; i < PP; ++i) {
+    const int t = PP * lane + i;
+    const float2 cs = a.rope_cs ? a.rope_cs[(size_t)pos * HALF + t]
+                                : g4mqf::rope_cos_sin(a.theta, a.apply_divisor, a.rope_freqs[t], t, HD, pos);
+    const T x0 = lo[i] * (T)g4d::f16_bits_to_f32(w[t]), x1 = hi[i] * (T)g4d::f16_bits_to_f32(w[t + HALF]);
+    lo[i] = x0 * (T)cs.x - x1 * (T)cs.y;
+    hi[i] = x0 * (T)cs.y + x1 * (T)cs.x;
+  }
+}
+
+template <int HD>
+__device__ __forceinline__ void q_row(const ProArgs& a) {
+  constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
+  const int lane = threadIdx.x & 63;
+  const uint64_t i = (uint64_t)blockIdx.x * NW + (threadIdx.x >> 6);
+  if (i >= (uint64_t)a.rows.num_rows * a.nqh) return;
+  const uint32_t row = (uint32_t)(i / a.nqh), head = (uint32_t)(i % a.nqh);
+  const uint32_t s = seq_of_row(a.rows, row);
+  if (s >= a.rows.num_seqs) return;
+  const Seq q = seq_rows(a.rows, s);
+  if (!q.len) return;
+  const size_t at = ((size_t)row * a.nqh + head) * HD;
+  float lo[PP], hi[PP], ss = 0.f;
+  load_row<HD>(a.q + at, (size_t)a.rows.num_rows * a.nqh * HD, a.nparts, lane, lo, hi);
+#pragma unroll
+  for (int e = 0; e < PP; ++e) ss += lo[e] * lo[e] + hi[e] * hi[e];
+  ss = g4d::wave_sum_dpp(ss);
+  const float inv = 1.0f / sqrtf(ss * (1.0f / (float)HD) + a.eps);
+#pragma unroll
+  for (int e = 0; e < PP; ++e) {
+    lo[e] *= inv;
+    hi[e] *= inv;
+  }
+  rotate<HD>(a, a.q_w, q.base + (row - q.first), lane, lo, hi);
+  if (lane < Row<HD>::ACT) {
+#pragma unroll
+    for (int e = 0; e < PP; ++e) {
+      a.q_out[at + PP * lane + e] = lo[e];
+      a.q_out[at + HALF + PP * lane + e] = hi[e];
+    }
+  }
+}
+
+// The scale of a page whose largest element is `am`: the least 2^e with
+// am <= 127 * 2^e, from its binary exponent; at least 2^-64 (all zeros).
+__device__ __forceinline__ float scale_of(double am) {
+  int x = 0;
+  const double m = frexp(am, &x);
+  return ldexpf(1.0f, am > 0.0 ? max(x - 7 + (m > 127.0 / 128.0), -64) : -64);
+}
+
+template <int HD>
+__global__ __launch_bounds__(NT) void kv8_prologue_kernel(ProArgs a) {
+  constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
+  __shared__ double s_am[NW];
+  __shared__ int s_bad;
+  if (blockIdx.x < a.q_blocks) {
+    q_row<HD>(a);
+    return;
+  }
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  uint32_t b = blockIdx.x - a.q_blocks;
+  const bool is_v = b & 1;
+  b >>= 1;
+  const uint32_t kvh = b % a.nkh;
+  b /= a.nkh;
+  const uint32_t j = b % a.seq_pages, s = b / a.seq_pages;
+  const Seq q = seq_rows(a.rows, s);
+  const uint32_t pi = q.base / a.page_size + j;
+  if (!q.len || pi > (q.len - 1) / a.page_size) return;  // (uniform)
+  const int32_t pg = a.page_table[(size_t)s * a.max_pages + pi];
+  if (pg < 0 || pg >= (int32_t)a.num_pages) return;
+  const uint32_t start = pi * a.page_size;
+  const uint32_t p0 = max(q.base, start), p1 = min(q.len, start + a.page_size), m = p1 - p0;
+  const float* src = (is_v ? a.v : a.k);
+  const size_t stride = (size_t)a.rows.num_rows * a.nkh * HD;
+
+  double lo[KEEP][PP], hi[KEEP][PP];
+  auto form = [&](uint32_t at) {  // the wave's rows p0 + at + w, + NW, ...
+#pragma unroll
+    for (int r = 0; r < KEEP; ++r) {
+      const uint32_t i = at + w + NW * r;
+#pragma unroll
+      for (int e = 0; e < PP; ++e) lo[r][e] = hi[r][e] = 0.0;
+      if (i >= m) continue;  // (uniform over the wave)
+      load_row<HD>(src + ((size_t)(q.first + (p0 - q.base) + i) * a.nkh + kvh) * HD, stride, a.nparts, lane, lo[r],
+                   hi[r]);
+      double ss = 0.0;
+#pragma unroll
+      for (int e = 0; e < PP; ++e) ss += lo[r][e] * lo[r][e] + hi[r][e] * hi[r][e];
+      const double inv = 1.0 / sqrt(wave_sum64(ss) * (1.0 / HD) + (double)a.eps);
+#pragma unroll
+      for (int e = 0; e < PP; ++e) {
+        lo[r][e] *= inv;
+        hi[r][e] *= inv;
+      }
+      if (!is_v) rotate<HD>(a, a.k_w, p0 + i, lane, lo[r], hi[r]);
+    }
+  };
+  double am = 0.0;
+  bool bad = false;
+  for (uint32_t at = 0; at < m; at += KEEP * NW) {
+    form(at);
+#pragma unroll
+    for (int r = 0; r < KEEP; ++r)
+#pragma unroll
+      for (int e = 0; e < PP; ++e) {
+        const double x = fmax(fabs(lo[r][e]), fabs(hi[r][e]));
+        am = fmax(am, x);  // (a NaN is not the larger one)
+        bad |= !(fabs(lo[r][e]) < INFINITY && fabs(hi[r][e]) < INFINITY);
+      }
+  }
+  am = wave_max64(am);
+  if (threadIdx.x == 0) s_bad = 0;
+  __syncthreads();
+  if (lane == 0) s_am[w] = am;
+  if (bad) s_bad = 1;
+  float* sp = (is_v ? a.vs : a.ks) + (size_t)pg * a.nkh + kvh;
+  const uint32_t before = p0 - start;  // codes of earlier calls
+  const float old = before ? *sp : 0.f;
+  __syncthreads();
+  am = fmax(fmax(s_am[0], s_am[1]), fmax(s_am[2], s_am[3]));
+  const bool poison = s_bad || old != old;
+  const float sc = poison ? __builtin_nanf("") : fmaxf(old, scale_of(am));
+  if (threadIdx.x == 0) *sp = sc;
+  int8_t* page = (is_v ? a.vp : a.kp) + ((size_t)pg * a.page_size * a.nkh + kvh) * HD;
+  const size_t rs = (size_t)a.nkh * HD;  // from one position's row to the next
+
+  if (before && sc != old && !poison) {  // (uniform) round the codes before to the grown scale
+    const float ratio = old / sc;
+    for (uint32_t i = threadIdx.x; i < before * (HD / 4); i += NT) {
+      uint32_t* d = (uint32_t*)(page + (size_t)(i / (HD / 4)) * rs + i % (HD / 4) * 4);
+      const uint32_t x = *d;
+      uint32_t y = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float c = rintf((float)(int8_t)(x >> (8 * e)) * ratio);
+        y |= ((uint32_t)(int)fminf(fmaxf(c, -127.f), 127.f) & 0xffu) << (8 * e);
+      }
+      *d = y;
+    }
+  }
+  const double up = poison ? 0.0 : 1.0 / (double)sc;
+  for (uint32_t at = 0; at < m; at += KEEP * NW) {
+    if (m > KEEP * NW) form(at);
+#pragma unroll
+    for (int r = 0; r < KEEP; ++r) {
+      const uint32_t i = at + w + NW * r;
+      if (i >= m || lane >= Row<HD>::ACT) continue;
+      int8_t* d = page + (size_t)(before + i) * rs + PP * lane;
+      uint32_t x = 0, y = 0;
+#pragma unroll
+      for (int e = 0; e < PP; ++e) {
+        x |= (poison ? 0u : (uint32_t)(int)rint(lo[r][e] * up) & 0xffu) << (8 * e);
+        y |= (poison ? 0u : (uint32_t)(int)rint(hi[r][e] * up) & 0xffu) << (8 * e);
+      }
+      if constexpr (PP == 1) {
+        d[0] = (int8_t)x;
+        d[HALF] = (int8_t)y;
+      } else if constexpr (PP == 2) {
+        *(uint16_t*)d = (uint16_t)x;
+        *(uint16_t*)(d + HALF) = (uint16_t)y;
+      } else {
+        *(uint32_t*)d = x;
+        *(uint32_t*)(d + HALF) = y;
+      }
+    }
+  }
+}
+
+struct ValArgs {
+  const int8_t* pool[2];
+  const float* scale[2];
+  uint16_t* out[2];
+  const int32_t* pages;
+  uint32_t page_size, nkh, hd, num_pages;
+};
+
+// 16 codes a thread. A code times its scale has 7 bits: exact in f16 from
+// 2^-24 to 65504.
+__global__ __launch_bounds__(NT) void kv8_values_kernel(ValArgs a) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const uint32_t bytes = a.page_size * a.nkh * a.hd;  // of a page
+  const uint32_t i = (blockIdx.y * NT + threadIdx.x) * 16;
+  if (i >= bytes) return;
+  const uint32_t which = blockIdx.z;
+  const int32_t pg = a.pages[blockIdx.x];
+  const bool in = pg >= 0 && pg < (int32_t)a.num_pages;
+  const size_t at = (size_t)(in ? pg : 0) * bytes + i;
+  const u32x4 x = *(const u32x4*)(a.pool[which] + at);
+  const float sc = in ? a.scale[which][(size_t)pg * a.nkh + i / a.hd % a.nkh] : 0.f;
+  u32x4 y[2];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = x[e / 2] >> (16 * (e & 1));
+    y[e / 4][e % 4] = (uint32_t)g4d::f32_to_f16_bits((float)(int8_t)b * sc) |
+                      (uint32_t)g4d::f32_to_f16_bits((float)(int8_t)(b >> 8) * sc) << 16;
+  }
+  u32x4* o = (u32x4*)(a.out[which] + (size_t)blockIdx.x * bytes + i);
+  o[0] = in ? y[0] : u32x4{0, 0, 0, 0};
+  o[1] = in ? y[1] : u32x4{0, 0, 0, 0};
+}
+
+}  // namespace
+
+int g4_internal_kv8_check(const char* fn, const g4_kv8_params& p, const uint32_t* row_starts) {
+  G4_REQUIRE(p.num_seqs > 0 && p.num_seqs <= 65535 && p.num_rows > 0 && p.num_rows <= 65535 && p.max_rows > 0 &&
+                 p.max_rows <= p.num_rows,
+             "%s: 1..65535 sequences and rows, max_rows (%u) from 1 to num_rows (%u)", fn, p.max_rows, p.num_rows);
+  G4_REQUIRE(row_starts || (p.max_rows == 1 && p.num_rows == p.num_seqs),
+             "%s: without row_starts every sequence has one row (num_rows = num_seqs, max_rows 1)", fn);
+  G4_REQUIRE(p.num_kv_heads > 0 && p.num_q_heads > 0 && p.num_q_heads % p.num_kv_heads == 0 &&
+                 p.num_q_heads / p.num_kv_heads <= 16 && p.num_kv_heads <= 64,
+             "%s: num_q_heads %u must be a multiple (<= 16x) of num_kv_heads %u (<= 64)", fn, p.num_q_heads,
+             p.num_kv_heads);
+  G4_REQUIRE(p.head_dim == 64 || p.head_dim == 128 || p.head_dim == 256 || p.head_dim == 512,
+             "%s: head_dim %u not in {64, 128, 256, 512}", fn, p.head_dim);
+  G4_REQUIRE(p.page_size > 0 && p.page_size % 16 == 0 && p.page_size <= 1024,
+             "%s: page_size %u is not a multiple of 16 up to 1024", fn, p.page_size);
+  G4_REQUIRE(p.max_pages > 0 && p.num_pages > 0 && p.num_pages <= 0x7fffffffu && p.max_seq_len > 0 &&
+                 p.max_seq_len <= 0x7fffffffu && (uint64_t)p.max_seq_len <= (uint64_t)p.page_size * p.max_pages,
+             "%s: max_seq_len %u exceeds the page table (%u x %u)", fn, p.max_seq_len, p.max_pages, p.page_size);
+  return G4_OK;
+}
+
+extern "C" {
+
+int g4_pagedAttnPrologue8(g4_ctx* ctx, const float* q_parts, const float* k_parts, const float* v_parts,
+                          uint32_t nparts, const uint16_t* q_norm_w, const uint16_t* k_norm_w,
+                          const uint16_t* rope_freqs, float* q_out, int8_t* k_pool, int8_t* v_pool, float* k_scale,
+                          float* v_scale, const int32_t* page_table, const uint32_t* seq_lens,
+                          const uint32_t* row_starts, g4_kv8_params p, const float* rope_cs, uint32_t rope_rows) {
+  G4_ENTER(ctx);
+  int rc = g4_internal_kv8_check(__func__, p, row_starts);
+  if (rc) return rc;
+  const bool q = q_parts != nullptr, kv = k_parts != nullptr;
+  G4_REQUIRE((q || kv) && nparts >= 1 && seq_lens, "g4_pagedAttnPrologue8: no rows, no parts or null seq_lens");
+  G4_REQUIRE(!q || (q_norm_w && q_out), "g4_pagedAttnPrologue8: q_parts, q_norm_w and q_out go together");
+  G4_REQUIRE(!q || q_out != q_parts || nparts == 1, "g4_pagedAttnPrologue8: q_out over q_parts needs one part");
+  G4_REQUIRE(kv ? (v_parts && k_norm_w && k_pool && v_pool && k_scale && v_scale && page_table) : !v_parts,
+             "g4_pagedAttnPrologue8: k_parts, v_parts, k_norm_w, the pools, their scales and the page table go together");
+  G4_REQUIRE((((uintptr_t)q_parts | (uintptr_t)k_parts | (uintptr_t)v_parts | (uintptr_t)q_out) & 15) == 0 &&
+                 (!kv || (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0),
+             "g4_pagedAttnPrologue8: rows and pools must be 16-byte aligned");
+  G4_REQUIRE(!rope_cs || (rope_rows >= p.max_seq_len && ((uintptr_t)rope_cs & 7) == 0),
+             "g4_pagedAttnPrologue8: RoPE table of %u rows < max_seq_len %u, or not 8-byte aligned", rope_rows,
+             p.max_seq_len);
+  G4_REQUIRE(!p.apply_divisor || rope_freqs || rope_cs, "g4_pagedAttnPrologue8: apply_divisor needs rope_freqs");
+  ProArgs a{};
+  a.q = q_parts;
+  a.k = k_parts;
+  a.v = v_parts;
+  a.nparts = nparts;
+  a.q_w = q_norm_w;
+  a.k_w = k_norm_w;
+  a.rope_freqs = rope_freqs ? rope_freqs : (q ? q_norm_w : k_norm_w);  // read, used only with the divisor
+  a.rope_cs = (const float2*)rope_cs;
+  a.q_out = q_out;
+  a.kp = k_pool;
+  a.vp = v_pool;
+  a.ks = k_scale;
+  a.vs = v_scale;
+  a.page_table = page_table;
+  a.rows = {seq_lens, row_starts, p.num_seqs, p.num_rows, p.max_rows, p.max_seq_len};
+  a.nqh = p.num_q_heads;
+  a.nkh = p.num_kv_heads;
+  a.page_size = p.page_size;
+  a.max_pages = p.max_pages;
+  a.num_pages = p.num_pages;
+  a.eps = p.eps;
+  a.theta = p.theta;
+  a.apply_divisor = p.apply_divisor;
+  a.q_blocks = q ? ceil_div((uint64_t)p.num_rows * p.num_q_heads, NW) : 0;
+  a.seq_pages = ceil_div(p.max_rows - 1, p.page_size) + 1;
+  const uint64_t blocks = a.q_blocks + (kv ? 2ull * p.num_seqs * a.seq_pages * p.num_kv_heads : 0ull);
+  G4_REQUIRE(blocks <= 0x7fffffffull, "g4_pagedAttnPrologue8: %llu workgroups", (unsigned long long)blocks);
+  const dim3 grid((unsigned)blocks);
+  switch (p.head_dim) {
+    case 64: hipLaunchKernelGGL(kv8_prologue_kernel<64>, grid, dim3(NT), 0, ctx->stream, a); break;
+    case 128: hipLaunchKernelGGL(kv8_prologue_kernel<128>, grid, dim3(NT), 0, ctx->stream, a); break;
+    case 256: hipLaunchKernelGGL(kv8_prologue_kernel<256>, grid, dim3(NT), 0, ctx->stream, a); break;
+    default: hipLaunchKernelGGL(kv8_prologue_kernel<512>, grid, dim3(NT), 0, ctx->stream, a); break;
+  }
+  G4_LAUNCHED(ctx, "kv8_prologue");
+  return G4_OK;
+}
+
+int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const float* k_scale, const float* v_scale,
+                 const int32_t* pages, uint32_t count, uint32_t page_size, uint32_t num_kv_heads, uint32_t head_dim,
+                 uint32_t num_pages, uint16_t* k_out, uint16_t* v_out) {
+  G4_ENTER(ctx);
+  G4_REQUIRE(k_pool && v_pool && k_scale && v_scale && pages && k_out && v_out, "g4_kv8Values: null buffer");
+  G4_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0,
+             "g4_kv8Values: pools and outputs must be 16-byte aligned");
+  g4_kv8_params p{};
+  p.num_seqs = p.num_rows = p.max_rows = p.max_pages = p.max_seq_len = 1;
+  p.num_q_heads = p.num_kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.page_size = page_size;
+  p.num_pages = num_pages;
+  int rc = g4_internal_kv8_check(__func__, p, nullptr);
+  if (rc) return rc;
+  G4_REQUIRE(count > 0 && count <= 0x7fffffffu, "g4_kv8Values: %u pages", count);
+  const ValArgs a{{k_pool, v_pool}, {k_scale, v_scale}, {k_out, v_out}, pages, page_size, num_kv_heads, head_dim, num_pages};
+  hipLaunchKernelGGL(kv8_values_kernel, dim3(count, ceil_div((uint64_t)page_size * num_kv_heads * head_dim, 16 * NT), 2),
+                     dim3(NT), 0, ctx->stream, a);
+  G4_LAUNCHED(ctx, "kv8_values");
+  return G4_OK;
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@ from ._lib import (  # noqa: F401
     SoftmaxParams,
     AttnOutputParams,
     AttnFusedParams,
+    Kv8Params,
     PagedAttnParams,
     PerHeadNormParams,
     NormRopeParams,

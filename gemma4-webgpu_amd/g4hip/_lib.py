@@ -77,6 +77,16 @@ class PagedAttnFusedParams(ctypes.Structure):
                                            ("apply_divisor", ctypes.c_uint32)]
 
 
+class Kv8Params(ctypes.Structure):  # g4_kv8_params
+    _fields_ = [("num_seqs", ctypes.c_uint32), ("num_q_heads", ctypes.c_uint32),
+                ("num_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("page_size", ctypes.c_uint32), ("max_pages", ctypes.c_uint32),
+                ("max_seq_len", ctypes.c_uint32), ("num_pages", ctypes.c_uint32),
+                ("num_rows", ctypes.c_uint32), ("max_rows", ctypes.c_uint32),
+                ("sliding_window", ctypes.c_uint32), ("scale", ctypes.c_float),
+                ("eps", ctypes.c_float), ("theta", ctypes.c_float), ("apply_divisor", ctypes.c_uint32)]
+
+
 class PerHeadNormParams(ctypes.Structure):  # shaders/per_head_rms_norm_no_weight.wgsl:8
     _fields_ = [("num_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
                 ("eps", ctypes.c_float), ("pad", ctypes.c_uint32)]
@@ -182,6 +192,13 @@ SIGNATURES = {
     "g4_pagedAttnDecodeFused_workspace_size": (_I, [PagedAttnFusedParams, ctypes.POINTER(_SZ)]),
     "g4_pagedAttnDecodeFused": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, PagedAttnFusedParams, _P,
                                      _SZ]),
+    "g4_pagedAttnPrologue8": (_I, [_P, _P, _P, _P, _U32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, Kv8Params, _P,
+                                   _U32]),
+    "g4_pagedAttn8_workspace_size": (_I, [Kv8Params, ctypes.POINTER(_SZ)]),
+    "g4_pagedAttn8": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, Kv8Params, _P, _SZ]),
+    "g4_kv8Values": (_I, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P]),
+    "g4_logprobsBatch_workspace_size": (_I, [_U32, _U32, _U32, ctypes.POINTER(_SZ)]),
+    "g4_logprobsBatch": (_I, [_P, _P, _P, _U32, _U32, _P, _P, _U32, _P, _P, _P, _SZ]),
     "g4_advanceSeqLens": (_I, [_P, _P, _U32, _U32]),
     "g4_perHeadRmsNormNoWeight": (_I, [_P, _P, PerHeadNormParams]),
     "g4_fusedPerHeadNormRope": (_I, [_P, _P, _P, NormRopeParams, _P]),

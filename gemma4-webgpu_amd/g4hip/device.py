@@ -16,6 +16,7 @@ from ._lib import (
     AttnFusedParams,
     AttnOutputParams,
     AttnScoreParams,
+    Kv8Params,
     KvStoreParams,
     MatmulParams,
     NormAddParams,
@@ -693,6 +694,44 @@ class Context:
                                       _p(page_table), _p(seq_lens), _p(out), _p(ops), p, _p(workspace),
                                       workspace.nbytes, _p(rope_cs), rope_rows))
 
+    # ---- 8-bit paged K/V cache ----
+    @staticmethod
+    def kv8_params(num_seqs, nqh, nkh, hd, page_size, max_pages, max_seq_len, num_pages, num_rows=None, max_rows=1,
+                   window=0, scale=1.0, eps=1e-6, theta=1e4, apply_divisor=0) -> Kv8Params:
+        """num_rows None: one row per sequence."""
+        return Kv8Params(num_seqs, nqh, nkh, hd, page_size, max_pages, max_seq_len, num_pages,
+                         num_seqs if num_rows is None else num_rows, max_rows, window, scale, eps, theta,
+                         apply_divisor)
+
+    @staticmethod
+    def attn8_workspace_bytes(p: Kv8Params) -> int:
+        n = ctypes.c_size_t()
+        check(lib().g4_pagedAttn8_workspace_size(p, ctypes.byref(n)))
+        return int(n.value)
+
+    def pagedAttnPrologue8(self, q_parts: Ptr, k_parts: Ptr, v_parts: Ptr, nparts: int, q_norm_w: Ptr, k_norm_w: Ptr,
+                           rope_freqs: Ptr, q_out: Ptr, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr,
+                           page_table: Ptr, seq_lens: Ptr, p: Kv8Params, row_starts: Ptr = None, rope_cs: Ptr = None,
+                           rope_rows: int = 0) -> None:
+        """pagedAttnPrologue over an 8-bit pool, rows row_starts[s] .. row_starts[s + 1] - 1 of each sequence
+        (None: one row each): q after norm + RoPE into q_out, k and v appended as codes, scales grown."""
+        check(lib().g4_pagedAttnPrologue8(self.h, _p(q_parts), _p(k_parts), _p(v_parts), nparts, _p(q_norm_w),
+                                          _p(k_norm_w), _p(rope_freqs), _p(q_out), _p(k_pool), _p(v_pool),
+                                          _p(k_scale), _p(v_scale), _p(page_table), _p(seq_lens), _p(row_starts), p,
+                                          _p(rope_cs), rope_rows))
+
+    def pagedAttn8(self, q: Ptr, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr, page_table: Ptr,
+                   seq_lens: Ptr, out: Ptr, p: Kv8Params, workspace: Buffer, row_starts: Ptr = None) -> None:
+        """Attention of every row over its sequence's 8-bit pages, up to its own position."""
+        check(lib().g4_pagedAttn8(self.h, _p(q), _p(k_pool), _p(v_pool), _p(k_scale), _p(v_scale), _p(page_table),
+                                  _p(seq_lens), _p(row_starts), _p(out), p, _p(workspace), workspace.nbytes))
+
+    def kv8Values(self, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr, pages: Ptr, count: int, page_size: int,
+                  nkh: int, hd: int, num_pages: int, k_out: Ptr, v_out: Ptr) -> None:
+        """The listed pages of an 8-bit pool as f16 pages."""
+        check(lib().g4_kv8Values(self.h, _p(k_pool), _p(v_pool), _p(k_scale), _p(v_scale), _p(pages), count,
+                                 page_size, nkh, hd, num_pages, _p(k_out), _p(v_out)))
+
     def advanceSeqLens(self, seq_lens: Ptr, num_seqs: int, delta: int = 1) -> None:
         check(lib().g4_advanceSeqLens(self.h, _p(seq_lens), num_seqs, delta))
 
@@ -760,6 +799,19 @@ class Context:
 
     def topk256Batch(self, logits: Ptr, result: Ptr, size: int, batch: int) -> None:
         check(lib().g4_topk256Batch(self.h, _p(logits), _p(result), size, batch))
+
+    @staticmethod
+    def logprobs_workspace_bytes(size: int, batch: int, ntop: int) -> int:
+        n = ctypes.c_size_t()
+        check(lib().g4_logprobsBatch_workspace_size(size, batch, ntop, ctypes.byref(n)))
+        return int(n.value)
+
+    def logprobsBatch(self, logits: Ptr, tokens: Ptr, size: int, batch: int, logprobs: Ptr, entropy: Ptr, ntop: int,
+                      top_ids: Ptr, top_logprobs: Ptr, workspace: Buffer) -> None:
+        """Per row of `batch` rows of logits: the log probability of tokens[r], the entropy, and the ntop likeliest
+        tokens with theirs."""
+        check(lib().g4_logprobsBatch(self.h, _p(logits), _p(tokens), size, batch, _p(logprobs), _p(entropy), ntop,
+                                     _p(top_ids), _p(top_logprobs), _p(workspace), workspace.nbytes))
 
     # ---- debug / synthetic inputs ----
     def dequant_q4k(self, blocks: Ptr, nblocks: int, out: Ptr) -> None:

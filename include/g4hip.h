@@ -771,6 +771,92 @@ int g4_prefillAttn(g4_ctx* ctx, const float* q, const uint16_t* k_pool, const ui
                    g4_paged_attn_fused_params p, float scale, void* workspace, size_t workspace_bytes);
 
 /* ------------------------------------------------------------------------ */
+/* 8-bit paged K/V cache, log probabilities                                  */
+/* (no counterpart in the reference, whose cache is f32 and whose sampler    */
+/*  reads argmax or top-k only: src/engine.ts:1053-1063, 1686-1740)          */
+/* ------------------------------------------------------------------------ */
+
+/* A K/V pool of signed 8-bit codes: pool[num_pages][page_size][num_kv_heads]
+ * [head_dim], one f32 scale per page and KV head (scale[num_pages]
+ * [num_kv_heads]); a value is code * scale. Scales are powers of two: the
+ * least 2^e (e >= -64) with |x| <= 127 * 2^e for every x of the page and head.
+ *
+ * Rows: num_rows rows of q (k, v, output), in num_seqs sequences. Sequence s
+ * has rows row_starts[s] .. row_starts[s + 1] - 1 (row_starts[num_seqs + 1],
+ * ascending, on the device), at most max_rows of them; row_starts NULL: one
+ * row per sequence (max_rows 1, num_rows = num_seqs). seq_lens[s] counts the
+ * rows (a step advances it first), so with n rows its row i is position
+ * seq_lens[s] - n + i. Rows outside every sequence are left as they are, as
+ * are those of a sequence whose starts descend, pass num_rows or hold more
+ * than max_rows rows. A sequence shorter than its rows or longer than
+ * max_seq_len appends nothing, its q_out is not written and its attention
+ * output is 0. Page ids outside [0, num_pages) store nothing and are clamped
+ * when read, as in the f16 pool.
+ *
+ * page_size: a multiple of 16, at most 1024. head_dim 64, 128, 256 or 512, at
+ * most 64 KV heads with at most 16 query heads each. */
+typedef struct {
+  uint32_t num_seqs, num_q_heads, num_kv_heads, head_dim;
+  uint32_t page_size, max_pages, max_seq_len, num_pages;
+  uint32_t num_rows, max_rows;
+  uint32_t sliding_window;
+  float scale;
+  float eps, theta;
+  uint32_t apply_divisor;
+} g4_kv8_params;
+/* g4_pagedAttnPrologue over such a pool and any number of rows a sequence:
+ * q_out = rope(norm(q) * q_norm_w), and k = rope(norm(k) * k_norm_w) and the
+ * weightless norm of v appended. parts: [nparts][num_rows][heads * head_dim],
+ * added in order (q_out may be q_parts when nparts is 1). A page that the call
+ * begins (its slot 0 is one of the rows) gets the scale of its rows; in a page
+ * begun earlier the scale grows to theirs where they need it, and the codes
+ * before them are rounded again to the new scale. The append rounds from 64-bit
+ * values: |value - x| <= scale / 2, and as much again of the then scale for
+ * each growth. A NaN or an infinity among a page and head's rows makes its
+ * scale NaN, and every value read from them NaN, until the page is begun again.
+ * Each page is appended to by one sequence of a call. k_parts = v_parts = NULL:
+ * q only; q_parts = NULL (with q_norm_w, q_out): k and v only.
+ * p.scale and p.sliding_window are unused. */
+int g4_pagedAttnPrologue8(g4_ctx* ctx, const float* q_parts, const float* k_parts, const float* v_parts,
+                          uint32_t nparts, const uint16_t* q_norm_w, const uint16_t* k_norm_w,
+                          const uint16_t* rope_freqs, float* q_out, int8_t* k_pool, int8_t* v_pool, float* k_scale,
+                          float* v_scale, const int32_t* page_table, const uint32_t* seq_lens,
+                          const uint32_t* row_starts, g4_kv8_params p, const float* rope_cs, uint32_t rope_rows);
+/* Attention over the pool: output [num_rows][num_q_heads][head_dim] of the
+ * roped q; the row at position t sees positions max(0, t + 1 - sliding_window)
+ * .. t (from 0 without a window). All rows of a call are appended before it.
+ * workspace: g4_pagedAttn8_workspace_size bytes, 16-byte aligned, of any
+ * content; calls sharing it must not overlap. p.eps, theta and apply_divisor
+ * are unused. */
+int g4_pagedAttn8_workspace_size(g4_kv8_params p, size_t* bytes);
+int g4_pagedAttn8(g4_ctx* ctx, const float* q, const int8_t* k_pool, const int8_t* v_pool, const float* k_scale,
+                  const float* v_scale, const int32_t* page_table, const uint32_t* seq_lens,
+                  const uint32_t* row_starts, float* output, g4_kv8_params p, void* workspace,
+                  size_t workspace_bytes);
+/* k_out, v_out f16 [count][page_size][num_kv_heads][head_dim] = the values of
+ * the pages listed in `pages` (device, `count` ids; one outside [0, num_pages)
+ * gives zeros): what moves a sequence to an f16 pool. */
+int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const float* k_scale, const float* v_scale,
+                 const int32_t* pages, uint32_t count, uint32_t page_size, uint32_t num_kv_heads, uint32_t head_dim,
+                 uint32_t num_pages, uint16_t* k_out, uint16_t* v_out);
+
+/* Per row of `batch` rows of `size` logits (softcapped already), batch <= 65535:
+ *   logprobs[r] = x[tokens[r]] - log sum exp x    (a token >= size: NaN)
+ *   entropy[r] = -sum p log p                     (a p of 0 adds 0)
+ *   top_ids, top_logprobs [batch][ntop]: the ntop largest logits, largest
+ *   first, equal ones by index (NaN after everything else), ntop <= 64 and
+ *   <= size.
+ * A row with a NaN or +Inf, or of nothing but -Inf, has NaN for every
+ * probability; its ids are as stated. tokens and logprobs may be NULL together,
+ * entropy alone; ntop 0 takes no top buffers. workspace:
+ * g4_logprobsBatch_workspace_size bytes, 16-byte aligned, of any content; calls
+ * sharing it must not overlap. */
+int g4_logprobsBatch_workspace_size(uint32_t size, uint32_t batch, uint32_t ntop, size_t* bytes);
+int g4_logprobsBatch(g4_ctx* ctx, const float* logits, const uint32_t* tokens, uint32_t size, uint32_t batch,
+                     float* logprobs, float* entropy, uint32_t ntop, uint32_t* top_ids, float* top_logprobs,
+                     void* workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------ */
 /* Debug / test exports                                                      */
 /* ------------------------------------------------------------------------ */
 
