@@ -311,8 +311,9 @@ int g4_internal_kv8_check(const char* fn, const g4_kv8_params& p, const uint32_t
   G4_REQUIRE(p.page_size > 0 && p.page_size % 16 == 0 && p.page_size <= 1024,
              "%s: page_size %u is not a multiple of 16 up to 1024", fn, p.page_size);
   G4_REQUIRE(p.max_pages > 0 && p.num_pages > 0 && p.num_pages <= 0x7fffffffu && p.max_seq_len > 0 &&
-                 p.max_seq_len <= 0x7fffffffu && (uint64_t)p.max_seq_len <= (uint64_t)p.page_size * p.max_pages,
-             "%s: max_seq_len %u exceeds the page table (%u x %u)", fn, p.max_seq_len, p.max_pages, p.page_size);
+                 p.max_seq_len <= (1u << 30) && (uint64_t)p.max_seq_len <= (uint64_t)p.page_size * p.max_pages,
+             "%s: max_seq_len %u exceeds the page table (%u x %u) or 2^30", fn, p.max_seq_len, p.max_pages,
+             p.page_size);
   return G4_OK;
 }
 

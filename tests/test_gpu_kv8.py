@@ -9,7 +9,9 @@ rotation's few roundings: (parts + 10) * 2^-24 of what |x0| + |x1| would be with
 the parts' magnitudes in their place. Attention: each of a score's products is off
 by a few roundings of itself, the score by those of A = sum |q k|, so a weight p
 is off by some 6 * 2^-24 (8 + A) of itself (exp and the sums: the 8) and the
-output by that of sum p |v|."""
+output by that of sum p |v|; and p itself is held to 2^-50 of the largest (f16 hi,
+in steps of 2^-24 below 2^-14, at 2^15; the rest 2^11 finer), each of n times at
+most 127 scales."""
 import numpy as np
 import pytest
 
@@ -83,7 +85,8 @@ class Case:
             if pos < 0:
                 assert np.all(got[r] == 0), (what, r)
                 continue
-            tol = 6 * U * (8 + reach) * mag + 1e-30
+            pages = np.clip(self.table[s][:pos // self.k.codes.shape[1] + 1], 0, self.pages - 1)
+            tol = 6 * U * (8 + reach) * mag + 2.0 ** -50 * (pos + 1) * 127 * np.nanmax(self.v.scale[pages]) + 1e-30
             off = float((np.abs(got[r] - want) / tol).max())
             assert off <= 1, (what, r, s, pos, off)
         assert np.all(got[total:] == 7.5), what
@@ -312,6 +315,22 @@ def test_attention(ctx, lens, rows, nqh, nkh, hd, ps, window):
     rows = range(total) if total < 60 else sorted({*range(0, total, 7), total - 1, total - 2})
     c.check_attention(got, rows)
     assert np.array_equal(c.attention().view(np.uint32), got.view(np.uint32))  # the sums' order is fixed
+
+
+@pytest.mark.parametrize("nkh,ragged", [(1, False), (3, True)])
+def test_attention_of_many_sequences(ctx, nkh, ragged):
+    """More sequences than a wave has lanes, some without positions or rows; shares that end inside one."""
+    rng = np.random.default_rng(7)
+    lens, rows = rng.integers(0, 400, 300), np.ones(300, int)
+    lens[60:200] = 0
+    if ragged:
+        rows = rng.integers(0, 3, 300)
+    c = Case(ctx, lens, rows, 4 * nkh, nkh, 128, 32, 86, extra_rows=int(ragged)).up()
+    got = c.attention()
+    total = int(c.n.sum())
+    c.check_attention(got, range(0, total, 3))
+    for r in range(total):
+        assert np.any(got[r] != 0) == (c.row(r)[1] >= 0), r
 
 
 @pytest.mark.parametrize("rows", [1, 40])
