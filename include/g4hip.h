@@ -840,7 +840,7 @@ int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const 
                  const int32_t* pages, uint32_t count, uint32_t page_size, uint32_t num_kv_heads, uint32_t head_dim,
                  uint32_t num_pages, uint16_t* k_out, uint16_t* v_out);
 
-/* Per row of `batch` rows of `size` logits (softcapped already), batch <= 65535:
+/* Per row of `batch` <= 65535 rows of `size` <= 2^28 logits (softcapped already):
  *   logprobs[r] = x[tokens[r]] - log sum exp x    (a token >= size: NaN)
  *   entropy[r] = -sum p log p                     (a p of 0 adds 0)
  *   top_ids, top_logprobs [batch][ntop]: the ntop largest logits, largest

@@ -36,6 +36,6 @@ def test_logprobs_workspace_sizes():
     n = ctypes.c_size_t()
     f = _lib.lib().g4_logprobsBatch_workspace_size
     assert f(262144, 64, 20, ctypes.byref(n)) == 0 and 0 < n.value < 1 << 28
-    for bad in ((0, 1, 0), (1 << 31, 1, 0), (10, 0, 0), (10, 65536, 0), (10, 1, 11), (100, 1, 65)):
+    for bad in ((0, 1, 0), ((1 << 28) + 1, 1, 0), (10, 0, 0), (10, 65536, 0), (10, 1, 11), (100, 1, 65)):
         assert f(*bad, ctypes.byref(n)) == -1
     assert f(10, 1, 1, None) == -1
