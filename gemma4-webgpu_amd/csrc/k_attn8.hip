@@ -7,10 +7,10 @@
 // a column being one query row and head of a KV head. Both products read the
 // codes as they are stored or as exact f16:
 //  * scores: v_mfma_i32_16x16x64_i8 of 16 K rows by 64 dims straight from the
-//    pool's bytes. q is a 24-bit integer per element (times a power of two of
-//    its column) in three signed 8-bit digits, so a score is exact integer
-//    arithmetic, rounded to f32 when its three sums are joined: no conversion
-//    of K, and q keeps 24 bits below its largest element.
+//    pool's bytes. q is an integer per element (times a power of two of its
+//    column, the largest 2^21 .. 2^22) in three signed 8-bit digits, so a score
+//    is exact integer arithmetic, rounded to f32 when its three sums are joined:
+//    no conversion of K, and q is rounded to 2^-23 of its largest element.
 //  * P V: v_mfma_f32_16x16x32_f16, P * 2^15 as f16 hi and, times 2^11 more, its
 //    rest lo, in products of their own: 22 bits of every P down to 2^-40 of the
 //    row's largest (one pair in one sum, lo not scaled, has them down to 2^-16
@@ -35,6 +35,7 @@ using g4mm::h2;
 using g4mm::h8;
 using g4mm::static_for;
 typedef int i4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 
 constexpr int COLS = 16;                 // columns of a matrix product
 constexpr float kLog2e = 1.44269504f;    // the softmax works in powers of two
@@ -52,6 +53,8 @@ struct Args {
   uint32_t wgs;   // workgroups that share the work
   uint2* meta;    // per sequence and KV head: the workgroups that hold its partials
   float* part;    // their partials
+  // many rows: column tiles of the longest sequence, steps of a part, parts of the longest tile
+  uint32_t tiles, part_steps, nparts;
 };
 
 __device__ __forceinline__ float exp2_h(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -86,20 +89,21 @@ __device__ __forceinline__ uint32_t first_seen(const Args& a, const Seq& q) {
   return a.window && q.base + 1 > a.window ? (q.base + 1 - a.window) & ~15u : 0u;
 }
 
-// The power of two that makes the largest |q| of a column a 24-bit integer of
-// at most 0x7f7f7f (three signed digits), and its inverse; NaN where it is not finite.
+// The power of two that brings the largest |q| of a column to 2^21 .. 2^22, and
+// its inverse; NaN where it is not finite.
 __device__ __forceinline__ float digit_scale(float am, float& inverse) {
   int ex = 0;
-  const float m = frexpf(am, &ex);
-  const int k = am > 0.f ? min(max((m > 0.99f ? 22 : 23) - ex, -120), 120) : 0;
+  (void)frexpf(am, &ex);
+  const int k = am > 0.f ? min(max(22 - ex, -120), 120) : 0;
   const bool fin = am < INFINITY;
   inverse = fin ? ldexpf(1.0f, -k) : __builtin_nanf("");
   return fin ? ldexpf(1.0f, k) : 0.f;
 }
-// x as its three signed digits, one a byte (the top byte 0): x + 0x808080 has
-// the digits plus 128 as its bytes.
-__device__ __forceinline__ uint32_t digits(float x) {
-  return ((uint32_t)(int)rintf(x) + 0x808080u) ^ 0x808080u;
+// x * up, at most 2^22, as three signed digits, one a byte (the top byte is
+// not used): 1.5 * 2^23 + x up has the rounded integer in its low bits, and that
+// plus 0x808080 the digits plus 128 as its bytes.
+__device__ __forceinline__ uint32_t digits(float x, float up) {
+  return (__float_as_uint(fmaf(x, up, 12582912.f)) + (0x808080u - 0x4b400000u)) ^ 0x808080u;
 }
 // Bytes `d` of four such words as one.
 template <int D>
@@ -292,7 +296,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
       for (int e = 0; e < E; e += 4) {
         uint32_t d[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = digits(up > 0.f ? x[e + i] * up : 0.f);
+        for (int i = 0; i < 4; ++i) d[i] = digits(x[e + i], up);
         const uint32_t dim = part * E + e;
         uint32_t* dst = s_q + (((dim / 64) * 64 + dim % 64 / 16 * 16 + col) * 4 + dim % 16 / 4);
         dst[0] = plane<0>(d[0], d[1], d[2], d[3]);
@@ -513,57 +517,485 @@ __global__ __launch_bounds__(MT) void attn8_merge_kernel(Args a) {
   *(f4*)(a.out + ((size_t)(q.first + col / a.G) * a.nqh + kvh * a.G + col % a.G) * HD + d) = y * inv;
 }
 
-// One workgroup per row and query head: 256 positions at a time, one score a
-// thread, then one or two output dims a thread.
+// ---------------------------------------------------------------------------
+// many rows a sequence (prompts, mixed batches)
+// ---------------------------------------------------------------------------
+//
+// Workgroup (64 columns of a sequence and KV head, part of their positions),
+// steps of 64 positions through LDS: K as stored, V as f16 in the order of the
+// P V product's operand. A wave holds 16 columns: their q digits and output sums
+// in registers; two waves per SIMD, so that one's softmax runs beside the
+// other's products. The next step's rows are on their way in registers.
+//
+// Head dim 512 (eight waves): the two waves of a column tile have 256 dims each,
+// and 32 of the step's positions each for the softmax: they hand each other
+// their integer sums of the other's positions, then their maxima and P, through
+// LDS (q's digits of all 512 dims in one wave would spill).
+//
+// P is f16 hi + lo at 2^15 here, in one sum: its products go into the output
+// sums without further arithmetic (sums of their own per step, hi apart from lo,
+// cost as many VALU operations as the softmax). That holds P to 22 bits down to
+// 2^-17 of the row's largest and to 2^-40 of it below. P also carries the V
+// scale of its page relative to the largest of the pages so far.
+//
+// Page ids and scales come through LDS, 32 steps at a time: scalar loads share
+// their counter with LDS reads, so that the products of a step would wait for
+// those of the next one.
+//
+// Positions are cut into parts of `part_steps` steps where the tiles alone would
+// leave CUs idle (a causal prompt's last tiles are twice the average): a column
+// tile of one part is written by its workgroup, else its parts leave partials
+// that attn8_tile_merge_kernel adds in order. Later tiles, the longer ones, start
+// first.
+constexpr int TC = 64, TP = 64;  // columns of a workgroup, positions of a step
+constexpr float kTileP = 32768.f;
+constexpr float kNothing = -3e38f;  // the maximum of no positions: finite, so that differences are
 template <int HD>
-__global__ __launch_bounds__(NT) void attn8_kernel(Args a) {
-  __shared__ float s_q[512], s_p[NT], s_red[8];
-  __shared__ int s_pg[NT];
-  const uint32_t row = blockIdx.y, head = blockIdx.x, kvh = head / a.G, t = threadIdx.x, ps_ = a.page_tiles * 16;
-  const uint32_t s = seq_of_row(a.rows, row);
-  if (s >= a.rows.num_seqs) return;
+struct TileShape {
+  static constexpr bool PAIR = HD == 512;
+  static constexpr int NTH = PAIR ? 512 : 256;
+  static constexpr int KS = HD + 16;             // K row stride in LDS (bytes): 16 rows on different banks
+  static constexpr int KB = TP * KS;
+  static constexpr int VB = HD / 16;             // dims of a lane and its row's share
+  static constexpr int VBYTES = TP * HD * 2;
+  static constexpr int KP = TP * HD / 16 / NTH;  // 16-byte pieces of K a thread and step
+  static constexpr int VD = PAIR ? 16 : VB;      // dims a thread moves of 4 positions of V
+};
+
+// Columns [64 ct, + 64) of a sequence and KV head: rows r0 .. r1, which see positions lo .. end - 1.
+struct Tile {
+  uint32_t lo, end, steps, parts;
+};
+__device__ __forceinline__ Tile tile_of(const Args& a, const Seq& q, uint32_t ct) {
+  const uint32_t r0 = ct * TC / a.G, r1 = min(q.n - 1, (ct * TC + TC - 1) / a.G);
+  Tile t;
+  t.lo = a.window && q.base + r0 + 1 > a.window ? (q.base + r0 + 1 - a.window) & ~15u : 0u;
+  t.end = q.base + r1 + 1;
+  t.steps = (t.end - t.lo + TP - 1) / TP;
+  t.parts = (t.steps + a.part_steps - 1) / a.part_steps;
+  return t;
+}
+
+template <int HD>
+__global__ __launch_bounds__(TileShape<HD>::NTH, 2) void attn8_tile_kernel(Args a) {
+  using S_ = TileShape<HD>;
+  constexpr bool PAIR = S_::PAIR;
+  constexpr int KJ = PAIR ? 4 : HD / 64, KP = S_::KP, VD = S_::VD, VB = S_::VB;
+  constexpr int NE = PAIR ? 16 : VB;  // products over a wave's dims
+  constexpr int PT = PAIR ? 2 : 4;    // tiles of a wave's softmax
+  constexpr int CH = 32;              // steps whose tiles and scales are in LDS
+  __shared__ __align__(16) int8_t s_k[S_::KB];
+  __shared__ __align__(16) uint8_t s_v[S_::VBYTES];
+  __shared__ __align__(16) h8 s_p[PAIR ? 4 * 2 * 2 * 64 : 1];  // P: [column tile][32 positions][hi, lo][lane]
+  __shared__ __align__(16) i4 s_d[PAIR ? 4 * 2 * 2 * 2 * 64 : 1];  // sums: [column tile][half][tile][part][lane]
+  __shared__ float s_mx[PAIR ? 2 * TC : 1];
+  __shared__ uint32_t s_tile[4 * CH];
+  __shared__ __align__(16) float s_ks[4 * CH], s_vs[4 * CH];
+  __shared__ float s_big[2];
+  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), qd = l >> 4, c = l & 15;
+  const int wc = w & 3, wd = PAIR ? w >> 2 : 0;  // column tile; half
+
+  // (tile, sequence, KV head, part), the last tiles first
+  uint32_t b = blockIdx.x;
+  const uint32_t split = b % a.nparts;
+  b /= a.nparts;
+  const uint32_t kvh = b % a.nkh;
+  b /= a.nkh;
+  const uint32_t s = b % a.rows.num_seqs, ct = a.tiles - 1 - b / a.rows.num_seqs;
   const Seq sq = seq_rows(a.rows, s);
-  if (!sq.n) return;
-  float* out = a.out + ((size_t)row * a.nqh + head) * HD;
-  const uint32_t end = sq.len ? sq.base + (row - sq.first) + 1 : 0u;
-  const uint32_t lo = a.window && end > a.window ? end - a.window : 0u;
-  for (uint32_t d = t; d < HD; d += NT) s_q[d] = a.q[((size_t)row * a.nqh + head) * HD + d];
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (uint32_t p0 = lo; p0 < end; p0 += NT) {
-    const uint32_t pos = min(p0 + t, end - 1);
-    const uint32_t pg = page_id(a, s, pos / ps_);
+  const uint32_t ncols = uni(sq.n) * a.G, n = uni(sq.n), base = uni(sq.base), first = uni(sq.first);
+  if (ct * TC >= ncols) return;
+  if (!uni(sq.len)) {  // rows that see nothing
+    if (split == 0)
+      for (uint32_t i = tid; i < min((uint32_t)TC, ncols - ct * TC) * HD; i += S_::NTH) {
+        const uint32_t g = ct * TC + i / HD;
+        a.out[((size_t)(first + g / a.G) * a.nqh + kvh * a.G + g % a.G) * HD + i % HD] = 0.f;
+      }
+    return;
+  }
+  const Tile T = tile_of(a, Seq{first, n, base, uni(sq.len)}, ct);
+  const uint32_t lo = uni(T.lo), end = uni(T.end), parts = uni(T.parts);
+  if (split >= parts) return;
+  const uint32_t each = (uni(T.steps) + parts - 1) / parts;  // (parts of about the same length)
+  const uint32_t st0 = min(split * each, uni(T.steps)), st1 = min(uni(T.steps), st0 + each);
+  const size_t rs = (size_t)a.nkh * HD;
+  const uint32_t t0 = lo / 16, tlast = (end - 1) / 16;
+  const int32_t* list = a.page_table + (size_t)s * a.max_pages;
+
+  // this lane's column
+  const uint32_t g = ct * TC + 16 * wc + c, gr = min(g, ncols - 1);
+  const uint32_t cpos = base + gr / a.G;
+  const uint32_t clo = a.window && cpos + 1 > a.window ? cpos + 1 - a.window : 0u;
+  const uint32_t width = g < ncols ? cpos + 1 - clo : 0u;
+  // positions every column sees: those from the last row's window on, up to the first row's own
+  const uint32_t all0 = a.window && end > a.window ? end - a.window : 0u, all1 = base + ct * TC / a.G;
+
+  // ---- rows on their way ----
+  i4 kr[KP];
+  uint32_t vr_[4][VD / 4];
+  // This thread's V: positions 4 vq .. + 3 of tile vt, dims from vdim on. Its K pieces: round i in tile kt(i) (the
+  // same for all lanes of a wave).
+  const int vt = 2 * (PAIR ? (w >> 1) & 1 : w >> 1) + (l >> 5), vq = 2 * (w & 1) + ((l >> 4) & 1);
+  const uint32_t vdim = PAIR ? 256 * wd + 16 * c : VB * c;
+  constexpr int PR = HD / 16, RPI = S_::NTH / PR;  // pieces of a row, rows of a round
+  auto kt = [&](int i) { return RPI == 16 ? i : RPI == 32 ? 2 * i + (w >> 1) : w; };
+  uint32_t k_at[KP];
+#pragma unroll
+  for (int i = 0; i < KP; ++i) k_at[i] = ((i * RPI + tid / PR) % 16) * (uint32_t)rs + tid % PR * 16;
+  const uint32_t v_at = 4 * vq * (uint32_t)rs + vdim;
+  const int8_t *kp = a.kp + kvh * HD, *vp_ = a.vp + kvh * HD;
+  // Tiles (of the pool) and scales of the steps from `st` on; V's relative to the
+  // largest so far. Returns what that one grew by (1 / growth).
+  float v_ref = 0.f;
+  auto refill = [&](uint32_t st) __attribute__((always_inline)) -> float {
+    float vs = 0.f;
+    if (tid < 4 * CH) {
+      const uint32_t t = min(t0 + 4 * st + tid, tlast), at = page_of(a, t), pg = clamp_page(a, list[at]);
+      s_tile[tid] = pg * a.page_tiles + (t - at * a.page_tiles);
+      s_ks[tid] = a.ks[(size_t)pg * a.nkh + kvh];
+      vs = a.vs[(size_t)pg * a.nkh + kvh];
+      const float big = g4d::wave_max_dpp(vs);  // (a NaN is not the larger one)
+      if (l == 0) s_big[w] = big;
+    }
     __syncthreads();
-    s_pg[t] = pg;
-    const int8_t* k = a.kp + (((size_t)pg * ps_ + pos % ps_) * a.nkh + kvh) * HD;
-    float x = 0.f;
-    for (uint32_t d = 0; d < HD; ++d) x = fmaf(s_q[d], (float)k[d], x);
-    x = p0 + t < end ? x * a.scale * a.ks[(size_t)pg * a.nkh + kvh] : -INFINITY;
-    const float mx = g4d::wave_max(x);
-    if ((t & 63) == 0) s_red[t >> 6] = mx;
+    const float ref = fmaxf(v_ref, fmaxf(s_big[0], s_big[1])), by = v_ref / ref;
+    if (tid < 4 * CH) s_vs[tid] = vs / ref * kTileP;
     __syncthreads();
-    float mn = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    mn = fmaxf(m, mn);
-    const float al = m == mn ? 1.f : expf(m - mn);
-    const float p = p0 + t < end ? expf(x - mn) : 0.f;
-    s_p[t] = p;
-    const float ps = g4d::wave_sum(p);
-    if ((t & 63) == 0) s_red[4 + (t >> 6)] = ps;
+    v_ref = ref;
+    return by;
+  };
+  auto load_k = [&](uint32_t k) __attribute__((always_inline)) {  // (of the refilled steps)
+#pragma unroll
+    for (int i = 0; i < KP; ++i)
+      kr[i] = *(const i4*)((const int8_t*)uni((uint64_t)(kp + (size_t)uni(s_tile[4 * k + kt(i)]) * (16 * rs))) + k_at[i]);
+  };
+  auto load_v = [&](uint32_t k) __attribute__((always_inline)) {
+    const int8_t* vp = vp_ + (size_t)s_tile[4 * k + vt] * (16 * rs) + v_at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t* r = (const uint32_t*)(vp + i * rs);
+      if constexpr (VD == 16) {
+        const i4 x = *(const i4*)r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vr_[i][e] = (uint32_t)x[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < VD / 4; ++e) vr_[i][e] = r[e];
+      }
+    }
+  };
+  // K rows as they are; V [32 positions][product e][lane (q, c)] 16 B: slots 4 (tile & 1) + i of position 4 q + i
+  auto store_step = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < KP; ++i) *(i4*)(s_k + (i * RPI + tid / PR) * S_::KS + tid % PR * 16) = kr[i];
+    uint8_t* dst = s_v + (((vt >> 1) * (PAIR ? 2 : 1) + wd) * NE * 64 + vq * 16 + c) * 16 + (vt & 1) * 8;
+    static_for<VD>([&](auto e) __attribute__((always_inline)) {
+      constexpr int k = decltype(e)::value;
+      const h2 x = two_codes<k % 4>(vr_[0][k / 4], vr_[1][k / 4]), y = two_codes<k % 4>(vr_[2][k / 4], vr_[3][k / 4]);
+      *(g4mm::u32x2*)(dst + k * 1024) = g4mm::u32x2{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
+    });
+  };
+  (void)refill(st0);
+  load_k(0);
+  load_v(0);
+
+  // ---- q's digits of this lane's column: dims 64 j + 16 qd .. + 15 (PAIR: from 256 wd on) ----
+  i4 qb[3][KJ];
+  float s_scale;
+  {
+    const float* qg = a.q + ((size_t)(first + gr / a.G) * a.nqh + kvh * a.G + gr % a.G) * HD + 16 * qd;
+    float am = 0.f;
+    bool nan = false;
+    auto largest = [&](const f4& y) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        am = fmaxf(am, fabsf(y[i]));
+        nan |= y[i] != y[i];
+      }
+    };
+    f4 x[KJ][4];
+#pragma unroll
+    for (int j = 0; j < KJ; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[j][k] = *(const f4*)(qg + 256 * wd + 64 * j + 4 * k);
+#pragma unroll
+    for (int j = 0; j < KJ; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) largest(x[j][k]);
+    am = g4d::xmax32(g4d::xmax16(nan ? INFINITY : am));
+    if constexpr (PAIR) {  // one scale for all 512 dims
+      if (qd == 0) s_mx[wd * TC + 16 * wc + c] = am;
+      __syncthreads();
+      am = fmaxf(am, s_mx[(wd ^ 1) * TC + 16 * wc + c]);
+    }
+    float un;
+    float up = digit_scale(am, un);
+    // the joined sums are in units of the second digit; the scale's sign goes to q, a scale of 0 leaves equal scores
+    if (a.scale < 0.f) up = -up;
+    if (a.scale == 0.f) up = 0.f;
+    s_scale = a.scale == 0.f ? un : un * (fabsf(a.scale) * (kLog2e * 256.f));
+#pragma unroll
+    for (int j = 0; j < KJ; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t d[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = digits(x[j][k][i], up);
+        qb[0][j][k] = (int)plane<0>(d[0], d[1], d[2], d[3]);
+        qb[1][j][k] = (int)plane<1>(d[0], d[1], d[2], d[3]);
+        qb[2][j][k] = (int)plane<2>(d[0], d[1], d[2], d[3]);
+      }
+  }
+
+  f4 O[NE];
+#pragma unroll
+  for (int e = 0; e < NE; ++e) O[e] = f4{0.f, 0.f, 0.f, 0.f};
+  float m_run = kNothing, l_run = 0.f;  // of column c (PAIR: l of this wave's positions)
+
+  float ksc[PT], vsc[PT];  // scales of the step at hand: of this wave's tiles
+  bool odd;                // whether one of the step's is not finite
+  auto turn = [&](uint32_t st, uint32_t next, bool inside) __attribute__((always_inline)) {
+    // ---- scores of this wave's PT tiles ----
+    float x[PT][4];
+    auto score = [&](int p, const i4& hi, const i4& low) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[p][i] = fmaf((float)low[i], 1.f / 256, (float)hi[i]);
+    };
+    i4 own[PAIR ? 2 : 1][2];
+    // (PAIR: the other wave's two tiles first. A tile's rows are read while the one before is multiplied.)
+    i4 A[2][KJ];
+    const int8_t* ka = s_k + c * S_::KS + 256 * wd + 16 * qd;
+    auto read_a = [&](int pp, i4* to) __attribute__((always_inline)) {
+      const int p = PAIR ? (2 * (wd ^ 1) + pp) & 3 : pp;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) to[j] = *(const i4*)(ka + 16 * p * S_::KS + 64 * j);
+    };
+    read_a(0, A[0]);
+#pragma unroll
+    for (int pp = 0; pp < 4; ++pp) {
+      if (pp < 3) read_a(pp + 1, A[(pp + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      i4 D[3];
+#pragma unroll
+      for (int d = 0; d < 3; ++d) D[d] = i4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
+#pragma unroll
+        for (int d = 0; d < 3; ++d) D[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[pp & 1][j], qb[d][j], D[d], 0, 0, 0);
+      i4 hi;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) hi[i] = (D[2][i] << 8) + D[1][i];
+      if constexpr (!PAIR) {
+        score(pp, hi, D[0]);
+      } else if (pp < 2) {
+        i4* to = s_d + (((wc * 2 + wd) * 2 + pp) * 2) * 64 + l;
+        to[0] = hi;
+        to[64] = D[0];
+      } else {
+        own[pp - 2][0] = hi;
+        own[pp - 2][1] = D[0];
+      }
+    }
+    if constexpr (PAIR) {
+      __syncthreads();
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const i4* from = s_d + (((wc * 2 + (wd ^ 1)) * 2 + p) * 2) * 64 + l;
+        score(p, own[p][0] + from[0], own[p][1] + from[64]);
+      }
+    }
+    if (!inside) {  // (uniform; the whole step twice, with and without, spills)
+      const uint32_t pb = lo + TP * st + 32 * wd + 4 * qd - clo;
+#pragma unroll
+      for (int p = 0; p < PT; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[p][i] = pb + 16 * p + i < width ? x[p][i] : -INFINITY;
+    }
+    float mx = -INFINITY, sc[PT];  // (sc >= 0)
+#pragma unroll
+    for (int p = 0; p < PT; ++p) {
+      sc[p] = s_scale * ksc[p];
+      mx = fmaxf(mx, fmaxf(fmaxf(x[p][0], x[p][1]), fmaxf(x[p][2], x[p][3])) * sc[p]);
+    }
+    mx = g4d::xmax32(g4d::xmax16(mx));
+    // P relative to a power of two (PAIR: of this wave's positions), so that a later one rescales it exactly
+    const float m_own = fmaxf(m_run, ceilf(mx));
+    float ps = 0.f;
+    h8 ph[2], pl[2];  // of 32 positions each
+    auto weights = [&](int k) __attribute__((always_inline)) {
+      float e[2][4], es[2][4];
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[p][i] = exp2_h(fmaf(x[2 * k + p][i], sc[2 * k + p], -m_own));
+          es[p][i] = e[p][i] * vsc[2 * k + p];
+        }
+      if (odd) {  // (uniform) a page whose scale is not finite: 0 where it is masked
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[p][i] = x[2 * k + p][i] == -INFINITY ? 0.f : e[p][i];
+            es[p][i] = x[2 * k + p][i] == -INFINITY ? 0.f : es[p][i];
+          }
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        ps += (e[p][0] + e[p][1]) + (e[p][2] + e[p][3]);
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const h2 hi = __builtin_convertvector((f2{es[p][i], es[p][i + 1]}), h2);
+          const h2 lo = __builtin_convertvector(
+              (f2{fmaf((float)hi[0], -1.f, es[p][i]), fmaf((float)hi[1], -1.f, es[p][i + 1])}), h2);
+          ph[k][4 * p + i] = hi[0];
+          ph[k][4 * p + i + 1] = hi[1];
+          pl[k][4 * p + i] = lo[0];
+          pl[k][4 * p + i + 1] = lo[1];
+        }
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < PT / 2; ++k) weights(k);
+    ps = g4d::xsum32(g4d::xsum16(ps));
+    float m_new = m_own;
+    if constexpr (PAIR) {
+      h8* pp = s_p + (wc * 2 * 2) * 64 + l;
+      pp[(wd * 2) * 64] = ph[0];
+      pp[(wd * 2 + 1) * 64] = pl[0];
+      if (qd == 0) s_mx[wd * TC + 16 * wc + c] = m_own;
+      __syncthreads();
+      const float m_other = s_mx[(wd ^ 1) * TC + 16 * wc + c];
+      m_new = fmaxf(m_own, m_other);
+      const float f_own = exp2_h(m_own - m_new), f_other = exp2_h(m_other - m_new);
+      ps *= f_own;
+      ph[0] = pp[0];
+      pl[0] = pp[64];
+      ph[1] = pp[128];
+      pl[1] = pp[192];
+      if (__ballot(f_own != f_other)) {  // (one of them is 1)
+        const _Float16 f0 = (_Float16)(wd ? f_other : f_own), f1 = (_Float16)(wd ? f_own : f_other);
+        ph[0] *= f0;
+        pl[0] *= f0;
+        ph[1] *= f1;
+        pl[1] *= f1;
+      }
+    }
+    const float alpha = exp2_h(m_run - m_new);
+    l_run = l_run * alpha + ps;
+    m_run = m_new;
+    if (__ballot(alpha != 1.f)) {  // O's rows are columns 4 qd + i
+      float ar[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ar[i] = __shfl(alpha, 4 * qd + i, 64);
+#pragma unroll
+      for (int e = 0; e < NE; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[e][i] *= ar[i];
+    }
+    load_v(next);
+    // ---- P V ----
+    // groups of four dims and 32 positions, the next group's operands read while one is multiplied
+    const uint8_t* vb = s_v + wd * NE * 1024 + l * 16;
+    h8 B[2][4];
+    auto read_b = [&](int u, h8* to) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e] = *(const h8*)(vb + ((u & 1) * (PAIR ? 2 : 1) * NE + u / 2 * 4 + e) * 1024);
+    };
+    read_b(0, B[0]);
+#pragma unroll
+    for (int u = 0; u < NE / 2; ++u) {
+      if (u + 1 < NE / 2) read_b(u + 1, B[(u + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[u / 2 * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[u & 1], B[u & 1][e], O[u / 2 * 4 + e], 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[u / 2 * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[u & 1], B[u & 1][e], O[u / 2 * 4 + e], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  for (uint32_t st = st0; st < st1; ++st) {
+    __syncthreads();  // every wave is done with the previous step's rows
+    store_step();
+    {
+      const uint32_t k = 4 * ((st - st0) % CH);
+      const f4 kk = *(const f4*)(s_ks + k), vv = *(const f4*)(s_vs + k);
+      odd = __ballot(!((vv[0] + vv[1] + vv[2] + vv[3]) + (kk[0] + kk[1] + kk[2] + kk[3]) < INFINITY));
+#pragma unroll
+      for (int p = 0; p < PT; ++p) {
+        ksc[p] = kk[p];
+        vsc[p] = vv[p];
+        if (PAIR && wd) {
+          ksc[p] = kk[(p + 2) & 3];
+          vsc[p] = vv[(p + 2) & 3];
+        }
+      }
+    }
     __syncthreads();
-    l = l * al + ((s_red[4] + s_red[5]) + (s_red[6] + s_red[7]));
-    m = mn;
-    o0 *= al;
-    o1 *= al;
-    const uint32_t n = min((uint32_t)NT, end - p0);
-    for (uint32_t i = 0; i < n; ++i) {
-      const int32_t g = s_pg[i];
-      const int8_t* v = a.vp + (((size_t)g * ps_ + (p0 + i) % ps_) * a.nkh + kvh) * HD;
-      const float w = s_p[i] * a.vs[(size_t)g * a.nkh + kvh];
-      if (t < HD) o0 = fmaf(w, (float)v[t], o0);
-      if (t + NT < HD) o1 = fmaf(w, (float)v[t + NT], o1);
+    // the next step's rows are in flight during this one, K's from before its scores, V's from before its P V (past
+    // the last step: its own rows again, not used)
+    const uint32_t next = (min(st + 1, st1 - 1) - st0) % CH;
+    float by = 1.f;
+    if (next == 0 && st + 1 < st1) by = refill(st + 1);  // (uniform)
+    load_k(next);
+    const uint32_t p0 = lo + TP * st;
+    turn(st, next, p0 >= all0 && p0 + TP - 1 <= all1);
+    if (by != 1.f) {  // (uniform) V's scales are relative to a larger one from here on
+#pragma unroll
+      for (int e = 0; e < NE; ++e) O[e] *= by;
     }
   }
-  if (t < HD) out[t] = end ? o0 / l : 0.f;
-  if (t + NT < HD) out[t + NT] = end ? o1 / l : 0.f;
+
+  // ---- columns 4 qd + i of the wave's tile, dims VB c + e (PAIR: 256 wd + 16 c + e) ----
+  if constexpr (PAIR) {
+    __syncthreads();
+    if (qd == 0) s_mx[wd * TC + 16 * wc + c] = l_run;
+    __syncthreads();
+    l_run = s_mx[16 * wc + c] + s_mx[TC + 16 * wc + c];
+  }
+  const bool whole = parts == 1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float L = __shfl(l_run, 4 * qd + i, 64), f = (whole ? 1.0f / L : 1.f) * (v_ref * (1.f / kTileP));
+    const uint32_t og = ct * TC + 16 * wc + 4 * qd + i;
+    if (og < ncols) {
+      const size_t row = (size_t)(first + og / a.G) * a.nqh + kvh * a.G + og % a.G;
+      float* o = (whole ? a.out : a.part + 2 * (size_t)a.nparts * a.rows.num_rows * a.nqh +
+                                      (size_t)split * a.rows.num_rows * a.nqh * HD) + row * HD + vdim;
+#pragma unroll
+      for (int e = 0; e < NE; e += 4) *(f4*)(o + e) = f4{O[e][i] * f, O[e + 1][i] * f, O[e + 2][i] * f, O[e + 3][i] * f};
+    }
+  }
+  if (!whole && wd == 0 && qd == 0 && g < ncols) {
+    const size_t row = (size_t)(first + g / a.G) * a.nqh + kvh * a.G + g % a.G, n_ = (size_t)a.rows.num_rows * a.nqh;
+    a.part[split * n_ + row] = m_run;
+    a.part[(a.nparts + split) * n_ + row] = l_run;
+  }
+}
+
+// out of a row and head from its tile's parts, in order.
+template <int HD>
+__global__ __launch_bounds__(HD / 4) void attn8_tile_merge_kernel(Args a) {
+  const uint32_t row = blockIdx.x / a.nqh, head = blockIdx.x % a.nqh, d = threadIdx.x * 4;
+  const uint32_t s = seq_of_row(a.rows, row);
+  if (s >= a.rows.num_seqs) return;
+  const Seq q = seq_rows(a.rows, s);
+  if (!q.len) return;
+  const uint32_t parts = tile_of(a, q, ((row - q.first) * a.G + head % a.G) / TC).parts;
+  if (parts == 1) return;
+  const size_t n = (size_t)a.rows.num_rows * a.nqh;
+  const float *pm = a.part + blockIdx.x, *pl = pm + a.nparts * n;
+  const float* po = a.part + 2 * a.nparts * n + (size_t)blockIdx.x * HD + d;
+  float M = -INFINITY, L = 0.f;
+  for (uint32_t k = 0; k < parts; ++k) M = fmaxf(M, pm[k * n]);
+  f4 o = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (uint32_t k = 0; k < parts; ++k) {
+    const float m = pm[k * n], f = m == -INFINITY ? 1.f : exp2_h(m - M);  // (-Inf: sums of 0, or NaN)
+    L += f * pl[k * n];
+    o += f * *(const f4*)(po + k * n * HD);
+  }
+  *(f4*)(a.out + (size_t)blockIdx.x * HD + d) = o * (1.0f / L);
 }
 
 bool step_fits(const g4_kv8_params& p) {
@@ -587,6 +1019,31 @@ size_t step_bytes(const g4_kv8_params& p) {
   return meta_bytes(p) + 2ull * step_wgs<HD>(p) * StepShape<HD>::SLOT * sizeof(float);
 }
 
+// Column tiles of the longest sequence; of all of them together (at most); steps of the longest tile.
+uint32_t tiles_of(const g4_kv8_params& p) {
+  return ceil_div((uint64_t)p.max_rows * (p.num_q_heads / p.num_kv_heads), TC);
+}
+uint64_t all_tiles(const g4_kv8_params& p) {
+  const uint64_t G = p.num_q_heads / p.num_kv_heads;
+  return (std::min<uint64_t>(ceil_div(p.num_rows * G, TC) + p.num_seqs, (uint64_t)tiles_of(p) * p.num_seqs)) *
+         p.num_kv_heads;
+}
+uint32_t most_steps(const g4_kv8_params& p) {
+  const uint64_t rows = TC / (p.num_q_heads / p.num_kv_heads) + 2;  // of a tile
+  uint64_t span = p.max_seq_len;
+  if (p.sliding_window) span = std::min<uint64_t>(span, p.sliding_window + rows + 15);
+  return ceil_div(span, TP);
+}
+// Steps of a part: about two parts for every workgroup that runs at once if every tile were the longest, at least 4.
+uint32_t part_steps(const g4_kv8_params& p) {
+  const uint64_t parts = p.head_dim == 512 ? 512 : 1024;
+  return (uint32_t)std::max<uint64_t>(4, (all_tiles(p) * most_steps(p) + parts - 1) / parts);
+}
+size_t tile_bytes(const g4_kv8_params& p) {
+  const uint32_t np = ceil_div(most_steps(p), part_steps(p));
+  return np > 1 ? (size_t)np * p.num_rows * p.num_q_heads * (p.head_dim + 2) * sizeof(float) : 256;
+}
+
 template <int HD>
 int attend(g4_ctx* ctx, const g4_kv8_params& p, Args a, void* workspace) {
   if (step_fits(p)) {
@@ -608,8 +1065,18 @@ int attend(g4_ctx* ctx, const g4_kv8_params& p, Args a, void* workspace) {
     G4_LAUNCHED(ctx, "attn8_merge");
     return G4_OK;
   }
-  hipLaunchKernelGGL(attn8_kernel<HD>, dim3(p.num_q_heads, p.num_rows), dim3(NT), 0, ctx->stream, a);
-  G4_LAUNCHED(ctx, "attn8");
+  a.tiles = tiles_of(p);
+  a.part_steps = part_steps(p);
+  a.nparts = ceil_div(most_steps(p), a.part_steps);
+  a.part = (float*)workspace;
+  const uint64_t grid = (uint64_t)a.tiles * p.num_seqs * p.num_kv_heads * a.nparts;
+  G4_REQUIRE(grid < (1ull << 31), "g4_pagedAttn8: %u sequences of up to %u rows and %u positions in one call", p.num_seqs,
+             p.max_rows, p.max_seq_len);
+  hipLaunchKernelGGL(attn8_tile_kernel<HD>, dim3((unsigned)grid), dim3(TileShape<HD>::NTH), 0, ctx->stream, a);
+  G4_LAUNCHED(ctx, "attn8_tile");
+  if (a.nparts == 1) return G4_OK;
+  hipLaunchKernelGGL(attn8_tile_merge_kernel<HD>, dim3(p.num_rows * p.num_q_heads), dim3(HD / 4), 0, ctx->stream, a);
+  G4_LAUNCHED(ctx, "attn8_tile_merge");
   return G4_OK;
 }
 
@@ -621,7 +1088,7 @@ int g4_pagedAttn8_workspace_size(g4_kv8_params p, size_t* bytes) {
   G4_REQUIRE(bytes, "g4_pagedAttn8_workspace_size: null out");
   int rc = g4_internal_kv8_check(__func__, p, p.max_rows == 1 && p.num_rows == p.num_seqs ? nullptr : &p.num_rows);
   if (rc) return rc;
-  *bytes = 256;
+  *bytes = tile_bytes(p);
   if (step_fits(p))
     *bytes = p.head_dim == 64 ? step_bytes<64>(p) : p.head_dim == 128 ? step_bytes<128>(p)
              : p.head_dim == 256 ? step_bytes<256>(p) : step_bytes<512>(p);
@@ -648,7 +1115,7 @@ int g4_pagedAttn8(g4_ctx* ctx, const float* q, const int8_t* k_pool, const int8_
                {seq_lens, row_starts, p.num_seqs, p.num_rows, p.max_rows, p.max_seq_len},
                p.num_q_heads, p.num_kv_heads, p.num_q_heads / p.num_kv_heads, tiles,
                tiles == 1 ? 0u : (uint32_t)(((1ull << 32) + tiles - 1) / tiles), tiles == 1 ? ~0u : 0u, p.max_pages, p.num_pages, p.sliding_window, p.scale,
-               output, 0, nullptr, nullptr};
+               output, 0, nullptr, nullptr, 0, 0, 0};
   switch (p.head_dim) {
     case 64: return attend<64>(ctx, p, a, workspace);
     case 128: return attend<128>(ctx, p, a, workspace);

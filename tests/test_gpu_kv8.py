@@ -9,9 +9,9 @@ rotation's few roundings: (parts + 10) * 2^-24 of what |x0| + |x1| would be with
 the parts' magnitudes in their place. Attention: each of a score's products is off
 by a few roundings of itself, the score by those of A = sum |q k|, so a weight p
 is off by some 6 * 2^-24 (8 + A) of itself (exp and the sums: the 8) and the
-output by that of sum p |v|; and p itself is held to 2^-50 of the largest (f16 hi,
-in steps of 2^-24 below 2^-14, at 2^15; the rest 2^11 finer), each of n times at
-most 127 scales."""
+output by that of sum p |v|; and p itself is held to 2^-40 of the largest (f16
+pairs at 2^15: the steps below 2^-14 are 2^-24, half of one is 2^-25), each of n
+times at most 127 scales."""
 import numpy as np
 import pytest
 
@@ -86,7 +86,7 @@ class Case:
                 assert np.all(got[r] == 0), (what, r)
                 continue
             pages = np.clip(self.table[s][:pos // self.k.codes.shape[1] + 1], 0, self.pages - 1)
-            tol = 6 * U * (8 + reach) * mag + 2.0 ** -50 * (pos + 1) * 127 * np.nanmax(self.v.scale[pages]) + 1e-30
+            tol = 6 * U * (8 + reach) * mag + 2.0 ** -40 * (pos + 1) * 127 * np.nanmax(self.v.scale[pages]) + 1e-30
             off = float((np.abs(got[r] - want) / tol).max())
             assert off <= 1, (what, r, s, pos, off)
         assert np.all(got[total:] == 7.5), what
