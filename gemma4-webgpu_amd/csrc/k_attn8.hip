@@ -53,8 +53,7 @@ struct Args {
   uint32_t wgs;   // workgroups that share the work
   uint2* meta;    // per sequence and KV head: the workgroups that hold its partials
   float* part;    // their partials
-  // many rows: column tiles of the longest sequence, steps of a part, parts of the longest tile
-  uint32_t tiles, part_steps, nparts;
+  uint32_t tiles;  // many rows: column tiles of the longest sequence
 };
 
 __device__ __forceinline__ float exp2_h(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -542,13 +541,15 @@ __global__ __launch_bounds__(MT) void attn8_merge_kernel(Args a) {
 // their counter with LDS reads, so that the products of a step would wait for
 // those of the next one.
 //
-// Positions are cut into parts of `part_steps` steps where the tiles alone would
-// leave CUs idle (a causal prompt's last tiles are twice the average): a column
-// tile of one part is written by its workgroup, else its parts leave partials
-// that attn8_tile_merge_kernel adds in order. Later tiles, the longer ones, start
-// first.
+// The steps of all column tiles, and kTileCost more for each tile (its q, its
+// output: about as long as so many steps), are dealt to the workgroups in equal
+// shares, one or two workgroups a CU: a causal prompt's last tiles are twice the
+// average, and a tile each, or tiles cut into parts, leaves CUs idle at the end. A
+// tile held by one workgroup is written by it, else its workgroups leave partials
+// that attn8_tile_merge_kernel adds in order.
 constexpr int TC = 64, TP = 64;  // columns of a workgroup, positions of a step
 constexpr float kTileP = 32768.f;
+constexpr uint32_t kTileCost = 3, kLeast = 4;  // cost of a tile besides its steps; least cost of a share
 constexpr float kNothing = -3e38f;  // the maximum of no positions: finite, so that differences are
 template <int HD>
 struct TileShape {
@@ -560,11 +561,13 @@ struct TileShape {
   static constexpr int VBYTES = TP * HD * 2;
   static constexpr int KP = TP * HD / 16 / NTH;  // 16-byte pieces of K a thread and step
   static constexpr int VD = PAIR ? 16 : VB;      // dims a thread moves of 4 positions of V
+  static constexpr uint32_t WGS = HD == 512 ? 256 : HD == 256 ? 512 : 768;  // that run at once (registers, LDS)
+  static constexpr uint32_t SLOT = TC * (HD + 2);                           // floats of a partial: max, sum [64], o
 };
 
 // Columns [64 ct, + 64) of a sequence and KV head: rows r0 .. r1, which see positions lo .. end - 1.
 struct Tile {
-  uint32_t lo, end, steps, parts;
+  uint32_t lo, end, steps;
 };
 __device__ __forceinline__ Tile tile_of(const Args& a, const Seq& q, uint32_t ct) {
   const uint32_t r0 = ct * TC / a.G, r1 = min(q.n - 1, (ct * TC + TC - 1) / a.G);
@@ -572,12 +575,17 @@ __device__ __forceinline__ Tile tile_of(const Args& a, const Seq& q, uint32_t ct
   t.lo = a.window && q.base + r0 + 1 > a.window ? (q.base + r0 + 1 - a.window) & ~15u : 0u;
   t.end = q.base + r1 + 1;
   t.steps = (t.end - t.lo + TP - 1) / TP;
-  t.parts = (t.steps + a.part_steps - 1) / a.part_steps;
   return t;
+}
+// Cost of column tile j % tiles of sequence j / tiles: kTileCost, then its steps (0: there is none).
+__device__ __forceinline__ uint32_t cost_of(const Args& a, uint32_t j) {
+  const Seq q = seq_rows(a.rows, j / a.tiles);
+  const uint32_t ct = j % a.tiles;
+  return q.len && ct * TC < q.n * a.G ? kTileCost + tile_of(a, q, ct).steps : 0u;
 }
 
 template <int HD>
-__global__ __launch_bounds__(TileShape<HD>::NTH, 2) void attn8_tile_kernel(Args a) {
+__global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_tile_kernel(Args a) {
   using S_ = TileShape<HD>;
   constexpr bool PAIR = S_::PAIR;
   constexpr int KJ = PAIR ? 4 : HD / 64, KP = S_::KP, VD = S_::VD, VB = S_::VB;
@@ -592,32 +600,67 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, 2) void attn8_tile_kernel(Args 
   __shared__ uint32_t s_tile[4 * CH];
   __shared__ __align__(16) float s_ks[4 * CH], s_vs[4 * CH];
   __shared__ float s_big[2];
+  __shared__ uint32_t s_upto[S_::NTH + 1], s_sum[S_::NTH / 64], s_at[2];  // s_upto: units before each thread's run
   const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), qd = l >> 4, c = l & 15;
   const int wc = w & 3, wd = PAIR ? w >> 2 : 0;  // column tile; half
 
-  // (tile, sequence, KV head, part), the last tiles first
-  uint32_t b = blockIdx.x;
-  const uint32_t split = b % a.nparts;
-  b /= a.nparts;
-  const uint32_t kvh = b % a.nkh;
-  b /= a.nkh;
-  const uint32_t s = b % a.rows.num_seqs, ct = a.tiles - 1 - b / a.rows.num_seqs;
+  // ---- this workgroup's share of the whole cost: a run of column tiles a thread, summed up ----
+  const uint32_t wg = blockIdx.x, pairs = a.rows.num_seqs * a.tiles, run = (pairs + S_::NTH - 1) / S_::NTH;
+  const uint32_t j0 = min(tid * run, pairs), j1 = min(j0 + run, pairs);
+  uint32_t mine = 0;
+  for (uint32_t j = j0; j < j1; ++j) mine += cost_of(a, j) * a.nkh;
+  uint32_t upto = wave_scan(mine);
+  if (l == 63) s_sum[w] = upto;
+  __syncthreads();
+  uint32_t total = 0;
+#pragma unroll
+  for (int i = 0; i < S_::NTH / 64; ++i) {
+    if (i < w) upto += s_sum[i];
+    total += s_sum[i];
+  }
+  total = uni(total);
+  s_upto[tid + 1] = upto;
+  if (tid == 0) s_upto[0] = 0;
+  __syncthreads();
+  const Share sh{total, min(a.wgs, (total + kLeast - 1) / kLeast)};
+  const uint32_t ub = wg < sh.W ? sh.first(wg) : 0u, ue = wg < sh.W ? sh.first(wg + 1) : 0u;
+  uint32_t pair = 0, before = 0, used = 0;  // column tile at hand, the units before it; partials written
+  auto locate = [&](uint32_t unit) {  // the column tile of a unit, by the thread whose run holds it
+    if (s_upto[tid] <= unit && s_upto[tid + 1] > unit) {
+      uint32_t j = tid * run, at = s_upto[tid];
+      for (uint32_t n; at + (n = cost_of(a, j) * a.nkh) <= unit; ++j) at += n;
+      s_at[0] = j;
+      s_at[1] = at;
+    }
+    __syncthreads();
+    pair = uni(s_at[0]);
+    before = uni(s_at[1]);
+    __syncthreads();
+  };
+  if (ub < ue) locate(ub);
+
+  for (uint32_t u = ub; u < ue;) {
+  const uint32_t s = pair / a.tiles, ct = pair % a.tiles;
   const Seq sq = seq_rows(a.rows, s);
-  const uint32_t ncols = uni(sq.n) * a.G, n = uni(sq.n), base = uni(sq.base), first = uni(sq.first);
-  if (ct * TC >= ncols) return;
-  if (!uni(sq.len)) {  // rows that see nothing
-    if (split == 0)
-      for (uint32_t i = tid; i < min((uint32_t)TC, ncols - ct * TC) * HD; i += S_::NTH) {
-        const uint32_t g = ct * TC + i / HD;
-        a.out[((size_t)(first + g / a.G) * a.nqh + kvh * a.G + g % a.G) * HD + i % HD] = 0.f;
-      }
-    return;
+  const uint32_t n = uni(sq.n), ncols = n * a.G, base = uni(sq.base), first = uni(sq.first);
+  if (!uni(sq.len) || ct * TC >= ncols) {  // behind the sequence's last tile
+    locate(u);
+    continue;
   }
   const Tile T = tile_of(a, Seq{first, n, base, uni(sq.len)}, ct);
-  const uint32_t lo = uni(T.lo), end = uni(T.end), parts = uni(T.parts);
-  if (split >= parts) return;
-  const uint32_t each = (uni(T.steps) + parts - 1) / parts;  // (parts of about the same length)
-  const uint32_t st0 = min(split * each, uni(T.steps)), st1 = min(uni(T.steps), st0 + each);
+  const uint32_t lo = uni(T.lo), end = uni(T.end), steps = uni(T.steps), cost = kTileCost + steps;
+  if (u >= before + cost * a.nkh) {
+    before += cost * a.nkh;
+    ++pair;
+    if (pair >= pairs) locate(u);
+    continue;
+  }
+  const uint32_t kvh = a.nkh == 1 ? 0u : uni((u - before) / cost);
+  const uint32_t seg = before + kvh * cost, stop = min(seg + cost, ue);  // the tile's first unit, the last here
+  const uint32_t st0 = max(u, seg + kTileCost) - (seg + kTileCost), st1 = max(stop, seg + kTileCost) - (seg + kTileCost);
+  u = stop;
+  if (st0 == st1) continue;  // (the share ends before the tile's first step)
+  __syncthreads();  // the previous tile's rows are done with
   const size_t rs = (size_t)a.nkh * HD;
   const uint32_t t0 = lo / 16, tlast = (end - 1) / 16;
   const int32_t* list = a.page_table + (size_t)s * a.max_pages;
@@ -953,27 +996,42 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, 2) void attn8_tile_kernel(Args 
     __syncthreads();
     l_run = s_mx[16 * wc + c] + s_mx[TC + 16 * wc + c];
   }
-  const bool whole = parts == 1;
+  const bool whole = st1 - st0 == steps;
+  const uint32_t slot = 2 * wg + used;  // (0 for a tile begun by another workgroup: it comes first)
+  used = 1;
+  float* part = a.part + (size_t)slot * TileShape<HD>::SLOT;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    const uint32_t col = 16 * wc + 4 * qd + i, og = ct * TC + col;
     const float L = __shfl(l_run, 4 * qd + i, 64), f = (whole ? 1.0f / L : 1.f) * (v_ref * (1.f / kTileP));
-    const uint32_t og = ct * TC + 16 * wc + 4 * qd + i;
     if (og < ncols) {
-      const size_t row = (size_t)(first + og / a.G) * a.nqh + kvh * a.G + og % a.G;
-      float* o = (whole ? a.out : a.part + 2 * (size_t)a.nparts * a.rows.num_rows * a.nqh +
-                                      (size_t)split * a.rows.num_rows * a.nqh * HD) + row * HD + vdim;
+      float* o = (whole ? a.out + ((size_t)(first + og / a.G) * a.nqh + kvh * a.G + og % a.G) * HD
+                        : part + 2 * TC + col * HD) + vdim;
 #pragma unroll
       for (int e = 0; e < NE; e += 4) *(f4*)(o + e) = f4{O[e][i] * f, O[e + 1][i] * f, O[e + 2][i] * f, O[e + 3][i] * f};
     }
   }
-  if (!whole && wd == 0 && qd == 0 && g < ncols) {
-    const size_t row = (size_t)(first + g / a.G) * a.nqh + kvh * a.G + g % a.G, n_ = (size_t)a.rows.num_rows * a.nqh;
-    a.part[split * n_ + row] = m_run;
-    a.part[(a.nparts + split) * n_ + row] = l_run;
+  if (!whole && wd == 0 && qd == 0) {
+    part[16 * wc + c] = m_run;
+    part[TC + 16 * wc + c] = l_run;
+  }
+  if (st0 == 0 && tid == 0) a.meta[(size_t)pair * a.nkh + kvh] = make_uint2(slot, sh.owner(seg + cost - 1));
+  }
+
+  // rows that see nothing
+  for (uint32_t j = wg; j < pairs; j += gridDim.x) {
+    const Seq q = seq_rows(a.rows, j / a.tiles);
+    const uint32_t g0 = j % a.tiles * TC, ncols = q.n * a.G;
+    if (q.len || g0 >= ncols) continue;
+    for (uint32_t i = tid; i < min((uint32_t)TC, ncols - g0) * a.nkh * HD; i += S_::NTH) {
+      const uint32_t g = g0 + i / HD / a.nkh, kvh = i / HD % a.nkh;
+      a.out[((size_t)(q.first + g / a.G) * a.nqh + kvh * a.G + g % a.G) * HD + i % HD] = 0.f;
+    }
   }
 }
 
-// out of a row and head from its tile's parts, in order.
+// out of a row and head from its tile's partials, in order: that of workgroup
+// meta.x / 2 (slot meta.x), then slot 0 of each up to meta.y.
 template <int HD>
 __global__ __launch_bounds__(HD / 4) void attn8_tile_merge_kernel(Args a) {
   const uint32_t row = blockIdx.x / a.nqh, head = blockIdx.x % a.nqh, d = threadIdx.x * 4;
@@ -981,19 +1039,20 @@ __global__ __launch_bounds__(HD / 4) void attn8_tile_merge_kernel(Args a) {
   if (s >= a.rows.num_seqs) return;
   const Seq q = seq_rows(a.rows, s);
   if (!q.len) return;
-  const uint32_t parts = tile_of(a, q, ((row - q.first) * a.G + head % a.G) / TC).parts;
-  if (parts == 1) return;
-  const size_t n = (size_t)a.rows.num_rows * a.nqh;
-  const float *pm = a.part + blockIdx.x, *pl = pm + a.nparts * n;
-  const float* po = a.part + 2 * a.nparts * n + (size_t)blockIdx.x * HD + d;
+  const uint32_t g = (row - q.first) * a.G + head % a.G, col = g % TC;
+  const uint2 mt = a.meta[((size_t)s * a.tiles + g / TC) * a.nkh + head / a.G];
+  const uint32_t w0 = mt.x / 2, n = mt.y - w0 + 1;
+  if (n == 1) return;  // written by its workgroup
+  auto part = [&](uint32_t k) { return a.part + (size_t)(k ? 2 * (w0 + k) : mt.x) * TileShape<HD>::SLOT; };
   float M = -INFINITY, L = 0.f;
-  for (uint32_t k = 0; k < parts; ++k) M = fmaxf(M, pm[k * n]);
+  for (uint32_t k = 0; k < n; ++k) M = fmaxf(M, part(k)[col]);
   f4 o = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (uint32_t k = 0; k < parts; ++k) {
-    const float m = pm[k * n], f = m == -INFINITY ? 1.f : exp2_h(m - M);  // (-Inf: sums of 0, or NaN)
-    L += f * pl[k * n];
-    o += f * *(const f4*)(po + k * n * HD);
+  for (uint32_t k = 0; k < n; ++k) {
+    const float* p = part(k);
+    const float f = exp2_h(p[col] - M);
+    L += f * p[TC + col];
+    o += f * *(const f4*)(p + 2 * TC + col * HD + d);
   }
   *(f4*)(a.out + (size_t)blockIdx.x * HD + d) = o * (1.0f / L);
 }
@@ -1019,29 +1078,31 @@ size_t step_bytes(const g4_kv8_params& p) {
   return meta_bytes(p) + 2ull * step_wgs<HD>(p) * StepShape<HD>::SLOT * sizeof(float);
 }
 
-// Column tiles of the longest sequence; of all of them together (at most); steps of the longest tile.
+// Column tiles of the longest sequence; cost of all tiles (at most).
 uint32_t tiles_of(const g4_kv8_params& p) {
   return ceil_div((uint64_t)p.max_rows * (p.num_q_heads / p.num_kv_heads), TC);
 }
-uint64_t all_tiles(const g4_kv8_params& p) {
-  const uint64_t G = p.num_q_heads / p.num_kv_heads;
-  return (std::min<uint64_t>(ceil_div(p.num_rows * G, TC) + p.num_seqs, (uint64_t)tiles_of(p) * p.num_seqs)) *
-         p.num_kv_heads;
-}
-uint32_t most_steps(const g4_kv8_params& p) {
-  const uint64_t rows = TC / (p.num_q_heads / p.num_kv_heads) + 2;  // of a tile
+uint64_t all_cost(const g4_kv8_params& p) {
+  const uint64_t G = p.num_q_heads / p.num_kv_heads, rows = TC / G + 2;  // of a tile
+  const uint64_t tiles = std::min<uint64_t>(ceil_div(p.num_rows * G, TC) + p.num_seqs, (uint64_t)tiles_of(p) * p.num_seqs);
   uint64_t span = p.max_seq_len;
   if (p.sliding_window) span = std::min<uint64_t>(span, p.sliding_window + rows + 15);
-  return ceil_div(span, TP);
+  return tiles * p.num_kv_heads * (kTileCost + ceil_div(span, TP));
 }
-// Steps of a part: about two parts for every workgroup that runs at once if every tile were the longest, at least 4.
-uint32_t part_steps(const g4_kv8_params& p) {
-  const uint64_t parts = p.head_dim == 512 ? 512 : 1024;
-  return (uint32_t)std::max<uint64_t>(4, (all_tiles(p) * most_steps(p) + parts - 1) / parts);
+template <int HD>
+uint32_t tile_wgs(const g4_kv8_params& p) {
+  return (uint32_t)std::min<uint64_t>(TileShape<HD>::WGS, (all_cost(p) + kLeast - 1) / kLeast);
 }
+size_t tile_meta_bytes(const g4_kv8_params& p) {
+  return ((size_t)p.num_seqs * tiles_of(p) * p.num_kv_heads * sizeof(uint2) + 255) / 256 * 256;
+}
+template <int HD>
 size_t tile_bytes(const g4_kv8_params& p) {
-  const uint32_t np = ceil_div(most_steps(p), part_steps(p));
-  return np > 1 ? (size_t)np * p.num_rows * p.num_q_heads * (p.head_dim + 2) * sizeof(float) : 256;
+  return tile_meta_bytes(p) + 2ull * tile_wgs<HD>(p) * TileShape<HD>::SLOT * sizeof(float);
+}
+template <int HD>
+size_t attn_bytes(const g4_kv8_params& p) {
+  return step_fits(p) ? step_bytes<HD>(p) : tile_bytes<HD>(p);
 }
 
 template <int HD>
@@ -1066,15 +1127,15 @@ int attend(g4_ctx* ctx, const g4_kv8_params& p, Args a, void* workspace) {
     return G4_OK;
   }
   a.tiles = tiles_of(p);
-  a.part_steps = part_steps(p);
-  a.nparts = ceil_div(most_steps(p), a.part_steps);
-  a.part = (float*)workspace;
-  const uint64_t grid = (uint64_t)a.tiles * p.num_seqs * p.num_kv_heads * a.nparts;
-  G4_REQUIRE(grid < (1ull << 31), "g4_pagedAttn8: %u sequences of up to %u rows and %u positions in one call", p.num_seqs,
-             p.max_rows, p.max_seq_len);
-  hipLaunchKernelGGL(attn8_tile_kernel<HD>, dim3((unsigned)grid), dim3(TileShape<HD>::NTH), 0, ctx->stream, a);
+  G4_REQUIRE(all_cost(p) < (1ull << 31) && (uint64_t)a.tiles * p.num_seqs * p.num_kv_heads < (1ull << 31),
+             "g4_pagedAttn8: %u sequences of up to %u rows and %u positions in one call", p.num_seqs, p.max_rows,
+             p.max_seq_len);
+  a.wgs = tile_wgs<HD>(p);
+  a.meta = (uint2*)workspace;
+  a.part = (float*)((uint8_t*)workspace + tile_meta_bytes(p));
+  hipLaunchKernelGGL(attn8_tile_kernel<HD>, dim3(a.wgs), dim3(TileShape<HD>::NTH), 0, ctx->stream, a);
   G4_LAUNCHED(ctx, "attn8_tile");
-  if (a.nparts == 1) return G4_OK;
+  if (a.wgs == 1) return G4_OK;  // no tile has partials
   hipLaunchKernelGGL(attn8_tile_merge_kernel<HD>, dim3(p.num_rows * p.num_q_heads), dim3(HD / 4), 0, ctx->stream, a);
   G4_LAUNCHED(ctx, "attn8_tile_merge");
   return G4_OK;
@@ -1088,10 +1149,8 @@ int g4_pagedAttn8_workspace_size(g4_kv8_params p, size_t* bytes) {
   G4_REQUIRE(bytes, "g4_pagedAttn8_workspace_size: null out");
   int rc = g4_internal_kv8_check(__func__, p, p.max_rows == 1 && p.num_rows == p.num_seqs ? nullptr : &p.num_rows);
   if (rc) return rc;
-  *bytes = tile_bytes(p);
-  if (step_fits(p))
-    *bytes = p.head_dim == 64 ? step_bytes<64>(p) : p.head_dim == 128 ? step_bytes<128>(p)
-             : p.head_dim == 256 ? step_bytes<256>(p) : step_bytes<512>(p);
+  *bytes = p.head_dim == 64 ? attn_bytes<64>(p) : p.head_dim == 128 ? attn_bytes<128>(p)
+           : p.head_dim == 256 ? attn_bytes<256>(p) : attn_bytes<512>(p);
   return G4_OK;
 }
 
@@ -1115,7 +1174,7 @@ int g4_pagedAttn8(g4_ctx* ctx, const float* q, const int8_t* k_pool, const int8_
                {seq_lens, row_starts, p.num_seqs, p.num_rows, p.max_rows, p.max_seq_len},
                p.num_q_heads, p.num_kv_heads, p.num_q_heads / p.num_kv_heads, tiles,
                tiles == 1 ? 0u : (uint32_t)(((1ull << 32) + tiles - 1) / tiles), tiles == 1 ? ~0u : 0u, p.max_pages, p.num_pages, p.sliding_window, p.scale,
-               output, 0, nullptr, nullptr, 0, 0, 0};
+               output, 0, nullptr, nullptr, 0};
   switch (p.head_dim) {
     case 64: return attend<64>(ctx, p, a, workspace);
     case 128: return attend<128>(ctx, p, a, workspace);
