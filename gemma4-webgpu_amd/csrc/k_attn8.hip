@@ -60,6 +60,7 @@ __device__ __forceinline__ float exp2_h(float x) { return __builtin_amdgcn_exp2f
 
 // Wave-uniform values into scalar registers.
 __device__ __forceinline__ uint32_t uni(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int32_t uni_i(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ uint64_t uni(uint64_t x) {
   return (uint64_t)uni((uint32_t)(x >> 32)) << 32 | uni((uint32_t)x);
 }
@@ -69,12 +70,6 @@ __device__ __forceinline__ uint64_t uni(uint64_t x) {
 // (one tile a page: a magic of 0 and all of t).
 __device__ __forceinline__ uint32_t page_of(const Args& a, uint32_t t) {
   return __umulhi(t, a.page_magic) + (t & a.page_same);
-}
-// A wave-uniform word that no kernel of the launch writes, by a scalar load:
-// it does not queue behind the vector loads in flight.
-template <typename T>
-__device__ __forceinline__ T scalar_load(const T* p) {
-  return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
 }
 __device__ __forceinline__ uint32_t clamp_page(const Args& a, int32_t pg) {
   return pg < 0 ? 0u : min((uint32_t)pg, a.num_pages - 1);
@@ -215,19 +210,28 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     i4 K[2][KJ];
     uint32_t V[8][VB / 4];
     float ks[2], vs[2];
-    // page ids of the next step and, on their way, of the one after it
+    // page ids of the next step and, on their way, of the one after it (vector loads, issued before the rows that
+    // go before them in use: a scalar load's wait is that of the LDS reads too)
     int32_t pg[2], pg_far[2];
     const uint32_t st1 = 4 * (off + take), tiles = (end - lo + 15) / 16, t0 = lo / 16;
     const uint32_t k_at = c * (uint32_t)rs + 16 * qd, v_at = 4 * qd * (uint32_t)rs + VB * c;
     const int32_t* list = a.page_table + (size_t)s * a.max_pages;
     auto pages = [&](uint32_t st, int32_t* to) {
 #pragma unroll
-      for (int p = 0; p < 2; ++p) to[p] = scalar_load(list + page_of(a, t0 + min(2 * st + p, tiles - 1)));
+      for (int p = 0; p < 2; ++p) to[p] = list[page_of(a, t0 + min(2 * st + p, tiles - 1))];
     };
     auto tile_at = [&](const int8_t* pool, uint32_t st, int p) -> const int8_t* {  // the tile's first row
       const uint32_t t = t0 + min(2 * st + p, tiles - 1), slot = (t - page_of(a, t) * a.page_tiles) * 16;
       return (const int8_t*)uni(
-          (uint64_t)(pool + ((size_t)clamp_page(a, pg[p]) * (a.page_tiles * 16) + slot) * rs + kvh * HD));
+          (uint64_t)(pool + ((size_t)clamp_page(a, uni_i(pg[p])) * (a.page_tiles * 16) + slot) * rs + kvh * HD));
+    };
+    auto load_scales = [&](float* k, float* v) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const size_t at = (size_t)clamp_page(a, uni_i(pg[p])) * a.nkh + kvh;
+        k[p] = a.ks[at];
+        v[p] = a.vs[at];
+      }
     };
     auto load_k = [&](uint32_t st) {
 #pragma unroll
@@ -235,7 +239,6 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
         const int8_t* base = tile_at(a.kp, st, p);
 #pragma unroll
         for (int j = 0; j < KJ; ++j) K[p][j] = *(const i4*)(base + k_at + 64 * j);
-        ks[p] = scalar_load(a.ks + (size_t)clamp_page(a, pg[p]) * a.nkh + kvh);
       }
     };
     auto load_v = [&](uint32_t st) {
@@ -257,7 +260,6 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
             for (int e = 0; e < VB / 4; ++e) V[4 * p + i][e] = r[e];
           }
         }
-        vs[p] = scalar_load(a.vs + (size_t)clamp_page(a, pg[p]) * a.nkh + kvh);
       }
     };
 
@@ -265,6 +267,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     const uint32_t steps = min(st1, (tiles + 1) / 2);  // (the last unit may be short)
     if (st < steps) {
       pages(st, pg);
+      load_scales(ks, vs);
       load_k(st);
       load_v(st);
       pages(min(st + 4, steps - 1), pg);
@@ -332,6 +335,8 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
         }
       const float sc[2] = {s_scale * ks[0], s_scale * ks[1]};
       pages(min(st + 8, steps - 1), pg_far);
+      float ksn[2], vsn[2];
+      load_scales(ksn, vsn);
       load_k(next);
       // ---- softmax over the step's 32 positions ----
       const uint32_t pb = lo + 32 * st + 4 * qd;
@@ -394,7 +399,11 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
       static_for<VB>(product);
       load_v(next);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) pg[p] = pg_far[p];
+      for (int p = 0; p < 2; ++p) {
+        pg[p] = pg_far[p];
+        ks[p] = ksn[p];
+        vs[p] = vsn[p];
+      }
     }
 
     // ---- the four waves' sums, in their order ----

@@ -11,11 +11,12 @@
 //
 // kv8_prologue_kernel: every page of a KV head that a call touches belongs to
 // one workgroup (K and V apart), which forms its rows' largest element before
-// it stores any code; other workgroups take the query rows, one wave a row and
-// head. Norms, rotation and rounding of K and V are in f64: a value near the
+// it stores any code; other workgroups take the query rows, a wave four heads of
+// one. Whatever depends on the row's place only (parts, norm weights, rotation)
+// is loaded before the first sum. Norms, rotation and rounding of K and V are in f64: a value near the
 // border of two codes then gets the same code as in exact arithmetic, whatever
-// the order of the sums (the f64 units are idle otherwise). q is f32. Up to 16
-// rows of a page stay in registers between the two steps; more are formed
+// the order of the sums (the f64 units are idle otherwise). q is f32. Up to 32
+// rows of a page (16 at head dim 512) stay in registers between the two steps; more are formed
 // again for the second.
 #include "kv8.hpp"
 #include "mqf_core.hpp"
@@ -24,8 +25,9 @@ namespace {
 
 using namespace g4kv8;
 
-constexpr int NT = 256, NW = NT / 64;
-constexpr int KEEP = 4;  // rows a wave keeps in registers
+constexpr int NT = 512, NW = NT / 64;
+constexpr int VT = 256;  // threads of the values kernel
+constexpr int QH = 4;    // query heads of a row that a wave takes
 
 struct ProArgs {
   const float *q, *k, *v;
@@ -39,7 +41,7 @@ struct ProArgs {
   const int32_t* page_table;
   Rows rows;
   uint32_t nqh, nkh, page_size, max_pages, num_pages;
-  uint32_t q_blocks, seq_pages;  // workgroups of the query rows; pages a sequence's rows may touch
+  uint32_t kv_blocks, seq_pages;  // workgroups of the pages; pages a sequence's rows may touch
   float eps, theta;
   uint32_t apply_divisor;
 };
@@ -50,11 +52,6 @@ struct Row {
   static constexpr int HALF = HD / 2, PP = HALF >= 64 ? HALF / 64 : 1, ACT = HALF / PP;
 };
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
 __device__ __forceinline__ double wave_max64(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
@@ -86,50 +83,97 @@ __device__ __forceinline__ void load_row(const float* p, size_t stride, uint32_t
   }
 }
 
-template <int HD, typename T>
-__device__ __forceinline__ void rotate(const ProArgs& a, const uint16_t* w, uint32_t pos, int lane, T* lo, T* hi) {
+// Cos and sin of a lane's pairs at a position, and a norm's weights at them (1 without one).
+template <int HD>
+struct Turn {
+  static constexpr int PP = Row<HD>::PP;
+  float2 cs[PP];
+};
+template <int HD>
+__device__ __forceinline__ void load_turn(const ProArgs& a, uint32_t pos, int lane, Turn<HD>& t) {
   constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
-  if (lane >= Row<HD>::ACT) return;
 #pragma unroll
   for (int i = 0; i < PP; ++i) {
-    const int t = PP * lane + i;
-    const float2 cs = a.rope_cs ? a.rope_cs[(size_t)pos * HALF + t]
-                                : g4mqf::rope_cos_sin(a.theta, a.apply_divisor, a.rope_freqs[t], t, HD, pos);
-    const T x0 = lo[i] * (T)g4d::f16_bits_to_f32(w[t]), x1 = hi[i] * (T)g4d::f16_bits_to_f32(w[t + HALF]);
-    lo[i] = x0 * (T)cs.x - x1 * (T)cs.y;
-    hi[i] = x0 * (T)cs.y + x1 * (T)cs.x;
+    const int k = min(PP * lane + i, HALF - 1);
+    t.cs[i] = a.rope_cs ? a.rope_cs[(size_t)pos * HALF + k]
+                        : g4mqf::rope_cos_sin(a.theta, a.apply_divisor, a.rope_freqs[k], k, HD, pos);
+  }
+}
+template <int HD>
+struct Weights {
+  static constexpr int PP = Row<HD>::PP;
+  float lo[PP], hi[PP];
+};
+template <int HD>
+__device__ __forceinline__ void load_weights(const uint16_t* w, int lane, Weights<HD>& t) {
+  constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
+#pragma unroll
+  for (int i = 0; i < PP; ++i) {
+    const int k = min(PP * lane + i, HALF - 1);
+    t.lo[i] = g4d::f16_bits_to_f32(w[k]);
+    t.hi[i] = g4d::f16_bits_to_f32(w[k + HALF]);
+  }
+}
+template <int HD, typename T>
+__device__ __forceinline__ void rotate(const Weights<HD>& w, const Turn<HD>& t, T* lo, T* hi) {
+#pragma unroll
+  for (int i = 0; i < Row<HD>::PP; ++i) {
+    const T x0 = lo[i] * (T)w.lo[i], x1 = hi[i] * (T)w.hi[i];
+    lo[i] = x0 * (T)t.cs[i].x - x1 * (T)t.cs[i].y;
+    hi[i] = x0 * (T)t.cs[i].y + x1 * (T)t.cs[i].x;
   }
 }
 
 template <int HD>
-__device__ __forceinline__ void q_row(const ProArgs& a) {
+__device__ __forceinline__ void q_row(const ProArgs& a, uint32_t block) {
   constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
   const int lane = threadIdx.x & 63;
-  const uint64_t i = (uint64_t)blockIdx.x * NW + (threadIdx.x >> 6);
-  if (i >= (uint64_t)a.rows.num_rows * a.nqh) return;
-  const uint32_t row = (uint32_t)(i / a.nqh), head = (uint32_t)(i % a.nqh);
+  const uint32_t groups = (a.nqh + QH - 1) / QH;
+  const uint64_t i = (uint64_t)block * NW + (threadIdx.x >> 6);
+  if (i >= (uint64_t)a.rows.num_rows * groups) return;
+  const uint32_t row = (uint32_t)(i / groups), h0 = (uint32_t)(i % groups) * QH;
+  const size_t at = ((size_t)row * a.nqh + h0) * HD, stride = (size_t)a.rows.num_rows * a.nqh * HD;
+  Weights<HD> w;
+  load_weights<HD>(a.q_w, lane, w);
+  float lo[QH][PP], hi[QH][PP];
+#pragma unroll
+  for (int h = 0; h < QH; ++h) load_row<HD>(a.q + at + min((uint32_t)h, a.nqh - 1 - h0) * HD, stride, a.nparts, lane, lo[h], hi[h]);
   const uint32_t s = seq_of_row(a.rows, row);
   if (s >= a.rows.num_seqs) return;
   const Seq q = seq_rows(a.rows, s);
   if (!q.len) return;
-  const size_t at = ((size_t)row * a.nqh + head) * HD;
-  float lo[PP], hi[PP], ss = 0.f;
-  load_row<HD>(a.q + at, (size_t)a.rows.num_rows * a.nqh * HD, a.nparts, lane, lo, hi);
+  Turn<HD> t;
+  load_turn<HD>(a, q.base + (row - q.first), lane, t);
 #pragma unroll
-  for (int e = 0; e < PP; ++e) ss += lo[e] * lo[e] + hi[e] * hi[e];
-  ss = g4d::wave_sum_dpp(ss);
-  const float inv = 1.0f / sqrtf(ss * (1.0f / (float)HD) + a.eps);
+  for (int h = 0; h < QH; ++h) {
+    if (h0 + h >= a.nqh) return;
+    float ss = 0.f;
 #pragma unroll
-  for (int e = 0; e < PP; ++e) {
-    lo[e] *= inv;
-    hi[e] *= inv;
-  }
-  rotate<HD>(a, a.q_w, q.base + (row - q.first), lane, lo, hi);
-  if (lane < Row<HD>::ACT) {
+    for (int e = 0; e < PP; ++e) ss += lo[h][e] * lo[h][e] + hi[h][e] * hi[h][e];
+    ss = g4d::wave_sum_dpp(ss);
+    const float inv = 1.0f / sqrtf(ss * (1.0f / (float)HD) + a.eps);
 #pragma unroll
     for (int e = 0; e < PP; ++e) {
-      a.q_out[at + PP * lane + e] = lo[e];
-      a.q_out[at + HALF + PP * lane + e] = hi[e];
+      lo[h][e] *= inv;
+      hi[h][e] *= inv;
+    }
+    rotate<HD>(w, t, lo[h], hi[h]);
+    if (lane < Row<HD>::ACT) {
+      float* o = a.q_out + at + h * HD + PP * lane;
+      if constexpr (PP == 1) {
+        o[0] = lo[h][0];
+        o[HALF] = hi[h][0];
+      } else {
+        typedef float vec __attribute__((ext_vector_type(PP)));
+        vec x, y;
+#pragma unroll
+        for (int e = 0; e < PP; ++e) {
+          x[e] = lo[h][e];
+          y[e] = hi[h][e];
+        }
+        *(vec*)o = x;
+        *(vec*)(o + HALF) = y;
+      }
     }
   }
 }
@@ -142,17 +186,17 @@ __device__ __forceinline__ float scale_of(double am) {
   return ldexpf(1.0f, am > 0.0 ? max(x - 7 + (m > 127.0 / 128.0), -64) : -64);
 }
 
-template <int HD>
-__global__ __launch_bounds__(NT) void kv8_prologue_kernel(ProArgs a) {
+template <int HD, int KEEP>
+__global__ __launch_bounds__(NT, 4) void kv8_prologue_kernel(ProArgs a) {
   constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
   __shared__ double s_am[NW];
   __shared__ int s_bad;
-  if (blockIdx.x < a.q_blocks) {
-    q_row<HD>(a);
+  if (blockIdx.x >= a.kv_blocks) {  // (the pages, which take longer, start first)
+    q_row<HD>(a, blockIdx.x - a.kv_blocks);
     return;
   }
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  uint32_t b = blockIdx.x - a.q_blocks;
+  uint32_t b = blockIdx.x;
   const bool is_v = b & 1;
   b >>= 1;
   const uint32_t kvh = b % a.nkh;
@@ -169,25 +213,43 @@ __global__ __launch_bounds__(NT) void kv8_prologue_kernel(ProArgs a) {
   const size_t stride = (size_t)a.rows.num_rows * a.nkh * HD;
 
   double lo[KEEP][PP], hi[KEEP][PP];
-  auto form = [&](uint32_t at) {  // the wave's rows p0 + at + w, + NW, ...
+  Weights<HD> wt;
+  if (!is_v) load_weights<HD>(a.k_w, lane, wt);
+  auto form = [&](uint32_t at) {  // the wave's rows p0 + at + w, + NW, ... (past the last: 0)
+    Turn<HD> turn[KEEP];
 #pragma unroll
     for (int r = 0; r < KEEP; ++r) {
       const uint32_t i = at + w + NW * r;
+      if (i < m) {  // (uniform over the wave)
+        load_row<HD>(src + ((size_t)(q.first + (p0 - q.base) + i) * a.nkh + kvh) * HD, stride, a.nparts, lane, lo[r],
+                     hi[r]);
+        if (!is_v) load_turn<HD>(a, p0 + i, lane, turn[r]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < PP; ++e) lo[r][e] = hi[r][e] = 0.0;
-      if (i >= m) continue;  // (uniform over the wave)
-      load_row<HD>(src + ((size_t)(q.first + (p0 - q.base) + i) * a.nkh + kvh) * HD, stride, a.nparts, lane, lo[r],
-                   hi[r]);
-      double ss = 0.0;
+        for (int e = 0; e < PP; ++e) lo[r][e] = hi[r][e] = 0.0;
+      }
+    }
+    double ss[KEEP];
 #pragma unroll
-      for (int e = 0; e < PP; ++e) ss += lo[r][e] * lo[r][e] + hi[r][e] * hi[r][e];
-      const double inv = 1.0 / sqrt(wave_sum64(ss) * (1.0 / HD) + (double)a.eps);
+    for (int r = 0; r < KEEP; ++r) {
+      ss[r] = 0.0;
+#pragma unroll
+      for (int e = 0; e < PP; ++e) ss[r] += lo[r][e] * lo[r][e] + hi[r][e] * hi[r][e];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+#pragma unroll
+      for (int r = 0; r < KEEP; ++r) ss[r] += __shfl_xor(ss[r], o, 64);
+#pragma unroll
+    for (int r = 0; r < KEEP; ++r) {
+      if (at + w + NW * r >= m) continue;
+      const double inv = 1.0 / sqrt(ss[r] * (1.0 / HD) + (double)a.eps);
 #pragma unroll
       for (int e = 0; e < PP; ++e) {
         lo[r][e] *= inv;
         hi[r][e] *= inv;
       }
-      if (!is_v) rotate<HD>(a, a.k_w, p0 + i, lane, lo[r], hi[r]);
+      if (!is_v) rotate<HD>(wt, turn[r], lo[r], hi[r]);
     }
   };
   double am = 0.0;
@@ -212,7 +274,8 @@ __global__ __launch_bounds__(NT) void kv8_prologue_kernel(ProArgs a) {
   const uint32_t before = p0 - start;  // codes of earlier calls
   const float old = before ? *sp : 0.f;
   __syncthreads();
-  am = fmax(fmax(s_am[0], s_am[1]), fmax(s_am[2], s_am[3]));
+#pragma unroll
+  for (int i = 0; i < NW; ++i) am = fmax(am, s_am[i]);
   const bool poison = s_bad || old != old;
   const float sc = poison ? __builtin_nanf("") : fmaxf(old, scale_of(am));
   if (threadIdx.x == 0) *sp = sc;
@@ -271,10 +334,10 @@ struct ValArgs {
 
 // 16 codes a thread. A code times its scale has 7 bits: exact in f16 from
 // 2^-24 to 65504.
-__global__ __launch_bounds__(NT) void kv8_values_kernel(ValArgs a) {
+__global__ __launch_bounds__(VT) void kv8_values_kernel(ValArgs a) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   const uint32_t bytes = a.page_size * a.nkh * a.hd;  // of a page
-  const uint32_t i = (blockIdx.y * NT + threadIdx.x) * 16;
+  const uint32_t i = (blockIdx.y * VT + threadIdx.x) * 16;
   if (i >= bytes) return;
   const uint32_t which = blockIdx.z;
   const int32_t pg = a.pages[blockIdx.x];
@@ -292,6 +355,15 @@ __global__ __launch_bounds__(NT) void kv8_values_kernel(ValArgs a) {
   u32x4* o = (u32x4*)(a.out[which] + (size_t)blockIdx.x * bytes + i);
   o[0] = in ? y[0] : u32x4{0, 0, 0, 0};
   o[1] = in ? y[1] : u32x4{0, 0, 0, 0};
+}
+
+// Rows a wave keeps: one where no sequence has more than the workgroup's eight
+// waves (a step of 64 rows at head dim 256 9.8 us with four, 8.3 with one), else
+// four, two at head dim 512 (four spill).
+template <int HD>
+void prologue(g4_ctx* ctx, const g4_kv8_params& p, dim3 grid, const ProArgs& a) {
+  if (p.max_rows <= NW) hipLaunchKernelGGL((kv8_prologue_kernel<HD, 1>), grid, dim3(NT), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((kv8_prologue_kernel<HD, HD == 512 ? 2 : 4>), grid, dim3(NT), 0, ctx->stream, a);
 }
 
 }  // namespace
@@ -314,6 +386,8 @@ int g4_internal_kv8_check(const char* fn, const g4_kv8_params& p, const uint32_t
                  p.max_seq_len <= (1u << 30) && (uint64_t)p.max_seq_len <= (uint64_t)p.page_size * p.max_pages,
              "%s: max_seq_len %u exceeds the page table (%u x %u) or 2^30", fn, p.max_seq_len, p.max_pages,
              p.page_size);
+  G4_REQUIRE((uint64_t)p.num_pages * (p.page_size / 16) < 1ull << 32, "%s: %u pages of %u: 2^36 positions or more", fn,
+             p.num_pages, p.page_size);
   return G4_OK;
 }
 
@@ -364,16 +438,17 @@ int g4_pagedAttnPrologue8(g4_ctx* ctx, const float* q_parts, const float* k_part
   a.eps = p.eps;
   a.theta = p.theta;
   a.apply_divisor = p.apply_divisor;
-  a.q_blocks = q ? ceil_div((uint64_t)p.num_rows * p.num_q_heads, NW) : 0;
   a.seq_pages = ceil_div(p.max_rows - 1, p.page_size) + 1;
-  const uint64_t blocks = a.q_blocks + (kv ? 2ull * p.num_seqs * a.seq_pages * p.num_kv_heads : 0ull);
+  const uint64_t kv_blocks = kv ? 2ull * p.num_seqs * a.seq_pages * p.num_kv_heads : 0ull;
+  const uint64_t blocks = kv_blocks + (q ? ceil_div((uint64_t)p.num_rows * ceil_div(p.num_q_heads, QH), NW) : 0);
   G4_REQUIRE(blocks <= 0x7fffffffull, "g4_pagedAttnPrologue8: %llu workgroups", (unsigned long long)blocks);
+  a.kv_blocks = (uint32_t)kv_blocks;
   const dim3 grid((unsigned)blocks);
   switch (p.head_dim) {
-    case 64: hipLaunchKernelGGL(kv8_prologue_kernel<64>, grid, dim3(NT), 0, ctx->stream, a); break;
-    case 128: hipLaunchKernelGGL(kv8_prologue_kernel<128>, grid, dim3(NT), 0, ctx->stream, a); break;
-    case 256: hipLaunchKernelGGL(kv8_prologue_kernel<256>, grid, dim3(NT), 0, ctx->stream, a); break;
-    default: hipLaunchKernelGGL(kv8_prologue_kernel<512>, grid, dim3(NT), 0, ctx->stream, a); break;
+    case 64: prologue<64>(ctx, p, grid, a); break;
+    case 128: prologue<128>(ctx, p, grid, a); break;
+    case 256: prologue<256>(ctx, p, grid, a); break;
+    default: prologue<512>(ctx, p, grid, a); break;
   }
   G4_LAUNCHED(ctx, "kv8_prologue");
   return G4_OK;
@@ -396,8 +471,8 @@ int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const 
   if (rc) return rc;
   G4_REQUIRE(count > 0 && count <= 0x7fffffffu, "g4_kv8Values: %u pages", count);
   const ValArgs a{{k_pool, v_pool}, {k_scale, v_scale}, {k_out, v_out}, pages, page_size, num_kv_heads, head_dim, num_pages};
-  hipLaunchKernelGGL(kv8_values_kernel, dim3(count, ceil_div((uint64_t)page_size * num_kv_heads * head_dim, 16 * NT), 2),
-                     dim3(NT), 0, ctx->stream, a);
+  hipLaunchKernelGGL(kv8_values_kernel, dim3(count, ceil_div((uint64_t)page_size * num_kv_heads * head_dim, 16 * VT), 2),
+                     dim3(VT), 0, ctx->stream, a);
   G4_LAUNCHED(ctx, "kv8_values");
   return G4_OK;
 }

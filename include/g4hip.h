@@ -794,7 +794,8 @@ int g4_prefillAttn(g4_ctx* ctx, const float* q, const uint16_t* k_pool, const ui
  * when read, as in the f16 pool.
  *
  * page_size: a multiple of 16, at most 1024. head_dim 64, 128, 256 or 512, at
- * most 64 KV heads with at most 16 query heads each. */
+ * most 64 KV heads with at most 16 query heads each. max_seq_len: at most 2^30
+ * and page_size * max_pages; the pool holds fewer than 2^36 positions. */
 typedef struct {
   uint32_t num_seqs, num_q_heads, num_kv_heads, head_dim;
   uint32_t page_size, max_pages, max_seq_len, num_pages;

@@ -39,3 +39,9 @@ def test_logprobs_workspace_sizes():
     for bad in ((0, 1, 0), ((1 << 28) + 1, 1, 0), (10, 0, 0), (10, 65536, 0), (10, 1, 11), (100, 1, 65)):
         assert f(*bad, ctypes.byref(n)) == -1
     assert f(10, 1, 1, None) == -1
+
+
+def test_a_pool_of_too_many_positions_is_refused():
+    big = dict(page_size=1024, max_seq_len=1024, max_pages=1)
+    assert size(num_pages=(1 << 26) - 1, **big)[0] == 0
+    assert size(num_pages=1 << 26, **big)[0] == -1
