@@ -824,7 +824,8 @@ class Decoder(_SyntheticModel):
 
 class BatchDecoder(_SyntheticModel):
     """Ragged multi-sequence decode: `num_seqs` sequences with their own cached
-    lengths share one set of weights and, per layer, one paged f16 K/V pool.
+    lengths share one set of weights and, per layer, one paged K/V pool (f16
+    or 8-bit).
 
     Pages are handed out on the host when the decoder is built: sequence i
     owns ceil((context_lens[i] + reserve) / page_size) pages, taken from a
@@ -842,11 +843,20 @@ class BatchDecoder(_SyntheticModel):
 
     def __init__(self, ctx: Context, context_lens, shape: Optional[E2BShape] = None, page_size: int = 16,
                  reserve: int = 64, seed: int = 0, n_layers: Optional[int] = None, lm_head: bool = True,
-                 page_seed: int = 7, shared_pages: bool = False, embed: bool = False, wtypes=None, gguf=None):
+                 page_seed: int = 7, shared_pages: bool = False, embed: bool = False, wtypes=None, gguf=None, kv: str = "f16",
+                 logprobs: Optional[int] = None):
         """shared_pages: every row reads and appends through one page list
         (the rows are tokens of one sequence: batched prefill). embed: an f16
         token table; each step starts from the embedding of every row's
-        token in `tokens` (the previous step's sample, or the prompt)."""
+        token in `tokens` (the previous step's sample, or the prompt). kv:
+        "f16" or "int8" pages (8-bit codes with a scale per page and KV head,
+        half the pool's bytes; page_size a multiple of 16). logprobs: a step
+        that samples leaves every row's token_logprobs (of its argmax),
+        entropy and this many alternatives (top_ids, top_logprobs [B][n])."""
+        if kv not in ("f16", "int8"):
+            raise ValueError(f"kv {kv!r}: f16 or int8")
+        if logprobs is not None and not lm_head:
+            raise ValueError("logprobs need the LM head")
         lens = np.asarray(context_lens, dtype=np.int64)
         if lens.ndim != 1 or lens.size == 0 or lens.size > 64 or np.any(lens < 0):
             raise ValueError("context_lens: 1..64 non-negative lengths")
@@ -870,10 +880,15 @@ class BatchDecoder(_SyntheticModel):
         self.page_table_host = table
         self.lens_host = lens.astype(np.uint32)
         rows = self.num_pages * page_size
+        self.kv8 = kv == "int8"
+        code = np.int8 if self.kv8 else np.uint16
         self._build_weights(ctx, shape, n_layers, seed, lm_head,
-                            lambda il: (ctx.zeros(rows * self.s.kv_dim_of(il), np.uint16),
-                                        ctx.zeros(rows * self.s.kv_dim_of(il), np.uint16)), embed=embed,
+                            lambda il: (ctx.zeros(rows * self.s.kv_dim_of(il), code),
+                                        ctx.zeros(rows * self.s.kv_dim_of(il), code)), embed=embed,
                             wtypes=wtypes, gguf=gguf)
+        # 8-bit pools: the scales of each producer's pages (k, v), f32 [num_pages][KV heads]
+        self.kv_scales = {il: tuple(ctx.zeros(self.num_pages * self.s.n_kv_heads, np.float32) for _ in "kv")
+                          for il in range(self.s.n_layers) if self.kv8 and self.s.is_producer(il)}
         s, B, f32 = self.s, self.B, np.float32
         self.page_table = ctx.from_numpy(table)
         self.seq_lens = ctx.from_numpy(self.lens_host)
@@ -905,6 +920,13 @@ class BatchDecoder(_SyntheticModel):
         self.logits = ctx.empty(B * s.vocab, f32) if lm_head else None
         self.tokens = ctx.zeros(B, np.uint32)
         self.topk = ctx.empty(B * 512, f32)
+        self.ntop = logprobs
+        if logprobs is not None:
+            self.token_logprobs = ctx.zeros(B, f32)
+            self.entropy = ctx.zeros(B, f32)
+            self.top_ids = ctx.zeros(B * logprobs, np.uint32) if logprobs else None
+            self.top_logprobs = ctx.zeros(B * logprobs, f32) if logprobs else None
+            self.logprobs_ws = ctx.alloc(ctx.logprobs_workspace_bytes(s.vocab, B, logprobs))
         if s.ple_dim:
             LD = s.n_layers * s.ple_dim
             self.ple_projected = ctx.empty(B * LD, f32)
@@ -926,10 +948,18 @@ class BatchDecoder(_SyntheticModel):
         # except where the rows share pages (prefill), whose prologue must
         # append every row before the attention reads any
         # (its own workspace: its arrival counters stay zero between calls)
-        self.block_attn = not shared_pages
-        self.attn_ws = ctx.zeros(max(ctx.paged_workspace_bytes(p) for p in self.attn_params), np.uint8)
-        self.block_ws = ctx.zeros(max(ctx.paged_block_workspace_bytes(p, self.ks_h) for p in self.pro_params),
-                                  np.uint8)
+        self.block_attn = not shared_pages and not self.kv8
+        if self.kv8:
+            # a shared page list holds one sequence: its length after the step
+            # and the first and past-the-last row that are its
+            self.span = ctx.zeros(3, np.uint32)
+            self.span_rows = 0
+            self.attn8_ws, self.attn8_cap = None, 0
+            self._attn8_workspace([self._kv8_params(il, B, B if shared_pages else 1) for il in range(s.n_layers)])
+        else:
+            self.attn_ws = ctx.zeros(max(ctx.paged_workspace_bytes(p) for p in self.attn_params), np.uint8)
+            self.block_ws = ctx.zeros(max(ctx.paged_block_workspace_bytes(p, self.ks_h) for p in self.pro_params),
+                                      np.uint8)
         self.rope_cs = self._rope_tables(self.max_seq)
         # prompts longer than one chunk of B rows go through the layers this
         # many rows at a time (0: B at a time); the buffers of such a pass come
@@ -947,6 +977,15 @@ class BatchDecoder(_SyntheticModel):
             if not self.s.is_producer(il):
                 continue
             n = self.num_pages * self.page_size * self.s.kv_dim_of(il)
+            if self.kv8:  # codes ~ N(0, 32^2) under a scale of 1/32 (past 2^22 of them, repeated)
+                rng = np.random.default_rng(splitmix64(seed, 2 * il))
+                for pool, scale in zip((L.k_cache, L.v_cache), self.kv_scales[il]):
+                    m = min(n, 1 << 22)
+                    pool.upload(np.clip(np.rint(rng.normal(0, 32, m)), -127, 127).astype(np.int8))
+                    for at in range(m, n, m):
+                        self.ctx.copy(pool.offset(at), pool, min(m, n - at))
+                    scale.upload(np.full(self.num_pages * self.s.n_kv_heads, 1 / 32, np.float32))
+                continue
             self.ctx.fill_normal_f16(L.k_cache, n, splitmix64(seed, 2 * il), 0.0, 1.0)
             self.ctx.fill_normal_f16(L.v_cache, n, splitmix64(seed, 2 * il + 1), 0.0, 1.0)
 
@@ -970,8 +1009,43 @@ class BatchDecoder(_SyntheticModel):
                 n = int(L) + 1
                 if not s.is_global(il):
                     n = min(n, s.window)
-                total += n * 2 * s.kv_dim_of(il) * 2
+                total += n * 2 * s.kv_dim_of(il) * (1 if self.kv8 else 2)
+                if self.kv8:
+                    total += -(-n // self.page_size) * 2 * s.n_kv_heads * 4
         return total
+
+    def _kv8_params(self, il: int, rows: int, valid: int, end: Optional[int] = None):
+        """Layer il's 8-bit attention over `rows` rows: of one sequence up to position `end`, of which the first
+        `valid` are its (shared_pages), or one of each sequence."""
+        s, glob = self.s, self.s.is_global(il)
+        return self.ctx.kv8_params(1 if self.shared_pages else rows, s.n_q_heads, s.n_kv_heads, s.hd(il),
+                                   self.page_size, self.max_pages, end or self.max_seq, self.num_pages, rows, valid,
+                                   0 if glob else s.window, 1.0, s.eps, s.theta_global if glob else s.theta_local,
+                                   int(glob))
+
+    def _attn8_workspace(self, params) -> None:
+        need = max(self.ctx.attn8_workspace_bytes(p) for p in params)
+        if need > self.attn8_cap:
+            self.attn8_ws = None  # (the old one is given back first)
+            self.attn8_ws, self.attn8_cap = self.ctx.alloc(need), need
+
+    def _attend8(self, il: int, q_parts, k_parts, v_parts, nq: int, q, out, p) -> None:
+        """Layer il's prologue and attention over its 8-bit pages. Of a shared page list, the spare rows past
+        the sequence's get its last row's output, as if they were that row again."""
+        c, s, L = self.ctx, self.s, self.layers[il]
+        src = il if s.is_producer(il) else s.producer(il)
+        prod = src == il
+        starts, lens = (self.span.offset(4), self.span) if self.shared_pages else (None, self.seq_lens)
+        if self.shared_pages:  # (few rows take another kernel than many)
+            self._attn8_workspace([p])
+        c.pagedAttnPrologue8(q_parts, k_parts if prod else None, v_parts if prod else None, nq, L.q_norm,
+                             L.k_norm if prod else None, self.rope_freqs, q, L.k_cache, L.v_cache,
+                             *self.kv_scales[src], self.page_table, lens, p, row_starts=starts,
+                             rope_cs=self.rope_cs[s.is_global(il)], rope_rows=self.rope_rows)
+        c.pagedAttn8(q, L.k_cache, L.v_cache, *self.kv_scales[src], self.page_table, lens, out, p, self.attn8_ws,
+                     row_starts=starts)
+        if self.shared_pages and p.max_rows < p.num_rows:
+            c.repeatRow(out, s.q_dim_of(il), p.max_rows - 1, p.max_rows, p.num_rows - p.max_rows)
 
     def step(self, sample: str = "argmax", probe=None, head: bool = True,
              rows: Optional[int] = None) -> None:
@@ -1005,6 +1079,8 @@ class BatchDecoder(_SyntheticModel):
         partial sums and the appended rows by all B sequences."""
         if rows is not None and not (self.shared_pages and 1 <= rows <= self.B):
             raise ValueError(f"step: rows={rows} needs shared_pages and 1..{self.B} rows")
+        if self.kv8 and self.shared_pages and not self.span_rows:
+            raise ValueError("step: 8-bit shared pages hold one sequence, whose rows prefill and score place")
         c, s, B = self.ctx, self.s, self.B if rows is None else rows
         H = s.hidden
         if self.embedding is not None:
@@ -1053,6 +1129,10 @@ class BatchDecoder(_SyntheticModel):
                                  L.q_norm, L.k_norm, self.rope_freqs, self.q, L.k_cache, L.v_cache, self.page_table,
                                  self.seq_lens, self.attn, self.pro_params[il], self.block_ws, ops=ops,
                                  rope_cs=self.rope_cs[s.is_global(il)], rope_rows=self.rope_rows)
+            elif self.kv8:
+                ops = None  # the o projection's own launch prepares its operands
+                self._attend8(il, self.q_parts, self.k_parts, self.v_parts, nq, self.q, self.attn,
+                              self._kv8_params(il, B, min(self.span_rows, B) if self.shared_pages else 1))
             else:
                 c.pagedAttnPrologue(self.q_parts, self.k_parts if prod else None, self.v_parts if prod else None, nq,
                                     L.q_norm, L.k_norm, self.rope_freqs, self.q, L.k_cache if prod else None,
@@ -1132,6 +1212,11 @@ class BatchDecoder(_SyntheticModel):
             c.argmaxBatch(self.logits, self.tokens, s.vocab, B)
         else:
             c.topk256Batch(self.logits, self.topk, s.vocab, B)
+        if self.ntop is not None:  # (the host samples of the top-k: no token's log probability then)
+            drawn = sample == "argmax"
+            c.logprobsBatch(self.logits, self.tokens if drawn else None, s.vocab, B,
+                            self.token_logprobs if drawn else None, self.entropy, self.ntop, self.top_ids,
+                            self.top_logprobs, self.logprobs_ws)
 
     def _ffn_handoff(self, il: int) -> bool:
         """Layer il's gate/up launch hands its product to the down projection
@@ -1199,20 +1284,66 @@ class BatchDecoder(_SyntheticModel):
         # a single chunk takes only as many rows as its matrix-core tiles need
         rows = next((r for r in (16, 32) if T <= r < B), B) if nch == 1 and probe is None else B
         for k in range(nch):
-            self.ctx.copy(self.tokens, dtok.offset(4 * B * k), 4 * B)
-            self.ctx.copy(self.seq_lens, dpos.offset(4 * B * k), 4 * B)
-            self.lens_host = cpos[B * k:B * (k + 1)].copy()
+            self._place_chunk(dtok, dpos, cpos, k, T, start)
             self.step(sample, probe=probe, head=k == nch - 1, rows=rows)
+        self.span_rows = 0
         if rows < B:  # the rows left out: the last token's again, as in a step over all B
             outs = [(self.hidden, self.s.hidden)]
             if self.lm_head is not None:
                 outs += [(self.logits, self.s.vocab)] + ([(self.tokens, 1)] if sample == "argmax" else [(self.topk, 512)])
+            if self.lm_head is not None and self.ntop is not None:
+                outs += [(self.entropy, 1)] + ([(self.token_logprobs, 1)] if sample == "argmax" else [])
+                outs += [(self.top_ids, self.ntop), (self.top_logprobs, self.ntop)] if self.ntop else []
             for buf, words in outs:
                 self.ctx.repeatRow(buf, words, n - 1, rows, B - rows)
         self.ctx.sync()
         dtok.free()
         dpos.free()
         return n - 1
+
+    def _place_chunk(self, dtok, dpos, cpos, k: int, T: int, start: int) -> None:
+        """Chunk k of a prompt of T tokens from position `start`: its tokens and its rows' lengths, as the step
+        expects them, from the prompt's (8-bit pages: the sequence's length after the chunk and its rows)."""
+        c, B = self.ctx, self.B
+        c.copy(self.tokens, dtok.offset(4 * B * k), 4 * B)
+        c.copy(self.seq_lens, dpos.offset(4 * B * k), 4 * B)
+        self.lens_host = cpos[B * k:B * (k + 1)].copy()
+        if self.kv8:
+            self._place_span(start + min(T, B * (k + 1)), min(T - B * k, B))
+
+    def _place_span(self, end: int, rows: int) -> None:
+        self.span.upload(np.array([end, 0, rows], np.uint32))
+        self.span_rows = rows
+
+    def score(self, tokens, start: int = 0) -> np.ndarray:
+        """The log probability of each token but the first under the model, given those before it (a
+        shared_pages decoder with an embedding table; the prompt at positions start, start + 1, ..., its K/V
+        rows appended as by prefill): f32 [len(tokens) - 1]. The LM head runs over every row, B at a time."""
+        if not self.shared_pages or self.embedding is None or self.lm_head is None:
+            raise ValueError("score needs a shared_pages decoder with an embedding table and the LM head")
+        toks = np.asarray(tokens, np.uint32)
+        T, B, c, s = int(toks.size), self.B, self.ctx, self.s
+        if T < 2 or start + T > self.max_seq - 1:
+            raise ValueError(f"score: {T} tokens from {start}: two or more within {self.max_seq} positions")
+        n = T - 1  # the last token is only asked for
+        nch = -(-n // B)
+        pad = nch * B - n
+        ctok = np.concatenate([toks[:n], np.repeat(toks[n - 1], pad)]).astype(np.uint32)
+        cpos = np.concatenate([start + np.arange(n), np.repeat(start + n - 1, pad)]).astype(np.uint32)
+        dtok, dpos, want = c.from_numpy(ctok), c.from_numpy(cpos), c.from_numpy(toks[1:])
+        out = c.empty(n, np.float32)
+        ws = c.alloc(c.logprobs_workspace_bytes(s.vocab, B, 0))
+        for k in range(nch):
+            self._place_chunk(dtok, dpos, cpos, k, n, start)
+            self.step()
+            rows = min(n - B * k, B)
+            c.logprobsBatch(self.logits, want.offset(4 * B * k), s.vocab, rows, out.offset(4 * B * k), None, 0, None,
+                            None, ws)
+        self.span_rows = 0
+        got = out.download(np.float32)
+        for b in (dtok, dpos, want, out, ws):
+            b.free()
+        return got
 
     def _wide_prefill(self) -> bool:
         """Whether prompts may take the layers many rows at a time: one prompt
@@ -1245,8 +1376,10 @@ class BatchDecoder(_SyntheticModel):
              "v": 4 * R * s.kv_dim, "attn": 4 * R * s.q_dim, "aops": ob(s.q_dim, R), "fops": ob(s.max_ffn, R),
              "parts": 4 * self.wide_parts}
         need, ws = 0, 0
+        if self.kv8:
+            self._attn8_workspace([self._kv8_params(il, R, R) for il in range(s.n_layers)])
         for il, L in enumerate(self.layers):
-            ws = max(ws, c.prefill_attn_workspace_bytes(c.paged_fused_params(
+            ws = 16 if self.kv8 else max(ws, c.prefill_attn_workspace_bytes(c.paged_fused_params(
                 R, s.n_q_heads, s.n_kv_heads, s.hd(il), self.page_size, self.max_pages, self.max_seq, self.num_pages,
                 0, s.eps, 1.0, 0)))
             Q, KV, I = s.q_dim_of(il), s.kv_dim_of(il), s.ffn_of(il)
@@ -1288,7 +1421,10 @@ class BatchDecoder(_SyntheticModel):
         n = 0
         for at in range(0, T + pad, self.wide_rows):
             n = min(self.wide_rows, T + pad - at)
+            if self.kv8:
+                self._place_span(start + min(T, at + n), min(T - at, n))
             self._wide_pass(dtok.offset(4 * at), dlen.offset(4 * at), n, int(clen[at:at + n].max()))
+        self.span_rows = 0
         # the last B rows are what the last chunk of B rows leaves: the residual
         # stream, its tokens and lengths, then the head and the sample
         c.copy(self.hidden, w["hidden"].offset(4 * H * (n - B)), 4 * H * B)
@@ -1347,10 +1483,15 @@ class BatchDecoder(_SyntheticModel):
             p = c.paged_fused_params(n, s.n_q_heads, s.n_kv_heads, s.hd(il), self.page_size, self.max_pages, end,
                                      self.num_pages, 0 if glob else s.window, s.eps,
                                      s.theta_global if glob else s.theta_local, int(glob))
-            c.prefillAttnPrologue(w["q"], w["k"] if prod else None, w["v"] if prod else None, L.q_norm, L.k_norm,
-                                  self.rope_freqs, w["q"], L.k_cache if prod else None, L.v_cache if prod else None,
-                                  self.page_table, lens, p, self.rope_cs[glob], self.rope_rows)
-            c.prefillAttn(w["q"], L.k_cache, L.v_cache, self.page_table, lens, w["attn"], p, w["attn_ws"])
+            if self.kv8:
+                self._attend8(il, w["q"], w["k"], w["v"], 1, w["q"], w["attn"],
+                              self._kv8_params(il, n, self.span_rows, end))
+            else:
+                c.prefillAttnPrologue(w["q"], w["k"] if prod else None, w["v"] if prod else None, L.q_norm, L.k_norm,
+                                      self.rope_freqs, w["q"], L.k_cache if prod else None,
+                                      L.v_cache if prod else None, self.page_table, lens, p, self.rope_cs[glob],
+                                      self.rope_rows)
+                c.prefillAttn(w["q"], L.k_cache, L.v_cache, self.page_table, lens, w["attn"], p, w["attn_ws"])
             lo = w["aops_lo"] if L.qt["wo"] == "f16" else None
             c.prefillPrep(w["attn"], 1, None, None, None, None, None, None, Q, n, s.eps, ops=w["aops"], ops_lo=lo)
             no = c.prefillMatmul(L.qt["wo"], [L.wo], [w["parts"]], [H], Q, w["aops"], n, wops, max_ks, ops_lo=lo)
