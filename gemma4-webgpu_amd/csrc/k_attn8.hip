@@ -40,6 +40,7 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 constexpr int COLS = 16;                 // columns of a matrix product
 constexpr float kLog2e = 1.44269504f;    // the softmax works in powers of two
 constexpr float kPScale = 32768.f, kLoScale = 2048.f;
+constexpr float kLeastScale = 0x1p-100f;  // V scales are taken relative to one of at least this (theirs: 2^-64 or 0)
 
 struct Args {
   const float* q;
@@ -56,6 +57,8 @@ struct Args {
   uint32_t tiles;  // many rows: column tiles of the longest sequence
 };
 
+// A V scale, NaN where it is infinite (relative to that one the others would be lost).
+__device__ __forceinline__ float finite(float x) { return x < INFINITY ? x : __builtin_nanf(""); }
 __device__ __forceinline__ float exp2_h(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Wave-uniform values into scalar registers.
@@ -73,9 +76,6 @@ __device__ __forceinline__ uint32_t page_of(const Args& a, uint32_t t) {
 }
 __device__ __forceinline__ uint32_t clamp_page(const Args& a, int32_t pg) {
   return pg < 0 ? 0u : min((uint32_t)pg, a.num_pages - 1);
-}
-__device__ __forceinline__ uint32_t page_id(const Args& a, uint32_t s, uint32_t index) {
-  return clamp_page(a, a.page_table[(size_t)s * a.max_pages + index]);
 }
 
 // First position (of a whole tile) that any row of the sequence sees.
@@ -353,8 +353,9 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
       mx = g4d::xmax32(g4d::xmax16(mx));
       const float m_new = fmaxf(m_run, mx), m_fin = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = exp2_h(m_run - m_fin);
-      const float vmax = fmaxf(vs[0], vs[1]);
-      const float vr[2] = {vs[0] / vmax * kPScale, vs[1] / vmax * kPScale};
+      // (vmax finite where both are NaN: not every column sees them)
+      const float v0 = finite(vs[0]), v1 = finite(vs[1]), vmax = fmaxf(fmaxf(v0, v1), kLeastScale);
+      const float vr[2] = {v0 / vmax * kPScale, v1 / vmax * kPScale};
       float ps = 0.f;
       h8 ph, pl;
 #pragma unroll
@@ -698,14 +699,14 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
   const int8_t *kp = a.kp + kvh * HD, *vp_ = a.vp + kvh * HD;
   // Tiles (of the pool) and scales of the steps from `st` on; V's relative to the
   // largest so far. Returns what that one grew by (1 / growth).
-  float v_ref = 0.f;
+  float v_ref = kLeastScale;
   auto refill = [&](uint32_t st) __attribute__((always_inline)) -> float {
     float vs = 0.f;
     if (tid < 4 * CH) {
       const uint32_t t = min(t0 + 4 * st + tid, tlast), at = page_of(a, t), pg = clamp_page(a, list[at]);
       s_tile[tid] = pg * a.page_tiles + (t - at * a.page_tiles);
       s_ks[tid] = a.ks[(size_t)pg * a.nkh + kvh];
-      vs = a.vs[(size_t)pg * a.nkh + kvh];
+      vs = finite(a.vs[(size_t)pg * a.nkh + kvh]);
       const float big = g4d::wave_max_dpp(vs);  // (a NaN is not the larger one)
       if (l == 0) s_big[w] = big;
     }
@@ -867,6 +868,7 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
 #pragma unroll
     for (int p = 0; p < PT; ++p) {
       sc[p] = s_scale * ksc[p];
+      sc[p] = sc[p] < 1.2e-38f ? 1.2e-38f : sc[p];  // (0 times a masked -Inf would be NaN; a NaN stays)
       mx = fmaxf(mx, fmaxf(fmaxf(x[p][0], x[p][1]), fmaxf(x[p][2], x[p][3])) * sc[p]);
     }
     mx = g4d::xmax32(g4d::xmax16(mx));
@@ -1120,6 +1122,9 @@ int attend(g4_ctx* ctx, const g4_kv8_params& p, Args a, void* workspace) {
     G4_REQUIRE(most_units(p) * p.num_seqs * p.num_kv_heads < (1ull << 31),
                "g4_pagedAttn8: %u sequences of up to %u positions and %u KV heads in one call", p.num_seqs,
                p.max_seq_len, p.num_kv_heads);
+    G4_REQUIRE((uint64_t)p.num_seqs * p.num_kv_heads * p.max_rows * a.G < 1u << 24,
+               "g4_pagedAttn8: %u sequences of up to %u rows of %u heads in one call", p.num_seqs, p.max_rows,
+               p.num_q_heads);
     a.wgs = step_wgs<HD>(p);
     a.meta = (uint2*)workspace;
     a.part = (float*)((uint8_t*)workspace + meta_bytes(p));
@@ -1128,7 +1133,7 @@ int attend(g4_ctx* ctx, const g4_kv8_params& p, Args a, void* workspace) {
     const uint64_t units = most_units(p);
     if (units == 1) return G4_OK;  // no sequence has partials
     const dim3 grid(p.num_seqs * p.num_kv_heads * p.max_rows * a.G);
-    if (std::min<uint64_t>(units, a.wgs) <= 32)
+    if (std::min<uint64_t>(units, a.wgs) <= 32 || grid.x >= 1u << 22)
       hipLaunchKernelGGL((attn8_merge_kernel<HD, 256>), grid, dim3(256), 0, ctx->stream, a);
     else
       hipLaunchKernelGGL((attn8_merge_kernel<HD, 1024>), grid, dim3(1024), 0, ctx->stream, a);
@@ -1139,6 +1144,8 @@ int attend(g4_ctx* ctx, const g4_kv8_params& p, Args a, void* workspace) {
   G4_REQUIRE(all_cost(p) < (1ull << 31) && (uint64_t)a.tiles * p.num_seqs * p.num_kv_heads < (1ull << 31),
              "g4_pagedAttn8: %u sequences of up to %u rows and %u positions in one call", p.num_seqs, p.max_rows,
              p.max_seq_len);
+  G4_REQUIRE((uint64_t)p.num_rows * p.num_q_heads < 1u << 25, "g4_pagedAttn8: %u rows of %u heads in one call",
+             p.num_rows, p.num_q_heads);
   a.wgs = tile_wgs<HD>(p);
   a.meta = (uint2*)workspace;
   a.part = (float*)((uint8_t*)workspace + tile_meta_bytes(p));

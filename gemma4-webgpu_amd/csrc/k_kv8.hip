@@ -441,7 +441,9 @@ int g4_pagedAttnPrologue8(g4_ctx* ctx, const float* q_parts, const float* k_part
   a.seq_pages = ceil_div(p.max_rows - 1, p.page_size) + 1;
   const uint64_t kv_blocks = kv ? 2ull * p.num_seqs * a.seq_pages * p.num_kv_heads : 0ull;
   const uint64_t blocks = kv_blocks + (q ? ceil_div((uint64_t)p.num_rows * ceil_div(p.num_q_heads, QH), NW) : 0);
-  G4_REQUIRE(blocks <= 0x7fffffffull, "g4_pagedAttnPrologue8: %llu workgroups", (unsigned long long)blocks);
+  G4_REQUIRE(blocks < (1ull << 32) / NT,
+             "g4_pagedAttnPrologue8: %u sequences of up to %u rows of %u and %u heads in one call", p.num_seqs,
+             p.max_rows, p.num_q_heads, p.num_kv_heads);
   a.kv_blocks = (uint32_t)kv_blocks;
   const dim3 grid((unsigned)blocks);
   switch (p.head_dim) {
@@ -469,7 +471,7 @@ int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const 
   p.num_pages = num_pages;
   int rc = g4_internal_kv8_check(__func__, p, nullptr);
   if (rc) return rc;
-  G4_REQUIRE(count > 0 && count <= 0x7fffffffu, "g4_kv8Values: %u pages", count);
+  G4_REQUIRE(count > 0 && count < (1ull << 32) / VT, "g4_kv8Values: %u pages", count);
   const ValArgs a{{k_pool, v_pool}, {k_scale, v_scale}, {k_out, v_out}, pages, page_size, num_kv_heads, head_dim, num_pages};
   hipLaunchKernelGGL(kv8_values_kernel, dim3(count, ceil_div((uint64_t)page_size * num_kv_heads * head_dim, 16 * VT), 2),
                      dim3(VT), 0, ctx->stream, a);

@@ -368,6 +368,94 @@ def test_attention_masks_and_extremes(ctx, rows):
     c.check_attention(c.attention())
 
 
+@pytest.mark.parametrize("hd,rows,window", [(256, 2, 0), (256, 2, 20), (512, 2, 0), (128, 70, 0), (256, 40, 30),
+                                            (512, 40, 0), (64, 300, 0)])
+def test_a_page_that_is_not_finite_stays_with_the_rows_that_see_it(ctx, hd, rows, window):
+    """The rows before a page's first position do not see it, though their step of positions may hold nothing else."""
+    c = Case(ctx, [97 if rows == 2 else 80 + rows], [rows], 8, 1, hd, 16, 111, window=window).up()
+    page = 6  # from position 96 on
+    for k, v in ((np.nan, 1.0), (1.0, np.nan), (np.nan, np.nan), (1.0, np.inf)):
+        ks, vs = c.k.scale.copy(), c.v.scale.copy()
+        ks[c.table[0, page]] *= k
+        vs[c.table[0, page]] *= v
+        c.dks.upload(ks)
+        c.dvs.upload(vs)
+        got = c.attention()
+        pos = c.lens[0] - rows + np.arange(rows)
+        sees = (pos >= 16 * page) & ((window == 0) | (pos - window + 1 < 16 * page + 16))
+        assert 0 < sees.sum() < rows
+        assert not np.isfinite(got[sees]).any()
+        c.check_attention(got, np.flatnonzero(~sees), what=(k, v))
+
+
+@pytest.mark.parametrize("hd,rows", [(256, 1), (512, 1), (64, 90), (128, 90), (256, 90), (512, 90)])
+def test_scales_and_q_of_nothing(ctx, hd, rows):
+    """Pages of zeros as the append leaves them (2^-64) or never begun (0), next to pages that hold something; q so
+    small that every score is 0 in f32, and q of zeros."""
+    for what in ("least", "never begun", "all never begun", "small q", "small q, least", "q of zeros"):
+        c = Case(ctx, [150], [rows], 8, 1, hd, 16, 121, scale=0.7)
+        for pool in (c.k, c.v):
+            if "least" in what:
+                pool.scale[c.table[0, 2:10]] = 2.0 ** -64
+                pool.codes[c.table[0, 2:10]] = 0
+            if "never" in what:
+                pool.scale[c.table[0, 2 if what[0] == "n" else 0:]] = 0
+        c.q *= np.float32(1e-33 if "small" in what else 0.0 if "zeros" in what else 1.0)
+        c.up()
+        c.check_attention(c.attention(), sorted({0, 5, 63, 64, rows - 1} & set(range(rows))), what=what)
+
+
+@pytest.mark.parametrize("scale", [-0.9, 0.0, 1e-30])
+@pytest.mark.parametrize("hd,rows,window", [(256, 1, 0), (512, 1, 40), (64, 50, 0), (256, 50, 60), (512, 50, 0)])
+def test_scale_of_any_sign(ctx, hd, rows, window, scale):
+    c = Case(ctx, [170, 60], [rows, rows], 8, 1, hd, 32, 131, window=window, scale=scale).up()
+    c.check_attention(c.attention(), sorted({0, 7, 8, rows - 1, rows, 2 * rows - 1} & set(range(2 * rows))))
+
+
+@pytest.mark.parametrize("hd,most,sequences", [(128, 9, 700), (256, 40, 300), (512, 17, 200)])
+def test_many_rows_of_many_sequences(ctx, hd, most, sequences):
+    """More column tiles than a workgroup has threads; sequences without rows, without positions, of one row."""
+    rng = np.random.default_rng(141)
+    lens, rows = rng.integers(0, 90, sequences), rng.integers(0, most + 1, sequences)
+    rows = np.minimum(rows, rng.choice([0, 1, most], sequences))
+    rows[3] = most
+    lens = np.where(rng.random(sequences) < 0.1, 0, np.maximum(lens, rows))
+    lens[100:140] = 0  # a run of nothing
+    lens[-2:] = 0
+    c = Case(ctx, lens, rows, 8, 1, hd, 16, 142, extra_rows=1).up()
+    got = c.attention()
+    total = int(c.n.sum())
+    short = [r for r in range(total) if c.lens[c.row(r)[0]] < c.n[c.row(r)[0]]]
+    assert short and np.all(got[short] == 0)
+    c.check_attention(got, sorted((set(range(0, total, 11)) | {total - 1}) - set(short)))
+
+
+def test_two_graphs_share_a_workspace(ctx):
+    """Prompts and steps captured apart into graphs over one workspace, replayed in turn with eager calls between."""
+    a = Case(ctx, [300], [120], 8, 1, 256, 16, 151).up()
+    b = Case(ctx, [700, 40], [1, 1], 8, 1, 512, 16, 152).up()
+    bytes_ = max(ctx.attn8_workspace_bytes(c.p) for c in (a, b))
+    ws = ctx.from_numpy(np.full(bytes_, 0xff, np.uint8))
+    want = [c.attention() for c in (a, b)]
+    runs = []
+    for c in (a, b):
+        q, out = ctx.from_numpy(c.q), ctx.from_numpy(np.full(c.q.shape, 7.5, np.float32))
+        ctx.graph_begin()
+        ctx.pagedAttn8(q, *c.cache, c.dt, c.dl, out, c.p, ws, row_starts=c.ds)
+        runs.append((ctx.graph_end(), q, out, c))
+    for _ in range(4):
+        for i in (0, 1, 1, 0):
+            g, _, out, c = runs[i]
+            out.upload(np.full(c.q.shape, 7.5, np.float32))
+            ctx.graph_launch(g)
+            got = out.download(np.float32).reshape(c.q.shape)
+            assert np.array_equal(got.view(np.uint32), want[i].view(np.uint32))
+            eager = runs[1 - i][3]
+            assert np.array_equal(eager.attention(ws).view(np.uint32), want[1 - i].view(np.uint32))
+    for g, *_ in runs:
+        ctx.graph_destroy(g)
+
+
 def test_attention_of_far_pages(ctx):
     """Pools of more than 4 GiB: page offsets past 32 bits."""
     hd, ps, pages = 512, 16, (1 << 32) // (16 * 512) + 40
