@@ -927,12 +927,15 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
       pl[0] = pp[64];
       ph[1] = pp[128];
       pl[1] = pp[192];
-      if (__ballot(f_own != f_other)) {  // (one of them is 1)
-        const _Float16 f0 = (_Float16)(wd ? f_other : f_own), f1 = (_Float16)(wd ? f_own : f_other);
-        ph[0] *= f0;
-        pl[0] *= f0;
-        ph[1] *= f1;
-        pl[1] *= f1;
+      if (__ballot(f_own != f_other)) {  // (one of them is 1; f16 ends at 2^-24, so the powers of two in two halves)
+        const float d0 = (wd ? m_other : m_own) - m_new, d1 = (wd ? m_own : m_other) - m_new;
+        const float a0 = ceilf(d0 * 0.5f), a1 = ceilf(d1 * 0.5f);
+        const _Float16 f0 = (_Float16)exp2_h(a0), g0 = (_Float16)exp2_h(d0 - a0);
+        const _Float16 f1 = (_Float16)exp2_h(a1), g1 = (_Float16)exp2_h(d1 - a1);
+        ph[0] = ph[0] * f0 * g0;
+        pl[0] = pl[0] * f0 * g0;
+        ph[1] = ph[1] * f1 * g1;
+        pl[1] = pl[1] * f1 * g1;
       }
     }
     const float alpha = exp2_h(m_run - m_new);

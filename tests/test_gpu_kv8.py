@@ -456,6 +456,24 @@ def test_two_graphs_share_a_workspace(ctx):
         ctx.graph_destroy(g)
 
 
+@pytest.mark.parametrize("far", [2.0 ** -12, 2.0 ** -26, 2.0 ** -36])
+@pytest.mark.parametrize("hd,rows", [(256, 1), (512, 1), (64, 20), (256, 20), (512, 20)])
+def test_a_weight_far_below_the_largest_keeps_its_share(ctx, hd, rows, far):
+    """One key holds all the weight, its values are 0; another's weight is `far` of it, in the same half of 64
+    positions or in the other."""
+    for a, b in ((3, 10), (3, 40), (40, 3), (70, 3)):
+        c = Case(ctx, [100], [rows], 8, 1, hd, 16, 161)
+        for pos in range(100):
+            pg, slot = c.table[0, pos // 16], pos % 16
+            c.k.codes[pg, slot], c.k.scale[pg] = 0, 1.0
+            c.k.codes[pg, slot, 0, 0] = {a: 100, b: 80}.get(pos, -100)
+            c.v.codes[pg, slot] *= np.int8(pos != a)
+        c.q[:] = 0
+        c.q[..., 0] = -np.log(far) / 20
+        c.up()
+        c.check_attention(c.attention(), what=(a, b))
+
+
 def test_attention_of_far_pages(ctx):
     """Pools of more than 4 GiB: page offsets past 32 bits."""
     hd, ps, pages = 512, 16, (1 << 32) // (16 * 512) + 40

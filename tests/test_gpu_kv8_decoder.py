@@ -144,6 +144,19 @@ def test_prefill_in_chunks(ctx, kind, T, start):
     assert all(bits_equal(H[r], H[last]) for r in range(last + 1, B))
 
 
+@pytest.mark.parametrize("T,start", [(5, 0), (16, 3), (20, 40)])
+def test_a_short_prompt_leaves_rows_out(ctx, T, start):
+    d = BatchDecoder(ctx, [0] * 64, shape(), seed=65, reserve=128, shared_pages=True, embed=True, kv="int8", logprobs=4)
+    d.fill_kv(seed=66)
+    toks = np.random.default_rng(67).integers(0, d.s.vocab, T).astype(np.uint32)
+    assert d.prefill(toks, start) == T - 1
+    il, s = d.s.n_layers - 1, d.s
+    n = T * s.q_dim_of(il)
+    check_rows(d, il, d.q.download(np.float32, n), d.attn.download(np.float32, n),
+               [(r, 0, start + r) for r in range(T)])
+    check_logprobs(d, range(64))
+
+
 @pytest.mark.parametrize("kind,B,T,start", [("real", 16, 100, 0), ("real", 64, 700, 0), ("uniform", 64, 201, 100),
                                             ("uniform", 16, 97, 530), ("real", 1, 33, 3)])
 def test_prefill_many_rows_a_pass(ctx, kind, B, T, start):
