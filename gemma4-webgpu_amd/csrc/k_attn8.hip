@@ -263,6 +263,13 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
       }
     };
 
+    // q, 16 threads a column (asked for before the rows, whose arrival its digits then do not wait for)
+    constexpr int E = HD / 16;
+    const uint32_t col = tid >> 4, part_of = tid & 15, cc = min(col, ncols - 1);
+    const float* qg = a.q + ((size_t)(sq.first + cc / a.G) * a.nqh + kvh * a.G + cc % a.G) * HD + part_of * E;
+    f4 x[E / 4];
+#pragma unroll
+    for (int e = 0; e < E / 4; ++e) x[e] = *(const f4*)(qg + 4 * e);
     uint32_t st = 4 * off + w;
     const uint32_t steps = min(st1, (tiles + 1) / 2);  // (the last unit may be short)
     if (st < steps) {
@@ -272,34 +279,26 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
       load_v(st);
       pages(min(st + 4, steps - 1), pg);
     }
-    // ---- q's digits: 16 threads a column ----
+    // ---- q's digits ----
     __syncthreads();  // the previous sequence's are done with
     {
-      constexpr int E = HD / 16;
-      const uint32_t col = tid >> 4, part = tid & 15, cc = min(col, ncols - 1);
-      const float* qg = a.q + ((size_t)(sq.first + cc / a.G) * a.nqh + kvh * a.G + cc % a.G) * HD + part * E;
-      float x[E], am = 0.f;
+      float am = 0.f;
       bool nan = false;
 #pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        const f4 y = *(const f4*)(qg + e);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[e + i] = y[i];
-          am = fmaxf(am, fabsf(y[i]));
-          nan |= y[i] != y[i];
-        }
+      for (int e = 0; e < E; ++e) {
+        am = fmaxf(am, fabsf(x[e / 4][e % 4]));
+        nan |= x[e / 4][e % 4] != x[e / 4][e % 4];
       }
       am = g4d::max16(nan ? INFINITY : am);
       float un;
       const float up = digit_scale(am, un);
-      if (part == 0) s_un[col] = un;
+      if (part_of == 0) s_un[col] = un;
 #pragma unroll
       for (int e = 0; e < E; e += 4) {
         uint32_t d[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = digits(x[e + i], up);
-        const uint32_t dim = part * E + e;
+        for (int i = 0; i < 4; ++i) d[i] = digits(x[e / 4][i], up);
+        const uint32_t dim = part_of * E + e;
         uint32_t* dst = s_q + (((dim / 64) * 64 + dim % 64 / 16 * 16 + col) * 4 + dim % 16 / 4);
         dst[0] = plane<0>(d[0], d[1], d[2], d[3]);
         dst[KJ * 256] = plane<1>(d[0], d[1], d[2], d[3]);
@@ -317,7 +316,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     for (int e = 0; e < VB; ++e) O[e] = f4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;  // of column c
     for (; st < steps; st += 4) {
-      const uint32_t next = min(st + 4, steps - 1);  // (past the end: its own last rows again, not used)
+      const uint32_t next = min(st + 4, steps - 1);  // (past the end: its own last rows again; a branch here spills)
       asm volatile("" ::: "memory");  // q's digits stay in LDS (in registers they would spill)
       // ---- scores ----
       i4 D[2][3];

@@ -11,13 +11,18 @@
 //
 // kv8_prologue_kernel: every page of a KV head that a call touches belongs to
 // one workgroup (K and V apart), which forms its rows' largest element before
-// it stores any code; other workgroups take the query rows, a wave four heads of
-// one. Whatever depends on the row's place only (parts, norm weights, rotation)
-// is loaded before the first sum. Norms, rotation and rounding of K and V are in f64: a value near the
+// it stores any code; other workgroups take the query rows, a wave some heads of
+// one. Norms, rotation and rounding of K and V are in f64: a value near the
 // border of two codes then gets the same code as in exact arithmetic, whatever
-// the order of the sums (the f64 units are idle otherwise). q is f32. Up to 32
-// rows of a page (16 at head dim 512) stay in registers between the two steps; more are formed
-// again for the second.
+// the order of the sums (the f64 units are idle otherwise). q is f32. The rows a
+// wave keeps stay in registers between the two steps; where a page has more they
+// are formed again for the second.
+//
+// A step's append is bound by latency, and much of that by instructions, which a
+// launch finds in no cache: 27 KB of code (loops unrolled, the rotation without a
+// table in line, library square root, division and frexp, maxima in f64 through
+// LDS) took 8.3 us for 64 sequences, the same steps in 8 KB 4.0. A prompt of 1900
+// rows at head dim 512 (its 35 MB at the copy rate: 8 us) takes 18.
 #include "kv8.hpp"
 #include "mqf_core.hpp"
 
@@ -25,9 +30,7 @@ namespace {
 
 using namespace g4kv8;
 
-constexpr int NT = 512, NW = NT / 64;
 constexpr int VT = 256;  // threads of the values kernel
-constexpr int QH = 4;    // query heads of a row that a wave takes
 
 struct ProArgs {
   const float *q, *k, *v;
@@ -52,13 +55,27 @@ struct Row {
   static constexpr int HALF = HD / 2, PP = HALF >= 64 ? HALF / 64 : 1, ACT = HALF / PP;
 };
 
-__device__ __forceinline__ double wave_max64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
-  return v;
+// Sum over the wave, in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_from(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v = add_from<0x111, 0xf>(v);
+  v = add_from<0x112, 0xf>(v);
+  v = add_from<0x114, 0xf>(v);
+  v = add_from<0x118, 0xf>(v);
+  v = add_from<0x142, 0xa>(v);
+  v = add_from<0x143, 0xc>(v);
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)b, 63), hi = __builtin_amdgcn_readlane((int)(b >> 32), 63);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// Parts added in order, in T.
+// Parts added in order, in T; four of them on their way.
 template <int HD, typename T>
 __device__ __forceinline__ void load_row(const float* p, size_t stride, uint32_t nparts, int lane, T* lo, T* hi) {
   constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
@@ -67,19 +84,27 @@ __device__ __forceinline__ void load_row(const float* p, size_t stride, uint32_t
   for (int i = 0; i < PP; ++i) lo[i] = hi[i] = 0;
   if (lane >= Row<HD>::ACT) return;
   const float* b = p + PP * lane;
-#pragma unroll 4
-  for (uint32_t c = 0; c < nparts; ++c, b += stride) {
-    if constexpr (PP == 1) {
-      lo[0] += (T)b[0];
-      hi[0] += (T)b[HALF];
-    } else {
-      const vec x = *(const vec*)b, y = *(const vec*)(b + HALF);
+#pragma nounroll
+  for (uint32_t c = 0; c < nparts; c += 4) {
+    vec x[4], y[4];
 #pragma unroll
-      for (int i = 0; i < PP; ++i) {
-        lo[i] += (T)x[i];
-        hi[i] += (T)y[i];
+    for (int k = 0; k < 4; ++k) {  // (past the last one: that one again, not added)
+      const float* r = b + (size_t)min(c + k, nparts - 1) * stride;
+      if constexpr (PP == 1) {
+        x[k][0] = r[0];
+        y[k][0] = r[HALF];
+      } else {
+        x[k] = *(const vec*)r;
+        y[k] = *(const vec*)(r + HALF);
       }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < PP; ++i) {
+        lo[i] += c + k < nparts ? (T)x[k][i] : (T)-0.0;
+        hi[i] += c + k < nparts ? (T)y[k][i] : (T)-0.0;
+      }
   }
 }
 
@@ -89,14 +114,14 @@ struct Turn {
   static constexpr int PP = Row<HD>::PP;
   float2 cs[PP];
 };
-template <int HD>
+template <int HD, bool TABLE>
 __device__ __forceinline__ void load_turn(const ProArgs& a, uint32_t pos, int lane, Turn<HD>& t) {
   constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
 #pragma unroll
   for (int i = 0; i < PP; ++i) {
     const int k = min(PP * lane + i, HALF - 1);
-    t.cs[i] = a.rope_cs ? a.rope_cs[(size_t)pos * HALF + k]
-                        : g4mqf::rope_cos_sin(a.theta, a.apply_divisor, a.rope_freqs[k], k, HD, pos);
+    t.cs[i] = TABLE ? a.rope_cs[(size_t)pos * HALF + k]
+                    : g4mqf::rope_cos_sin(a.theta, a.apply_divisor, a.rope_freqs[k], k, HD, pos);
   }
 }
 template <int HD>
@@ -124,9 +149,10 @@ __device__ __forceinline__ void rotate(const Weights<HD>& w, const Turn<HD>& t, 
   }
 }
 
-template <int HD>
+// The heads of a row QH at a time, a wave each.
+template <int HD, int NT, int QH, bool TABLE>
 __device__ __forceinline__ void q_row(const ProArgs& a, uint32_t block) {
-  constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
+  constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF, NW = NT / 64;
   const int lane = threadIdx.x & 63;
   const uint32_t groups = (a.nqh + QH - 1) / QH;
   const uint64_t i = (uint64_t)block * NW + (threadIdx.x >> 6);
@@ -143,7 +169,7 @@ __device__ __forceinline__ void q_row(const ProArgs& a, uint32_t block) {
   const Seq q = seq_rows(a.rows, s);
   if (!q.len) return;
   Turn<HD> t;
-  load_turn<HD>(a, q.base + (row - q.first), lane, t);
+  load_turn<HD, TABLE>(a, q.base + (row - q.first), lane, t);
 #pragma unroll
   for (int h = 0; h < QH; ++h) {
     if (h0 + h >= a.nqh) return;
@@ -178,21 +204,30 @@ __device__ __forceinline__ void q_row(const ProArgs& a, uint32_t block) {
   }
 }
 
-// The scale of a page whose largest element is `am`: the least 2^e with
-// am <= 127 * 2^e, from its binary exponent; at least 2^-64 (all zeros).
-__device__ __forceinline__ float scale_of(double am) {
-  int x = 0;
-  const double m = frexp(am, &x);
-  return ldexpf(1.0f, am > 0.0 ? max(x - 7 + (m > 127.0 / 128.0), -64) : -64);
+// The least e >= -64 with x <= 127 * 2^e, of a double's magnitude bits: the binary
+// exponent less 7, one more where the fraction passes that of 127 / 128. kBad
+// where it is not finite.
+constexpr int kBad = 1000;
+__device__ __forceinline__ int exponent_of(uint64_t bits) {
+  constexpr uint64_t carry = (1ull << 52) - 1 - 0xfc00000000000ull;
+  return bits >= 0x7ffull << 52 ? kBad : max((int)((bits + carry) >> 52) - 1022 - 7, -64);
+}
+__device__ __forceinline__ uint64_t magnitude(double x) { return __builtin_bit_cast(uint64_t, x) & ~(1ull << 63); }
+// 1 / sqrt(x), from the hardware's estimate by two steps of Newton's iteration.
+__device__ __forceinline__ double rsqrt64(double x) {
+  double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
+  return y;
 }
 
-template <int HD, int KEEP>
+// KEEP rows a wave; 1 where no sequence of the call has more than there are waves.
+template <int HD, int NT, int KEEP, int QH, bool TABLE>
 __global__ __launch_bounds__(NT, 4) void kv8_prologue_kernel(ProArgs a) {
-  constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF;
-  __shared__ double s_am[NW];
-  __shared__ int s_bad;
+  constexpr int PP = Row<HD>::PP, HALF = Row<HD>::HALF, NW = NT / 64;
+  __shared__ float s_e[NW];
   if (blockIdx.x >= a.kv_blocks) {  // (the pages, which take longer, start first)
-    q_row<HD>(a, blockIdx.x - a.kv_blocks);
+    q_row<HD, NT, QH, TABLE>(a, blockIdx.x - a.kv_blocks);
     return;
   }
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -206,7 +241,6 @@ __global__ __launch_bounds__(NT, 4) void kv8_prologue_kernel(ProArgs a) {
   const uint32_t pi = q.base / a.page_size + j;
   if (!q.len || pi > (q.len - 1) / a.page_size) return;  // (uniform)
   const int32_t pg = a.page_table[(size_t)s * a.max_pages + pi];
-  if (pg < 0 || pg >= (int32_t)a.num_pages) return;
   const uint32_t start = pi * a.page_size;
   const uint32_t p0 = max(q.base, start), p1 = min(q.len, start + a.page_size), m = p1 - p0;
   const float* src = (is_v ? a.v : a.k);
@@ -214,36 +248,36 @@ __global__ __launch_bounds__(NT, 4) void kv8_prologue_kernel(ProArgs a) {
 
   double lo[KEEP][PP], hi[KEEP][PP];
   Weights<HD> wt;
+  Turn<HD> turn[KEEP];
   if (!is_v) load_weights<HD>(a.k_w, lane, wt);
-  auto form = [&](uint32_t at) {  // the wave's rows p0 + at + w, + NW, ... (past the last: 0)
-    Turn<HD> turn[KEEP];
+  auto load = [&](uint32_t at) {  // the wave's rows p0 + at + w, + NW, ... (past the last: 0)
 #pragma unroll
     for (int r = 0; r < KEEP; ++r) {
       const uint32_t i = at + w + NW * r;
       if (i < m) {  // (uniform over the wave)
         load_row<HD>(src + ((size_t)(q.first + (p0 - q.base) + i) * a.nkh + kvh) * HD, stride, a.nparts, lane, lo[r],
                      hi[r]);
-        if (!is_v) load_turn<HD>(a, p0 + i, lane, turn[r]);
+        if (!is_v) load_turn<HD, TABLE>(a, p0 + i, lane, turn[r]);
       } else {
 #pragma unroll
         for (int e = 0; e < PP; ++e) lo[r][e] = hi[r][e] = 0.0;
       }
     }
+  };
+  auto form = [&](uint32_t at) {
     double ss[KEEP];
 #pragma unroll
     for (int r = 0; r < KEEP; ++r) {
       ss[r] = 0.0;
 #pragma unroll
-      for (int e = 0; e < PP; ++e) ss[r] += lo[r][e] * lo[r][e] + hi[r][e] * hi[r][e];
+      for (int e = 0; e < PP; ++e) ss[r] = fma(lo[r][e], lo[r][e], fma(hi[r][e], hi[r][e], ss[r]));
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-#pragma unroll
-      for (int r = 0; r < KEEP; ++r) ss[r] += __shfl_xor(ss[r], o, 64);
+    for (int r = 0; r < KEEP; ++r) ss[r] = wave_sum64(ss[r]);
 #pragma unroll
     for (int r = 0; r < KEEP; ++r) {
       if (at + w + NW * r >= m) continue;
-      const double inv = 1.0 / sqrt(ss[r] * (1.0 / HD) + (double)a.eps);
+      const double inv = rsqrt64(ss[r] * (1.0 / HD) + (double)a.eps);
 #pragma unroll
       for (int e = 0; e < PP; ++e) {
         lo[r][e] *= inv;
@@ -252,32 +286,29 @@ __global__ __launch_bounds__(NT, 4) void kv8_prologue_kernel(ProArgs a) {
       if (!is_v) rotate<HD>(wt, turn[r], lo[r], hi[r]);
     }
   };
-  double am = 0.0;
-  bool bad = false;
+  load(0);
+  if (pg < 0 || pg >= (int32_t)a.num_pages) return;
+  float* sp = (is_v ? a.vs : a.ks) + (size_t)pg * a.nkh + kvh;
+  const uint32_t before = p0 - start;  // codes of earlier calls
+  const float old = before ? *sp : 0.f;
+  uint64_t am = 0;  // the lane's largest magnitude (an infinity and a NaN are larger than any number)
   for (uint32_t at = 0; at < m; at += KEEP * NW) {
+    if (KEEP > 1 && at) load(at);
     form(at);
 #pragma unroll
     for (int r = 0; r < KEEP; ++r)
 #pragma unroll
-      for (int e = 0; e < PP; ++e) {
-        const double x = fmax(fabs(lo[r][e]), fabs(hi[r][e]));
-        am = fmax(am, x);  // (a NaN is not the larger one)
-        bad |= !(fabs(lo[r][e]) < INFINITY && fabs(hi[r][e]) < INFINITY);
-      }
+      for (int e = 0; e < PP; ++e) am = max(am, max(magnitude(lo[r][e]), magnitude(hi[r][e])));
+    if (KEEP == 1) break;
   }
-  am = wave_max64(am);
-  if (threadIdx.x == 0) s_bad = 0;
-  __syncthreads();
-  if (lane == 0) s_am[w] = am;
-  if (bad) s_bad = 1;
-  float* sp = (is_v ? a.vs : a.ks) + (size_t)pg * a.nkh + kvh;
-  const uint32_t before = p0 - start;  // codes of earlier calls
-  const float old = before ? *sp : 0.f;
-  __syncthreads();
+  const float ew = g4d::wave_max_dpp((float)exponent_of(am));
+  if (lane == 0) s_e[w] = ew;
+  __syncthreads();  // (and every thread has read the scale)
+  float ex = s_e[0];
 #pragma unroll
-  for (int i = 0; i < NW; ++i) am = fmax(am, s_am[i]);
-  const bool poison = s_bad || old != old;
-  const float sc = poison ? __builtin_nanf("") : fmaxf(old, scale_of(am));
+  for (int i = 1; i < NW; ++i) ex = fmaxf(ex, s_e[i]);
+  const bool poison = ex == (float)kBad || old != old;
+  const float sc = poison ? __builtin_nanf("") : fmaxf(old, __uint_as_float((uint32_t)(min((int)ex, 127) + 127) << 23));
   if (threadIdx.x == 0) *sp = sc;
   int8_t* page = (is_v ? a.vp : a.kp) + ((size_t)pg * a.page_size * a.nkh + kvh) * HD;
   const size_t rs = (size_t)a.nkh * HD;  // from one position's row to the next
@@ -296,9 +327,12 @@ __global__ __launch_bounds__(NT, 4) void kv8_prologue_kernel(ProArgs a) {
       *d = y;
     }
   }
-  const double up = poison ? 0.0 : 1.0 / (double)sc;
+  const double up = (double)__uint_as_float(0x7f000000u - __float_as_uint(sc));  // 1 / sc
   for (uint32_t at = 0; at < m; at += KEEP * NW) {
-    if (m > KEEP * NW) form(at);
+    if (KEEP > 1 && m > KEEP * NW) {
+      load(at);
+      form(at);
+    }
 #pragma unroll
     for (int r = 0; r < KEEP; ++r) {
       const uint32_t i = at + w + NW * r;
@@ -321,6 +355,7 @@ __global__ __launch_bounds__(NT, 4) void kv8_prologue_kernel(ProArgs a) {
         *(uint32_t*)(d + HALF) = y;
       }
     }
+    if (KEEP == 1) break;
   }
 }
 
@@ -357,13 +392,31 @@ __global__ __launch_bounds__(VT) void kv8_values_kernel(ValArgs a) {
   o[1] = in ? y[1] : u32x4{0, 0, 0, 0};
 }
 
-// Rows a wave keeps: one where no sequence has more than the workgroup's eight
-// waves (a step of 64 rows at head dim 256 9.8 us with four, 8.3 with one), else
-// four, two at head dim 512 (four spill).
+// The launch: few rows (at most four a sequence), a row and two of q's heads a
+// wave (64 sequences 3.6 us, with four heads 4.1); more rows, KEEP of them and four
+// heads (1900 rows 20.7 us, with two heads 21.6), in workgroups of four waves where
+// a page is 16 rows (18.7 us, eight waves 20.5) and eight where it is more (301
+// rows in pages of 32 7.4 us, four waves 13.2).
+struct Shape {
+  int threads, heads;
+  bool few;
+};
+Shape shape_of(const g4_kv8_params& p) {
+  if (p.max_rows <= 4) return {256, 2, true};
+  return {p.page_size <= 16 ? 256 : 512, 4, false};
+}
+template <int HD, bool TABLE>
+void prologue_of(g4_ctx* ctx, const Shape& s, dim3 grid, const ProArgs& a) {
+  constexpr int KEEP = HD == 512 ? 2 : 4;  // (four spill)
+  if (s.few) hipLaunchKernelGGL((kv8_prologue_kernel<HD, 256, 1, 2, TABLE>), grid, dim3(256), 0, ctx->stream, a);
+  else if (s.threads == 256)
+    hipLaunchKernelGGL((kv8_prologue_kernel<HD, 256, KEEP, 4, TABLE>), grid, dim3(256), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((kv8_prologue_kernel<HD, 512, KEEP, 4, TABLE>), grid, dim3(512), 0, ctx->stream, a);
+}
 template <int HD>
-void prologue(g4_ctx* ctx, const g4_kv8_params& p, dim3 grid, const ProArgs& a) {
-  if (p.max_rows <= NW) hipLaunchKernelGGL((kv8_prologue_kernel<HD, 1>), grid, dim3(NT), 0, ctx->stream, a);
-  else hipLaunchKernelGGL((kv8_prologue_kernel<HD, HD == 512 ? 2 : 4>), grid, dim3(NT), 0, ctx->stream, a);
+void prologue(g4_ctx* ctx, const Shape& s, dim3 grid, const ProArgs& a) {
+  if (a.rope_cs) prologue_of<HD, true>(ctx, s, grid, a);
+  else prologue_of<HD, false>(ctx, s, grid, a);
 }
 
 }  // namespace
@@ -439,18 +492,19 @@ int g4_pagedAttnPrologue8(g4_ctx* ctx, const float* q_parts, const float* k_part
   a.theta = p.theta;
   a.apply_divisor = p.apply_divisor;
   a.seq_pages = ceil_div(p.max_rows - 1, p.page_size) + 1;
+  const Shape s = shape_of(p);
   const uint64_t kv_blocks = kv ? 2ull * p.num_seqs * a.seq_pages * p.num_kv_heads : 0ull;
-  const uint64_t blocks = kv_blocks + (q ? ceil_div((uint64_t)p.num_rows * ceil_div(p.num_q_heads, QH), NW) : 0);
-  G4_REQUIRE(blocks < (1ull << 32) / NT,
+  const uint64_t blocks = kv_blocks + (q ? ceil_div((uint64_t)p.num_rows * ceil_div(p.num_q_heads, s.heads), s.threads / 64) : 0);
+  G4_REQUIRE(blocks < (1ull << 32) / s.threads,
              "g4_pagedAttnPrologue8: %u sequences of up to %u rows of %u and %u heads in one call", p.num_seqs,
              p.max_rows, p.num_q_heads, p.num_kv_heads);
   a.kv_blocks = (uint32_t)kv_blocks;
   const dim3 grid((unsigned)blocks);
   switch (p.head_dim) {
-    case 64: prologue<64>(ctx, p, grid, a); break;
-    case 128: prologue<128>(ctx, p, grid, a); break;
-    case 256: prologue<256>(ctx, p, grid, a); break;
-    default: prologue<512>(ctx, p, grid, a); break;
+    case 64: prologue<64>(ctx, s, grid, a); break;
+    case 128: prologue<128>(ctx, s, grid, a); break;
+    case 256: prologue<256>(ctx, s, grid, a); break;
+    default: prologue<512>(ctx, s, grid, a); break;
   }
   G4_LAUNCHED(ctx, "kv8_prologue");
   return G4_OK;
