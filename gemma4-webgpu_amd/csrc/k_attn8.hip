@@ -214,16 +214,21 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     // go before them in use: a scalar load's wait is that of the LDS reads too)
     int32_t pg[2], pg_far[2];
     const uint32_t st1 = 4 * (off + take), tiles = (end - lo + 15) / 16, t0 = lo / 16;
+    const uint32_t steps = min(st1, (tiles + 1) / 2);  // (the last unit may be short)
     const uint32_t k_at = c * (uint32_t)rs + 16 * qd, v_at = 4 * qd * (uint32_t)rs + VB * c;
     const int32_t* list = a.page_table + (size_t)s * a.max_pages;
     auto pages = [&](uint32_t st, int32_t* to) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) to[p] = list[page_of(a, t0 + min(2 * st + p, tiles - 1))];
     };
-    auto tile_at = [&](const int8_t* pool, uint32_t st, int p) -> const int8_t* {  // the tile's first row
+    // a tile's rows as a buffer; of no bytes past the last step, so that nothing is read there (a branch around the
+    // loads of the next step would spill)
+    auto tile_at = [&](const int8_t* pool, uint32_t st, int p) -> __amdgpu_buffer_rsrc_t {
       const uint32_t t = t0 + min(2 * st + p, tiles - 1), slot = (t - page_of(a, t) * a.page_tiles) * 16;
-      return (const int8_t*)uni(
-          (uint64_t)(pool + ((size_t)clamp_page(a, uni_i(pg[p])) * (a.page_tiles * 16) + slot) * rs + kvh * HD));
+      const uint64_t at = uni((uint64_t)(pool + ((size_t)clamp_page(a, uni_i(pg[p])) * (a.page_tiles * 16) + slot) * rs +
+                                         kvh * HD));
+      return __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, st < steps ? (int)(15 * (uint32_t)rs + HD) : 0,
+                                               0x00020000);
     };
     auto load_scales = [&](float* k, float* v) {
 #pragma unroll
@@ -236,28 +241,30 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     auto load_k = [&](uint32_t st) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const int8_t* base = tile_at(a.kp, st, p);
+        const __amdgpu_buffer_rsrc_t r = tile_at(a.kp, st, p);
 #pragma unroll
-        for (int j = 0; j < KJ; ++j) K[p][j] = *(const i4*)(base + k_at + 64 * j);
+        for (int j = 0; j < KJ; ++j)
+          K[p][j] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(r, k_at + 64 * j, 0, 0));
       }
     };
     auto load_v = [&](uint32_t st) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const int8_t* base = tile_at(a.vp, st, p);
+        const __amdgpu_buffer_rsrc_t r = tile_at(a.vp, st, p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t* r = (const uint32_t*)(base + i * rs + v_at);
           if constexpr (VB >= 16) {
 #pragma unroll
             for (int k = 0; k < VB / 16; ++k) {
-              const i4 x = *(const i4*)(r + 4 * k);
+              const i4 x = __builtin_bit_cast(
+                  i4, __builtin_amdgcn_raw_buffer_load_b128(r, v_at + 16 * k, i * (uint32_t)rs, 0));
 #pragma unroll
               for (int e = 0; e < 4; ++e) V[4 * p + i][4 * k + e] = (uint32_t)x[e];
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < VB / 4; ++e) V[4 * p + i][e] = r[e];
+            for (int e = 0; e < VB / 4; ++e)
+              V[4 * p + i][e] = __builtin_amdgcn_raw_buffer_load_b32(r, v_at + 4 * e, i * (uint32_t)rs, 0);
           }
         }
       }
@@ -271,7 +278,6 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
 #pragma unroll
     for (int e = 0; e < E / 4; ++e) x[e] = *(const f4*)(qg + 4 * e);
     uint32_t st = 4 * off + w;
-    const uint32_t steps = min(st1, (tiles + 1) / 2);  // (the last unit may be short)
     if (st < steps) {
       pages(st, pg);
       load_scales(ks, vs);
@@ -316,7 +322,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     for (int e = 0; e < VB; ++e) O[e] = f4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;  // of column c
     for (; st < steps; st += 4) {
-      const uint32_t next = min(st + 4, steps - 1);  // (past the end: its own last rows again; a branch here spills)
+      const uint32_t next = st + 4;
       asm volatile("" ::: "memory");  // q's digits stay in LDS (in registers they would spill)
       // ---- scores ----
       i4 D[2][3];
