@@ -255,6 +255,26 @@ __device__ __forceinline__ float wave_max_dpp(float v) {
   return fmaxf(fmaxf(lane_value(v, 0), lane_value(v, 16)), fmaxf(lane_value(v, 32), lane_value(v, 48)));
 }
 
+// The same of doubles, each 16 lanes' last sum added to the rows behind.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_from(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_dpp(double v) {
+  v = add_from<0x111, 0xf>(v);
+  v = add_from<0x112, 0xf>(v);
+  v = add_from<0x114, 0xf>(v);
+  v = add_from<0x118, 0xf>(v);
+  v = add_from<0x142, 0xa>(v);
+  v = add_from<0x143, 0xc>(v);
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)b, 63), hi = __builtin_amdgcn_readlane((int)(b >> 32), 63);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
 // Block-wide sum for blockDim.x == 64 * nwaves; `red` holds >= nwaves floats.
 // Every thread gets the total. Contains __syncthreads.
 template <int NWAVES>

@@ -55,26 +55,6 @@ struct Row {
   static constexpr int HALF = HD / 2, PP = HALF >= 64 ? HALF / 64 : 1, ACT = HALF / PP;
 };
 
-// Sum over the wave, in every lane.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double add_from(double v) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
-  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
-  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-__device__ __forceinline__ double wave_sum64(double v) {
-  v = add_from<0x111, 0xf>(v);
-  v = add_from<0x112, 0xf>(v);
-  v = add_from<0x114, 0xf>(v);
-  v = add_from<0x118, 0xf>(v);
-  v = add_from<0x142, 0xa>(v);
-  v = add_from<0x143, 0xc>(v);
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __builtin_amdgcn_readlane((int)b, 63), hi = __builtin_amdgcn_readlane((int)(b >> 32), 63);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-
 // Parts added in order, in T; four of them on their way.
 template <int HD, typename T>
 __device__ __forceinline__ void load_row(const float* p, size_t stride, uint32_t nparts, int lane, T* lo, T* hi) {
@@ -273,7 +253,7 @@ __global__ __launch_bounds__(NT, 4) void kv8_prologue_kernel(ProArgs a) {
       for (int e = 0; e < PP; ++e) ss[r] = fma(lo[r][e], lo[r][e], fma(hi[r][e], hi[r][e], ss[r]));
     }
 #pragma unroll
-    for (int r = 0; r < KEEP; ++r) ss[r] = wave_sum64(ss[r]);
+    for (int r = 0; r < KEEP; ++r) ss[r] = g4d::wave_sum_dpp(ss[r]);
 #pragma unroll
     for (int r = 0; r < KEEP; ++r) {
       if (at + w + NW * r >= m) continue;

@@ -60,10 +60,14 @@ struct Args {
   Top* top;    // [row][chunk][ntop], in order
 };
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(v, 63);
 }
 __device__ __forceinline__ Top wave_first(Top t) {
 #pragma unroll
@@ -75,12 +79,15 @@ __device__ __forceinline__ Top wave_first(Top t) {
 // that exactly `need` reach (0: fewer keys are not 0).
 template <int N>
 __device__ __forceinline__ uint32_t reached_by(const uint32_t (&key)[N], uint32_t need) {
-  uint32_t hi = 0, lo = 0;  // lo: reached by enough; above hi: by too few
+  uint32_t most = 0, least = 0, some = 0;  // (of those that are not 0; the least as its complement)
 #pragma unroll
-  for (int i = 0; i < N; ++i) hi = max(hi, key[i]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) hi = max(hi, (uint32_t)__shfl_xor((int)hi, o, 64));
-  hi = __builtin_amdgcn_readfirstlane(hi);
+  for (int i = 0; i < N; ++i) {
+    most = max(most, key[i]);
+    least = max(least, key[i] ? ~key[i] : 0u);
+    some += __popcll(__ballot(key[i] != 0));
+  }
+  if (some < need) return 0;
+  uint32_t hi = wave_max_u32(most), lo = ~wave_max_u32(least);  // lo: reached by enough; above hi: by too few
   while (lo < hi) {
     const uint32_t mid = hi - (hi - lo) / 2;
     uint32_t n = 0;
@@ -184,8 +191,8 @@ __global__ __launch_bounds__(NT) void logprobs_chunk_kernel(Args a) {
     z += (double)zs[0];
     h += (double)hs[0];
   }
-  z = wave_sum64(z);
-  h = wave_sum64(h);
+  z = g4d::wave_sum_dpp(z);
+  h = g4d::wave_sum_dpp(h);
   if (l == 0) {
     s_z[w] = z;
     s_h[w] = h;
@@ -278,8 +285,8 @@ __global__ __launch_bounds__(NT) void logprobs_row_kernel(Args a) {
     z += f * s.z;
     h += f * (s.h + d * s.z);
   }
-  z = wave_sum64(z);
-  h = wave_sum64(h);
+  z = g4d::wave_sum_dpp(z);
+  h = g4d::wave_sum_dpp(h);
   if (l == 0) {
     s_z[w] = z;
     s_h[w] = h;
