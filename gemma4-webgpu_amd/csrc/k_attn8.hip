@@ -55,6 +55,8 @@ struct Args {
   uint2* meta;    // per sequence and KV head: the workgroups that hold its partials
   float* part;    // their partials
   uint32_t tiles;  // many rows: column tiles of the longest sequence
+  uint8_t* ops;    // few rows, or null: the output as operand blocks, in ntv tiles of 16 rows
+  int ntv;
 };
 
 // A V scale, NaN where it is infinite (relative to that one the others would be lost).
@@ -158,9 +160,44 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t pick(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
+// The output's super-block kb of a row, lane l holding its values 4 l .. + 3, as
+// an operand block of the o projection (g4d::Ops), what the batch's norms write of
+// the same values.
+__device__ __forceinline__ void write_ops(const Args& a, uint32_t row, uint32_t kb, int l, const f4& y) {
+  typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+  const float am = g4d::wave_max_dpp(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
+  float inverse;
+  const float up = g4d::f16_pair_scale(am, inverse);
+  const uint32_t t = row >> 4, c = row & 15u, s = l >> 3, q = (l >> 1) & 3, j = 4 * (l & 1);
+  uint8_t* base = a.ops + (size_t)kb * g4d::Ops::bytes(a.ntv);
+  h4 hi, lo;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = y[i] * up;
+    hi[i] = (_Float16)x;
+    lo[i] = (_Float16)(x - (float)hi[i]);
+    sum += x;
+  }
+  uint8_t* mp = base + t * g4d::Ops::MAIN_T + s * 2048 + (c + 16 * q) * 16 + j * 2;
+  *(h4*)mp = hi;
+  *(h4*)(mp + 1024) = lo;
+  sum = g4d::sum8(sum) * 0.015625f;  // of the sub-block, in three parts
+  if ((l & 7) == 0) {
+    h4 p;
+    p[0] = (_Float16)sum;
+    const float r = sum - (float)p[0];
+    p[1] = (_Float16)r;
+    p[2] = (_Float16)(r - (float)p[1]);
+    p[3] = (_Float16)0.f;
+    *(h4*)(base + g4d::Ops::sums_off(a.ntv) + t * 1024 + (c + 16 * (s >> 1)) * 16 + (s & 1) * 8) = p;
+  }
+  if (l == 0) *(float*)(base + g4d::Ops::scale_off(a.ntv) + t * 64 + c * 4) = inverse;
+}
+
 template <int HD>
 __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args a) {
-  constexpr int VB = HD / 16, KJ = HD / 64;
+  constexpr int VB = HD / 16, KJ = HD / 64, BL = HD < 256 ? 1 : HD / 256;
   __shared__ __align__(16) uint32_t s_q[3 * KJ * 64 * 4];  // digits as B operands: [digit][64 dims][lane] 16 B
   __shared__ __align__(16) float s_o[4 * COLS * HD];
   __shared__ float s_m[4 * COLS], s_l[4 * COLS], s_un[COLS];
@@ -448,7 +485,12 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
       }
       float* o = whole ? a.out + ((size_t)(sq.first + col / a.G) * a.nqh + kvh * a.G + col % a.G) * HD
                        : part + 2 * COLS + col * HD;
-      *(f4*)(o + d) = whole ? y * (1.0f / L) : y;
+      if (whole) y *= 1.0f / L;
+      *(f4*)(o + d) = y;
+      if constexpr (HD >= 256) {
+        if (whole && a.ops)  // (uniform; a wave holds 256 values of one row and head)
+          write_ops(a, sq.first + col / a.G, (kvh * a.G + col % a.G) * BL + d / 256, l, y);
+      }
       if (!whole && d == 0) {
         part[col] = M;
         part[COLS + col] = L;
@@ -463,6 +505,9 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     if (q.len || !q.n) continue;
     for (uint32_t d = tid; d < q.n * a.G * HD; d += NT)
       a.out[((size_t)(q.first + d / (a.G * HD)) * a.nqh + i % a.nkh * a.G) * HD + d % (a.G * HD)] = 0.f;
+    if (HD >= 256 && a.ops)
+      for (uint32_t b = w; b < q.n * a.G * BL; b += NT / 64)
+        write_ops(a, q.first + b / (a.G * BL), i % a.nkh * a.G * BL + b % (a.G * BL), l, f4{0.f, 0.f, 0.f, 0.f});
   }
 }
 
@@ -527,8 +572,10 @@ __global__ __launch_bounds__(MT) void attn8_merge_kernel(Args a) {
     L += f * s_l[i];
     y += f * *(const f4*)(s_o + i * HD + d);
   }
-  const float inv = 1.0f / L;
-  *(f4*)(a.out + ((size_t)(q.first + col / a.G) * a.nqh + kvh * a.G + col % a.G) * HD + d) = y * inv;
+  y *= 1.0f / L;
+  const uint32_t row = q.first + col / a.G, head = kvh * a.G + col % a.G;
+  *(f4*)(a.out + ((size_t)row * a.nqh + head) * HD + d) = y;
+  if (HD >= 256 && a.ops) write_ops(a, row, head * (HD / 256) + d / 256, threadIdx.x & 63, y);
 }
 
 // ---------------------------------------------------------------------------
@@ -1182,6 +1229,14 @@ int g4_pagedAttn8(g4_ctx* ctx, const float* q, const int8_t* k_pool, const int8_
                   const float* v_scale, const int32_t* page_table, const uint32_t* seq_lens,
                   const uint32_t* row_starts, float* output, g4_kv8_params p, void* workspace,
                   size_t workspace_bytes) {
+  return g4_pagedAttn8Ops(ctx, q, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens, row_starts, output, p,
+                          workspace, workspace_bytes, nullptr);
+}
+
+int g4_pagedAttn8Ops(g4_ctx* ctx, const float* q, const int8_t* k_pool, const int8_t* v_pool, const float* k_scale,
+                     const float* v_scale, const int32_t* page_table, const uint32_t* seq_lens,
+                     const uint32_t* row_starts, float* output, g4_kv8_params p, void* workspace,
+                     size_t workspace_bytes, void* ops) {
   G4_ENTER(ctx);
   G4_REQUIRE(q && k_pool && v_pool && k_scale && v_scale && page_table && seq_lens && output && workspace,
              "g4_pagedAttn8: null buffer");
@@ -1193,12 +1248,15 @@ int g4_pagedAttn8(g4_ctx* ctx, const float* q, const int8_t* k_pool, const int8_
   G4_REQUIRE(workspace_bytes >= need, "g4_pagedAttn8: workspace %zu bytes < %zu required", workspace_bytes, need);
   G4_REQUIRE((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)output | (uintptr_t)workspace) & 15) == 0,
              "g4_pagedAttn8: rows, pools and workspace must be 16-byte aligned");
+  G4_REQUIRE(!ops || (p.head_dim % 256 == 0 && p.num_rows <= 64 && step_fits(p) && ((uintptr_t)ops & 15) == 0),
+             "g4_pagedAttn8Ops: operand blocks need head_dim a multiple of 256, <= 64 rows, <= 16 rows x heads of a "
+             "KV head and a 16-byte aligned buffer");
   const uint32_t tiles = p.page_size / 16;
   const Args a{q, k_pool, v_pool, k_scale, v_scale, page_table,
                {seq_lens, row_starts, p.num_seqs, p.num_rows, p.max_rows, p.max_seq_len},
                p.num_q_heads, p.num_kv_heads, p.num_q_heads / p.num_kv_heads, tiles,
                tiles == 1 ? 0u : (uint32_t)(((1ull << 32) + tiles - 1) / tiles), tiles == 1 ? ~0u : 0u, p.max_pages, p.num_pages, p.sliding_window, p.scale,
-               output, 0, nullptr, nullptr, 0};
+               output, 0, nullptr, nullptr, 0, (uint8_t*)ops, (int)(g4d::pad_batch(p.num_rows) / 16)};
   switch (p.head_dim) {
     case 64: return attend<64>(ctx, p, a, workspace);
     case 128: return attend<128>(ctx, p, a, workspace);

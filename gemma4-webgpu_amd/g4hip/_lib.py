@@ -196,6 +196,7 @@ SIGNATURES = {
                                    _U32]),
     "g4_pagedAttn8_workspace_size": (_I, [Kv8Params, ctypes.POINTER(_SZ)]),
     "g4_pagedAttn8": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, Kv8Params, _P, _SZ]),
+    "g4_pagedAttn8Ops": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, Kv8Params, _P, _SZ, _P]),
     "g4_kv8Values": (_I, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P]),
     "g4_logprobsBatch_workspace_size": (_I, [_U32, _U32, _U32, ctypes.POINTER(_SZ)]),
     "g4_logprobsBatch": (_I, [_P, _P, _P, _U32, _U32, _P, _P, _U32, _P, _P, _P, _SZ]),

@@ -1029,7 +1029,7 @@ class BatchDecoder(_SyntheticModel):
             self.attn8_ws = None  # (the old one is given back first)
             self.attn8_ws, self.attn8_cap = self.ctx.alloc(need), need
 
-    def _attend8(self, il: int, q_parts, k_parts, v_parts, nq: int, q, out, p) -> None:
+    def _attend8(self, il: int, q_parts, k_parts, v_parts, nq: int, q, out, p, ops=None) -> None:
         """Layer il's prologue and attention over its 8-bit pages. Of a shared page list, the spare rows past
         the sequence's get its last row's output, as if they were that row again."""
         c, s, L = self.ctx, self.s, self.layers[il]
@@ -1043,7 +1043,7 @@ class BatchDecoder(_SyntheticModel):
                              *self.kv_scales[src], self.page_table, lens, p, row_starts=starts,
                              rope_cs=self.rope_cs[s.is_global(il)], rope_rows=self.rope_rows)
         c.pagedAttn8(q, L.k_cache, L.v_cache, *self.kv_scales[src], self.page_table, lens, out, p, self.attn8_ws,
-                     row_starts=starts)
+                     row_starts=starts, ops=ops)
         if self.shared_pages and p.max_rows < p.num_rows:
             c.repeatRow(out, s.q_dim_of(il), p.max_rows - 1, p.max_rows, p.num_rows - p.max_rows)
 
@@ -1130,9 +1130,10 @@ class BatchDecoder(_SyntheticModel):
                                  self.seq_lens, self.attn, self.pro_params[il], self.block_ws, ops=ops,
                                  rope_cs=self.rope_cs[s.is_global(il)], rope_rows=self.rope_rows)
             elif self.kv8:
-                ops = None  # the o projection's own launch prepares its operands
+                if self.shared_pages:  # (many rows of one sequence: the o projection's launch makes its operands)
+                    ops = None
                 self._attend8(il, self.q_parts, self.k_parts, self.v_parts, nq, self.q, self.attn,
-                              self._kv8_params(il, B, min(self.span_rows, B) if self.shared_pages else 1))
+                              self._kv8_params(il, B, min(self.span_rows, B) if self.shared_pages else 1), ops)
             else:
                 c.pagedAttnPrologue(self.q_parts, self.k_parts if prod else None, self.v_parts if prod else None, nq,
                                     L.q_norm, L.k_norm, self.rope_freqs, self.q, L.k_cache if prod else None,

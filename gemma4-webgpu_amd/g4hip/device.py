@@ -721,10 +721,13 @@ class Context:
                                           _p(rope_cs), rope_rows))
 
     def pagedAttn8(self, q: Ptr, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr, page_table: Ptr,
-                   seq_lens: Ptr, out: Ptr, p: Kv8Params, workspace: Buffer, row_starts: Ptr = None) -> None:
-        """Attention of every row over its sequence's 8-bit pages, up to its own position."""
-        check(lib().g4_pagedAttn8(self.h, _p(q), _p(k_pool), _p(v_pool), _p(k_scale), _p(v_scale), _p(page_table),
-                                  _p(seq_lens), _p(row_starts), _p(out), p, _p(workspace), workspace.nbytes))
+                   seq_lens: Ptr, out: Ptr, p: Kv8Params, workspace: Buffer, row_starts: Ptr = None,
+                   ops: Ptr = None) -> None:
+        """Attention of every row over its sequence's 8-bit pages, up to its own position (`ops`: also as the o
+        projection's operand blocks)."""
+        check(lib().g4_pagedAttn8Ops(self.h, _p(q), _p(k_pool), _p(v_pool), _p(k_scale), _p(v_scale), _p(page_table),
+                                     _p(seq_lens), _p(row_starts), _p(out), p, _p(workspace), workspace.nbytes,
+                                     _p(ops)))
 
     def kv8Values(self, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr, pages: Ptr, count: int, page_size: int,
                   nkh: int, hd: int, num_pages: int, k_out: Ptr, v_out: Ptr) -> None:

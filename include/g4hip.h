@@ -834,6 +834,15 @@ int g4_pagedAttn8(g4_ctx* ctx, const float* q, const int8_t* k_pool, const int8_
                   const float* v_scale, const int32_t* page_table, const uint32_t* seq_lens,
                   const uint32_t* row_starts, float* output, g4_kv8_params p, void* workspace,
                   size_t workspace_bytes);
+/* The same, with the output also as the operand blocks of the o projection (ops:
+ * g4_batchOperandBytes(num_q_heads * head_dim, num_rows) bytes, as
+ * g4_pagedAttnDecodeOps writes them; row r is vector r). head_dim 256 or 512, at
+ * most 64 rows and max_rows * query heads per KV head <= 16; ops NULL is
+ * g4_pagedAttn8. */
+int g4_pagedAttn8Ops(g4_ctx* ctx, const float* q, const int8_t* k_pool, const int8_t* v_pool, const float* k_scale,
+                     const float* v_scale, const int32_t* page_table, const uint32_t* seq_lens,
+                     const uint32_t* row_starts, float* output, g4_kv8_params p, void* workspace,
+                     size_t workspace_bytes, void* ops);
 /* k_out, v_out f16 [count][page_size][num_kv_heads][head_dim] = the values of
  * the pages listed in `pages` (device, `count` ids; one outside [0, num_pages)
  * gives zeros): what moves a sequence to an f16 pool. */
