@@ -43,6 +43,11 @@ class Buffer:
         self.nbytes = nbytes
         self._owned = owned
 
+    @property
+    def _as_parameter_(self) -> int:
+        """A Buffer as an argument of a C entry: its address (an int and None are taken as they are)."""
+        return self.ptr
+
     def offset(self, nbytes: int) -> "Buffer":
         assert 0 <= nbytes <= self.nbytes
         return Buffer(self.ctx, self.ptr + nbytes, self.nbytes - nbytes, owned=False)
@@ -715,25 +720,23 @@ class Context:
                            rope_rows: int = 0) -> None:
         """pagedAttnPrologue over an 8-bit pool, rows row_starts[s] .. row_starts[s + 1] - 1 of each sequence
         (None: one row each): q after norm + RoPE into q_out, k and v appended as codes, scales grown."""
-        check(lib().g4_pagedAttnPrologue8(self.h, _p(q_parts), _p(k_parts), _p(v_parts), nparts, _p(q_norm_w),
-                                          _p(k_norm_w), _p(rope_freqs), _p(q_out), _p(k_pool), _p(v_pool),
-                                          _p(k_scale), _p(v_scale), _p(page_table), _p(seq_lens), _p(row_starts), p,
-                                          _p(rope_cs), rope_rows))
+        check(lib().g4_pagedAttnPrologue8(self.h, q_parts, k_parts, v_parts, nparts, q_norm_w, k_norm_w,
+                                          rope_freqs, q_out, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens,
+                                          row_starts, p, rope_cs, rope_rows))
 
     def pagedAttn8(self, q: Ptr, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr, page_table: Ptr,
                    seq_lens: Ptr, out: Ptr, p: Kv8Params, workspace: Buffer, row_starts: Ptr = None,
                    ops: Ptr = None) -> None:
         """Attention of every row over its sequence's 8-bit pages, up to its own position (`ops`: also as the o
         projection's operand blocks)."""
-        check(lib().g4_pagedAttn8Ops(self.h, _p(q), _p(k_pool), _p(v_pool), _p(k_scale), _p(v_scale), _p(page_table),
-                                     _p(seq_lens), _p(row_starts), _p(out), p, _p(workspace), workspace.nbytes,
-                                     _p(ops)))
+        check(lib().g4_pagedAttn8Ops(self.h, q, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens,
+                                     row_starts, out, p, workspace, workspace.nbytes, ops))
 
     def kv8Values(self, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr, pages: Ptr, count: int, page_size: int,
                   nkh: int, hd: int, num_pages: int, k_out: Ptr, v_out: Ptr) -> None:
         """The listed pages of an 8-bit pool as f16 pages."""
-        check(lib().g4_kv8Values(self.h, _p(k_pool), _p(v_pool), _p(k_scale), _p(v_scale), _p(pages), count,
-                                 page_size, nkh, hd, num_pages, _p(k_out), _p(v_out)))
+        check(lib().g4_kv8Values(self.h, k_pool, v_pool, k_scale, v_scale, pages, count, page_size, nkh, hd,
+                                 num_pages, k_out, v_out))
 
     def advanceSeqLens(self, seq_lens: Ptr, num_seqs: int, delta: int = 1) -> None:
         check(lib().g4_advanceSeqLens(self.h, _p(seq_lens), num_seqs, delta))
@@ -813,8 +816,8 @@ class Context:
                       top_ids: Ptr, top_logprobs: Ptr, workspace: Buffer) -> None:
         """Per row of `batch` rows of logits: the log probability of tokens[r], the entropy, and the ntop likeliest
         tokens with theirs."""
-        check(lib().g4_logprobsBatch(self.h, _p(logits), _p(tokens), size, batch, _p(logprobs), _p(entropy), ntop,
-                                     _p(top_ids), _p(top_logprobs), _p(workspace), workspace.nbytes))
+        check(lib().g4_logprobsBatch(self.h, logits, tokens, size, batch, logprobs, entropy, ntop, top_ids,
+                                     top_logprobs, workspace, workspace.nbytes))
 
     # ---- debug / synthetic inputs ----
     def dequant_q4k(self, blocks: Ptr, nblocks: int, out: Ptr) -> None:
