@@ -19,6 +19,10 @@
 //
 // Sums: eight values in f32, the rest in f64: behind a likely token's 1 the
 // 30000 others of 1e-7 each would otherwise fall below half a step.
+//
+// Measured: 500 rows of 100003 (200 MB) 38 us, 5.2 TB/s, and 5 for the join; 64 of
+// 262144 17.6 and 5.1 (a workgroup has one round of loads, whose arrival nothing
+// hides); one row 5.4 and 4.2, two launches of 2.3 when empty.
 #include <algorithm>
 
 #include "g4_internal.hpp"
