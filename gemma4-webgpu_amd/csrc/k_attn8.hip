@@ -321,13 +321,12 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
 #pragma unroll
     for (int e = 0; e < E / 4; ++e) x[e] = *(const f4*)(qg + 4 * e);
     uint32_t st = 4 * off + w;
-    if (st < steps) {
-      pages(st, pg);
-      load_scales(ks, vs);
-      load_k(st);
-      load_v(st);
-      pages(min(st + 4, steps - 1), pg);
-    }
+    // (a wave without a step too, of no bytes: behind a branch q would be waited for together with the rows)
+    pages(st, pg);
+    load_scales(ks, vs);
+    load_k(st);
+    load_v(st);
+    pages(min(st + 4, steps - 1), pg);
     // ---- q's digits ----
     __syncthreads();  // the previous sequence's are done with
     {
