@@ -323,10 +323,12 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     uint32_t st = 4 * off + w;
     // (a wave without a step too, of no bytes: behind a branch q would be waited for together with the rows)
     pages(st, pg);
+    pages(min(st + 4, steps - 1), pg_far);  // (before the rows: what comes after them is waited for with them)
     load_scales(ks, vs);
     load_k(st);
     load_v(st);
-    pages(min(st + 4, steps - 1), pg);
+    pg[0] = pg_far[0];
+    pg[1] = pg_far[1];
     // ---- q's digits ----
     __syncthreads();  // the previous sequence's are done with
     {
