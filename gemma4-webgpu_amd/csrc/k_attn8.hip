@@ -781,10 +781,16 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
     v_ref = ref;
     return by;
   };
+  // (K as buffers: an address made scalar would be a generic one, whose loads the LDS reads of the step wait for)
   auto load_k = [&](uint32_t k) __attribute__((always_inline)) {  // (of the refilled steps)
 #pragma unroll
-    for (int i = 0; i < KP; ++i)
-      kr[i] = *(const i4*)((const int8_t*)uni((uint64_t)(kp + (size_t)uni(s_tile[4 * k + kt(i)]) * (16 * rs))) + k_at[i]);
+    for (int i = 0; i < KP; ++i) {
+      const uint64_t at = uni((uint64_t)(kp + (size_t)uni(s_tile[4 * k + kt(i)]) * (16 * rs)));
+      kr[i] = __builtin_bit_cast(
+          i4, __builtin_amdgcn_raw_buffer_load_b128(
+                  __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, (int)(15 * (uint32_t)rs + HD), 0x00020000),
+                  k_at[i], 0, 0));
+    }
   };
   auto load_v = [&](uint32_t k) __attribute__((always_inline)) {
     const int8_t* vp = vp_ + (size_t)s_tile[4 * k + vt] * (16 * rs) + v_at;
