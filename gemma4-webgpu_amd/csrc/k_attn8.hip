@@ -702,7 +702,8 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
   auto locate = [&](uint32_t unit) {  // the column tile of a unit, by the thread whose run holds it
     if (s_upto[tid] <= unit && s_upto[tid + 1] > unit) {
       uint32_t j = tid * run, at = s_upto[tid];
-      for (uint32_t n; at + (n = cost_of(a, j) * a.nkh) <= unit; ++j) at += n;
+      if (run > 1)  // (a run of one is that tile)
+        for (uint32_t n; at + (n = cost_of(a, j) * a.nkh) <= unit; ++j) at += n;
       s_at[0] = j;
       s_at[1] = at;
     }
@@ -768,9 +769,10 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
     float vs = 0.f;
     if (tid < 4 * CH) {
       const uint32_t t = min(t0 + 4 * st + tid, tlast), at = page_of(a, t), pg = clamp_page(a, list[at]);
+      const float ks = a.ks[(size_t)pg * a.nkh + kvh], v = a.vs[(size_t)pg * a.nkh + kvh];
       s_tile[tid] = pg * a.page_tiles + (t - at * a.page_tiles);
-      s_ks[tid] = a.ks[(size_t)pg * a.nkh + kvh];
-      vs = finite(a.vs[(size_t)pg * a.nkh + kvh]);
+      vs = finite(v);
+      s_ks[tid] = ks;
       const float big = g4d::wave_max_dpp(vs);  // (a NaN is not the larger one)
       if (l == 0) s_big[w] = big;
     }
@@ -818,15 +820,20 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
       *(g4mm::u32x2*)(dst + k * 1024) = g4mm::u32x2{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
     });
   };
+  const float* qg = a.q + ((size_t)(first + gr / a.G) * a.nqh + kvh * a.G + gr % a.G) * HD + 16 * qd;
+  f4 qx[KJ][4];  // q of this lane's column: dims 64 j + 16 qd .. + 15 (PAIR: from 256 wd on), asked for first
+#pragma unroll
+  for (int j = 0; j < KJ; ++j)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) qx[j][k] = *(const f4*)(qg + 256 * wd + 64 * j + 4 * k);
   (void)refill(st0);
   load_k(0);
   load_v(0);
 
-  // ---- q's digits of this lane's column: dims 64 j + 16 qd .. + 15 (PAIR: from 256 wd on) ----
+  // ---- q's digits ----
   i4 qb[3][KJ];
   float s_scale;
   {
-    const float* qg = a.q + ((size_t)(first + gr / a.G) * a.nqh + kvh * a.G + gr % a.G) * HD + 16 * qd;
     float am = 0.f;
     bool nan = false;
     auto largest = [&](const f4& y) {
@@ -836,15 +843,10 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
         nan |= y[i] != y[i];
       }
     };
-    f4 x[KJ][4];
 #pragma unroll
     for (int j = 0; j < KJ; ++j)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[j][k] = *(const f4*)(qg + 256 * wd + 64 * j + 4 * k);
-#pragma unroll
-    for (int j = 0; j < KJ; ++j)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) largest(x[j][k]);
+      for (int k = 0; k < 4; ++k) largest(qx[j][k]);
     am = g4d::xmax32(g4d::xmax16(nan ? INFINITY : am));
     if constexpr (PAIR) {  // one scale for all 512 dims
       if (qd == 0) s_mx[wd * TC + 16 * wc + c] = am;
@@ -863,7 +865,7 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
       for (int k = 0; k < 4; ++k) {
         uint32_t d[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = digits(x[j][k][i], up);
+        for (int i = 0; i < 4; ++i) d[i] = digits(qx[j][k][i], up);
         qb[0][j][k] = (int)plane<0>(d[0], d[1], d[2], d[3]);
         qb[1][j][k] = (int)plane<1>(d[0], d[1], d[2], d[3]);
         qb[2][j][k] = (int)plane<2>(d[0], d[1], d[2], d[3]);

@@ -18,12 +18,12 @@ struct Seq {
 };
 __device__ __forceinline__ Seq seq_rows(const Rows& r, uint32_t s) {
   Seq q{s, 1, 0, 0};
+  const uint32_t L = r.seq_lens[s];  // (all three on their way at once)
   if (r.row_starts) {
     const uint32_t a = r.row_starts[s], b = r.row_starts[s + 1];
     q.first = a;
     q.n = b >= a && b <= r.num_rows && b - a <= r.max_rows ? b - a : 0u;
   }
-  const uint32_t L = r.seq_lens[s];
   if (q.n > 0 && L >= q.n && L <= r.max_seq_len) {
     q.len = L;
     q.base = L - q.n;
