@@ -1075,7 +1075,7 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
     }
   }
 
-  // ---- columns 4 qd + i of the wave's tile, dims VB c + e (PAIR: 256 wd + 16 c + e) ----
+  // ---- columns 4 qd + i of the wave's tile, dims NE c + e (PAIR: 256 wd + 16 c + e) ----
   if constexpr (PAIR) {
     __syncthreads();
     if (qd == 0) s_mx[wd * TC + 16 * wc + c] = l_run;
@@ -1086,16 +1086,31 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_t
   const uint32_t slot = 2 * wg + used;  // (0 for a tile begun by another workgroup: it comes first)
   used = 1;
   float* part = a.part + (size_t)slot * TileShape<HD>::SLOT;
+  // Row by row through LDS (where V was), so that a wave stores whole KB: lanes storing their own 16 bytes of every 64
+  // take four times the requests. Four dims of a lane turned by c: its 16 lanes meet different banks.
+  constexpr int RD = NE * 16, QG = NE / 4, RPS = 16 / NE;  // a wave's dims of a row; groups of four of a lane; rows a store
+  if constexpr (!PAIR) __syncthreads();  // (every wave is done with V)
+  float* turn_s = (float*)s_v + w * 4 * RD;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t col = 16 * wc + 4 * qd + i, og = ct * TC + col;
     const float L = __shfl(l_run, 4 * qd + i, 64), f = (whole ? 1.0f / L : 1.f) * (v_ref * (1.f / kTileP));
-    if (og < ncols) {
-      float* o = (whole ? a.out + ((size_t)(first + og / a.G) * a.nqh + kvh * a.G + og % a.G) * HD
-                        : part + 2 * TC + col * HD) + vdim;
 #pragma unroll
-      for (int e = 0; e < NE; e += 4) *(f4*)(o + e) = f4{O[e][i] * f, O[e + 1][i] * f, O[e + 2][i] * f, O[e + 3][i] * f};
+    for (int e = 0; e < QG; ++e)
+      *(f4*)(turn_s + qd * RD + c * NE + 4 * ((e + c) % QG)) =
+          f4{O[4 * e][i] * f, O[4 * e + 1][i] * f, O[4 * e + 2][i] * f, O[4 * e + 3][i] * f};
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");  // (the wave's own region: its LDS operations are in order)
+#pragma unroll
+    for (int r0 = 0; r0 < 4; r0 += RPS) {
+      const int r = r0 + l / (RD / 4), d4 = l % (RD / 4), lc = d4 / QG;
+      const f4 y = *(const f4*)(turn_s + r * RD + lc * NE + 4 * ((d4 % QG + lc) % QG));
+      const uint32_t col = 16 * wc + 4 * r + i, og = ct * TC + col;
+      if (og < ncols)
+        *(f4*)((whole ? a.out + ((size_t)(first + og / a.G) * a.nqh + kvh * a.G + og % a.G) * HD
+                      : part + 2 * TC + col * HD) + 256 * wd + 4 * d4) = y;
     }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
   }
   if (!whole && wd == 0 && qd == 0) {
     part[16 * wc + c] = m_run;
