@@ -635,7 +635,7 @@ struct TileShape {
   static constexpr int VBYTES = TP * HD * 2;
   static constexpr int KP = TP * HD / 16 / NTH;  // 16-byte pieces of K a thread and step
   static constexpr int VD = PAIR ? 16 : VB;      // dims a thread moves of 4 positions of V
-  static constexpr uint32_t WGS = HD == 512 ? 256 : HD == 256 ? 512 : 768;  // that run at once (registers, LDS)
+  static constexpr uint32_t WGS = HD == 512 ? 256 : HD >= 128 ? 512 : 768;  // that run at once (registers, LDS)
   static constexpr uint32_t SLOT = TC * (HD + 2);                           // floats of a partial: max, sum [64], o
 };
 
@@ -659,7 +659,7 @@ __device__ __forceinline__ uint32_t cost_of(const Args& a, uint32_t j) {
 }
 
 template <int HD>
-__global__ __launch_bounds__(TileShape<HD>::NTH, HD <= 128 ? 3 : 2) void attn8_tile_kernel(Args a) {
+__global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn8_tile_kernel(Args a) {
   using S_ = TileShape<HD>;
   constexpr bool PAIR = S_::PAIR;
   constexpr int KJ = PAIR ? 4 : HD / 64, KP = S_::KP, VD = S_::VD, VB = S_::VB;
