@@ -205,6 +205,21 @@ def test_score(ctx, kv):
         assert abs(got[i] - ref) <= 8 * U * (abs(float(x[toks[i + 1]]) - float(x.max())) + np.log(x.size) + 1), i
 
 
+def test_log_probabilities_without_alternatives_and_of_a_topk_sample(ctx):
+    """A step whose host samples has no token yet: entropy and alternatives only."""
+    x = BatchDecoder(ctx, [3, 20], shape(), seed=85, embed=True, kv="int8", logprobs=0)
+    y = BatchDecoder(ctx, [3, 20], shape(), seed=85, embed=True, kv="int8", logprobs=6)
+    for d in (x, y):
+        d.fill_kv(seed=86)
+        d.token_logprobs.upload(np.full(2, 7.0, np.float32))
+    x.step()
+    y.step("topk")
+    assert np.all(x.token_logprobs.download(np.float32) < 0) and x.top_ids is None
+    assert np.all(y.token_logprobs.download(np.float32) == 7.0)
+    assert bits_equal(x.entropy.download(np.float32), y.entropy.download(np.float32))
+    assert np.array_equal(y.top_ids.download(np.uint32).reshape(2, 6)[:, 0], x.tokens.download(np.uint32))
+
+
 def test_refusals(ctx):
     s = shape()
     with pytest.raises(ValueError):
