@@ -130,10 +130,10 @@ __device__ __forceinline__ h2 two_codes(uint32_t x0, uint32_t x1) {
 // held by one workgroup is written by it; else its workgroups leave partials
 // (max, sum, o), which attn8_merge_kernel adds in order.
 //
-// Measured: 32 long contexts at head dim 512 (362 MB) 83 us, 4.4 TB/s of the 4.8
-// of a copy; 64 mixed ones at 256 (93 MB) 26 us; one window of 512 8.6 us, the
+// Measured: 32 long contexts at head dim 512 (362 MB) 80 us, 4.5 TB/s of the 4.8
+// of a copy; 64 mixed ones at 256 (93 MB) 25 us; one window of 512 8.0 us, the
 // latency of a unit (lengths, page ids, rows, products, the waves' sums); the
-// partials 3.4 to 4.8 us more. Units of 1024, so that a window has no partials,
+// partials 3 to 4.8 us more. Units of 1024, so that a window has no partials,
 // took 15.6 us instead of 11.4: a wave's step of 32 positions is 1.8 us.
 constexpr int NT = 256, UNIT = 128;
 template <int HD>
@@ -1145,15 +1145,33 @@ __global__ __launch_bounds__(HD / 4) void attn8_tile_merge_kernel(Args a) {
   const uint32_t w0 = mt.x / 2, n = mt.y - w0 + 1;
   if (n == 1) return;  // written by its workgroup
   auto part = [&](uint32_t k) { return a.part + (size_t)(k ? 2 * (w0 + k) : mt.x) * TileShape<HD>::SLOT; };
-  float M = -INFINITY, L = 0.f;
-  for (uint32_t k = 0; k < n; ++k) M = fmaxf(M, part(k)[col]);
+  constexpr int MS = 4;  // partials on their way
+  float M = kNothing, L = 0.f;
   f4 o = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (uint32_t k = 0; k < n; ++k) {
-    const float* p = part(k);
-    const float f = exp2_h(p[col] - M);
-    L += f * p[TC + col];
-    o += f * *(const f4*)(p + 2 * TC + col * HD + d);
+  for (uint32_t k0 = 0; k0 < n; k0 += MS) {
+    float pm[MS], pl[MS];
+    f4 po[MS];
+#pragma unroll
+    for (int k = 0; k < MS; ++k) {
+      const float* p = part(min(k0 + k, n - 1));
+      pm[k] = p[col];
+      pl[k] = p[TC + col];
+      po[k] = *(const f4*)(p + 2 * TC + col * HD + d);
+    }
+    float mn = M;
+#pragma unroll
+    for (int k = 0; k < MS; ++k) mn = fmaxf(mn, pm[k]);
+    const float al = exp2_h(M - mn);
+    L *= al;
+    o *= al;
+#pragma unroll
+    for (int k = 0; k < MS; ++k) {
+      if (k0 + k >= n) continue;
+      const float f = exp2_h(pm[k] - mn);
+      L += f * pl[k];
+      o += f * po[k];
+    }
+    M = mn;
   }
   *(f4*)(a.out + (size_t)blockIdx.x * HD + d) = o * (1.0f / L);
 }
