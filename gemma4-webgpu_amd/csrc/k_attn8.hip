@@ -48,7 +48,7 @@ struct Args {
   const float *ks, *vs;
   const int32_t* page_table;
   Rows rows;
-  uint32_t nqh, nkh, G, page_tiles, page_magic, page_same, max_pages, num_pages, window;
+  uint32_t nqh, nkh, G, g_magic, g_same, page_tiles, page_magic, page_same, max_pages, num_pages, window;
   float scale;
   float* out;
   uint32_t wgs;   // workgroups that share the work
@@ -68,6 +68,14 @@ __device__ __forceinline__ uint32_t uni(uint32_t x) { return __builtin_amdgcn_re
 __device__ __forceinline__ int32_t uni_i(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ uint64_t uni(uint64_t x) {
   return (uint64_t)uni((uint32_t)(x >> 32)) << 32 | uni((uint32_t)x);
+}
+
+// x / G for x < 2^28 (G <= 16: x times the rounded-up 2^32 / G is off by less than 1 / G; a G of 1: a magic of 0 and
+// all of x).
+__device__ __forceinline__ uint32_t div_g(const Args& a, uint32_t x) { return __umulhi(x, a.g_magic) + (x & a.g_same); }
+// Row of q and of the output (of nqh heads a row) that is a sequence's column of a KV head.
+__device__ __forceinline__ size_t row_of(const Args& a, uint32_t first, uint32_t kvh, uint32_t col) {
+  return (size_t)first * a.nqh + kvh * a.G + (size_t)div_g(a, col) * (a.nqh - a.G) + col;
 }
 
 // Page (of the sequence's list) that holds tile t: t < 2^26, at most 64 tiles
@@ -316,7 +324,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     // q, 16 threads a column (asked for before the rows, whose arrival its digits then do not wait for)
     constexpr int E = HD / 16;
     const uint32_t col = tid >> 4, part_of = tid & 15, cc = min(col, ncols - 1);
-    const float* qg = a.q + ((size_t)(sq.first + cc / a.G) * a.nqh + kvh * a.G + cc % a.G) * HD + part_of * E;
+    const float* qg = a.q + row_of(a, sq.first, kvh, cc) * HD + part_of * E;
     f4 x[E / 4];
 #pragma unroll
     for (int e = 0; e < E / 4; ++e) x[e] = *(const f4*)(qg + 4 * e);
@@ -358,7 +366,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     __syncthreads();
     // this lane's column: positions clo .. clo + width - 1
     const float s_scale = s_un[c] * (a.scale * kLog2e);
-    const uint32_t cpos = sq.base + c / a.G;
+    const uint32_t cpos = sq.base + div_g(a, c);
     const uint32_t clo = a.window && cpos + 1 > a.window ? cpos + 1 - a.window : 0u;
     const uint32_t width = (uint32_t)c < ncols ? cpos + 1 - clo : 0u;
     f4 O[VB];
@@ -490,13 +498,12 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
         L += s_l[k * COLS + col] * f;
         y += *(const f4*)(s_o + (k * COLS + col) * HD + d / VB * VB + 4 * ((d % VB / 4 + d / VB) % QG)) * f;
       }
-      float* o = whole ? a.out + ((size_t)(sq.first + col / a.G) * a.nqh + kvh * a.G + col % a.G) * HD
-                       : part + 2 * COLS + col * HD;
+      float* o = whole ? a.out + row_of(a, sq.first, kvh, col) * HD : part + 2 * COLS + col * HD;
       if (whole) y *= 1.0f / L;
       *(f4*)(o + d) = y;
       if constexpr (HD >= 256) {
         if (whole && a.ops)  // (uniform; a wave holds 256 values of one row and head)
-          write_ops(a, sq.first + col / a.G, (kvh * a.G + col % a.G) * BL + d / 256, l, y);
+          write_ops(a, sq.first + div_g(a, col), (kvh * a.G + col - div_g(a, col) * a.G) * BL + d / 256, l, y);
       }
       if (!whole && d == 0) {
         part[col] = M;
@@ -644,7 +651,7 @@ struct Tile {
   uint32_t lo, end, steps;
 };
 __device__ __forceinline__ Tile tile_of(const Args& a, const Seq& q, uint32_t ct) {
-  const uint32_t r0 = ct * TC / a.G, r1 = min(q.n - 1, (ct * TC + TC - 1) / a.G);
+  const uint32_t r0 = div_g(a, ct * TC), r1 = min(q.n - 1, div_g(a, ct * TC + TC - 1));
   Tile t;
   t.lo = a.window && q.base + r0 + 1 > a.window ? (q.base + r0 + 1 - a.window) & ~15u : 0u;
   t.end = q.base + r1 + 1;
@@ -742,11 +749,11 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn8_ti
 
   // this lane's column
   const uint32_t g = ct * TC + 16 * wc + c, gr = min(g, ncols - 1);
-  const uint32_t cpos = base + gr / a.G;
+  const uint32_t cpos = base + div_g(a, gr);
   const uint32_t clo = a.window && cpos + 1 > a.window ? cpos + 1 - a.window : 0u;
   const uint32_t width = g < ncols ? cpos + 1 - clo : 0u;
   // positions every column sees: those from the last row's window on, up to the first row's own
-  const uint32_t all0 = a.window && end > a.window ? end - a.window : 0u, all1 = base + ct * TC / a.G;
+  const uint32_t all0 = a.window && end > a.window ? end - a.window : 0u, all1 = base + div_g(a, ct * TC);
 
   // ---- rows on their way ----
   i4 kr[KP];
@@ -820,7 +827,7 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn8_ti
       *(g4mm::u32x2*)(dst + k * 1024) = g4mm::u32x2{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
     });
   };
-  const float* qg = a.q + ((size_t)(first + gr / a.G) * a.nqh + kvh * a.G + gr % a.G) * HD + 16 * qd;
+  const float* qg = a.q + row_of(a, first, kvh, gr) * HD + 16 * qd;
   f4 qx[KJ][4];  // q of this lane's column: dims 64 j + 16 qd .. + 15 (PAIR: from 256 wd on), asked for first
 #pragma unroll
   for (int j = 0; j < KJ; ++j)
@@ -1106,8 +1113,7 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn8_ti
       const f4 y = *(const f4*)(turn_s + r * RD + lc * NE + 4 * ((d4 % QG + lc) % QG));
       const uint32_t col = 16 * wc + 4 * r + i, og = ct * TC + col;
       if (og < ncols)
-        *(f4*)((whole ? a.out + ((size_t)(first + og / a.G) * a.nqh + kvh * a.G + og % a.G) * HD
-                      : part + 2 * TC + col * HD) + 256 * wd + 4 * d4) = y;
+        *(f4*)((whole ? a.out + row_of(a, first, kvh, og) * HD : part + 2 * TC + col * HD) + 256 * wd + 4 * d4) = y;
     }
     __builtin_amdgcn_wave_barrier();
     asm volatile("" ::: "memory");
@@ -1126,7 +1132,7 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn8_ti
     if (q.len || g0 >= ncols) continue;
     for (uint32_t i = tid; i < min((uint32_t)TC, ncols - g0) * a.nkh * HD; i += S_::NTH) {
       const uint32_t g = g0 + i / HD / a.nkh, kvh = i / HD % a.nkh;
-      a.out[((size_t)(q.first + g / a.G) * a.nqh + kvh * a.G + g % a.G) * HD + i % HD] = 0.f;
+      a.out[row_of(a, q.first, kvh, g) * HD + i % HD] = 0.f;
     }
   }
 }
@@ -1304,12 +1310,12 @@ int g4_pagedAttn8Ops(g4_ctx* ctx, const float* q, const int8_t* k_pool, const in
   G4_REQUIRE(!ops || (p.head_dim % 256 == 0 && p.num_rows <= 64 && step_fits(p) && ((uintptr_t)ops & 15) == 0),
              "g4_pagedAttn8Ops: operand blocks need head_dim a multiple of 256, <= 64 rows, <= 16 rows x heads of a "
              "KV head and a 16-byte aligned buffer");
-  const uint32_t tiles = p.page_size / 16;
+  const uint32_t tiles = p.page_size / 16, G = p.num_q_heads / p.num_kv_heads;
+  auto magic = [](uint32_t d) { return d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d); };
   const Args a{q, k_pool, v_pool, k_scale, v_scale, page_table,
                {seq_lens, row_starts, p.num_seqs, p.num_rows, p.max_rows, p.max_seq_len},
-               p.num_q_heads, p.num_kv_heads, p.num_q_heads / p.num_kv_heads, tiles,
-               tiles == 1 ? 0u : (uint32_t)(((1ull << 32) + tiles - 1) / tiles), tiles == 1 ? ~0u : 0u, p.max_pages, p.num_pages, p.sliding_window, p.scale,
-               output, 0, nullptr, nullptr, 0, (uint8_t*)ops, (int)(g4d::pad_batch(p.num_rows) / 16)};
+               p.num_q_heads, p.num_kv_heads, G, magic(G), G == 1 ? ~0u : 0u, tiles, magic(tiles),
+               tiles == 1 ? ~0u : 0u, p.max_pages, p.num_pages, p.sliding_window, p.scale, output, 0, nullptr, nullptr, 0, (uint8_t*)ops, (int)(g4d::pad_batch(p.num_rows) / 16)};
   switch (p.head_dim) {
     case 64: return attend<64>(ctx, p, a, workspace);
     case 128: return attend<128>(ctx, p, a, workspace);
