@@ -276,8 +276,8 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn8_step_kernel(Args 
     // loads of the next step would spill)
     auto tile_at = [&](const int8_t* pool, uint32_t st, int p) -> __amdgpu_buffer_rsrc_t {
       const uint32_t t = t0 + min(2 * st + p, tiles - 1), slot = (t - page_of(a, t) * a.page_tiles) * 16;
-      const uint64_t at = uni((uint64_t)(pool + ((size_t)clamp_page(a, uni_i(pg[p])) * (a.page_tiles * 16) + slot) * rs +
-                                         kvh * HD));
+      const size_t row = (size_t)clamp_page(a, uni_i(pg[p])) * (a.page_tiles * 16) + slot;
+      const uint64_t at = uni((uint64_t)(pool + row * rs + kvh * HD));
       return __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, st < steps ? (int)(15 * (uint32_t)rs + HD) : 0,
                                                0x00020000);
     };
@@ -739,7 +739,7 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn8_ti
   }
   const uint32_t kvh = a.nkh == 1 ? 0u : uni((u - before) / cost);
   const uint32_t seg = before + kvh * cost, stop = min(seg + cost, ue);  // the tile's first unit, the last here
-  const uint32_t st0 = max(u, seg + kTileCost) - (seg + kTileCost), st1 = max(stop, seg + kTileCost) - (seg + kTileCost);
+  const uint32_t seg0 = seg + kTileCost, st0 = max(u, seg0) - seg0, st1 = max(stop, seg0) - seg0;
   u = stop;
   if (st0 == st1) continue;  // (the share ends before the tile's first step)
   __syncthreads();  // the previous tile's rows are done with
@@ -1044,9 +1044,15 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn8_ti
       if (u + 1 < NE / 2) read_b(u + 1, B[(u + 1) & 1]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) O[u / 2 * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[u & 1], B[u & 1][e], O[u / 2 * 4 + e], 0, 0, 0);
+      for (int e = 0; e < 4; ++e) {
+        f4& o = O[u / 2 * 4 + e];
+        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[u & 1], B[u & 1][e], o, 0, 0, 0);
+      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) O[u / 2 * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[u & 1], B[u & 1][e], O[u / 2 * 4 + e], 0, 0, 0);
+      for (int e = 0; e < 4; ++e) {
+        f4& o = O[u / 2 * 4 + e];
+        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[u & 1], B[u & 1][e], o, 0, 0, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -1095,7 +1101,7 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn8_ti
   float* part = a.part + (size_t)slot * TileShape<HD>::SLOT;
   // Row by row through LDS (where V was), so that a wave stores whole KB: lanes storing their own 16 bytes of every 64
   // take four times the requests. Four dims of a lane turned by c: its 16 lanes meet different banks.
-  constexpr int RD = NE * 16, QG = NE / 4, RPS = 16 / NE;  // a wave's dims of a row; groups of four of a lane; rows a store
+  constexpr int RD = NE * 16, QG = NE / 4, RPS = 16 / NE;  // a wave's dims of a row; a lane's groups; rows a store
   if constexpr (!PAIR) __syncthreads();  // (every wave is done with V)
   float* turn_s = (float*)s_v + w * 4 * RD;
 #pragma unroll
@@ -1185,7 +1191,8 @@ __global__ __launch_bounds__(HD / 4) void attn8_tile_merge_kernel(Args a) {
 bool step_fits(const g4_kv8_params& p) {
   return (uint64_t)p.max_rows * (p.num_q_heads / p.num_kv_heads) <= COLS;
 }
-// Units a sequence may have (a window of several rows spans max_rows - 1 more positions, and up to 15 of its first tile).
+// Units a sequence may have (a window of several rows spans max_rows - 1 more positions, and up to 15 of its first
+// tile).
 uint64_t most_units(const g4_kv8_params& p) {
   uint64_t span = p.max_seq_len;
   if (p.sliding_window) span = std::min<uint64_t>(span, (uint64_t)p.sliding_window + p.max_rows - 1 + 15);
@@ -1209,7 +1216,8 @@ uint32_t tiles_of(const g4_kv8_params& p) {
 }
 uint64_t all_cost(const g4_kv8_params& p) {
   const uint64_t G = p.num_q_heads / p.num_kv_heads, rows = TC / G + 2;  // of a tile
-  const uint64_t tiles = std::min<uint64_t>(ceil_div(p.num_rows * G, TC) + p.num_seqs, (uint64_t)tiles_of(p) * p.num_seqs);
+  const uint64_t tiles =
+      std::min<uint64_t>(ceil_div(p.num_rows * G, TC) + p.num_seqs, (uint64_t)tiles_of(p) * p.num_seqs);
   uint64_t span = p.max_seq_len;
   if (p.sliding_window) span = std::min<uint64_t>(span, p.sliding_window + rows + 15);
   return tiles * p.num_kv_heads * (kTileCost + ceil_div(span, TP));
@@ -1305,7 +1313,8 @@ int g4_pagedAttn8Ops(g4_ctx* ctx, const float* q, const int8_t* k_pool, const in
   rc = g4_pagedAttn8_workspace_size(p, &need);
   if (rc) return rc;
   G4_REQUIRE(workspace_bytes >= need, "g4_pagedAttn8: workspace %zu bytes < %zu required", workspace_bytes, need);
-  G4_REQUIRE((((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)output | (uintptr_t)workspace) & 15) == 0,
+  const uintptr_t all = (uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)output | (uintptr_t)workspace;
+  G4_REQUIRE((all & 15) == 0,
              "g4_pagedAttn8: rows, pools and workspace must be 16-byte aligned");
   G4_REQUIRE(!ops || (p.head_dim % 256 == 0 && p.num_rows <= 64 && step_fits(p) && ((uintptr_t)ops & 15) == 0),
              "g4_pagedAttn8Ops: operand blocks need head_dim a multiple of 256, <= 64 rows, <= 16 rows x heads of a "
@@ -1315,7 +1324,8 @@ int g4_pagedAttn8Ops(g4_ctx* ctx, const float* q, const int8_t* k_pool, const in
   const Args a{q, k_pool, v_pool, k_scale, v_scale, page_table,
                {seq_lens, row_starts, p.num_seqs, p.num_rows, p.max_rows, p.max_seq_len},
                p.num_q_heads, p.num_kv_heads, G, magic(G), G == 1 ? ~0u : 0u, tiles, magic(tiles),
-               tiles == 1 ? ~0u : 0u, p.max_pages, p.num_pages, p.sliding_window, p.scale, output, 0, nullptr, nullptr, 0, (uint8_t*)ops, (int)(g4d::pad_batch(p.num_rows) / 16)};
+               tiles == 1 ? ~0u : 0u, p.max_pages, p.num_pages, p.sliding_window, p.scale, output,
+               0, nullptr, nullptr, 0, (uint8_t*)ops, (int)(g4d::pad_batch(p.num_rows) / 16)};
   switch (p.head_dim) {
     case 64: return attend<64>(ctx, p, a, workspace);
     case 128: return attend<128>(ctx, p, a, workspace);

@@ -22,7 +22,7 @@
 // launch finds in no cache: 27 KB of code (loops unrolled, the rotation without a
 // table in line, library square root, division and frexp, maxima in f64 through
 // LDS) took 8.3 us for 64 sequences, the same steps in 8 KB 4.0. A prompt of 1900
-// rows at head dim 512 (its 35 MB at the copy rate: 8 us) takes 18.
+// rows at head dim 512 (72 MB, 15 us at a copy's rate) takes 18.7.
 #include "kv8.hpp"
 #include "mqf_core.hpp"
 
@@ -143,7 +143,8 @@ __device__ __forceinline__ void q_row(const ProArgs& a, uint32_t block) {
   load_weights<HD>(a.q_w, lane, w);
   float lo[QH][PP], hi[QH][PP];
 #pragma unroll
-  for (int h = 0; h < QH; ++h) load_row<HD>(a.q + at + min((uint32_t)h, a.nqh - 1 - h0) * HD, stride, a.nparts, lane, lo[h], hi[h]);
+  for (int h = 0; h < QH; ++h)
+    load_row<HD>(a.q + at + min((uint32_t)h, a.nqh - 1 - h0) * HD, stride, a.nparts, lane, lo[h], hi[h]);
   const uint32_t s = seq_of_row(a.rows, row);
   if (s >= a.rows.num_seqs) return;
   const Seq q = seq_rows(a.rows, s);
@@ -474,7 +475,8 @@ int g4_pagedAttnPrologue8(g4_ctx* ctx, const float* q_parts, const float* k_part
   a.seq_pages = ceil_div(p.max_rows - 1, p.page_size) + 1;
   const Shape s = shape_of(p);
   const uint64_t kv_blocks = kv ? 2ull * p.num_seqs * a.seq_pages * p.num_kv_heads : 0ull;
-  const uint64_t blocks = kv_blocks + (q ? ceil_div((uint64_t)p.num_rows * ceil_div(p.num_q_heads, s.heads), s.threads / 64) : 0);
+  const uint64_t q_waves = q ? (uint64_t)p.num_rows * ceil_div(p.num_q_heads, s.heads) : 0ull;
+  const uint64_t blocks = kv_blocks + ceil_div(q_waves, s.threads / 64);
   G4_REQUIRE(blocks < (1ull << 32) / s.threads,
              "g4_pagedAttnPrologue8: %u sequences of up to %u rows of %u and %u heads in one call", p.num_seqs,
              p.max_rows, p.num_q_heads, p.num_kv_heads);
@@ -506,9 +508,10 @@ int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const 
   int rc = g4_internal_kv8_check(__func__, p, nullptr);
   if (rc) return rc;
   G4_REQUIRE(count > 0 && count < (1ull << 32) / VT, "g4_kv8Values: %u pages", count);
-  const ValArgs a{{k_pool, v_pool}, {k_scale, v_scale}, {k_out, v_out}, pages, page_size, num_kv_heads, head_dim, num_pages};
-  hipLaunchKernelGGL(kv8_values_kernel, dim3(count, ceil_div((uint64_t)page_size * num_kv_heads * head_dim, 16 * VT), 2),
-                     dim3(VT), 0, ctx->stream, a);
+  const ValArgs a{{k_pool, v_pool}, {k_scale, v_scale}, {k_out, v_out}, pages, page_size, num_kv_heads, head_dim,
+                  num_pages};
+  const dim3 grid(count, ceil_div((uint64_t)page_size * num_kv_heads * head_dim, 16 * VT), 2);
+  hipLaunchKernelGGL(kv8_values_kernel, grid, dim3(VT), 0, ctx->stream, a);
   G4_LAUNCHED(ctx, "kv8_values");
   return G4_OK;
 }

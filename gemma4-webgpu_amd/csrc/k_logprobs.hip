@@ -216,7 +216,8 @@ __global__ __launch_bounds__(NT) void logprobs_chunk_kernel(Args a) {
       if (who) {
         uint32_t at = 0;
         if (l == 0) at = atomicAdd(&s_n, (uint32_t)__popcll(who));
-        at = __builtin_amdgcn_readfirstlane(at) + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+        const uint32_t below = __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0);
+        at = __builtin_amdgcn_readfirstlane(at) + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), below);
         if (in && at < CAP) s_list[at] = make_top(v[e], index(e));
       }
     }

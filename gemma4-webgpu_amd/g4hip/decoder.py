@@ -843,8 +843,8 @@ class BatchDecoder(_SyntheticModel):
 
     def __init__(self, ctx: Context, context_lens, shape: Optional[E2BShape] = None, page_size: int = 16,
                  reserve: int = 64, seed: int = 0, n_layers: Optional[int] = None, lm_head: bool = True,
-                 page_seed: int = 7, shared_pages: bool = False, embed: bool = False, wtypes=None, gguf=None, kv: str = "f16",
-                 logprobs: Optional[int] = None):
+                 page_seed: int = 7, shared_pages: bool = False, embed: bool = False, wtypes=None, gguf=None,
+                 kv: str = "f16", logprobs: Optional[int] = None):
         """shared_pages: every row reads and appends through one page list
         (the rows are tokens of one sequence: batched prefill). embed: an f16
         token table; each step starts from the embedding of every row's

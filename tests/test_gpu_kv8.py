@@ -581,7 +581,8 @@ def test_step_prompt_and_replays_together(ctx):
         c.lens += 1
         for s, L in enumerate(c.lens):
             cs = host_table[L - 1:L]
-            c.k.append(K8.rotated(K8.normed(k[0, s:s + 1], (kw * np.float16(0.1)).astype(np.float16)), cs), c.table[s], L - 1)
+            kn = K8.normed(k[0, s:s + 1], (kw * np.float16(0.1)).astype(np.float16))
+            c.k.append(K8.rotated(kn, cs), c.table[s], L - 1)
             c.v.append(K8.normed(v[0, s:s + 1]), c.table[s], L - 1)
         c.q = qo.download(np.float32).reshape(2, 8, 256)
         c.check_attention(out.download(np.float32).reshape(2, 8, 256), what=step)
