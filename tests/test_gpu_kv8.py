@@ -171,6 +171,18 @@ def test_prologue(ctx, lens, rows, nqh, nkh, hd, ps, parts, with_table):
     prologue(c, q, k, v, table, qw, kw)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("rows,ps", [(1, 16), (3, 16), (4, 64), (5, 16), (40, 16), (70, 64), (130, 128)])
+@pytest.mark.parametrize("with_table", [False, True])
+def test_prologue_of_each_launch(ctx, hd, rows, ps, with_table):
+    """Few rows, many rows of small pages and of large ones, at each head dim; rows that begin within a page and end
+    in another, a sequence of one row and one of none beside them."""
+    nqh, nkh = (6, 2) if hd == 64 else (8, 1)
+    c = Case(ctx, [3 * ps + rows // 2 + 1, 7, 2 * ps, rows], [rows, 1, 0, rows], nqh, nkh, hd, ps, 13, parts=5).up()
+    q, k, v, qw, kw = projections(c, 14)
+    prologue(c, q, k, v, table_of(ctx, hd, c.p.max_seq_len)[0] if with_table else None, qw, kw)
+
+
 def test_prologue_q_alone_and_kv_alone(ctx):
     c = Case(ctx, [20, 9], [3, 9], 8, 2, 128, 16, 21).up()
     q, k, v, qw, kw = projections(c, 22)
@@ -339,6 +351,15 @@ def test_attention_of_a_long_cache(ctx, rows):
     got = c.attention()
     total = int(c.n.sum())
     c.check_attention(got, sorted({0, rows // 2, rows - 1, total - 1}))
+
+
+@pytest.mark.parametrize("hd,nkh", [(64, 2), (128, 1), (512, 1)])
+@pytest.mark.parametrize("rows", [1, 20])
+def test_attention_of_a_long_cache_at_each_head_dim(ctx, rows, hd, nkh):
+    """More than 32 workgroups of one sequence; more than one round of a tile's pages."""
+    c = Case(ctx, [9003, 31], [rows, 1], 8 * nkh, nkh, hd, 48, 92).up()
+    got = c.attention()
+    c.check_attention(got, sorted({0, rows // 2, rows - 1, rows}))
 
 
 @pytest.mark.parametrize("rows", [1, 20])
