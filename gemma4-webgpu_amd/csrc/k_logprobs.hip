@@ -342,8 +342,9 @@ __global__ __launch_bounds__(NT) void logprobs_row_kernel(Args a) {
   }
 }
 
-// Values a thread: 32, or 8 where 32 would leave the launch with less than two
-// workgroups per CU.
+// Values a thread: 32 (64 rows of 262144 22.2 us; 16 values 25.8, 24 23.5, 48 22.5,
+// 64 22.1), or 8 where 32 would leave the launch with less than two workgroups per
+// CU (one row 9.5 us, with 32 9.8).
 uint32_t chunks_of(uint32_t size, uint32_t e) { return ceil_div(size, NT * e); }
 uint32_t pick_e(uint32_t size, uint32_t batch) { return (uint64_t)chunks_of(size, 32) * batch >= 512 ? 32 : 8; }
 
