@@ -346,7 +346,14 @@ __global__ __launch_bounds__(NT) void logprobs_row_kernel(Args a) {
 // 64 22.1), or 8 where 32 would leave the launch with less than two workgroups per
 // CU (one row 9.5 us, with 32 9.8).
 uint32_t chunks_of(uint32_t size, uint32_t e) { return ceil_div(size, NT * e); }
-uint32_t pick_e(uint32_t size, uint32_t batch) { return (uint64_t)chunks_of(size, 32) * batch >= 512 ? 32 : 8; }
+constexpr uint32_t kManyChunks = 512;
+uint32_t pick_e(uint32_t size, uint32_t batch) { return (uint64_t)chunks_of(size, 32) * batch >= kManyChunks ? 32 : 8; }
+// Chunks of the batch or of any smaller one, whichever has most: the most rows that take 8 values a thread may have
+// more of them than the batch, whose workspace serves those calls too.
+size_t most_chunks(uint32_t size, uint32_t batch) {
+  const uint32_t few = std::min(batch, (kManyChunks - 1) / chunks_of(size, 32));
+  return std::max((size_t)batch * chunks_of(size, pick_e(size, batch)), (size_t)few * chunks_of(size, 8));
+}
 
 int check_shape(uint32_t size, uint32_t batch, uint32_t ntop) {
   G4_REQUIRE(size > 0 && size <= (1u << 28) && batch > 0 && batch <= 65535 && ntop <= 64 && ntop <= size,
@@ -363,7 +370,7 @@ int g4_logprobsBatch_workspace_size(uint32_t size, uint32_t batch, uint32_t ntop
   G4_REQUIRE(bytes, "g4_logprobsBatch_workspace_size: null out");
   int rc = check_shape(size, batch, ntop);
   if (rc) return rc;
-  *bytes = (size_t)batch * chunks_of(size, pick_e(size, batch)) * (sizeof(Stat) + ntop * sizeof(Top));
+  *bytes = most_chunks(size, batch) * (sizeof(Stat) + ntop * sizeof(Top));
   return G4_OK;
 }
 

@@ -859,8 +859,8 @@ int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const 
  * A row with a NaN or +Inf, or of nothing but -Inf, has NaN for every
  * probability; its ids are as stated. tokens and logprobs may be NULL together,
  * entropy alone; ntop 0 takes no top buffers. workspace:
- * g4_logprobsBatch_workspace_size bytes, 16-byte aligned, of any content; calls
- * sharing it must not overlap. */
+ * g4_logprobsBatch_workspace_size bytes, 16-byte aligned, of any content, which
+ * serve any smaller batch, too; calls sharing it must not overlap. */
 int g4_logprobsBatch_workspace_size(uint32_t size, uint32_t batch, uint32_t ntop, size_t* bytes);
 int g4_logprobsBatch(g4_ctx* ctx, const float* logits, const uint32_t* tokens, uint32_t size, uint32_t batch,
                      float* logprobs, float* entropy, uint32_t ntop, uint32_t* top_ids, float* top_logprobs,

@@ -234,3 +234,22 @@ def test_refusals(ctx):
     assert d.prefill([1, 2, 3]) == 2
     with pytest.raises(ValueError):
         d.step()
+
+
+def test_fewer_rows_than_the_decoder_has_at_a_large_vocabulary(ctx):
+    """A short prompt and a text's last rows take the log probabilities of fewer rows, whose launch holds fewer values
+    a thread and leaves more partials a row."""
+    s = E2BShape.real(n_layers=2, n_unshared=1, global_layers=(1,), vocab=128256)
+    d = BatchDecoder(ctx, [0] * 40, s, seed=91, reserve=160, shared_pages=True, embed=True, kv="int8", logprobs=4)
+    d.fill_kv(seed=92)
+    toks = np.random.default_rng(93).integers(0, s.vocab, 61).astype(np.uint32)
+    for T in (12, 25):  # 16 and 32 rows of the 40
+        assert d.prefill(toks[:T]) == T - 1
+        check_logprobs(d, range(40))
+    got = d.score(toks, 3)
+    assert got.shape == (60,)
+    last = d.logits.download(np.float32).reshape(40, -1)[:20]  # what the second pass left
+    d.prefill(toks[:40], 3)
+    for i, x in enumerate(np.concatenate([d.logits.download(np.float32).reshape(40, -1), last])):
+        ref = K8.logprobs(x, int(toks[i + 1]), 0)[0]
+        assert abs(got[i] - ref) <= 8 * U * (abs(float(x[toks[i + 1]]) - float(x.max())) + np.log(x.size) + 1), i

@@ -45,3 +45,14 @@ def test_a_pool_of_too_many_positions_is_refused():
     big = dict(page_size=1024, max_seq_len=1024, max_pages=1)
     assert size(num_pages=(1 << 26) - 1, **big)[0] == 0
     assert size(num_pages=1 << 26, **big)[0] == -1
+
+
+@pytest.mark.parametrize("ntop", [0, 5, 64])
+@pytest.mark.parametrize("vocab", [64, 4096, 32003, 100003, 128256, 262144])
+def test_a_logprobs_workspace_serves_fewer_rows(vocab, ntop):
+    """A decoder sizes it for all its rows; a short prompt and a text's last rows are fewer."""
+    f, n, most = _lib.lib().g4_logprobsBatch_workspace_size, ctypes.c_size_t(), 0
+    for rows in [*range(1, 70), 127, 128, 500, 511, 512, 513, 2000, 65535]:
+        assert f(vocab, rows, ntop, ctypes.byref(n)) == 0
+        assert n.value >= most, (rows, n.value, most)
+        most = n.value
