@@ -239,7 +239,7 @@ def test_refusals(ctx):
 def test_fewer_rows_than_the_decoder_has_at_a_large_vocabulary(ctx):
     """A short prompt and a text's last rows take the log probabilities of fewer rows, whose launch holds fewer values
     a thread and leaves more partials a row."""
-    s = E2BShape.real(n_layers=2, n_unshared=1, global_layers=(1,), vocab=128256)
+    s = E2BShape.real(n_layers=4, n_unshared=2, global_layers=(1, 3), vocab=128256)
     d = BatchDecoder(ctx, [0] * 40, s, seed=91, reserve=160, shared_pages=True, embed=True, kv="int8", logprobs=4)
     d.fill_kv(seed=92)
     toks = np.random.default_rng(93).integers(0, s.vocab, 61).astype(np.uint32)
