@@ -1284,10 +1284,12 @@ class BatchDecoder(_SyntheticModel):
         dtok, dpos = self.ctx.from_numpy(ctok), self.ctx.from_numpy(cpos)
         # a single chunk takes only as many rows as its matrix-core tiles need
         rows = next((r for r in (16, 32) if T <= r < B), B) if nch == 1 and probe is None else B
-        for k in range(nch):
-            self._place_chunk(dtok, dpos, cpos, k, T, start)
-            self.step(sample, probe=probe, head=k == nch - 1, rows=rows)
-        self.span_rows = 0
+        try:
+            for k in range(nch):
+                self._place_chunk(dtok, dpos, cpos, k, T, start)
+                self.step(sample, probe=probe, head=k == nch - 1, rows=rows)
+        finally:
+            self.span_rows = 0
         if rows < B:  # the rows left out: the last token's again, as in a step over all B
             outs = [(self.hidden, self.s.hidden)]
             if self.lm_head is not None:
@@ -1334,13 +1336,15 @@ class BatchDecoder(_SyntheticModel):
         dtok, dpos, want = c.from_numpy(ctok), c.from_numpy(cpos), c.from_numpy(toks[1:])
         out = c.empty(n, np.float32)
         ws = c.alloc(c.logprobs_workspace_bytes(s.vocab, B, 0))
-        for k in range(nch):
-            self._place_chunk(dtok, dpos, cpos, k, n, start)
-            self.step()
-            rows = min(n - B * k, B)
-            c.logprobsBatch(self.logits, want.offset(4 * B * k), s.vocab, rows, out.offset(4 * B * k), None, 0, None,
-                            None, ws)
-        self.span_rows = 0
+        try:
+            for k in range(nch):
+                self._place_chunk(dtok, dpos, cpos, k, n, start)
+                self.step()
+                rows = min(n - B * k, B)
+                c.logprobsBatch(self.logits, want.offset(4 * B * k), s.vocab, rows, out.offset(4 * B * k), None, 0,
+                                None, None, ws)
+        finally:
+            self.span_rows = 0
         got = out.download(np.float32)
         for b in (dtok, dpos, want, out, ws):
             b.free()
@@ -1420,12 +1424,14 @@ class BatchDecoder(_SyntheticModel):
         clen = (np.concatenate([np.arange(T), np.repeat(T - 1, pad)]) + start + 1).astype(np.uint32)
         dtok, dlen = c.from_numpy(ctok), c.from_numpy(clen)
         n = 0
-        for at in range(0, T + pad, self.wide_rows):
-            n = min(self.wide_rows, T + pad - at)
-            if self.kv8:
-                self._place_span(start + min(T, at + n), min(T - at, n))
-            self._wide_pass(dtok.offset(4 * at), dlen.offset(4 * at), n, int(clen[at:at + n].max()))
-        self.span_rows = 0
+        try:
+            for at in range(0, T + pad, self.wide_rows):
+                n = min(self.wide_rows, T + pad - at)
+                if self.kv8:
+                    self._place_span(start + min(T, at + n), min(T - at, n))
+                self._wide_pass(dtok.offset(4 * at), dlen.offset(4 * at), n, int(clen[at:at + n].max()))
+        finally:
+            self.span_rows = 0
         # the last B rows are what the last chunk of B rows leaves: the residual
         # stream, its tokens and lengths, then the head and the sample
         c.copy(self.hidden, w["hidden"].offset(4 * H * (n - B)), 4 * H * B)
