@@ -1282,11 +1282,12 @@ class BatchDecoder(_SyntheticModel):
         ctok = np.concatenate([toks, np.repeat(toks[-1], pad)]).astype(np.uint32)
         cpos = np.concatenate([start + np.arange(T), np.repeat(start + T - 1, pad)]).astype(np.uint32)
         dtok, dpos = self.ctx.from_numpy(ctok), self.ctx.from_numpy(cpos)
+        spans = self._spans(T, start, B)
         # a single chunk takes only as many rows as its matrix-core tiles need
         rows = next((r for r in (16, 32) if T <= r < B), B) if nch == 1 and probe is None else B
         try:
             for k in range(nch):
-                self._place_chunk(dtok, dpos, cpos, k, T, start)
+                self._place_chunk(dtok, dpos, cpos, k, spans)
                 self.step(sample, probe=probe, head=k == nch - 1, rows=rows)
         finally:
             self.span_rows = 0
@@ -1304,19 +1305,30 @@ class BatchDecoder(_SyntheticModel):
         dpos.free()
         return n - 1
 
-    def _place_chunk(self, dtok, dpos, cpos, k: int, T: int, start: int) -> None:
-        """Chunk k of a prompt of T tokens from position `start`: its tokens and its rows' lengths, as the step
-        expects them, from the prompt's (8-bit pages: the sequence's length after the chunk and its rows)."""
+    def _place_chunk(self, dtok, dpos, cpos, k: int, spans) -> None:
+        """Chunk k of a prompt, from the prompt's: its tokens and its rows' lengths, as the step expects them, and
+        over 8-bit pages its span."""
         c, B = self.ctx, self.B
         c.copy(self.tokens, dtok.offset(4 * B * k), 4 * B)
         c.copy(self.seq_lens, dpos.offset(4 * B * k), 4 * B)
         self.lens_host = cpos[B * k:B * (k + 1)].copy()
-        if self.kv8:
-            self._place_span(start + min(T, B * (k + 1)), min(T - B * k, B))
+        self._place_span(spans, k)
 
-    def _place_span(self, end: int, rows: int) -> None:
-        self.span.upload(np.array([end, 0, rows], np.uint32))
-        self.span_rows = rows
+    def _spans(self, T: int, start: int, rows: int):
+        """8-bit pages: the spans of a prompt of T tokens from position `start` that takes the layers `rows` at a
+        time, uploaded at once (an upload waits for the stream): per pass the sequence's length after it and the
+        first and past-the-last row that are its."""
+        if not self.kv8:
+            return None
+        first = np.arange(0, T, rows)
+        own = np.minimum(T - first, rows)
+        spans = np.stack([start + first + own, np.zeros_like(own), own], 1).astype(np.uint32)
+        return self.ctx.from_numpy(spans), own
+
+    def _place_span(self, spans, k: int) -> None:
+        if spans is not None:
+            self.ctx.copy(self.span, spans[0].offset(12 * k), 12)
+            self.span_rows = int(spans[1][k])
 
     def score(self, tokens, start: int = 0) -> np.ndarray:
         """The log probability of each token but the first under the model, given those before it (a
@@ -1334,11 +1346,12 @@ class BatchDecoder(_SyntheticModel):
         ctok = np.concatenate([toks[:n], np.repeat(toks[n - 1], pad)]).astype(np.uint32)
         cpos = np.concatenate([start + np.arange(n), np.repeat(start + n - 1, pad)]).astype(np.uint32)
         dtok, dpos, want = c.from_numpy(ctok), c.from_numpy(cpos), c.from_numpy(toks[1:])
+        spans = self._spans(n, start, B)
         out = c.empty(n, np.float32)
         ws = c.alloc(c.logprobs_workspace_bytes(s.vocab, B, 0))
         try:
             for k in range(nch):
-                self._place_chunk(dtok, dpos, cpos, k, n, start)
+                self._place_chunk(dtok, dpos, cpos, k, spans)
                 self.step()
                 rows = min(n - B * k, B)
                 c.logprobsBatch(self.logits, want.offset(4 * B * k), s.vocab, rows, out.offset(4 * B * k), None, 0,
@@ -1423,12 +1436,12 @@ class BatchDecoder(_SyntheticModel):
         ctok = np.concatenate([toks, np.repeat(toks[-1], pad)]).astype(np.uint32)
         clen = (np.concatenate([np.arange(T), np.repeat(T - 1, pad)]) + start + 1).astype(np.uint32)
         dtok, dlen = c.from_numpy(ctok), c.from_numpy(clen)
+        spans = self._spans(T, start, self.wide_rows)
         n = 0
         try:
             for at in range(0, T + pad, self.wide_rows):
                 n = min(self.wide_rows, T + pad - at)
-                if self.kv8:
-                    self._place_span(start + min(T, at + n), min(T - at, n))
+                self._place_span(spans, at // self.wide_rows)
                 self._wide_pass(dtok.offset(4 * at), dlen.offset(4 * at), n, int(clen[at:at + n].max()))
         finally:
             self.span_rows = 0

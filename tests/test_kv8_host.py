@@ -125,3 +125,11 @@ def test_a_step_that_fails_leaves_no_rows_placed(wide_rows, call):
     assert d.span_rows == 0
     with pytest.raises(ValueError, match="shared pages"):
         BatchDecoder.step(d)
+
+
+@pytest.mark.parametrize("wide_rows,call", CALLS, ids=NAMES)
+def test_no_wait_between_steps(wide_rows, call):
+    """What places the steps goes up before the first; they run back to back, as over f16 pages."""
+    d = decoder(wide_rows=wide_rows)
+    call(d)
+    assert len(d.seen) == 3 and len({x[4] for x in d.seen}) == 1, [x[4] for x in d.seen]
