@@ -1026,7 +1026,7 @@ class BatchDecoder(_SyntheticModel):
     def _attn8_workspace(self, params) -> None:
         need = max(self.ctx.attn8_workspace_bytes(p) for p in params)
         if need > self.attn8_cap:
-            self.attn8_ws = None  # (the old one is given back first)
+            self.attn8_ws, self.attn8_cap = None, 0  # (the old one is given back first)
             self.attn8_ws, self.attn8_cap = self.ctx.alloc(need), need
 
     def _attend8(self, il: int, q_parts, k_parts, v_parts, nq: int, q, out, p, ops=None) -> None:

@@ -133,3 +133,21 @@ def test_no_wait_between_steps(wide_rows, call):
     d = decoder(wide_rows=wide_rows)
     call(d)
     assert len(d.seen) == 3 and len({x[4] for x in d.seen}) == 1, [x[4] for x in d.seen]
+
+
+def test_a_workspace_that_could_not_grow_is_asked_for_again():
+    """The old one is given back before the larger one is asked for; without either, the next call gets its own."""
+    d, sizes, asked = decoder(), {"long": 100, "short": 40}, []
+    d.attn8_ws, d.attn8_cap = d.ctx.alloc(60), 60
+
+    def alloc(n):
+        asked.append(n)
+        if n == 100:
+            raise MemoryError
+        return Buf(d.ctx, np.zeros(n, np.uint8))
+
+    d.ctx.alloc, d.ctx.attn8_workspace_bytes = alloc, sizes.get
+    with pytest.raises(MemoryError):
+        d._attn8_workspace(["long"])
+    d._attn8_workspace(["short"])
+    assert asked == [100, 40] and d.attn8_ws.nbytes == d.attn8_cap == 40
