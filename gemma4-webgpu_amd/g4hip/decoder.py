@@ -852,11 +852,15 @@ class BatchDecoder(_SyntheticModel):
         "f16" or "int8" pages (8-bit codes with a scale per page and KV head,
         half the pool's bytes; page_size a multiple of 16). logprobs: a step
         that samples leaves every row's token_logprobs (of its argmax),
-        entropy and this many alternatives (top_ids, top_logprobs [B][n])."""
+        entropy and this many alternatives, at most 64 (top_ids, top_logprobs
+        [B][n]); a top-k 256 step, whose token the host draws, leaves
+        token_logprobs as they were."""
         if kv not in ("f16", "int8"):
             raise ValueError(f"kv {kv!r}: f16 or int8")
         if logprobs is not None and not lm_head:
             raise ValueError("logprobs need the LM head")
+        if logprobs is not None and not 0 <= logprobs <= 64:
+            raise ValueError(f"logprobs {logprobs}: 0..64 alternatives")
         lens = np.asarray(context_lens, dtype=np.int64)
         if lens.ndim != 1 or lens.size == 0 or lens.size > 64 or np.any(lens < 0):
             raise ValueError("context_lens: 1..64 non-negative lengths")

@@ -151,3 +151,10 @@ def test_a_workspace_that_could_not_grow_is_asked_for_again():
         d._attn8_workspace(["long"])
     d._attn8_workspace(["short"])
     assert asked == [100, 40] and d.attn8_ws.nbytes == d.attn8_cap == 40
+
+
+@pytest.mark.parametrize("n", [-1, 65])
+def test_alternatives_that_no_call_gives_are_refused(n):
+    """Before anything is allocated for them."""
+    with pytest.raises(ValueError, match="logprobs"):
+        BatchDecoder(None, [3], kv="int8", logprobs=n)
