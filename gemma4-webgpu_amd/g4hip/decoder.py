@@ -1266,7 +1266,7 @@ class BatchDecoder(_SyntheticModel):
             raise ValueError("prefill needs a shared_pages decoder with an embedding table")
         toks = np.asarray(tokens, np.uint32)
         T, B = int(toks.size), self.B
-        if T == 0 or start + T > self.max_seq - 1:
+        if T == 0 or start < 0 or start + T > self.max_seq - 1:
             raise ValueError(f"prefill: {T} tokens from {start} do not fit {self.max_seq} positions")
         nch = -(-T // B)
         n = T - (nch - 1) * B
@@ -1342,7 +1342,7 @@ class BatchDecoder(_SyntheticModel):
             raise ValueError("score needs a shared_pages decoder with an embedding table and the LM head")
         toks = np.asarray(tokens, np.uint32)
         T, B, c, s = int(toks.size), self.B, self.ctx, self.s
-        if T < 2 or start + T > self.max_seq - 1:
+        if T < 2 or start < 0 or start + T > self.max_seq - 1:
             raise ValueError(f"score: {T} tokens from {start}: two or more within {self.max_seq} positions")
         n = T - 1  # the last token is only asked for
         nch = -(-n // B)

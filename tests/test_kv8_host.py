@@ -158,3 +158,16 @@ def test_alternatives_that_no_call_gives_are_refused(n):
     """Before anything is allocated for them."""
     with pytest.raises(ValueError, match="logprobs"):
         BatchDecoder(None, [3], kv="int8", logprobs=n)
+
+
+@pytest.mark.parametrize("wide_rows,call", [(0, lambda d: d.prefill(np.arange(11), -3)),
+                                            (8, lambda d: d.prefill(np.arange(19), -1)),
+                                            (0, lambda d: d.score(np.arange(11), -3))], ids=NAMES)
+def test_positions_before_the_first_are_refused(wide_rows, call):
+    d = decoder(wide_rows=wide_rows)
+    with pytest.raises(ValueError, match="from -"):
+        call(d)
+    d.kv8 = False
+    with pytest.raises(ValueError, match="from -"):
+        call(d)
+    assert not d.seen
