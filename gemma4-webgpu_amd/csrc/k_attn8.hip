@@ -682,22 +682,36 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn8_ti
   __shared__ __align__(16) float s_ks[4 * CH], s_vs[4 * CH];
   __shared__ float s_big[2];
   __shared__ uint32_t s_upto[S_::NTH + 1], s_sum[S_::NTH / 64], s_at[2];  // s_upto: units before each thread's run
+  __shared__ float s_all[S_::NTH / 64];
   const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), qd = l >> 4, c = l & 15;
   const int wc = w & 3, wd = PAIR ? w >> 2 : 0;  // column tile; half
 
   // ---- this workgroup's share of the whole cost: a run of column tiles a thread, summed up ----
   const uint32_t wg = blockIdx.x, pairs = a.rows.num_seqs * a.tiles, run = (pairs + S_::NTH - 1) / S_::NTH;
   const uint32_t j0 = min(tid * run, pairs), j1 = min(j0 + run, pairs);
-  uint32_t mine = 0;
-  for (uint32_t j = j0; j < j1; ++j) mine += cost_of(a, j) * a.nkh;
-  uint32_t upto = wave_scan(mine);
-  if (l == 63) s_sum[w] = upto;
+  uint64_t mine = 0;
+  for (uint32_t j = j0; j < j1; ++j) mine += (uint64_t)cost_of(a, j) * a.nkh;
+  uint32_t upto = wave_scan((uint32_t)mine);
+  const float wave_all = g4d::wave_sum_dpp((float)mine);
+  if (l == 63) {
+    s_sum[w] = upto;
+    s_all[w] = wave_all;
+  }
   __syncthreads();
   uint32_t total = 0;
+  float all = 0.f;
 #pragma unroll
   for (int i = 0; i < S_::NTH / 64; ++i) {
     if (i < w) upto += s_sum[i];
     total += s_sum[i];
+    all += s_all[i];
+  }
+  // Rows that are one sequence's each cost less than 2^31 (checked by the host). Starts that descend in between may
+  // give rows to many sequences, past what 32 bits number: nothing is written then, and nothing added up.
+  if (all > 3e9f) {  // (uniform)
+    for (uint64_t i = (uint64_t)wg * S_::NTH + tid; i < (uint64_t)pairs * a.nkh; i += (uint64_t)gridDim.x * S_::NTH)
+      a.meta[i] = make_uint2(0, 0);
+    return;
   }
   total = uni(total);
   s_upto[tid + 1] = upto;

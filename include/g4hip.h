@@ -788,7 +788,10 @@ int g4_prefillAttn(g4_ctx* ctx, const float* q, const uint16_t* k_pool, const ui
  * rows (a step advances it first), so with n rows its row i is position
  * seq_lens[s] - n + i. Rows outside every sequence are left as they are, as
  * are those of a sequence whose starts descend, pass num_rows or hold more
- * than max_rows rows. A sequence shorter than its rows or longer than
+ * than max_rows rows (a row that starts which descend give to several
+ * sequences is any one's; where so many share rows that the attention would
+ * have 3 * 10^9 steps of 64 positions or more, it writes nothing). A sequence
+ * shorter than its rows or longer than
  * max_seq_len appends nothing, its q_out is not written and its attention
  * output is 0. Page ids outside [0, num_pages) store nothing and are clamped
  * when read, as in the f16 pool.

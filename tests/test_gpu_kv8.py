@@ -654,3 +654,18 @@ def test_operand_blocks_that_are_refused(ctx):
                                      num_pages=9), **change})
         with pytest.raises(g4hip.G4Error):
             ctx.pagedAttn8(b, b, b, b, b, b, b, b, p, ws, row_starts=b if p.num_rows != p.num_seqs else None, ops=ops)
+
+
+def test_starts_that_give_rows_to_many_sequences(ctx):
+    """Every other sequence's starts descend, the others hold all rows each: 1024 x 4096 tiles of some 1900 steps are
+    more than 32 bits number. Nothing is written, and every wait ends."""
+    S, rows, hd, top = 2048, 16384, 64, 1 << 17
+    p = ctx.kv8_params(S, 16, 1, hd, 1024, top // 1024, top, 2, num_rows=rows, max_rows=rows)
+    assert S // 2 * (rows * 16 // 64) * ((top - rows) // 64) > 2 ** 32
+    pool, scale = ctx.zeros(2 * 1024 * hd, np.int8), ctx.from_numpy(np.ones(2, np.float32))
+    table, lens = ctx.zeros(S * (top // 1024), np.int32), ctx.from_numpy(np.full(S, top, np.uint32))
+    starts = ctx.from_numpy(np.where(np.arange(S + 1) % 2, rows, 0).astype(np.uint32))
+    q, out = ctx.zeros(rows * 16 * hd, np.float32), ctx.from_numpy(np.full(rows * 16 * hd, 7.5, np.float32))
+    ws = ctx.from_numpy(np.full(ctx.attn8_workspace_bytes(p), 0xff, np.uint8))
+    ctx.pagedAttn8(q, pool, pool, scale, scale, table, lens, out, p, ws, row_starts=starts)
+    assert np.all(out.download(np.float32) == 7.5)
