@@ -669,3 +669,81 @@ def test_starts_that_give_rows_to_many_sequences(ctx):
     ws = ctx.from_numpy(np.full(ctx.attn8_workspace_bytes(p), 0xff, np.uint8))
     ctx.pagedAttn8(q, pool, pool, scale, scale, table, lens, out, p, ws, row_starts=starts)
     assert np.all(out.download(np.float32) == 7.5)
+
+
+@pytest.mark.parametrize("hd,theta,divisor", [(64, 1e4, 1), (256, 1e6, 0), (512, 1e6, 1), (128, 5e5, 1)])
+def test_prologue_by_theta_and_divisor(ctx, hd, theta, divisor):
+    """Angles formed in the launch: of its theta, divided by the frequencies' table where it says so; the same bits as
+    from a table, and cos and sin within 2^-22 of the f32 angle's."""
+    c = Case(ctx, [61, 300], [9, 40], 8, 2, hd, 32, 181)
+    c.p.theta, c.p.apply_divisor = theta, divisor
+    rng = np.random.default_rng(182)
+    freqs = rng.choice(np.array([1, 2, 8, 0.5], np.float16), hd // 2)
+    n = c.p.max_seq_len
+    t, df = ctx.empty(n * hd, np.float32), ctx.from_numpy(freqs)
+    ctx.ropeTable(theta, divisor, df, hd, n, t)
+    f = (1.0 / np.float64(np.float32(theta)) ** (2.0 * np.arange(hd // 2) / hd)).astype(np.float32)
+    angle = np.arange(n, dtype=np.float32)[:, None] * (f / freqs.astype(np.float32) if divisor else f)
+    host = t.download(np.float32).reshape(n, hd // 2, 2)
+    # (theta^x by another library: an angle may be the next f32, 2^-23 of it)
+    tol = 2.0 ** -22 * (1 + np.abs(angle.astype(np.float64)))
+    for i, fn in enumerate((np.cos, np.sin)):
+        assert (np.abs(host[..., i] - fn(angle.astype(np.float64))) <= tol).all()
+    q, k, v, qw, kw = projections(c, 183)
+    runs = []
+    for table in (None, t):
+        c.up()
+        out = ctx.from_numpy(np.full(q[0].shape, 3.25, np.float32))
+        ctx.pagedAttnPrologue8(*(ctx.from_numpy(x) for x in (q, k, v)), 1, ctx.from_numpy(qw), ctx.from_numpy(kw), df,
+                               out, *c.cache, c.dt, c.dl, c.p, row_starts=c.ds, rope_cs=table,
+                               rope_rows=n if table else 0)
+        runs.append([out.download(np.uint32)] + [b.download(np.uint8) for b in c.cache])
+    assert all(np.array_equal(a, b) for a, b in zip(*runs))
+    got = runs[0][0].view(np.float32).reshape(q[0].shape)
+    for s in range(2):
+        a, m, L = int(c.starts[s]), int(c.n[s]), int(c.lens[s])
+        x = K8.normed(q[0, a:a + m].astype(np.float64), qw)
+        half = hd // 2
+        mag = np.tile(np.abs(x[..., :half]) + np.abs(x[..., half:]), 2)
+        assert (np.abs(got[a:a + m] - K8.rotated(x, host[L - m:L])) <= 11 * U * mag + 1e-30).all()
+        c.k.append(K8.rotated(K8.normed(k[0, a:a + m], kw), host[L - m:L]), c.table[s], L - m)
+        c.v.append(K8.normed(v[0, a:a + m]), c.table[s], L - m)
+    check_pools(c)
+
+
+@pytest.mark.parametrize("hd,ps", [(64, 256), (128, 1024), (256, 512), (512, 256), (512, 1024)])
+def test_large_pages(ctx, hd, ps):
+    """Pages of more rows than a workgroup keeps: begun, filled and left within; then steps and their attention."""
+    c = Case(ctx, [ps + 700, 300, 2 * ps + 1], [ps + 333, 1, 2], 4, 2, hd, ps, 191, parts=2).up()
+    q, k, v, qw, kw = projections(c, 192)
+    got = prologue(c, q, k, v, table_of(ctx, hd, c.p.max_seq_len)[0], qw, kw)
+    c.q = got * np.float32(0.1)
+    total = int(c.n.sum())
+    c.check_attention(c.attention(), sorted({0, 63, 64, ps - 1, total - 4, total - 3, total - 2, total - 1}))
+
+
+def test_rows_taken_back(ctx):
+    """Drafted rows whose length is set back: their page keeps the scale that they made grow, the codes before them
+    the rounding to it, the next rows are appended under it; a page that they began is begun again."""
+    c = Case(ctx, [21, 40], [5, 9], 4, 2, 128, 16, 201, max_len=64, spare=4)
+    free = [p for p in range(c.pages) if p not in c.table]
+    c.table[0, 2:4], c.table[1, 3] = free[:2], free[2]
+    c.up()
+    for step, (lens, spread) in enumerate([([21, 40], 1), ([24, 44], 9), ([23, 39], 1), ([28, 48], 1)]):
+        c.lens[:] = lens
+        c.dl.upload(c.lens.astype(np.uint32))
+        q, k, v, qw, kw = projections(c, 202 + step)
+        k[..., 3] *= spread  # a spike: the norm leaves a larger element
+        v[..., 5] *= spread
+        prologue(c, q, k, v, None, qw, kw)
+        c.check_attention(c.attention(), what=step)
+
+
+def test_steps_beside_a_prompt(ctx):
+    rng = np.random.default_rng(211)
+    lens, rows = rng.integers(1, 900, 65), np.ones(65, int)
+    lens[20], rows[20] = 420, 300
+    c = Case(ctx, lens, rows, 8, 1, 256, 16, 212, window=512).up()
+    got = c.attention()
+    total = int(c.n.sum())
+    c.check_attention(got, sorted({*range(0, 20), *range(20, 320, 29), 319, *range(320, total)}))

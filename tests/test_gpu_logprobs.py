@@ -159,3 +159,19 @@ def test_refusals(ctx):
                  (b, b, 10, 1, b, b, 1, b, b, ws.offset(4))):
         with pytest.raises(g4hip.G4Error):
             ctx.logprobsBatch(*args)
+
+
+@pytest.mark.parametrize("low", [-np.inf, np.finfo(np.float32).min])
+@pytest.mark.parametrize("rows,size", [(17, 262144), (2, 100003)])
+def test_rows_under_a_mask(ctx, rows, size, low):
+    """A grammar leaves a few tokens of a large vocabulary: fewer than the alternatives asked for, or in few chunks."""
+    rng = np.random.default_rng(9)
+    x = np.full((rows, size), low, np.float32)
+    tokens = np.zeros(rows, int)
+    for r in range(rows):
+        kept = rng.choice(size, [1, 3, 19, 20, 21, 2000, size // 3][r % 7], replace=False)
+        if r % 2:
+            kept = kept // 64  # (one chunk or a few)
+        x[r, kept] = rng.normal(-4, 3, kept.size)
+        tokens[r] = kept[0] if r % 3 else rng.integers(0, size)
+    check(ctx, x, tokens, 20)
