@@ -180,7 +180,10 @@ _kept = {}
 
 
 def _context():
-    """One context and one workspace, kept as a serving program keeps them."""
+    """One context and one workspace, kept as a serving program keeps them. Its calls go to a stream of the context's
+    own, which torch's work neither waits for nor is waited for by: `prepare` ends with a wait for the device, and who
+    reads a pass's outputs waits first. A program without such waits has torch and the context on one stream
+    (Context.set_stream with a torch.cuda.Stream's handle; the default stream's, 0, stands for the context's own)."""
     if "ctx" not in _kept:
         sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                                         "gemma4-webgpu_amd"))
