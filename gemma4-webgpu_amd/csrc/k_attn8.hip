@@ -138,10 +138,10 @@ __device__ __forceinline__ h2 two_codes(uint32_t x0, uint32_t x1) {
 // held by one workgroup is written by it; else its workgroups leave partials
 // (max, sum, o), which attn8_merge_kernel adds in order.
 //
-// Measured: 32 long contexts at head dim 512 (362 MB) 80 us, 4.5 TB/s of the 4.8
-// of a copy; 64 mixed ones at 256 (93 MB) 25 us; one window of 512 8.0 us, the
-// latency of a unit (lengths, page ids, rows, products, the waves' sums); the
-// partials 3 to 4.8 us more. Units of 1024, so that a window has no partials,
+// Measured: 32 long contexts at head dim 512 (362 MB) 78 us, 4.6 TB/s where a copy
+// moves 4.7 and reads alone go at 5.3; 64 mixed ones at 256 (93 MB) 24.5 us; one
+// window of 512 7.9 us, the latency of a unit (lengths, page ids, rows, products,
+// the waves' sums); the partials 3 to 4.8 us more. Units of 1024, so that a window has no partials,
 // took 15.6 us instead of 11.4: a wave's step of 32 positions is 1.8 us.
 constexpr int NT = 256, UNIT = 128;
 template <int HD>
@@ -625,9 +625,9 @@ __global__ __launch_bounds__(MT) void attn8_merge_kernel(Args a) {
 // that attn8_tile_merge_kernel adds in order.
 //
 // Measured: a prompt of 1900 rows of 8 heads at head dim 512 (29.6 GFLOP of scores
-// and P V, 1.75 times that as digits and halves) 105 us, then 16.6 for the 95 MB of
-// partials and output; long prompts 460 TFLOP/s at 512 and 510 at 256, where the
-// card lowers its clock.
+// and P V, 1.75 times that as digits and halves) 94 us, then 12.3 for the 95 MB of
+// partials and output, by the trace's kernel times; both together 94 us in passes
+// one after the other without it.
 constexpr int TC = 64, TP = 64;  // columns of a workgroup, positions of a step
 constexpr float kTileP = 32768.f;
 constexpr uint32_t kTileCost = 3, kLeast = 4;  // cost of a tile besides its steps; least cost of a share

@@ -22,7 +22,7 @@
 // launch finds in no cache: 27 KB of code (loops unrolled, the rotation without a
 // table in line, library square root, division and frexp, maxima in f64 through
 // LDS) took 8.3 us for 64 sequences, the same steps in 8 KB 4.0. A prompt of 1900
-// rows at head dim 512 (72 MB, 15 us at a copy's rate) takes 18.7.
+// rows at head dim 512 (72 MB, 15 us at a copy's rate) takes 18.1 to 18.7.
 #include "kv8.hpp"
 #include "mqf_core.hpp"
 
@@ -374,10 +374,12 @@ __global__ __launch_bounds__(VT) void kv8_values_kernel(ValArgs a) {
 }
 
 // The launch: few rows (at most four a sequence), a row and two of q's heads a
-// wave (64 sequences 3.6 us, with four heads 4.1); more rows, KEEP of them and four
-// heads (1900 rows 20.7 us, with two heads 21.6), in workgroups of four waves where
-// a page is 16 rows (18.7 us, eight waves 20.5) and eight where it is more (301
-// rows in pages of 32 7.4 us, four waves 13.2).
+// wave (64 sequences 3.9 us, with four heads 4.3); more rows, KEEP of them and four
+// heads (1900 rows 18.1 to 18.6 us, with two heads 18.5), in workgroups of four waves
+// where a page is 16 rows (chunks of seven prompts at head dim 128 6.6 us, with
+// eight waves 7.7; at 256 7.7 and 8.0; 1900 rows alike; 300 rows at 512 alone 10.8
+// and 6.8) and eight where it is more (the chunks in pages of 32 7.4 us, four waves
+// 12.8; 1900 rows at 256 12.8 and 18.0, in pages of 64 at 512 27.2 and 36.8).
 struct Shape {
   int threads, heads;
   bool few;

@@ -797,8 +797,9 @@ int g4_prefillAttn(g4_ctx* ctx, const float* q, const uint16_t* k_pool, const ui
  * when read, as in the f16 pool.
  *
  * page_size: a multiple of 16, at most 1024. head_dim 64, 128, 256 or 512, at
- * most 64 KV heads with at most 16 query heads each. max_seq_len: at most 2^30
- * and page_size * max_pages; the pool holds fewer than 2^36 positions. */
+ * most 64 KV heads with at most 16 query heads each. At most 65535 sequences
+ * and rows a call. max_seq_len: at most 2^30 and page_size * max_pages; the
+ * pool holds fewer than 2^36 positions. */
 typedef struct {
   uint32_t num_seqs, num_q_heads, num_kv_heads, head_dim;
   uint32_t page_size, max_pages, max_seq_len, num_pages;
@@ -818,6 +819,12 @@ typedef struct {
  * values: |value - x| <= scale / 2, and as much again of the then scale for
  * each growth. A NaN or an infinity among a page and head's rows makes its
  * scale NaN, and every value read from them NaN, until the page is begun again.
+ * A sequence whose length is set back (drafted rows that were rejected) appends
+ * over them like any other: a page that the taken-back rows began is begun
+ * again; one that stays keeps the scale that they made grow, with the codes
+ * before them rounded to it, or their mark. A caller to whom that matters keeps
+ * the codes and the scale of the page that holds the first drafted row (one page
+ * a sequence and layer) and puts them back.
  * Each page is appended to by one sequence of a call. k_parts = v_parts = NULL:
  * q only; q_parts = NULL (with q_norm_w, q_out): k and v only.
  * p.scale and p.sliding_window are unused. */
@@ -829,8 +836,9 @@ int g4_pagedAttnPrologue8(g4_ctx* ctx, const float* q_parts, const float* k_part
 /* Attention over the pool: output [num_rows][num_q_heads][head_dim] of the
  * roped q; the row at position t sees positions max(0, t + 1 - sliding_window)
  * .. t (from 0 without a window). All rows of a call are appended before it.
- * workspace: g4_pagedAttn8_workspace_size bytes, 16-byte aligned, of any
- * content; calls sharing it must not overlap. p.eps, theta and apply_divisor
+ * workspace: g4_pagedAttn8_workspace_size bytes of these parameters (others
+ * may need more, with fewer rows, too), 16-byte aligned, of any content; calls
+ * sharing it must not overlap. p.eps, theta and apply_divisor
  * are unused. */
 int g4_pagedAttn8_workspace_size(g4_kv8_params p, size_t* bytes);
 int g4_pagedAttn8(g4_ctx* ctx, const float* q, const int8_t* k_pool, const int8_t* v_pool, const float* k_scale,
@@ -860,7 +868,10 @@ int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const 
  *   first, equal ones by index (NaN after everything else), ntop <= 64 and
  *   <= size.
  * A row with a NaN or +Inf, or of nothing but -Inf, has NaN for every
- * probability; its ids are as stated. tokens and logprobs may be NULL together,
+ * probability; its ids are as stated. A row's alternatives take ntop rounds over
+ * the parts of it where fewer than ntop values are above -Inf or a mask's lowest
+ * value: rows masked to a few tokens cost some ten times as much as others at
+ * ntop 20 (ntop 0 and the rest of the outputs cost the same). tokens and logprobs may be NULL together,
  * entropy alone; ntop 0 takes no top buffers. workspace:
  * g4_logprobsBatch_workspace_size bytes, 16-byte aligned, of any content, which
  * serve any smaller batch, too; calls sharing it must not overlap. */
