@@ -87,6 +87,9 @@ class Kv8Params(ctypes.Structure):  # g4_kv8_params
                 ("eps", ctypes.c_float), ("theta", ctypes.c_float), ("apply_divisor", ctypes.c_uint32)]
 
 
+Kv4Params = Kv8Params  # g4_kv4_params
+
+
 class PerHeadNormParams(ctypes.Structure):  # shaders/per_head_rms_norm_no_weight.wgsl:8
     _fields_ = [("num_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
                 ("eps", ctypes.c_float), ("pad", ctypes.c_uint32)]
@@ -198,6 +201,13 @@ SIGNATURES = {
     "g4_pagedAttn8": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, Kv8Params, _P, _SZ]),
     "g4_pagedAttn8Ops": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, Kv8Params, _P, _SZ, _P]),
     "g4_kv8Values": (_I, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P]),
+    "g4_pagedAttnPrologue4": (_I, [_P, _P, _P, _P, _U32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                   Kv4Params, _P, _U32]),
+    "g4_pagedAttn4_workspace_size": (_I, [Kv4Params, _I, ctypes.POINTER(_SZ)]),
+    "g4_pagedAttn4": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, Kv4Params, _P, _SZ, _P]),
+    "g4_kvEvict4_workspace_size": (_I, [Kv4Params, _U32, ctypes.POINTER(_SZ)]),
+    "g4_kvEvict4": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, Kv4Params, _U32, _U32, _U32, _P, _P, _SZ]),
+    "g4_kv4Values": (_I, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P]),
     "g4_logprobsBatch_workspace_size": (_I, [_U32, _U32, _U32, ctypes.POINTER(_SZ)]),
     "g4_logprobsBatch": (_I, [_P, _P, _P, _U32, _U32, _P, _P, _U32, _P, _P, _P, _SZ]),
     "g4_advanceSeqLens": (_I, [_P, _P, _U32, _U32]),

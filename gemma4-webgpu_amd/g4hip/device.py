@@ -16,6 +16,7 @@ from ._lib import (
     AttnFusedParams,
     AttnOutputParams,
     AttnScoreParams,
+    Kv4Params,
     Kv8Params,
     KvStoreParams,
     MatmulParams,
@@ -736,6 +737,53 @@ class Context:
                   nkh: int, hd: int, num_pages: int, k_out: Ptr, v_out: Ptr) -> None:
         """The listed pages of an 8-bit pool as f16 pages."""
         check(lib().g4_kv8Values(self.h, k_pool, v_pool, k_scale, v_scale, pages, count, page_size, nkh, hd,
+                                 num_pages, k_out, v_out))
+
+    # ---- 4-bit paged K/V cache whose rows are weighed and evicted ----
+    kv4_params = kv8_params
+
+    @staticmethod
+    def attn4_workspace_bytes(p: Kv4Params, mass: bool = False) -> int:
+        n = ctypes.c_size_t()
+        check(lib().g4_pagedAttn4_workspace_size(p, int(mass), ctypes.byref(n)))
+        return int(n.value)
+
+    def pagedAttnPrologue4(self, q_parts: Ptr, k_parts: Ptr, v_parts: Ptr, nparts: int, q_norm_w: Ptr, k_norm_w: Ptr,
+                           rope_freqs: Ptr, q_out: Ptr, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr,
+                           page_table: Ptr, seq_lens: Ptr, p: Kv4Params, row_starts: Ptr = None,
+                           positions: Ptr = None, mass: Ptr = None, rope_cs: Ptr = None,
+                           rope_rows: int = 0) -> None:
+        """pagedAttnPrologue8 over a 4-bit pool. positions: the tokens of each sequence's text, where its cache has
+        lost rows (None: seq_lens); mass: new rows begin at 0."""
+        check(lib().g4_pagedAttnPrologue4(self.h, q_parts, k_parts, v_parts, nparts, q_norm_w, k_norm_w,
+                                          rope_freqs, q_out, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens,
+                                          row_starts, positions, mass, p, rope_cs, rope_rows))
+
+    def pagedAttn4(self, q: Ptr, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr, page_table: Ptr,
+                   seq_lens: Ptr, out: Ptr, p: Kv4Params, workspace: Buffer, row_starts: Ptr = None,
+                   mass: Ptr = None, ops: Ptr = None) -> None:
+        """pagedAttn8 over a 4-bit pool; with `mass`, every cached row's attention weight is added to it."""
+        check(lib().g4_pagedAttn4(self.h, q, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens, row_starts, out,
+                                  mass, p, workspace, workspace.nbytes, ops))
+
+    @staticmethod
+    def evict4_workspace_bytes(p: Kv4Params, keep: int) -> int:
+        n = ctypes.c_size_t()
+        check(lib().g4_kvEvict4_workspace_size(p, keep, ctypes.byref(n)))
+        return int(n.value)
+
+    def kvEvict4(self, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr, mass: Ptr, page_table: Ptr,
+                 seq_lens: Ptr, p: Kv4Params, keep: int, first: int, recent: int, kept: Ptr,
+                 workspace: Buffer) -> None:
+        """Every sequence of more than `keep` rows keeps, per KV head, its first `first`, its last `recent` and the
+        heaviest others; `kept` says where they were."""
+        check(lib().g4_kvEvict4(self.h, k_pool, v_pool, k_scale, v_scale, mass, page_table, seq_lens, p, keep, first,
+                                recent, kept, workspace, workspace.nbytes))
+
+    def kv4Values(self, k_pool: Ptr, v_pool: Ptr, k_scale: Ptr, v_scale: Ptr, pages: Ptr, count: int, page_size: int,
+                  nkh: int, hd: int, num_pages: int, k_out: Ptr, v_out: Ptr) -> None:
+        """The listed pages of a 4-bit pool as f16 pages."""
+        check(lib().g4_kv4Values(self.h, k_pool, v_pool, k_scale, v_scale, pages, count, page_size, nkh, hd,
                                  num_pages, k_out, v_out))
 
     def advanceSeqLens(self, seq_lens: Ptr, num_seqs: int, delta: int = 1) -> None:

@@ -861,6 +861,82 @@ int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const 
                  const int32_t* pages, uint32_t count, uint32_t page_size, uint32_t num_kv_heads, uint32_t head_dim,
                  uint32_t num_pages, uint16_t* k_out, uint16_t* v_out);
 
+/* ------------------------------------------------------------------------ */
+/* 4-bit paged K/V cache whose rows are weighed and evicted                  */
+/* (no counterpart in the reference)                                         */
+/* ------------------------------------------------------------------------ */
+
+/* A K/V pool of 4-bit floats: codes e2m1 (magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6,
+ * bit 3 the sign), a scale for every 32 neighbouring dims of a row and KV head;
+ * a value is code * 2^(scale byte - 127). 4.25 bits a value.
+ *   codes   u8 [num_pages][page_size][num_kv_heads][head_dim / 2], byte i holds
+ *           dims 2 i (its low half) and 2 i + 1
+ *   k_scale u8 [num_pages][page_size][num_kv_heads][head_dim / 32]
+ *   v_scale u8 [num_pages][page_size / 16][num_kv_heads][head_dim / 32][16]: the
+ *           scales of 16 neighbouring rows next to each other
+ * The scale of a block is the least 2^e (e >= -20) with |x| <= 7 * 2^e for all of
+ * it; a code is the nearest, halves to the even code: |value - x| <= 2^e, a
+ * quarter of the largest at most and 11 % of a normal block's deviation on the
+ * average. A NaN or an infinity in a row and head makes all its scales 255, and
+ * every output that sees the row NaN. V scales above 2^13 (the f16 values of the
+ * products end there) are the caller's own: the weightless norm's are below 2^2.
+ *
+ * mass f32 [num_pages][page_size][num_kv_heads]: the attention weight that each
+ * cached row has got so far, added up over query heads, rows and calls.
+ *
+ * Rows, sequences, limits: as g4_kv8_params says. Each row has its own scales:
+ * rows move between slots unchanged, and a sequence set back leaves nothing.
+ * Each page belongs to one sequence of a call that appends, weighs or evicts. */
+typedef g4_kv8_params g4_kv4_params;
+/* g4_pagedAttnPrologue8 over such a pool. positions (or NULL: seq_lens):
+ * positions[s] counts the tokens of sequence s's text, the call's rows among
+ * them, where its cache has lost some (g4_kvEvict4): with n rows its row i is
+ * turned by position positions[s] - n + i. With rope_cs, a sequence whose
+ * positions[s] exceeds rope_rows, and always one whose positions[s] is below its
+ * rows, appends nothing and its q_out is not written. mass (or NULL): new rows
+ * begin at 0. */
+int g4_pagedAttnPrologue4(g4_ctx* ctx, const float* q_parts, const float* k_parts, const float* v_parts,
+                          uint32_t nparts, const uint16_t* q_norm_w, const uint16_t* k_norm_w,
+                          const uint16_t* rope_freqs, float* q_out, uint8_t* k_pool, uint8_t* v_pool,
+                          uint8_t* k_scale, uint8_t* v_scale, const int32_t* page_table, const uint32_t* seq_lens,
+                          const uint32_t* row_starts, const uint32_t* positions, float* mass, g4_kv4_params p,
+                          const float* rope_cs, uint32_t rope_rows);
+/* Attention over the pool, as g4_pagedAttn8 (a window is the last sliding_window
+ * cached rows). mass (or NULL): to each cached row and KV head is added the
+ * softmax weight that it gets here, over the head's query heads and the
+ * sequence's rows; the same sums in every run. ops (or NULL): as
+ * g4_pagedAttn8Ops. workspace: g4_pagedAttn4_workspace_size bytes of these
+ * parameters, with or without mass (others may need more), 16-byte aligned, of
+ * any content; calls sharing it must not overlap. */
+int g4_pagedAttn4_workspace_size(g4_kv4_params p, int with_mass, size_t* bytes);
+int g4_pagedAttn4(g4_ctx* ctx, const float* q, const uint8_t* k_pool, const uint8_t* v_pool, const uint8_t* k_scale,
+                  const uint8_t* v_scale, const int32_t* page_table, const uint32_t* seq_lens,
+                  const uint32_t* row_starts, float* output, float* mass, g4_kv4_params p, void* workspace,
+                  size_t workspace_bytes, void* ops);
+/* Cuts every sequence of more than `keep` (and at most max_seq_len) cached rows
+ * down to `keep`, each KV head by itself: it keeps its first `first` rows, its
+ * last `recent` and, of the others, the keep - first - recent with the largest
+ * mass (of equal ones the earliest; a mass that is not above 0 counts as 0). The
+ * kept rows move, in their order, to rows 0 .. keep - 1, their masses with them;
+ * later slots stay as they are, and seq_lens[s] becomes keep. Sequences of keep
+ * rows or fewer, or more than max_seq_len, stay as they are.
+ * kept i32 [num_seqs][num_kv_heads][keep]: where each row was (0, 1, .. for a
+ * sequence that stays; -1 past its last row, and for one longer than
+ * max_seq_len). first + recent <= keep <= max_seq_len. Rows whose page id is
+ * outside [0, num_pages) count 0, are read as page clamped and not written.
+ * workspace: g4_kvEvict4_workspace_size bytes, 16-byte aligned, of any content;
+ * calls sharing it must not overlap. Of p, the rows and the query heads, the
+ * window and what the norms and the rotation take are unused. */
+int g4_kvEvict4_workspace_size(g4_kv4_params p, uint32_t keep, size_t* bytes);
+int g4_kvEvict4(g4_ctx* ctx, uint8_t* k_pool, uint8_t* v_pool, uint8_t* k_scale, uint8_t* v_scale, float* mass,
+                const int32_t* page_table, uint32_t* seq_lens, g4_kv4_params p, uint32_t keep, uint32_t first,
+                uint32_t recent, int32_t* kept, void* workspace, size_t workspace_bytes);
+/* g4_kv8Values over such a pool: the listed pages' values in f16, rounded where
+ * they are below 2^-14 or above its range (a row of scales 255: NaN). */
+int g4_kv4Values(g4_ctx* ctx, const uint8_t* k_pool, const uint8_t* v_pool, const uint8_t* k_scale,
+                 const uint8_t* v_scale, const int32_t* pages, uint32_t count, uint32_t page_size,
+                 uint32_t num_kv_heads, uint32_t head_dim, uint32_t num_pages, uint16_t* k_out, uint16_t* v_out);
+
 /* Per row of `batch` <= 65535 rows of `size` <= 2^28 logits (softcapped already):
  *   logprobs[r] = x[tokens[r]] - log sum exp x    (a token >= size: NaN)
  *   entropy[r] = -sum p log p                     (a p of 0 adds 0)
