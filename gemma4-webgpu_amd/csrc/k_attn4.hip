@@ -1,24 +1,584 @@
 // k_attn4.hip — attention over the 4-bit paged K/V pool (k_kv4.hip writes it),
-// and the attention weight of its rows.
+// and the attention weight of its rows, on the gfx950 matrix cores.
 //
-//   p[t] = softmax over t of scale * (q . k[t]),  out = sum p[t] * v[t],
-//   mass[t] += sum of p[t] over a KV head's query heads and the sequence's rows
+//   S[pos][col] = k[pos] . q[col],  out[col] = sum P[pos][col] * v[pos],  P = softmax of scale * S,
+//   mass[pos] += sum over cols of P[pos][col]
 //
-// attn4_row_kernel: a workgroup one row and query head, a wave every fourth
-// position, one pass with the running maximum and sum. attn4_mass_kernel: a wave
-// one position and KV head, the scores again with the rows' maxima and sums.
+// a column being one query row and head of a KV head.
+//  * scores: v_mfma_scale_f32_16x16x128_f8f6f4 takes 16 K rows' codes and scales as
+//    they lie in the pool (e2m1, e8m0 per 32 dims). q is five e2m3 digits of 5 bits
+//    a block of 32 dims, each with a scale of its own, so that all sum up in one
+//    f32 accumulator: digits in [-16, 16] / 8, q rounded to 2^-24 of its block's
+//    largest. Products and sums of one instruction are exact but for one rounding
+//    (2^-23.2 of the magnitudes' sum at most, over random blocks and scales). No
+//    conversion of K, at 16 cycles for 128 dims and a digit; three digits of 8 bits
+//    with integer products (K expanded to bytes) take 24 for the five's 40 / 2 = 20.
+//  * P V: v_mfma_f32_16x16x32_f16, P * 2^15 as f16 hi + lo in one sum: 22 bits of
+//    every P down to 2^-17 of the row's largest and 2^-40 of it below. V is exact
+//    in f16 (codes of 2 bits, scales 2^-20 .. 2^13): one conversion for two codes
+//    with their scale, and one byte permutation for the order of the operand.
+// Sums over steps are f32. Maxima are taken to the next power of two, so that a
+// later one rescales exactly.
 #include <algorithm>
+#include <type_traits>
 
+#include "attn_paged.hpp"
 #include "kv4.hpp"
 
 namespace {
 
 using namespace g4kv8;
+using g4kv4::BAD;
 using g4kv4::BLOCK;
+using g4mm::h2;
+using g4mm::h8;
+using g4mm::static_for;
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef int i6 __attribute__((ext_vector_type(6)));
+typedef int i8 __attribute__((ext_vector_type(8)));
+typedef float f16x __attribute__((ext_vector_type(16)));
 
-constexpr int NT = 256, NW = NT / 64;
+constexpr int COLS = 16;               // columns of a matrix product
+constexpr float kLog2e = 1.44269504f;  // the softmax works in powers of two
+constexpr float kPScale = 32768.f;
+constexpr float kNothing = -3e38f;     // the maximum of no positions: finite, so that differences are
+constexpr int DIGITS = 5;
 
-struct Args {
+struct Args : PagedArgs {
+  const uint8_t *kp, *vp, *ks, *vs;
+  float* mass;              // or null
+  float2* sums;             // with mass: maximum and 1 / sum of each row and query head
+  float* scores;            // few rows, with mass: [sequence][KV head][unit][column][128 positions]
+  uint32_t units, columns;  // of a sequence and KV head there
+};
+
+// ---- q as digits ----
+
+// 32 neighbouring elements x of q: their digits' codes (24 bytes each, first the largest), and the scale bytes of the
+// five. Non-finite ones have a scale of NaN. Ones below 2^-106 count as 0 (the last digit's scale ends there).
+__device__ __forceinline__ void digits_of(const float* x, i6* code, uint32_t& scales, uint32_t& last) {
+  float am = 0.f;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < BLOCK; ++i) {
+    am = fmaxf(am, fabsf(x[i]));
+    nan |= x[i] != x[i];
+  }
+  const bool bad = nan || !(am < INFINITY);
+  int e = __builtin_amdgcn_frexp_expf(am) - 1;  // 2^e <= am < 2^(e + 1)
+  const bool none = bad || am == 0.f || e < -106;
+  e = none ? 0 : e;
+  f16x a, b;  // even, odd elements (the conversion takes them in turn)
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    a[i] = none ? 0.f : __builtin_amdgcn_ldexpf(x[2 * i], -e);
+    b[i] = none ? 0.f : __builtin_amdgcn_ldexpf(x[2 * i + 1], -e);
+  }
+  static_for<DIGITS>([&](auto d) __attribute__((always_inline)) {
+    constexpr int D = decltype(d)::value;
+    constexpr float unit = 1.f / (float)(1u << (5 * D)), border = 1572864.f * unit;  // 1.5 * 2^20: steps of 1 / 8
+    if constexpr (D == DIGITS - 1) {
+      code[D] = __builtin_bit_cast(i6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, unit));
+    } else {
+      f16x u, v;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        u[i] = (a[i] + border) - border;
+        v[i] = (b[i] + border) - border;
+        a[i] -= u[i];
+        b[i] -= v[i];
+      }
+      code[D] = __builtin_bit_cast(i6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(u, v, unit));
+    }
+  });
+  const uint32_t s = (uint32_t)(e + 127);
+  scales = bad ? 0x7f7f7f00u | BAD : s | (s - 5) << 8 | (s - 10) << 16 | (s - 15) << 24;
+  last = bad ? 127u : s - 20;
+}
+
+// One digit of q times 128 dims of 16 K rows, added to c. KS and QS: the bytes of ks and qs with their scales.
+template <int KS, int QS>
+__device__ __forceinline__ f4 product(const i4& k, const i6& q, f4 c, uint32_t ks, uint32_t qs) {
+  const i8 a{k[0], k[1], k[2], k[3], 0, 0, 0, 0}, b{q[0], q[1], q[2], q[3], q[4], q[5], 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 2, KS, (int)ks, QS, (int)qs);
+}
+
+// ---- V as f16 ----
+
+// Byte I of four as the power of two that it is the exponent of (255: infinity, 0: 0).
+template <int I>
+__device__ __forceinline__ float exponent(uint32_t w) {
+  return __uint_as_float(I < 3 ? (w << (24 - 8 * I) >> 24) << 23 : w >> 24 << 23);
+}
+__device__ __forceinline__ bool any_bad(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
+// The two codes of byte B of x and of y, each times its row's scale: (first of x, first of y), (second, second).
+template <int B>
+__device__ __forceinline__ void two_by_two(uint32_t x, float sx, uint32_t y, float sy, h2& first, h2& second) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sx, B));
+  const uint32_t v = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(y, sy, B));
+  first = __builtin_bit_cast(h2, __builtin_amdgcn_perm(v, u, 0x05040100u));
+  second = __builtin_bit_cast(h2, __builtin_amdgcn_perm(v, u, 0x07060302u));
+}
+
+// ---------------------------------------------------------------------------
+// few rows a sequence (a decode step): rows * query heads per KV head <= 16
+// ---------------------------------------------------------------------------
+//
+// HBM bounds it: every byte of K and V goes from the pool to a wave's registers
+// once, in the matrix operands' order (no LDS): a lane's 16 bytes of a K row are
+// 32 dims of its A operand, and its HD / 16 neighbouring dims of 8 V rows become
+// the B operands of HD / 16 products.
+//
+// The positions of all sequences, in units of 128, are dealt to the workgroups
+// in equal shares whatever the lengths (a share may end in one sequence and go
+// on in the next), 32 positions at a time to each of the four waves. A sequence
+// held by one workgroup is written by it; else its workgroups leave partials
+// (max, sum, o), which attn4_merge_kernel adds in order. With masses, the scores
+// go to the workspace, and attn4_weigh_kernel turns them into weights when the
+// maxima and sums are known: 4 bytes a position and column written and read, where
+// K again would be HD / 2 * 17 / 16 bytes a position and the products once more.
+constexpr int NT = 256, UNIT = 128;
+template <int HD>
+struct StepShape {
+  static constexpr uint32_t WGS = HD == 512 ? 256 : 512;  // one or two per CU (registers)
+  static constexpr uint32_t SLOT = COLS * (HD + 2);       // floats of a partial: max, sum [16], o [16][HD]
+};
+
+template <int HD, bool MASS>
+__global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn4_step_kernel(Args a) {
+  constexpr int VB = HD / 16, NB = HD / BLOCK, J = HD < 128 ? 1 : HD / 128, BL = HD < 256 ? 1 : HD / 256;
+  constexpr int VW = VB < 8 ? 1 : VB / 8;  // words of a lane's share of a V row
+  __shared__ __align__(16) float s_o[4 * COLS * HD];
+  // (the same bytes, before the waves' sums) digits as B operands: [digit][128 dims][lane] 24 B
+  uint8_t* s_q = (uint8_t*)s_o;
+  static_assert(DIGITS * J * 64 * 24 <= sizeof(s_o));
+  __shared__ __align__(8) uint2 s_qs[J * 64];
+  __shared__ float s_m[4 * COLS], s_l[4 * COLS];
+  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), qd = l >> 4, c = l & 15;
+  const uint32_t S = a.rows.num_seqs, wg = blockIdx.x;
+
+  // The sequences 64 at a time, one a lane (in every wave alike): their units
+  // summed up, T in all; then those that hold this workgroup's share.
+  Seq mine{};
+  uint32_t c0 = 0, mine_units = 0, incl = 0, total = 0;
+  auto load_chunk = [&](uint32_t first) {
+    c0 = first;
+    mine = first + l < S ? seq_rows(a.rows, first + l) : Seq{0, 0, 0, 0};
+    mine_units = mine.len ? (mine.len - first_seen(a, mine) + UNIT - 1) / UNIT : 0u;
+    incl = wave_scan(mine_units * a.nkh);
+    total = __builtin_amdgcn_readlane(incl, 63);
+  };
+  uint32_t T = 0;
+  for (uint32_t first = 0; first < S; first += 64) {
+    load_chunk(first);
+    T += total;
+  }
+  const Share sh{T, min(a.wgs, T)};
+  const uint32_t ub = wg < sh.W ? sh.first(wg) : 0u, ue = wg < sh.W ? sh.first(wg + 1) : 0u;
+  uint32_t before = 0;  // units before the chunk
+  if (S > 64 && ub < ue) {
+    for (load_chunk(0); before + total <= ub; load_chunk(c0 + 64)) before += total;
+  }
+
+  uint32_t u = ub;
+  while (u < ue) {
+    while (before + total <= u) {  // (u < T: a later chunk holds it)
+      before += total;
+      load_chunk(c0 + 64);
+    }
+    const int at = __ffsll((unsigned long long)__ballot(before + incl > u)) - 1;
+    const uint32_t s = c0 + at;
+    const Seq sq{pick(mine.first, at), pick(mine.n, at), pick(mine.base, at), pick(mine.len, at)};
+    const uint32_t units = pick(mine_units, at), seq0 = before + pick(incl, at) - units * a.nkh;
+    const uint32_t lo = first_seen(a, sq), end = sq.len;
+    const uint32_t kvh = a.nkh == 1 ? 0u : uni((u - seq0) / units);
+    const uint32_t seg = seq0 + kvh * units;  // its first unit
+    const uint32_t off = u - seg, take = min(units - off, ue - u);
+    const uint32_t ncols = sq.n * a.G;
+    const uint32_t rs = a.nkh * (HD / 2), ss = a.nkh * NB;  // bytes from a row to the next: codes, K scales
+
+    i4 K[2][J];
+    uint32_t V[8][VW], kw[2], vw[2];
+    // page ids of the next step and, on their way, of the one after it (vector loads, issued before the rows that
+    // go before them in use: a scalar load's wait is that of the LDS reads too)
+    int32_t pg[2], pg_far[2];
+    const uint32_t st1 = 4 * (off + take), tiles = (end - lo + 15) / 16, t0 = lo / 16;
+    const uint32_t steps = min(st1, (tiles + 1) / 2);  // (the last unit may be short)
+    const uint32_t none = 0x40000000u;  // past every tile: read as 0
+    const uint32_t k_at = HD == 64 && qd >= 2 ? none : c * rs + 16 * J * qd;
+    const uint32_t ks_at = HD == 64 && qd >= 2 ? none : c * ss + J * qd;
+    const uint32_t v_at = 4 * qd * rs + VB / 2 * c, vs_at = VB * c / BLOCK * 16 + 4 * qd;
+    const int32_t* list = a.page_table + (size_t)s * a.max_pages;
+    auto pages = [&](uint32_t st, int32_t* to) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) to[p] = list[page_of(a, t0 + min(2 * st + p, tiles - 1))];
+    };
+    // a tile's rows as buffers; of no bytes past the last step, so that nothing is read there (a branch around the
+    // loads of the next step would spill)
+    auto tile_at = [&](uint32_t st, int p) -> size_t {
+      const uint32_t t = t0 + min(2 * st + p, tiles - 1);
+      return (size_t)clamp_page(a, uni_i(pg[p])) * a.page_tiles + (t - page_of(a, t) * a.page_tiles);
+    };
+    auto buffer = [&](const uint8_t* base, uint32_t bytes, uint32_t st) -> __amdgpu_buffer_rsrc_t {
+      return __builtin_amdgcn_make_buffer_rsrc((void*)uni((uint64_t)base), (short)0, st < steps ? (int)bytes : 0,
+                                               0x00020000);
+    };
+    auto load_k = [&](uint32_t st) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const size_t t = tile_at(st, p);
+        const __amdgpu_buffer_rsrc_t r = buffer(a.kp + t * (16 * (size_t)rs) + kvh * (HD / 2), 15 * rs + HD / 2, st);
+        const __amdgpu_buffer_rsrc_t z = buffer(a.ks + t * (16 * (size_t)ss) + kvh * NB, 15 * ss + NB, st);
+        if constexpr (J == 4) kw[p] = __builtin_amdgcn_raw_buffer_load_b32(z, ks_at, 0, 0);
+        else if constexpr (J == 2) kw[p] = __builtin_amdgcn_raw_buffer_load_b16(z, ks_at, 0, 0);
+        else kw[p] = __builtin_amdgcn_raw_buffer_load_b8(z, ks_at, 0, 0);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          K[p][j] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(r, k_at + 16 * j, 0, 0));
+      }
+    };
+    auto load_v = [&](uint32_t st) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const size_t t = tile_at(st, p);
+        const __amdgpu_buffer_rsrc_t r = buffer(a.vp + t * (16 * (size_t)rs) + kvh * (HD / 2), 15 * rs + HD / 2, st);
+        const __amdgpu_buffer_rsrc_t z = buffer(a.vs + (t * a.nkh + kvh) * (NB * 16), NB * 16, st);
+        vw[p] = __builtin_amdgcn_raw_buffer_load_b32(z, vs_at, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (VW == 4) {
+            const i4 x = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(r, v_at, i * rs, 0));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) V[4 * p + i][e] = (uint32_t)x[e];
+          } else if constexpr (VW == 2) {
+            const auto x = __builtin_amdgcn_raw_buffer_load_b64(r, v_at, i * rs, 0);
+            V[4 * p + i][0] = x[0];
+            V[4 * p + i][1] = x[1];
+          } else if constexpr (VB == 8) {
+            V[4 * p + i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, v_at, i * rs, 0);
+          } else {
+            V[4 * p + i][0] = __builtin_amdgcn_raw_buffer_load_b16(r, v_at, i * rs, 0);
+          }
+        }
+      }
+    };
+
+    // q, a thread 32 dims of a column (asked for before the rows, whose arrival its digits then do not wait for)
+    const uint32_t col = tid / (4 * J), block = tid % (4 * J);
+    float x32[BLOCK];
+    if (tid < 64 * J) {
+      const float* qg = a.q + row_of(a, sq.first, kvh, min(col, ncols - 1)) * HD + BLOCK * (HD == 64 ? block & 1 : block);
+#pragma unroll
+      for (int e = 0; e < BLOCK; e += 4) {
+        const f4 y = *(const f4*)(qg + e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x32[e + i] = HD == 64 && block >= 2 ? 0.f : y[i];
+      }
+    }
+    uint32_t st = 4 * off + w;
+    // (a wave without a step too, of no bytes: behind a branch q would be waited for together with the rows)
+    pages(st, pg);
+    pages(min(st + 4, steps - 1), pg_far);  // (before the rows: what comes after them is waited for with them)
+    load_k(st);
+    load_v(st);
+    pg[0] = pg_far[0];
+    pg[1] = pg_far[1];
+    // ---- q's digits ----
+    __syncthreads();  // the previous sequence's are done with
+    if (tid < 64 * J) {
+      i6 code[DIGITS];
+      uint2 sc;
+      digits_of(x32, code, sc.x, sc.y);
+      const uint32_t j = block % J, lane = block / J * 16 + col;
+      s_qs[j * 64 + lane] = sc;
+#pragma unroll
+      for (int d = 0; d < DIGITS; ++d) {
+        uint2* to = (uint2*)(s_q + ((d * J + j) * 64 + lane) * 24);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) to[i] = make_uint2(code[d][2 * i], code[d][2 * i + 1]);
+      }
+    }
+    __syncthreads();
+    uint2 qs[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) qs[j] = s_qs[j * 64 + l];
+    // this lane's column: positions clo .. clo + width - 1
+    const float s_scale = a.scale * kLog2e;
+    const uint32_t cpos = sq.base + div_g(a, c);
+    const uint32_t clo = a.window && cpos + 1 > a.window ? cpos + 1 - a.window : 0u;
+    const uint32_t width = (uint32_t)c < ncols ? cpos + 1 - clo : 0u;
+    const uint32_t first = a.window && sq.base + 1 > a.window ? sq.base + 1 - a.window : 0u;  // of any column
+    float* score_at = nullptr;
+    if (MASS)
+      score_at = a.scores + (((size_t)(s * a.nkh + kvh) * a.units) * a.columns + min((uint32_t)c, a.columns - 1)) * UNIT;
+    f4 O[VB];
+#pragma unroll
+    for (int e = 0; e < VB; ++e) O[e] = f4{0.f, 0.f, 0.f, 0.f};
+    float m_run = kNothing, l_run = 0.f;  // of column c
+    for (; st < steps; st += 4) {
+      const uint32_t next = st + 4;
+      asm volatile("" ::: "memory");  // q's digits stay in LDS (in registers they would spill)
+      // ---- scores ----
+      f4 D[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) D[p] = f4{0.f, 0.f, 0.f, 0.f};
+      static_for<DIGITS * J>([&](auto k) __attribute__((always_inline)) {
+        constexpr int d = DIGITS - 1 - decltype(k)::value / J, j = decltype(k)::value % J;  // (the smallest first)
+        const uint2* from = (const uint2*)(s_q + ((d * J + j) * 64 + l) * 24);
+        i6 B;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const uint2 y = from[i];
+          B[2 * i] = (int)y.x;
+          B[2 * i + 1] = (int)y.y;
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) D[p] = product<j, d % 4>(K[p][j], B, D[p], kw[p], d == 4 ? qs[j].y : qs[j].x);
+      });
+      pages(min(st + 8, steps - 1), pg_far);
+      load_k(next);
+      // ---- softmax over the step's 32 positions ----
+      const uint32_t p0 = lo + 32 * st, pb = p0 + 4 * qd;
+      float x[8], vsc[8], mx = -INFINITY;
+      auto live = [&](int k) { return pb + 16 * (k / 4) + k % 4 - clo < width; };
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = D[k / 4][k % 4] * s_scale;
+      static_for<8>([&](auto k) __attribute__((always_inline)) {
+        constexpr int n = decltype(k)::value;
+        vsc[n] = exponent<n % 4>(vw[n / 4]);
+      });
+      // (uniform) rows that no column sees may hold anything; of the others, one that is not finite makes the weight of
+      // every column that sees it NaN
+      if (p0 < first || p0 + 32 > end || __ballot(any_bad(vw[0]) || any_bad(vw[1]))) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t pos = pb + 16 * (k / 4) + k % 4;
+          const bool bad = vsc[k] == INFINITY;
+          if (bad) x[k] = __builtin_nanf("");
+          if (bad || pos < first || pos >= end) vsc[k] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, live(k) ? x[k] : -INFINITY);
+      mx = g4d::xmax32(g4d::xmax16(mx));
+      const float m_new = fmaxf(m_run, ceilf(mx));
+      const float alpha = exp2_h(m_run - m_new);
+      float ps = 0.f;
+      h8 ph, pl;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float e = live(k) ? exp2_h(x[k] - m_new) : 0.f;
+        ps += e;
+        const float es = e * kPScale;
+        ph[k] = (_Float16)es;
+        pl[k] = (_Float16)(es - (float)ph[k]);
+      }
+      if (MASS && (uint32_t)c < ncols) {
+        float* to = score_at + (size_t)(st / 4) * a.columns * UNIT + st % 4 * 32 + 4 * qd;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          f4 y;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = live(4 * p + i) ? x[4 * p + i] : -INFINITY;
+          *(f4*)(to + 16 * p) = y;
+        }
+      }
+      ps = g4d::xsum32(g4d::xsum16(ps));
+      l_run = l_run * alpha + ps;
+      m_run = m_new;
+      if (__ballot(alpha != 1.f)) {
+        float ar[4];  // O's rows are columns 4 qd + i
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ar[i] = __shfl(alpha, 4 * qd + i, 64);
+#pragma unroll
+        for (int e = 0; e < VB; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) O[e][i] *= ar[i];
+      }
+      // ---- P V, two dims (a byte of V) at a time ----
+      static_for<VB / 2>([&](auto e) __attribute__((always_inline)) {
+        constexpr int b = decltype(e)::value % 4, k = decltype(e)::value / 4, n = 2 * decltype(e)::value;
+        h8 B[2];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          h2 y, z;
+          two_by_two<b>(V[j][k], vsc[j], V[j + 1][k], vsc[j + 1], y, z);
+          B[0][j] = y[0];
+          B[0][j + 1] = y[1];
+          B[1][j] = z[0];
+          B[1][j + 1] = z[1];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) O[n + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, B[i], O[n + i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) O[n + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, B[i], O[n + i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      load_v(next);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) pg[p] = pg_far[p];
+    }
+
+    // ---- the four waves' sums, in their order ----
+    __syncthreads();  // every wave is done with q's digits
+    if (qd == 0) {
+      s_m[w * COLS + c] = m_run;
+      s_l[w * COLS + c] = l_run;
+    }
+    // O of column 4 qd + i, dims VB c .. + VB - 1: groups of four dims turned by c, so that the 16 lanes meet
+    // different banks
+    constexpr int QG = VB / 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (4u * qd + i < ncols) {
+        float* o = s_o + (w * COLS + 4 * qd + i) * HD + VB * c;
+#pragma unroll
+        for (int e = 0; e < QG; ++e)
+          *(f4*)(o + 4 * ((e + c) % QG)) = f4{O[4 * e][i], O[4 * e + 1][i], O[4 * e + 2][i], O[4 * e + 3][i]};
+      }
+    }
+    __syncthreads();
+    const bool whole = take == units;
+    const uint32_t slot = 2 * wg + (u == ub ? 0u : 1u);
+    float* part = a.part + (size_t)slot * StepShape<HD>::SLOT;
+    for (uint32_t i = tid; i < ncols * (HD / 4); i += NT) {
+      const uint32_t col = i / (HD / 4), d = i % (HD / 4) * 4;
+      float M = kNothing, L = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) M = fmaxf(M, s_m[k * COLS + col]);
+      f4 y = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = exp2_h(s_m[k * COLS + col] - M);
+        L += s_l[k * COLS + col] * f;
+        y += *(const f4*)(s_o + (k * COLS + col) * HD + d / VB * VB + 4 * ((d % VB / 4 + d / VB) % QG)) * f;
+      }
+      y *= 1.f / kPScale;
+      const size_t row = row_of(a, sq.first, kvh, col);
+      float* o = whole ? a.out + row * HD : part + 2 * COLS + col * HD;
+      if (whole) y *= 1.0f / L;
+      *(f4*)(o + d) = y;
+      if constexpr (HD >= 256) {
+        if (whole && a.ops)  // (uniform; a wave holds 256 values of one row and head)
+          write_ops(a, sq.first + div_g(a, col), (kvh * a.G + col - div_g(a, col) * a.G) * BL + d / 256, l, y);
+      }
+      if (d == 0) {
+        if (!whole) {
+          part[col] = M;
+          part[COLS + col] = L;
+        } else if (MASS) {
+          a.sums[row] = make_float2(M, 1.0f / L);
+        }
+      }
+    }
+    if (off == 0 && tid == 0) a.meta[(size_t)s * a.nkh + kvh] = make_uint2(slot, sh.owner(seg + units - 1));
+    u += take;
+  }
+  // rows that see nothing
+  for (uint32_t i = wg; i < S * a.nkh; i += gridDim.x) {
+    const Seq q = seq_rows(a.rows, i / a.nkh);
+    if (q.len || !q.n) continue;
+    for (uint32_t d = tid; d < q.n * a.G * HD; d += NT)
+      a.out[((size_t)(q.first + d / (a.G * HD)) * a.nqh + i % a.nkh * a.G) * HD + d % (a.G * HD)] = 0.f;
+    if (HD >= 256 && a.ops)
+      for (uint32_t b = w; b < q.n * a.G * BL; b += NT / 64)
+        write_ops(a, q.first + b / (a.G * BL), i % a.nkh * a.G * BL + b % (a.G * BL), l, f4{0.f, 0.f, 0.f, 0.f});
+  }
+}
+
+// Adds the partials of one column: those of workgroup meta.x / 2 (slot meta.x)
+// and of the ones up to meta.y (slot 0 of each), in this order over groups of
+// threads: group g takes every NG-th, then the groups are added in order.
+template <int HD, int MT>
+__global__ __launch_bounds__(MT) void attn4_merge_kernel(Args a) {
+  constexpr int TG = HD / 4, NG = MT / TG, MS = 4;  // threads a partial row, groups, loads in flight of each
+  __shared__ float s_m[NG], s_l[NG];
+  __shared__ __align__(16) float s_o[NG * HD];
+  const uint32_t cols = a.rows.max_rows * a.G, col = blockIdx.x % cols;
+  const uint32_t sh = blockIdx.x / cols, s = sh / a.nkh, kvh = sh % a.nkh;
+  const Seq q = seq_rows(a.rows, s);
+  if (!q.len || col >= q.n * a.G) return;
+  const uint2 mt = a.meta[sh];
+  const uint32_t w0 = mt.x / 2, n = mt.y - w0 + 1;
+  if (n == 1) return;  // written by its workgroup
+  const uint32_t g = threadIdx.x / TG, d = threadIdx.x % TG * 4;
+  auto slot = [&](uint32_t i) -> const float* {
+    return a.part + (size_t)(i ? 2 * (w0 + i) : mt.x) * StepShape<HD>::SLOT;
+  };
+  float m = kNothing, l = 0.f;
+  f4 o = f4{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t i0 = g; i0 < n; i0 += NG * MS) {
+    float pm[MS], pl[MS];
+    f4 po[MS];
+#pragma unroll
+    for (int k = 0; k < MS; ++k) {
+      const float* p = slot(min(i0 + NG * k, n - 1));
+      pm[k] = p[col];
+      pl[k] = p[COLS + col];
+      po[k] = *(const f4*)(p + 2 * COLS + col * HD + d);
+    }
+    float mn = m;
+#pragma unroll
+    for (int k = 0; k < MS; ++k) mn = fmaxf(mn, i0 + NG * k < n ? pm[k] : kNothing);
+    const float al = exp2_h(m - mn);
+    l *= al;
+    o *= al;
+#pragma unroll
+    for (int k = 0; k < MS; ++k) {
+      if (i0 + NG * k >= n) continue;
+      const float f = exp2_h(pm[k] - mn);
+      l += f * pl[k];
+      o += f * po[k];
+    }
+    m = mn;
+  }
+  if (d == 0) {
+    s_m[g] = m;
+    s_l[g] = l;
+  }
+  *(f4*)(s_o + g * HD + d) = o;
+  __syncthreads();
+  if (g) return;
+  float M = kNothing, L = 0.f;
+  for (int i = 0; i < NG; ++i) M = fmaxf(M, s_m[i]);
+  f4 y = f4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < NG; ++i) {
+    const float f = exp2_h(s_m[i] - M);
+    L += f * s_l[i];
+    y += f * *(const f4*)(s_o + i * HD + d);
+  }
+  y *= 1.0f / L;
+  const uint32_t row = q.first + col / a.G, head = kvh * a.G + col % a.G;
+  *(f4*)(a.out + ((size_t)row * a.nqh + head) * HD + d) = y;
+  if (a.sums && d == 0) a.sums[(size_t)row * a.nqh + head] = make_float2(M, 1.0f / L);
+  if (HD >= 256 && a.ops) write_ops(a, row, head * (HD / 256) + d / 256, threadIdx.x & 63, y);
+}
+
+// The weights of a unit's positions from their scores, a thread each, added over the columns in order.
+__global__ __launch_bounds__(UNIT) void attn4_weigh_kernel(Args a) {
+  __shared__ float2 s_sum[COLS];
+  const uint32_t sh = blockIdx.y, s = sh / a.nkh, kvh = sh % a.nkh, i = threadIdx.x;
+  const Seq q = seq_rows(a.rows, s);
+  if (!q.len) return;
+  const uint32_t ncols = q.n * a.G, lo = first_seen(a, q);
+  if (i < ncols) s_sum[i] = a.sums[row_of(a, q.first, kvh, i)];
+  __syncthreads();
+  for (uint32_t unit = blockIdx.x; lo + unit * UNIT < q.len; unit += gridDim.x) {
+    const uint32_t t = lo + unit * UNIT + i;
+    if (t >= q.len) return;
+    const float* x = a.scores + ((size_t)sh * a.units + unit) * a.columns * UNIT + i;
+    float got = 0.f;
+    for (uint32_t c = 0; c < ncols; ++c) got += exp2_h(x[c * UNIT] - s_sum[c].x) * s_sum[c].y;
+    const uint32_t tile = t / 16, page = page_of(a, tile);
+    const int32_t id = a.page_table[(size_t)s * a.max_pages + page];
+    if (id >= 0 && id < (int32_t)a.num_pages)
+      a.mass[((size_t)id * (a.page_tiles * 16) + (t - page * a.page_tiles * 16)) * a.nkh + kvh] += got;
+  }
+}
+
+constexpr int NW = NT / 64;
+
+struct Plain {
   const float* q;
   g4kv4::Pool pool;
   g4kv4::Shape sh;
@@ -30,7 +590,7 @@ struct Args {
   float2* sums;  // maximum and 1 / sum of each row and query head
 };
 
-__device__ __forceinline__ uint32_t page_at(const Args& a, uint32_t s, uint32_t t) {
+__device__ __forceinline__ uint32_t page_at(const Plain& a, uint32_t s, uint32_t t) {
   const int32_t pg = a.page_table[(size_t)s * a.max_pages + t / a.sh.page_size];
   return pg < 0 ? 0u : min((uint32_t)pg, a.num_pages - 1);
 }
@@ -45,7 +605,7 @@ __device__ __forceinline__ void read_row(const uint8_t* codes, const uint8_t* sc
   }
 }
 template <int HD>
-__device__ __forceinline__ float score(const Args& a, const float* q, uint32_t pg, uint32_t slot, uint32_t h, int l) {
+__device__ __forceinline__ float score(const Plain& a, const float* q, uint32_t pg, uint32_t slot, uint32_t h, int l) {
   constexpr int D = HD / 64;
   float k[D], x = 0.f;
   read_row<HD>(a.pool.k + a.sh.code(pg, slot, h), a.pool.ks + a.sh.k_scale(pg, slot, h, 0), 1, l, k);
@@ -55,7 +615,7 @@ __device__ __forceinline__ float score(const Args& a, const float* q, uint32_t p
 }
 
 template <int HD>
-__global__ __launch_bounds__(NT) void attn4_row_kernel(Args a) {
+__global__ __launch_bounds__(NT) void attn4_row_kernel(Plain a) {
   constexpr int D = HD / 64;
   __shared__ float s_m[NW], s_l[NW], s_o[NW * HD];
   const uint32_t row = blockIdx.x / a.nqh, hq = blockIdx.x % a.nqh, h = hq / a.G;
@@ -110,7 +670,7 @@ __global__ __launch_bounds__(NT) void attn4_row_kernel(Args a) {
 }
 
 template <int HD>
-__global__ __launch_bounds__(NT) void attn4_mass_kernel(Args a) {
+__global__ __launch_bounds__(NT) void attn4_mass_kernel(Plain a) {
   constexpr int D = HD / 64;
   const uint32_t s = blockIdx.y / a.sh.nkh, h = blockIdx.y % a.sh.nkh;
   const int l = threadIdx.x & 63;
@@ -119,7 +679,7 @@ __global__ __launch_bounds__(NT) void attn4_mass_kernel(Args a) {
     const int32_t id = a.page_table[(size_t)s * a.max_pages + t / a.sh.page_size];
     if (id < 0 || id >= (int32_t)a.num_pages) continue;
     const uint32_t slot = t % a.sh.page_size;
-    float got = 0.f;
+    double got = 0.0;
     for (uint32_t r = 0; r < sq.n; ++r) {
       const uint32_t pos = sq.base + r;
       if (t > pos || (a.window && t + a.window <= pos)) continue;
@@ -132,17 +692,92 @@ __global__ __launch_bounds__(NT) void attn4_mass_kernel(Args a) {
         got += expf(score<HD>(a, q, (uint32_t)id, slot, h, l) - ml.x) * ml.y;
       }
     }
-    if (l == 0) a.pool.mass[a.sh.row((uint32_t)id, slot, h)] += got;
+    if (l == 0) a.pool.mass[a.sh.row((uint32_t)id, slot, h)] += (float)got;
   }
 }
 
+bool step_fits(const g4_kv4_params& p) {
+  return (uint64_t)p.max_rows * (p.num_q_heads / p.num_kv_heads) <= COLS;
+}
+// Units a sequence may have (a window of several rows spans max_rows - 1 more positions, and up to 15 of its first
+// tile).
+uint64_t most_units(const g4_kv4_params& p) {
+  uint64_t span = p.max_seq_len;
+  if (p.sliding_window) span = std::min<uint64_t>(span, (uint64_t)p.sliding_window + p.max_rows - 1 + 15);
+  return (span + UNIT - 1) / UNIT;
+}
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 template <int HD>
-int attend(g4_ctx* ctx, const g4_kv4_params& p, const Args& a) {
-  hipLaunchKernelGGL(attn4_row_kernel<HD>, dim3(p.num_rows * p.num_q_heads), dim3(NT), 0, ctx->stream, a);
+uint32_t step_wgs(const g4_kv4_params& p) {
+  return (uint32_t)std::min<uint64_t>(StepShape<HD>::WGS, most_units(p) * p.num_seqs * p.num_kv_heads);
+}
+// The parts of a workspace, one after the other.
+struct Sizes {
+  size_t meta, part, sums, scores;
+  size_t all() const { return meta + part + sums + scores; }
+};
+template <int HD>
+Sizes sizes_of(const g4_kv4_params& p, bool mass) {
+  Sizes z{};
+  const size_t pairs = (size_t)p.num_seqs * p.num_kv_heads;
+  if (step_fits(p)) {
+    z.meta = up256(pairs * sizeof(uint2));
+    z.part = up256(2ull * step_wgs<HD>(p) * StepShape<HD>::SLOT * sizeof(float));
+    if (mass)
+      z.scores = pairs * most_units(p) * (p.max_rows * (p.num_q_heads / p.num_kv_heads)) * UNIT * sizeof(float);
+  }
+  if (mass) z.sums = up256((size_t)p.num_rows * p.num_q_heads * sizeof(float2));
+  return z;
+}
+
+template <int HD>
+int attend(g4_ctx* ctx, const g4_kv4_params& p, Args a, void* workspace) {
+  const Sizes z = sizes_of<HD>(p, a.mass);
+  uint8_t* w = (uint8_t*)workspace;
+  a.meta = (uint2*)w;
+  a.part = (float*)(w + z.meta);
+  a.sums = a.mass ? (float2*)(w + z.meta + z.part) : nullptr;
+  a.scores = (float*)(w + z.meta + z.part + z.sums);
+  if (step_fits(p)) {
+    const uint64_t units = most_units(p), pairs = (uint64_t)p.num_seqs * p.num_kv_heads;
+    G4_REQUIRE(units * pairs < (1ull << 31), "g4_pagedAttn4: %u sequences of up to %u positions and %u KV heads in one "
+               "call", p.num_seqs, p.max_seq_len, p.num_kv_heads);
+    G4_REQUIRE(pairs * p.max_rows * a.G < 1u << 24, "g4_pagedAttn4: %u sequences of up to %u rows of %u heads in one "
+               "call", p.num_seqs, p.max_rows, p.num_q_heads);
+    a.wgs = step_wgs<HD>(p);
+    a.units = (uint32_t)units;
+    a.columns = p.max_rows * a.G;
+    const dim3 grid(a.wgs);
+    if (a.mass) hipLaunchKernelGGL((attn4_step_kernel<HD, true>), grid, dim3(NT), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((attn4_step_kernel<HD, false>), grid, dim3(NT), 0, ctx->stream, a);
+    G4_LAUNCHED(ctx, "attn4_step");
+    if (units > 1) {  // (else no sequence has partials)
+      const dim3 merges(p.num_seqs * p.num_kv_heads * p.max_rows * a.G);
+      if (std::min<uint64_t>(units, a.wgs) <= 32 || merges.x >= 1u << 22)
+        hipLaunchKernelGGL((attn4_merge_kernel<HD, 256>), merges, dim3(256), 0, ctx->stream, a);
+      else
+        hipLaunchKernelGGL((attn4_merge_kernel<HD, 1024>), merges, dim3(1024), 0, ctx->stream, a);
+      G4_LAUNCHED(ctx, "attn4_merge");
+    }
+    if (a.mass) {
+      hipLaunchKernelGGL(attn4_weigh_kernel, dim3((unsigned)std::min<uint64_t>(units, 4096), (unsigned)pairs), dim3(UNIT),
+                         0, ctx->stream, a);
+      G4_LAUNCHED(ctx, "attn4_weigh");
+    }
+    return G4_OK;
+  }
+  G4_REQUIRE((uint64_t)p.num_rows * p.num_q_heads < 1u << 24, "g4_pagedAttn4: %u rows of %u heads in one call",
+             p.num_rows, p.num_q_heads);
+  const Plain b{a.q,
+                {(uint8_t*)a.kp, (uint8_t*)a.vp, (uint8_t*)a.ks, (uint8_t*)a.vs, a.mass},
+                {p.page_size, p.num_kv_heads, p.head_dim},
+                a.page_table, a.rows, p.num_q_heads, a.G, p.max_pages, p.num_pages, p.sliding_window, p.scale, a.out,
+                a.sums};
+  hipLaunchKernelGGL(attn4_row_kernel<HD>, dim3(p.num_rows * p.num_q_heads), dim3(NT), 0, ctx->stream, b);
   G4_LAUNCHED(ctx, "attn4_row");
-  if (!a.sums) return G4_OK;
+  if (!a.mass) return G4_OK;
   const dim3 grid(std::min(ceil_div(p.max_seq_len, NW), 4096u), p.num_seqs * p.num_kv_heads);
-  hipLaunchKernelGGL(attn4_mass_kernel<HD>, grid, dim3(NT), 0, ctx->stream, a);
+  hipLaunchKernelGGL(attn4_mass_kernel<HD>, grid, dim3(NT), 0, ctx->stream, b);
   G4_LAUNCHED(ctx, "attn4_mass");
   return G4_OK;
 }
@@ -155,7 +790,10 @@ int g4_pagedAttn4_workspace_size(g4_kv4_params p, int with_mass, size_t* bytes) 
   G4_REQUIRE(bytes, "g4_pagedAttn4_workspace_size: null out");
   int rc = g4_internal_kv8_check(__func__, p, p.max_rows == 1 && p.num_rows == p.num_seqs ? nullptr : &p.num_rows);
   if (rc) return rc;
-  *bytes = with_mass ? (size_t)p.num_rows * p.num_q_heads * sizeof(float2) : 16;
+  const bool mass = with_mass != 0;
+  const Sizes z = p.head_dim == 64 ? sizes_of<64>(p, mass) : p.head_dim == 128 ? sizes_of<128>(p, mass)
+                  : p.head_dim == 256 ? sizes_of<256>(p, mass) : sizes_of<512>(p, mass);
+  *bytes = std::max<size_t>(z.all(), 16);
   return G4_OK;
 }
 
@@ -172,31 +810,21 @@ int g4_pagedAttn4(g4_ctx* ctx, const float* q, const uint8_t* k_pool, const uint
   rc = g4_pagedAttn4_workspace_size(p, mass != nullptr, &need);
   if (rc) return rc;
   G4_REQUIRE(workspace_bytes >= need, "g4_pagedAttn4: workspace %zu bytes < %zu required", workspace_bytes, need);
-  const uintptr_t all = (uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)output | (uintptr_t)workspace;
-  G4_REQUIRE((all & 15) == 0, "g4_pagedAttn4: rows, pools and workspace must be 16-byte aligned");
-  G4_REQUIRE(!ops, "g4_pagedAttn4: operand blocks are not written");
-  G4_REQUIRE((uint64_t)p.num_rows * p.num_q_heads < 1u << 24, "g4_pagedAttn4: %u rows of %u heads in one call",
-             p.num_rows, p.num_q_heads);
+  const uintptr_t all = (uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)output |
+                        (uintptr_t)workspace | (uintptr_t)k_scale | (uintptr_t)v_scale;
+  G4_REQUIRE((all & 15) == 0, "g4_pagedAttn4: rows, pools, scales and workspace must be 16-byte aligned");
+  G4_REQUIRE(!ops || (p.head_dim % 256 == 0 && p.num_rows <= 64 && step_fits(p) && ((uintptr_t)ops & 15) == 0),
+             "g4_pagedAttn4: operand blocks need head_dim a multiple of 256, <= 64 rows, <= 16 rows x heads of a KV "
+             "head and a 16-byte aligned buffer");
   G4_REQUIRE(!mass || (uint64_t)p.num_seqs * p.num_kv_heads <= 65535, "g4_pagedAttn4: %u sequences of %u KV heads",
              p.num_seqs, p.num_kv_heads);
-  const Args a{q,
-               {(uint8_t*)k_pool, (uint8_t*)v_pool, (uint8_t*)k_scale, (uint8_t*)v_scale, mass},
-               {p.page_size, p.num_kv_heads, p.head_dim},
-               page_table,
-               {seq_lens, row_starts, p.num_seqs, p.num_rows, p.max_rows, p.max_seq_len},
-               p.num_q_heads,
-               p.num_q_heads / p.num_kv_heads,
-               p.max_pages,
-               p.num_pages,
-               p.sliding_window,
-               p.scale,
-               output,
-               mass ? (float2*)workspace : nullptr};
+  const Args a{paged_args(p, q, page_table, seq_lens, row_starts, output, ops), k_pool, v_pool, k_scale, v_scale, mass,
+               nullptr, nullptr, 0, 0};
   switch (p.head_dim) {
-    case 64: return attend<64>(ctx, p, a);
-    case 128: return attend<128>(ctx, p, a);
-    case 256: return attend<256>(ctx, p, a);
-    default: return attend<512>(ctx, p, a);
+    case 64: return attend<64>(ctx, p, a, workspace);
+    case 128: return attend<128>(ctx, p, a, workspace);
+    case 256: return attend<256>(ctx, p, a, workspace);
+    default: return attend<512>(ctx, p, a, workspace);
   }
 }
 
