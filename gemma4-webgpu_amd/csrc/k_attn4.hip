@@ -49,7 +49,12 @@ struct Args : PagedArgs {
   float* mass;              // or null
   float2* sums;             // with mass: maximum and 1 / sum of each row and query head
   float* scores;            // few rows, with mass: [sequence][KV head][unit][column][128 positions]
-  uint32_t units, columns;  // of a sequence and KV head there
+  uint32_t units, columns;  // of a sequence and KV head there; many rows: 16 columns at a time, of a KV head
+  uint8_t* qdigits;         // many rows, with mass: [KV head][16 columns][digit][128 dims][lane] 24 B, and the scales
+  uint2* qscales;
+  float* weights;           // [sequence][KV head][256 positions][split][position]
+  uint32_t splits;
+  uint32_t* done;           // many rows, with mass: whether the tiles were written
 };
 
 // ---- q as digits ----
@@ -576,124 +581,587 @@ __global__ __launch_bounds__(UNIT) void attn4_weigh_kernel(Args a) {
   }
 }
 
-constexpr int NW = NT / 64;
-
-struct Plain {
-  const float* q;
-  g4kv4::Pool pool;
-  g4kv4::Shape sh;
-  const int32_t* page_table;
-  Rows rows;
-  uint32_t nqh, G, max_pages, num_pages, window;
-  float scale;
-  float* out;
-  float2* sums;  // maximum and 1 / sum of each row and query head
+// ---------------------------------------------------------------------------
+// many rows a sequence (prompts, mixed batches)
+// ---------------------------------------------------------------------------
+//
+// Workgroup (64 columns of a sequence and KV head, part of their positions),
+// steps of 64 positions through LDS: K and its scales as stored, V as f16 in the
+// order of the P V product's operand. A wave holds 16 columns: their q digits and
+// output sums in registers; two waves per SIMD, so that one's softmax runs beside
+// the other's products. The next step's rows are on their way in registers.
+//
+// Head dim 512 (eight waves): the two waves of a column tile have 256 dims each,
+// and 32 of the step's positions each for the softmax: they hand each other
+// their sums of the other's positions, then their maxima and P, through LDS (q's
+// digits of all 512 dims in one wave would spill).
+//
+// Page ids come through LDS, 32 steps at a time: scalar loads share their counter
+// with LDS reads, so that the products of a step would wait for those of the next
+// one.
+//
+// The work is dealt to the workgroups in equal shares (Walk), one or two
+// workgroups a CU. A tile held by one workgroup is written by it, else its
+// workgroups leave partials that attn4_tile_merge_kernel adds in order.
+template <int HD>
+struct TileShape {
+  static constexpr bool PAIR = HD == 512;
+  static constexpr int NTH = PAIR ? 512 : 256;
+  static constexpr int RB = HD / 2;              // bytes of a K row
+  static constexpr int KS = RB + 16;             // its stride in LDS: 16 rows on different banks
+  static constexpr int VBYTES = TP * HD * 2;
+  static constexpr int PR = RB / 16;             // 16-byte pieces of a K row
+  static constexpr int RPI = NTH / PR < TP ? NTH / PR : TP;  // rows of a round of pieces
+  static constexpr int KP = TP / RPI;            // rounds
+  static constexpr int VD = PAIR ? 16 : HD / 16; // dims a thread moves of 4 positions of V
+  static constexpr int J = HD == 64 ? 1 : PAIR ? 2 : HD / 128;  // products of a wave's dims
+  static constexpr uint32_t WGS = HD == 512 ? 256 : HD >= 128 ? 512 : 768;  // that run at once (registers, LDS)
+  static constexpr uint32_t SLOT = TC * (HD + 2);                           // floats of a partial: max, sum [64], o
 };
+// Where a sequence's columns, 16 at a time, stand among those of all.
+__device__ __forceinline__ uint32_t first_columns(const Args& a, uint32_t s, const Seq& q) { return q.first * a.G / 16 + s; }
 
-__device__ __forceinline__ uint32_t page_at(const Plain& a, uint32_t s, uint32_t t) {
-  const int32_t pg = a.page_table[(size_t)s * a.max_pages + t / a.sh.page_size];
-  return pg < 0 ? 0u : min((uint32_t)pg, a.num_pages - 1);
-}
-// Dims l * HD / 64 .. of a row.
-template <int HD>
-__device__ __forceinline__ void read_row(const uint8_t* codes, const uint8_t* scales, uint32_t stride, int l, float* x) {
-  constexpr int D = HD / 64;
-#pragma unroll
-  for (int e = 0; e < D; ++e) {
-    const int d = l * D + e;
-    x[e] = g4kv4::value_of(codes[d / 2] >> (4 * (d & 1))) * g4kv4::scale_of(scales[d / BLOCK * stride]);
-  }
-}
-template <int HD>
-__device__ __forceinline__ float score(const Plain& a, const float* q, uint32_t pg, uint32_t slot, uint32_t h, int l) {
-  constexpr int D = HD / 64;
-  float k[D], x = 0.f;
-  read_row<HD>(a.pool.k + a.sh.code(pg, slot, h), a.pool.ks + a.sh.k_scale(pg, slot, h, 0), 1, l, k);
-#pragma unroll
-  for (int e = 0; e < D; ++e) x = fmaf(q[e], k[e], x);
-  return g4d::wave_sum_dpp(x) * a.scale;
-}
+template <int HD, bool MASS>
+__global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn4_tile_kernel(Args a) {
+  using S_ = TileShape<HD>;
+  constexpr bool PAIR = S_::PAIR;
+  constexpr int J = S_::J, KP = S_::KP, VD = S_::VD, RB = S_::RB, NB = HD / BLOCK;
+  constexpr int NE = PAIR ? 16 : HD / 16;  // products over a wave's dims
+  constexpr int PT = PAIR ? 2 : 4;         // tiles of a wave's softmax
+  constexpr int CH = 32;                   // steps whose tiles are in LDS
+  constexpr int VW = VD < 8 ? 1 : VD / 8;  // words of a thread's share of a V row
+  constexpr int SB = NB < 4 ? NB : 4, SR = NB / SB;  // bytes of K scales a thread loads, threads of a row
+  __shared__ __align__(16) uint8_t s_k[TP * S_::KS];
+  __shared__ __align__(16) uint8_t s_z[TP * NB];  // K's scales
+  __shared__ __align__(16) uint8_t s_v[S_::VBYTES];
+  __shared__ __align__(16) h8 s_p[PAIR ? 4 * 2 * 2 * 64 : 1];  // P: [column tile][32 positions][hi, lo][lane]
+  __shared__ __align__(16) f4 s_d[PAIR ? 4 * 2 * 2 * 64 : 1];  // sums: [column tile][half][tile][lane]
+  __shared__ float s_mx[PAIR ? 2 * TC : 1];
+  __shared__ uint32_t s_tile[4 * CH], s_bad[TP / 4];  // s_bad: rows of V that are not finite, four a word
+  __shared__ WalkLds<S_::NTH> s_walk;
+  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), qd = l >> 4, c = l & 15;
+  const int wc = w & 3, wd = PAIR ? w >> 2 : 0;  // column tile; half
+  Walk<S_::NTH> walk{a, s_walk};
+  const bool ok = walk.begin();
+  if (MASS && blockIdx.x == 0 && tid == 0) *a.done = ok;
+  if (!ok) return;
 
-template <int HD>
-__global__ __launch_bounds__(NT) void attn4_row_kernel(Plain a) {
-  constexpr int D = HD / 64;
-  __shared__ float s_m[NW], s_l[NW], s_o[NW * HD];
-  const uint32_t row = blockIdx.x / a.nqh, hq = blockIdx.x % a.nqh, h = hq / a.G;
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const uint32_t s = seq_of_row(a.rows, row);
-  if (s >= a.rows.num_seqs) return;
-  const Seq sq = seq_rows(a.rows, s);
-  if (row - sq.first >= sq.n) return;
-  float* out = a.out + (size_t)blockIdx.x * HD;
-  if (!sq.len) {
-    for (int d = threadIdx.x; d < HD; d += NT) out[d] = 0.f;
-    return;
-  }
-  const uint32_t pos = sq.base + (row - sq.first), lo = a.window && pos + 1 > a.window ? pos + 1 - a.window : 0u;
-  float q[D], o[D], m = -INFINITY, sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < D; ++e) {
-    q[e] = a.q[(size_t)blockIdx.x * HD + l * D + e];
-    o[e] = 0.f;
-  }
-  for (uint32_t t = lo + w; t <= pos; t += NW) {
-    const uint32_t pg = page_at(a, s, t), slot = t % a.sh.page_size;
-    const float x = score<HD>(a, q, pg, slot, h, l);
-    const float mn = fmaxf(m, x), al = expf(m - mn), p = expf(x - mn);
-    float v[D];
-    read_row<HD>(a.pool.v + a.sh.code(pg, slot, h), a.pool.vs + a.sh.v_scale(pg, slot, h, 0), 16, l, v);
-    m = mn;
-    sum = sum * al + p;
-#pragma unroll
-    for (int e = 0; e < D; ++e) o[e] = o[e] * al + p * v[e];
-  }
-  if (l == 0) {
-    s_m[w] = m;
-    s_l[w] = sum;
-  }
-#pragma unroll
-  for (int e = 0; e < D; ++e) s_o[w * HD + l * D + e] = o[e];
-  __syncthreads();
-  float M = s_m[0], L = 0.f;
-  for (int i = 1; i < NW; ++i) M = fmaxf(M, s_m[i]);
-  float f[NW];
-  for (int i = 0; i < NW; ++i) {
-    f[i] = s_m[i] == -INFINITY ? 1.f : expf(s_m[i] - M);  // (-Inf: sums of 0, or NaN)
-    L += f[i] * s_l[i];
-  }
-  for (int d = threadIdx.x; d < HD; d += NT) {
-    float y = 0.f;
-    for (int i = 0; i < NW; ++i) y += f[i] * s_o[i * HD + d];
-    out[d] = y / L;
-  }
-  if (a.sums && threadIdx.x == 0) a.sums[blockIdx.x] = make_float2(M, 1.0f / L);
-}
+  Part pt;
+  while (walk.next(pt)) {
+    __syncthreads();  // the previous tile's rows are done with
+    const uint32_t ncols = pt.q.n * a.G, base = pt.q.base, first = pt.q.first, kvh = pt.kvh, ct = pt.ct;
+    const uint32_t lo = pt.t.lo, end = pt.t.end, st0 = pt.st0, st1 = pt.st1;
+    const uint32_t rs = a.nkh * RB, ss = a.nkh * NB;
+    const uint32_t t0 = lo / 16, tlast = (end - 1) / 16;
+    const int32_t* list = a.page_table + (size_t)pt.s * a.max_pages;
 
-template <int HD>
-__global__ __launch_bounds__(NT) void attn4_mass_kernel(Plain a) {
-  constexpr int D = HD / 64;
-  const uint32_t s = blockIdx.y / a.sh.nkh, h = blockIdx.y % a.sh.nkh;
-  const int l = threadIdx.x & 63;
-  const Seq sq = seq_rows(a.rows, s);
-  for (uint32_t t = blockIdx.x * NW + (threadIdx.x >> 6); t < sq.len; t += gridDim.x * NW) {
-    const int32_t id = a.page_table[(size_t)s * a.max_pages + t / a.sh.page_size];
-    if (id < 0 || id >= (int32_t)a.num_pages) continue;
-    const uint32_t slot = t % a.sh.page_size;
-    double got = 0.0;
-    for (uint32_t r = 0; r < sq.n; ++r) {
-      const uint32_t pos = sq.base + r;
-      if (t > pos || (a.window && t + a.window <= pos)) continue;
-      for (uint32_t g = 0; g < a.G; ++g) {
-        const size_t at = (size_t)(sq.first + r) * a.nqh + h * a.G + g;
-        float q[D];
+    // this lane's column
+    const uint32_t g = ct * TC + 16 * wc + c, gr = min(g, ncols - 1);
+    const uint32_t cpos = base + div_g(a, gr);
+    const uint32_t clo = a.window && cpos + 1 > a.window ? cpos + 1 - a.window : 0u;
+    const uint32_t width = g < ncols ? cpos + 1 - clo : 0u;
+    // positions every column sees: those from the last row's window on, up to the first row's own; and that any sees
+    const uint32_t r0 = base + div_g(a, ct * TC), all0 = a.window && end > a.window ? end - a.window : 0u, all1 = r0;
+    const uint32_t any0 = a.window && r0 + 1 > a.window ? r0 + 1 - a.window : 0u;
+
+    // ---- rows on their way ----
+    i4 kr[KP];
+    uint32_t zr = 0, vr_[4][VW], vw = 0;
+    // This thread's V: positions 4 vq .. + 3 of tile vt, dims from vdim on.
+    const int vt = 2 * (PAIR ? (w >> 1) & 1 : w >> 1) + (l >> 5), vq = 2 * (w & 1) + ((l >> 4) & 1);
+    const uint32_t vdim = PAIR ? 256 * wd + 16 * c : VD * c;
+    const bool has_k = S_::PR * S_::RPI >= S_::NTH || tid < S_::PR * S_::RPI;
+    const uint32_t kpiece = tid % S_::PR * 16, krow = tid / S_::PR;
+    const uint32_t v_at = 4 * vq * rs + vdim / 2, vs_at = vdim / BLOCK * 16 + 4 * vq;
+    const uint32_t zrow = tid / SR, zbyte = tid % SR * SB;
+    const uint8_t *kp = a.kp + kvh * RB, *vp = a.vp + kvh * RB, *kz = a.ks + kvh * NB;
+    auto refill = [&](uint32_t st) __attribute__((always_inline)) {  // tiles (of the pool) of the steps from `st` on
+      if (tid < 4 * CH) {
+        const uint32_t t = min(t0 + 4 * st + tid, tlast), at = page_of(a, t);
+        s_tile[tid] = clamp_page(a, list[at]) * a.page_tiles + (t - at * a.page_tiles);
+      }
+      __syncthreads();
+    };
+    auto load_k = [&](uint32_t k) __attribute__((always_inline)) {  // (of the refilled steps)
+      if (has_k) {
 #pragma unroll
-        for (int e = 0; e < D; ++e) q[e] = a.q[at * HD + l * D + e];
-        const float2 ml = a.sums[at];
-        got += expf(score<HD>(a, q, (uint32_t)id, slot, h, l) - ml.x) * ml.y;
+        for (int i = 0; i < KP; ++i) {
+          const uint32_t row = i * S_::RPI + krow;
+          kr[i] = *(const i4*)(kp + (size_t)s_tile[4 * k + row / 16] * (16 * rs) + (row % 16 * rs + kpiece));
+        }
+      }
+      if (SR * TP >= S_::NTH || tid < SR * TP) {
+        const uint8_t* z = kz + (size_t)s_tile[4 * k + zrow / 16] * (16 * ss) + (zrow % 16 * ss + zbyte);
+        zr = SB == 4 ? *(const uint32_t*)z : *(const uint16_t*)z;
+      }
+    };
+    auto load_v = [&](uint32_t k) __attribute__((always_inline)) {
+      const size_t t = s_tile[4 * k + vt];
+      const uint8_t* x = vp + t * (16 * rs) + v_at;
+      vw = *(const uint32_t*)(a.vs + (t * a.nkh + kvh) * (NB * 16) + vs_at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (VW == 2) {
+          const uint2 y = *(const uint2*)(x + i * rs);
+          vr_[i][0] = y.x;
+          vr_[i][1] = y.y;
+        } else if constexpr (VD == 8) {
+          vr_[i][0] = *(const uint32_t*)(x + i * rs);
+        } else {
+          vr_[i][0] = *(const uint16_t*)(x + i * rs);
+        }
+      }
+    };
+    // K rows as they are; V [32 positions][product e][lane (q, c)] 16 B: slots 4 (tile & 1) + i of position 4 q + i
+    auto store_step = [&](uint32_t st) __attribute__((always_inline)) {
+      if (has_k) {
+#pragma unroll
+        for (int i = 0; i < KP; ++i) *(i4*)(s_k + (i * S_::RPI + krow) * S_::KS + kpiece) = kr[i];
+      }
+      if (SR * TP >= S_::NTH || tid < SR * TP) {
+        if constexpr (SB == 4) *(uint32_t*)(s_z + zrow * NB + zbyte) = zr;
+        else *(uint16_t*)(s_z + zrow * NB + zbyte) = (uint16_t)zr;
+      }
+      float sc[4] = {exponent<0>(vw), exponent<1>(vw), exponent<2>(vw), exponent<3>(vw)};
+      const uint32_t p0 = lo + TP * st;
+      uint32_t bad = 0;
+      if (p0 < any0 || p0 + TP > end || __ballot(any_bad(vw))) {  // (uniform) rows that no column sees hold anything
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t pos = p0 + 16 * vt + 4 * vq + i;
+          const bool seen = pos >= any0 && pos < end;
+          if (seen && sc[i] == INFINITY) bad |= 1u << i;
+          if (!seen || sc[i] == INFINITY) sc[i] = 0.f;
+        }
+      }
+      if (wd == 0 && c == 0) s_bad[4 * vt + vq] = bad;
+      uint8_t* dst = s_v + (((vt >> 1) * (PAIR ? 2 : 1) + wd) * NE * 64 + vq * 16 + c) * 16 + (vt & 1) * 8;
+      static_for<VD / 2>([&](auto e) __attribute__((always_inline)) {
+        constexpr int k = decltype(e)::value;
+        h2 x, y, x2, y2;
+        two_by_two<k % 4>(vr_[0][k / 4], sc[0], vr_[1][k / 4], sc[1], x, y);
+        two_by_two<k % 4>(vr_[2][k / 4], sc[2], vr_[3][k / 4], sc[3], x2, y2);
+        *(g4mm::u32x2*)(dst + 2 * k * 1024) =
+            g4mm::u32x2{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x2)};
+        *(g4mm::u32x2*)(dst + (2 * k + 1) * 1024) =
+            g4mm::u32x2{__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, y2)};
+      });
+    };
+    refill(st0);
+    load_k(0);
+    load_v(0);
+
+    // ---- q's digits: the scale's sign goes to q; a scale of 0 leaves equal scores ----
+    i6 qb[DIGITS][J];
+    uint2 qs[J];
+    const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
+    const float sc = a.scale == 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);  // (0 times a masked -Inf: NaN)
+    static_for<J>([&](auto jj) __attribute__((always_inline)) {
+      constexpr int j = decltype(jj)::value;
+      const bool pad = HD == 64 && qd >= 2;
+      const float* qg = a.q + row_of(a, first, kvh, gr) * HD + BLOCK * (pad ? 0 : qd * J + j) + 256 * wd;
+      float x[BLOCK];
+#pragma unroll
+      for (int e = 0; e < BLOCK; e += 4) {
+        const f4 y = *(const f4*)(qg + e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[e + i] = pad ? 0.f : y[i] * sign;
+      }
+      i6 code[DIGITS];
+      digits_of(x, code, qs[j].x, qs[j].y);
+#pragma unroll
+      for (int d = 0; d < DIGITS; ++d) qb[d][j] = code[d];
+    });
+    if (MASS && st0 == 0 && ct * TC + 16 * wc < ncols) {  // (for the weights, by the one that begins the tile)
+      constexpr int JT = PAIR ? 4 : J;
+      const size_t tile = (size_t)kvh * a.columns + first_columns(a, pt.s, pt.q) + 4 * ct + wc;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int jt = PAIR ? 2 * wd + j : j;
+        a.qscales[(tile * JT + jt) * 64 + l] = qs[j];
+#pragma unroll
+        for (int d = 0; d < DIGITS; ++d) {
+          uint2* to = (uint2*)(a.qdigits + ((tile * DIGITS + d) * JT + jt) * (64 * 24) + l * 24);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) to[i] = make_uint2(qb[d][j][2 * i], qb[d][j][2 * i + 1]);
+        }
       }
     }
-    if (l == 0) a.pool.mass[a.sh.row((uint32_t)id, slot, h)] += (float)got;
+
+    f4 O[NE];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) O[e] = f4{0.f, 0.f, 0.f, 0.f};
+    float m_run = kNothing, l_run = 0.f;  // of column c, times 2^15 (PAIR: l of this wave's positions)
+    const uint8_t* ka = s_k + c * S_::KS + (HD == 64 ? 16 * (qd & 1) : 16 * J * qd) + 128 * wd;
+    const uint8_t* za = s_z + c * NB + (HD == 64 ? qd & 1 : J * qd) + 8 * wd;
+    auto turn = [&](uint32_t st, uint32_t next, bool inside) __attribute__((always_inline)) {
+      // ---- scores of this wave's PT tiles ----
+      f4 x[PT];
+      f4 own[PAIR ? 2 : 1];
+      // (PAIR: the other wave's two tiles first. A tile's rows are read while the one before is multiplied.)
+      i4 A[2][J];
+      uint32_t z[2];
+      auto read_a = [&](int pp, int to) __attribute__((always_inline)) {
+        const int p = PAIR ? (2 * (wd ^ 1) + pp) & 3 : pp;
+#pragma unroll
+        for (int j = 0; j < J; ++j) A[to][j] = *(const i4*)(ka + 16 * p * S_::KS + 16 * j);
+        z[to] = J == 2 ? *(const uint16_t*)(za + 16 * p * NB) : za[16 * p * NB];
+        if (HD == 64 && qd >= 2) z[to] = 127;  // (no dims there)
+      };
+      read_a(0, 0);
+#pragma unroll
+      for (int pp = 0; pp < 4; ++pp) {
+        if (pp < 3) read_a(pp + 1, (pp + 1) & 1);
+        __builtin_amdgcn_sched_barrier(0);
+        f4 D = f4{0.f, 0.f, 0.f, 0.f};
+        static_for<DIGITS * J>([&](auto k) __attribute__((always_inline)) {
+          constexpr int d = DIGITS - 1 - decltype(k)::value / J, j = decltype(k)::value % J;  // (the smallest first)
+          D = product<j, d % 4>(A[pp & 1][j], qb[d][j], D, z[pp & 1], d == 4 ? qs[j].y : qs[j].x);
+        });
+        if constexpr (!PAIR) x[pp] = D;
+        else if (pp < 2) s_d[((wc * 2 + wd) * 2 + pp) * 64 + l] = D;
+        else own[pp - 2] = D;
+      }
+      if constexpr (PAIR) {
+        __syncthreads();
+#pragma unroll
+        for (int p = 0; p < 2; ++p) x[p] = own[p] + s_d[((wc * 2 + (wd ^ 1)) * 2 + p) * 64 + l];
+      }
+      if (__ballot(s_bad[l & 15])) {  // (uniform) a row of V that is not finite: NaN where it is seen
+#pragma unroll
+        for (int p = 0; p < PT; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (s_bad[4 * (p + (PAIR ? 2 * wd : 0)) + qd] >> i & 1u) x[p][i] = __builtin_nanf("");
+      }
+      if (!inside) {  // (uniform; the whole step twice, with and without, spills)
+        const uint32_t pb = lo + TP * st + 32 * wd + 4 * qd - clo;
+#pragma unroll
+        for (int p = 0; p < PT; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[p][i] = pb + 16 * p + i < width ? x[p][i] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int p = 0; p < PT; ++p) mx = fmaxf(mx, fmaxf(fmaxf(x[p][0], x[p][1]), fmaxf(x[p][2], x[p][3])));
+      mx = g4d::xmax32(g4d::xmax16(mx)) * sc;
+      // P relative to a power of two (PAIR: of this wave's positions), so that a later one rescales it exactly
+      const float m_own = fmaxf(m_run, ceilf(mx)), m_up = 15.f - m_own;
+      float ps = 0.f;
+      h8 ph[2], pl[2];  // of 32 positions each
+#pragma unroll
+      for (int p = 0; p < PT; ++p) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = exp2_h(fmaf(x[p][i], sc, m_up));
+        ps += (e[0] + e[1]) + (e[2] + e[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const _Float16 hi = (_Float16)e[i];
+          ph[p / 2][4 * (p & 1) + i] = hi;
+          pl[p / 2][4 * (p & 1) + i] = (_Float16)(e[i] - (float)hi);
+        }
+      }
+      ps = g4d::xsum32(g4d::xsum16(ps));
+      float m_new = m_own;
+      if constexpr (PAIR) {
+        h8* pp = s_p + (wc * 2 * 2) * 64 + l;
+        pp[(wd * 2) * 64] = ph[0];
+        pp[(wd * 2 + 1) * 64] = pl[0];
+        if (qd == 0) s_mx[wd * TC + 16 * wc + c] = m_own;
+        __syncthreads();
+        const float m_other = s_mx[(wd ^ 1) * TC + 16 * wc + c];
+        m_new = fmaxf(m_own, m_other);
+        const float f_own = exp2_h(m_own - m_new), f_other = exp2_h(m_other - m_new);
+        ps *= f_own;
+        ph[0] = pp[0];
+        pl[0] = pp[64];
+        ph[1] = pp[128];
+        pl[1] = pp[192];
+        if (__ballot(f_own != f_other)) {  // (one of them is 1; f16 ends at 2^-24, so the powers of two in two halves)
+          const float d0 = (wd ? m_other : m_own) - m_new, d1 = (wd ? m_own : m_other) - m_new;
+          const float a0 = ceilf(d0 * 0.5f), a1 = ceilf(d1 * 0.5f);
+          const _Float16 f0 = (_Float16)exp2_h(a0), g0 = (_Float16)exp2_h(d0 - a0);
+          const _Float16 f1 = (_Float16)exp2_h(a1), g1 = (_Float16)exp2_h(d1 - a1);
+          ph[0] = ph[0] * f0 * g0;
+          pl[0] = pl[0] * f0 * g0;
+          ph[1] = ph[1] * f1 * g1;
+          pl[1] = pl[1] * f1 * g1;
+        }
+      }
+      const float alpha = exp2_h(m_run - m_new);
+      l_run = l_run * alpha + ps;
+      m_run = m_new;
+      if (__ballot(alpha != 1.f)) {  // O's rows are columns 4 qd + i
+        float ar[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ar[i] = __shfl(alpha, 4 * qd + i, 64);
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) O[e][i] *= ar[i];
+      }
+      load_v(next);
+      // ---- P V ----
+      // groups of four dims and 32 positions, the next group's operands read while one is multiplied
+      const uint8_t* vb = s_v + wd * NE * 1024 + l * 16;
+      h8 B[2][4];
+      auto read_b = [&](int u, h8* to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = *(const h8*)(vb + ((u & 1) * (PAIR ? 2 : 1) * NE + u / 2 * 4 + e) * 1024);
+      };
+      read_b(0, B[0]);
+#pragma unroll
+      for (int u = 0; u < NE / 2; ++u) {
+        if (u + 1 < NE / 2) read_b(u + 1, B[(u + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f4& o = O[u / 2 * 4 + e];
+          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[u & 1], B[u & 1][e], o, 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f4& o = O[u / 2 * 4 + e];
+          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[u & 1], B[u & 1][e], o, 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    for (uint32_t st = st0; st < st1; ++st) {
+      __syncthreads();  // every wave is done with the previous step's rows
+      store_step(st);
+      __syncthreads();
+      // the next step's rows are in flight during this one, K's from before its scores, V's from before its P V (past
+      // the last step: its own rows again, not used)
+      const uint32_t next = (min(st + 1, st1 - 1) - st0) % CH;
+      if (next == 0 && st + 1 < st1) refill(st + 1);  // (uniform)
+      load_k(next);
+      const uint32_t p0 = lo + TP * st;
+      turn(st, next, p0 >= all0 && p0 + TP - 1 <= all1);
+    }
+
+    // ---- columns 4 qd + i of the wave's tile, dims NE c + e (PAIR: 256 wd + 16 c + e) ----
+    if constexpr (PAIR) {
+      __syncthreads();
+      if (qd == 0) s_mx[wd * TC + 16 * wc + c] = l_run;
+      __syncthreads();
+      l_run = s_mx[16 * wc + c] + s_mx[TC + 16 * wc + c];
+    }
+    const bool whole = st1 - st0 == pt.t.steps;
+    float* part = a.part + (size_t)pt.slot * S_::SLOT;
+    // Row by row through LDS (where V was), so that a wave stores whole KB: lanes storing their own 16 bytes of every 64
+    // take four times the requests. Four dims of a lane turned by c: its 16 lanes meet different banks.
+    constexpr int RD = NE * 16, QG = NE / 4, RPS = 16 / NE;  // a wave's dims of a row; a lane's groups; rows a store
+    if constexpr (!PAIR) __syncthreads();  // (every wave is done with V)
+    float* turn_s = (float*)s_v + w * 4 * RD;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float L = __shfl(l_run, 4 * qd + i, 64), f = whole ? 1.0f / L : 1.f;
+#pragma unroll
+      for (int e = 0; e < QG; ++e)
+        *(f4*)(turn_s + qd * RD + c * NE + 4 * ((e + c) % QG)) =
+            f4{O[4 * e][i] * f, O[4 * e + 1][i] * f, O[4 * e + 2][i] * f, O[4 * e + 3][i] * f};
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");  // (the wave's own region: its LDS operations are in order)
+#pragma unroll
+      for (int r0 = 0; r0 < 4; r0 += RPS) {
+        const int r = r0 + l / (RD / 4), d4 = l % (RD / 4), lc = d4 / QG;
+        const f4 y = *(const f4*)(turn_s + r * RD + lc * NE + 4 * ((d4 % QG + lc) % QG));
+        const uint32_t col = 16 * wc + 4 * r + i, og = ct * TC + col;
+        if (og < ncols)
+          *(f4*)((whole ? a.out + row_of(a, first, kvh, og) * HD : part + 2 * TC + col * HD) + 256 * wd + 4 * d4) = y;
+      }
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
+    }
+    if (wd == 0 && qd == 0) {
+      if (!whole) {
+        part[16 * wc + c] = m_run;
+        part[TC + 16 * wc + c] = l_run;
+      } else if (MASS && g < ncols) {
+        a.sums[row_of(a, first, kvh, g)] = make_float2(m_run, kTileP / l_run);
+      }
+    }
+    if (st0 == 0 && tid == 0) a.meta[walk.tile_index(pt)] = pt.meta;
   }
+  clear_rows<HD, S_::NTH>(a);
+}
+
+// out of a row and head from its tile's partials, in order: that of workgroup
+// meta.x / 2 (slot meta.x), then slot 0 of each up to meta.y.
+template <int HD>
+__global__ __launch_bounds__(HD / 4) void attn4_tile_merge_kernel(Args a) {
+  const uint32_t row = blockIdx.x / a.nqh, head = blockIdx.x % a.nqh, d = threadIdx.x * 4;
+  const uint32_t s = seq_of_row(a.rows, row);
+  if (s >= a.rows.num_seqs) return;
+  const Seq q = seq_rows(a.rows, s);
+  if (!q.len) return;
+  const uint32_t g = (row - q.first) * a.G + head % a.G, col = g % TC;
+  const uint2 mt = a.meta[((size_t)s * a.tiles + g / TC) * a.nkh + head / a.G];
+  const uint32_t w0 = mt.x / 2, n = mt.y - w0 + 1;
+  if (n == 1) return;  // written by its workgroup
+  auto part = [&](uint32_t k) { return a.part + (size_t)(k ? 2 * (w0 + k) : mt.x) * TileShape<HD>::SLOT; };
+  constexpr int MS = 4;  // partials on their way
+  float M = kNothing, L = 0.f;
+  f4 o = f4{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t k0 = 0; k0 < n; k0 += MS) {
+    float pm[MS], pl[MS];
+    f4 po[MS];
+#pragma unroll
+    for (int k = 0; k < MS; ++k) {
+      const float* p = part(min(k0 + k, n - 1));
+      pm[k] = p[col];
+      pl[k] = p[TC + col];
+      po[k] = *(const f4*)(p + 2 * TC + col * HD + d);
+    }
+    float mn = M;
+#pragma unroll
+    for (int k = 0; k < MS; ++k) mn = fmaxf(mn, pm[k]);
+    const float al = exp2_h(M - mn);
+    L *= al;
+    o *= al;
+#pragma unroll
+    for (int k = 0; k < MS; ++k) {
+      if (k0 + k >= n) continue;
+      const float f = exp2_h(pm[k] - mn);
+      L += f * pl[k];
+      o += f * po[k];
+    }
+    M = mn;
+  }
+  *(f4*)(a.out + (size_t)blockIdx.x * HD + d) = o * (1.0f / L);
+  if (a.sums && d == 0) a.sums[blockIdx.x] = make_float2(M, kTileP / L);
+}
+
+// The weights of 256 positions of a sequence and KV head, a wave 64 of them: the
+// scores again, of K rows that stay in registers, with q's digits as the tiles left
+// them, 16 columns at a time through LDS; a lane adds up those of its column and
+// positions, over 16 column tiles and then over all (a sum of thousands in one chain
+// would be 2e-6 off), the lanes of a position at the end. Few blocks of positions:
+// the columns in `splits` parts, which attn4_mass_kernel adds in order.
+constexpr int WT = 256, WP = 256;  // threads, positions of a workgroup
+template <int HD>
+__global__ __launch_bounds__(WT, 2) void attn4_tile_weigh_kernel(Args a) {
+  constexpr int J = HD < 128 ? 1 : HD / 128, NB = HD / BLOCK, PT = 4;
+  constexpr int BYTES = DIGITS * J * 64 * 24, PIECES = BYTES / 16, PER = (PIECES + WT - 1) / WT;
+  __shared__ __align__(16) uint8_t s_q[2][BYTES];
+  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), qd = l >> 4, c = l & 15;
+  const uint32_t s = blockIdx.y / a.nkh, kvh = blockIdx.y % a.nkh;
+  const uint32_t block = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const Seq q = seq_rows(a.rows, s);
+  const uint32_t lo = first_seen(a, q), b0 = lo + block * WP;
+  if (b0 >= q.len || !*a.done) return;  // (a length of 0 too)
+  // rows that see any of the block's positions, and their columns, 16 at a time
+  const uint32_t r0 = max(b0, q.base) - q.base, last = b0 + WP - 1;
+  const bool leaves = a.window && a.window < q.len && last + a.window < q.len;  // the last rows do not see it
+  const uint32_t r1 = leaves ? last + a.window - q.base : q.n;                   // past the last that does
+  const uint32_t c0 = r0 * a.G / 16, c1 = (r1 * a.G + 15) / 16, per = (c1 - c0 + a.splits - 1) / a.splits;
+  const uint32_t ct0 = min(c0 + split * per, c1), ct1 = min(ct0 + per, c1);
+  const uint32_t ncols = q.n * a.G;
+
+  i4 A[PT][J];
+  uint32_t z[PT];
+  const uint32_t rs = a.nkh * (HD / 2), ss = a.nkh * NB, tlast = (q.len - 1) / 16;
+  const int32_t* list = a.page_table + (size_t)s * a.max_pages;
+#pragma unroll
+  for (int p = 0; p < PT; ++p) {
+    const uint32_t t = min(b0 / 16 + 4 * w + p, tlast), at = page_of(a, t);
+    const size_t tile = (size_t)clamp_page(a, list[at]) * a.page_tiles + (t - at * a.page_tiles);
+    // (dims as the tiles have them: two neighbouring blocks a lane; at head dim 512 of each half)
+    const uint32_t b = HD == 64 ? qd & 1 : HD == 128 ? qd : 2 * qd;
+    const uint8_t* k = a.kp + tile * (16 * (size_t)rs) + c * rs + kvh * (HD / 2) + 16 * b;
+    const uint8_t* y = a.ks + tile * (16 * (size_t)ss) + c * ss + kvh * NB + b;
+#pragma unroll
+    for (int j = 0; j < J; ++j) A[p][j] = *(const i4*)(k + 128 * (j / 2) + 16 * (j % 2));
+    z[p] = J == 1 ? *y : *(const uint16_t*)y;
+    if constexpr (J == 4) z[p] |= (uint32_t)*(const uint16_t*)(y + 8) << 16;
+    if (HD == 64 && qd >= 2) z[p] = 127;  // (no dims there)
+  }
+  const float sc = a.scale == 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
+  const size_t first = (size_t)kvh * a.columns + first_columns(a, s, q);
+  f4 sum[PT], part[PT];
+#pragma unroll
+  for (int p = 0; p < PT; ++p) sum[p] = part[p] = f4{0.f, 0.f, 0.f, 0.f};
+  i4 next[PER];
+  auto load = [&](uint32_t ct) __attribute__((always_inline)) {
+    const i4* from = (const i4*)(a.qdigits + (first + ct) * BYTES);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) next[i] = from[min(i * WT + tid, PIECES - 1)];
+  };
+  auto store = [&](int to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (i * WT + tid < PIECES) *(i4*)(s_q[to] + (i * WT + tid) * 16) = next[i];
+  };
+  if (ct0 < ct1) {
+    load(ct0);
+    store(0);
+  }
+  for (uint32_t ct = ct0; ct < ct1; ++ct) {
+    const int at = (ct - ct0) & 1;
+    __syncthreads();
+    if (ct + 1 < ct1) load(ct + 1);
+    const uint32_t g = 16 * ct + c, gr = min(g, ncols - 1), cpos = q.base + div_g(a, gr);
+    const uint32_t clo = a.window && cpos + 1 > a.window ? cpos + 1 - a.window : 0u;
+    const uint32_t width = g < ncols ? cpos + 1 - clo : 0u;
+    const float2 ml = a.sums[row_of(a, q.first, kvh, gr)];
+    uint2 qs[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) qs[j] = a.qscales[((first + ct) * J + j) * 64 + l];
+    f4 D[PT];
+#pragma unroll
+    for (int p = 0; p < PT; ++p) D[p] = f4{0.f, 0.f, 0.f, 0.f};
+    static_for<DIGITS * J>([&](auto k) __attribute__((always_inline)) {
+      constexpr int d = DIGITS - 1 - decltype(k)::value / J, j = decltype(k)::value % J;  // (the smallest first)
+      const uint2* from = (const uint2*)(s_q[at] + ((d * J + j) * 64 + l) * 24);
+      i6 B;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const uint2 y = from[i];
+        B[2 * i] = (int)y.x;
+        B[2 * i + 1] = (int)y.y;
+      }
+#pragma unroll
+      for (int p = 0; p < PT; ++p) D[p] = product<j, d % 4>(A[p][j], B, D[p], z[p], d == 4 ? qs[j].y : qs[j].x);
+    });
+    const uint32_t pb = b0 + 64 * w + 4 * qd - clo;
+#pragma unroll
+    for (int p = 0; p < PT; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        part[p][i] += pb + 16 * p + i < width ? exp2_h(fmaf(D[p][i], sc, -ml.x)) * ml.y : 0.f;
+    if ((ct - ct0) % 16 == 15 || ct + 1 == ct1) {
+#pragma unroll
+      for (int p = 0; p < PT; ++p) {
+        sum[p] += part[p];
+        part[p] = f4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+    if (ct + 1 < ct1) store(at ^ 1);
+  }
+  const size_t out = ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * WP;
+#pragma unroll
+  for (int p = 0; p < PT; ++p)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float y = g4d::sum16(sum[p][i]);
+      if (c == 4 * p + i) a.weights[out + 64 * w + 16 * p + 4 * qd + i] = y;
+    }
+}
+// Adds the parts of each position's weight, a thread each.
+__global__ __launch_bounds__(WP) void attn4_mass_kernel(Args a) {
+  const uint32_t s = blockIdx.y / a.nkh, kvh = blockIdx.y % a.nkh, i = threadIdx.x;
+  const Seq q = seq_rows(a.rows, s);
+  const uint32_t t = first_seen(a, q) + blockIdx.x * WP + i;
+  if (t >= q.len || !*a.done) return;
+  const float* from = a.weights + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * a.splits * WP + i;
+  float got = 0.f;
+  for (uint32_t k = 0; k < a.splits; ++k) got += from[(size_t)k * WP];
+  const uint32_t tile = t / 16, page = page_of(a, tile);
+  const int32_t id = a.page_table[(size_t)s * a.max_pages + page];
+  if (id >= 0 && id < (int32_t)a.num_pages)
+    a.mass[((size_t)id * (a.page_tiles * 16) + (t - page * a.page_tiles * 16)) * a.nkh + kvh] += got;
 }
 
 bool step_fits(const g4_kv4_params& p) {
@@ -713,9 +1181,27 @@ uint32_t step_wgs(const g4_kv4_params& p) {
 }
 // The parts of a workspace, one after the other.
 struct Sizes {
-  size_t meta, part, sums, scores;
-  size_t all() const { return meta + part + sums + scores; }
+  size_t meta, part, sums, scores, digits, scales, weights, done;
+  size_t all() const { return meta + part + sums + scores + digits + scales + weights + done; }
 };
+// Many rows: 256 positions at a time of a sequence, parts of their columns (so many that the workgroups fill the device,
+// of eight column tiles or more), and how often 16 columns may begin (those of each sequence by themselves).
+uint64_t weigh_blocks(const g4_kv4_params& p) {
+  uint64_t span = p.max_seq_len;
+  if (p.sliding_window) span = std::min<uint64_t>(span, (uint64_t)p.sliding_window + p.max_rows - 1 + 15);
+  return (span + WP - 1) / WP;
+}
+uint32_t weigh_splits(const g4_kv4_params& p) {
+  const uint64_t blocks = weigh_blocks(p) * p.num_seqs * p.num_kv_heads, tiles = tiles_of(p) * (TC / 16);
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / blocks, tiles / 8));
+}
+uint64_t weigh_columns(const g4_kv4_params& p) {
+  return (uint64_t)p.num_rows * (p.num_q_heads / p.num_kv_heads) / 16 + p.num_seqs + 1;
+}
+template <int HD>
+uint32_t tile_wgs(const g4_kv4_params& p) {
+  return (uint32_t)std::min<uint64_t>(TileShape<HD>::WGS, (all_cost(p) + kLeast - 1) / kLeast);
+}
 template <int HD>
 Sizes sizes_of(const g4_kv4_params& p, bool mass) {
   Sizes z{};
@@ -725,6 +1211,16 @@ Sizes sizes_of(const g4_kv4_params& p, bool mass) {
     z.part = up256(2ull * step_wgs<HD>(p) * StepShape<HD>::SLOT * sizeof(float));
     if (mass)
       z.scores = pairs * most_units(p) * (p.max_rows * (p.num_q_heads / p.num_kv_heads)) * UNIT * sizeof(float);
+  } else {
+    z.meta = up256(pairs * tiles_of(p) * sizeof(uint2));
+    z.part = up256(2ull * tile_wgs<HD>(p) * TileShape<HD>::SLOT * sizeof(float));
+    if (mass) {
+      const size_t lanes = p.num_kv_heads * weigh_columns(p) * (HD < 128 ? 1 : HD / 128) * 64;
+      z.digits = up256(lanes * DIGITS * 24);
+      z.scales = up256(lanes * sizeof(uint2));
+      z.weights = up256(pairs * weigh_blocks(p) * weigh_splits(p) * WP * sizeof(float));
+      z.done = 256;
+    }
   }
   if (mass) z.sums = up256((size_t)p.num_rows * p.num_q_heads * sizeof(float2));
   return z;
@@ -766,18 +1262,34 @@ int attend(g4_ctx* ctx, const g4_kv4_params& p, Args a, void* workspace) {
     }
     return G4_OK;
   }
-  G4_REQUIRE((uint64_t)p.num_rows * p.num_q_heads < 1u << 24, "g4_pagedAttn4: %u rows of %u heads in one call",
+  a.tiles = tiles_of(p);
+  G4_REQUIRE(all_cost(p) < (1ull << 31) && (uint64_t)a.tiles * p.num_seqs * p.num_kv_heads < (1ull << 31),
+             "g4_pagedAttn4: %u sequences of up to %u rows and %u positions in one call", p.num_seqs, p.max_rows,
+             p.max_seq_len);
+  G4_REQUIRE((uint64_t)p.num_rows * p.num_q_heads < 1u << 25, "g4_pagedAttn4: %u rows of %u heads in one call",
              p.num_rows, p.num_q_heads);
-  const Plain b{a.q,
-                {(uint8_t*)a.kp, (uint8_t*)a.vp, (uint8_t*)a.ks, (uint8_t*)a.vs, a.mass},
-                {p.page_size, p.num_kv_heads, p.head_dim},
-                a.page_table, a.rows, p.num_q_heads, a.G, p.max_pages, p.num_pages, p.sliding_window, p.scale, a.out,
-                a.sums};
-  hipLaunchKernelGGL(attn4_row_kernel<HD>, dim3(p.num_rows * p.num_q_heads), dim3(NT), 0, ctx->stream, b);
-  G4_LAUNCHED(ctx, "attn4_row");
+  a.wgs = tile_wgs<HD>(p);
+  if (a.mass) {
+    a.columns = (uint32_t)weigh_columns(p);
+    a.splits = weigh_splits(p);
+    a.qdigits = w + z.meta + z.part + z.sums + z.scores;
+    a.qscales = (uint2*)(a.qdigits + z.digits);
+    a.weights = (float*)((uint8_t*)a.qscales + z.scales);
+    a.done = (uint32_t*)((uint8_t*)a.weights + z.weights);
+  }
+  const dim3 grid(a.wgs), threads(TileShape<HD>::NTH);
+  if (a.mass) hipLaunchKernelGGL((attn4_tile_kernel<HD, true>), grid, threads, 0, ctx->stream, a);
+  else hipLaunchKernelGGL((attn4_tile_kernel<HD, false>), grid, threads, 0, ctx->stream, a);
+  G4_LAUNCHED(ctx, "attn4_tile");
+  if (a.wgs > 1) {  // (else no tile has partials)
+    hipLaunchKernelGGL(attn4_tile_merge_kernel<HD>, dim3(p.num_rows * p.num_q_heads), dim3(HD / 4), 0, ctx->stream, a);
+    G4_LAUNCHED(ctx, "attn4_tile_merge");
+  }
   if (!a.mass) return G4_OK;
-  const dim3 grid(std::min(ceil_div(p.max_seq_len, NW), 4096u), p.num_seqs * p.num_kv_heads);
-  hipLaunchKernelGGL(attn4_mass_kernel<HD>, grid, dim3(NT), 0, ctx->stream, b);
+  const unsigned blocks = (unsigned)weigh_blocks(p), pairs = p.num_seqs * p.num_kv_heads;
+  hipLaunchKernelGGL(attn4_tile_weigh_kernel<HD>, dim3(blocks * a.splits, pairs), dim3(WT), 0, ctx->stream, a);
+  G4_LAUNCHED(ctx, "attn4_tile_weigh");
+  hipLaunchKernelGGL(attn4_mass_kernel, dim3(blocks, pairs), dim3(WP), 0, ctx->stream, a);
   G4_LAUNCHED(ctx, "attn4_mass");
   return G4_OK;
 }
@@ -819,7 +1331,7 @@ int g4_pagedAttn4(g4_ctx* ctx, const float* q, const uint8_t* k_pool, const uint
   G4_REQUIRE(!mass || (uint64_t)p.num_seqs * p.num_kv_heads <= 65535, "g4_pagedAttn4: %u sequences of %u KV heads",
              p.num_seqs, p.num_kv_heads);
   const Args a{paged_args(p, q, page_table, seq_lens, row_starts, output, ops), k_pool, v_pool, k_scale, v_scale, mass,
-               nullptr, nullptr, 0, 0};
+               nullptr, nullptr, 0, 0, nullptr, nullptr, nullptr, 1, nullptr};
   switch (p.head_dim) {
     case 64: return attend<64>(ctx, p, a, workspace);
     case 128: return attend<128>(ctx, p, a, workspace);

@@ -524,9 +524,6 @@ __global__ __launch_bounds__(MT) void attn8_merge_kernel(Args a) {
 // and P V, 1.75 times that as digits and halves) 94 us, then 12.3 for the 95 MB of
 // partials and output, by the trace's kernel times; both together 94 us in passes
 // one after the other without it.
-constexpr int TC = 64, TP = 64;  // columns of a workgroup, positions of a step
-constexpr float kTileP = 32768.f;
-constexpr uint32_t kTileCost = 3, kLeast = 4;  // cost of a tile besides its steps; least cost of a share
 constexpr float kNothing = -3e38f;  // the maximum of no positions: finite, so that differences are
 template <int HD>
 struct TileShape {
@@ -541,25 +538,6 @@ struct TileShape {
   static constexpr uint32_t WGS = HD == 512 ? 256 : HD >= 128 ? 512 : 768;  // that run at once (registers, LDS)
   static constexpr uint32_t SLOT = TC * (HD + 2);                           // floats of a partial: max, sum [64], o
 };
-
-// Columns [64 ct, + 64) of a sequence and KV head: rows r0 .. r1, which see positions lo .. end - 1.
-struct Tile {
-  uint32_t lo, end, steps;
-};
-__device__ __forceinline__ Tile tile_of(const Args& a, const Seq& q, uint32_t ct) {
-  const uint32_t r0 = div_g(a, ct * TC), r1 = min(q.n - 1, div_g(a, ct * TC + TC - 1));
-  Tile t;
-  t.lo = a.window && q.base + r0 + 1 > a.window ? (q.base + r0 + 1 - a.window) & ~15u : 0u;
-  t.end = q.base + r1 + 1;
-  t.steps = (t.end - t.lo + TP - 1) / TP;
-  return t;
-}
-// Cost of column tile j % tiles of sequence j / tiles: kTileCost, then its steps (0: there is none).
-__device__ __forceinline__ uint32_t cost_of(const Args& a, uint32_t j) {
-  const Seq q = seq_rows(a.rows, j / a.tiles);
-  const uint32_t ct = j % a.tiles;
-  return q.len && ct * TC < q.n * a.G ? kTileCost + tile_of(a, q, ct).steps : 0u;
-}
 
 template <int HD>
 __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn8_tile_kernel(Args a) {
@@ -1120,18 +1098,6 @@ size_t step_bytes(const g4_kv8_params& p) {
   return meta_bytes(p) + 2ull * step_wgs<HD>(p) * StepShape<HD>::SLOT * sizeof(float);
 }
 
-// Column tiles of the longest sequence; cost of all tiles (at most).
-uint32_t tiles_of(const g4_kv8_params& p) {
-  return ceil_div((uint64_t)p.max_rows * (p.num_q_heads / p.num_kv_heads), TC);
-}
-uint64_t all_cost(const g4_kv8_params& p) {
-  const uint64_t G = p.num_q_heads / p.num_kv_heads, rows = TC / G + 2;  // of a tile
-  const uint64_t tiles =
-      std::min<uint64_t>(ceil_div(p.num_rows * G, TC) + p.num_seqs, (uint64_t)tiles_of(p) * p.num_seqs);
-  uint64_t span = p.max_seq_len;
-  if (p.sliding_window) span = std::min<uint64_t>(span, p.sliding_window + rows + 15);
-  return tiles * p.num_kv_heads * (kTileCost + ceil_div(span, TP));
-}
 template <int HD>
 uint32_t tile_wgs(const g4_kv8_params& p) {
   return (uint32_t)std::min<uint64_t>(TileShape<HD>::WGS, (all_cost(p) + kLeast - 1) / kLeast);

@@ -854,3 +854,18 @@ def test_refusals(ctx):
                  lambda: ctx.kv4Values(b, b, b, b, None, 1, 16, 1, 256, 4, b, b)):
         with pytest.raises(g4hip.G4Error):
             call()
+
+
+def test_starts_that_give_rows_to_many_sequences(ctx):
+    """Every other sequence's starts descend, the others hold all rows each: 1024 x 4096 tiles of some 1900 steps are
+    more than 32 bits number. Nothing is written or added, and every wait ends."""
+    S, rows, hd, top = 2048, 16384, 64, 1 << 17
+    p = ctx.kv4_params(S, 16, 1, hd, 1024, top // 1024, top, 2, num_rows=rows, max_rows=rows)
+    pool, scale = ctx.zeros(1024 * hd, np.uint8), ctx.from_numpy(np.full(2 * 1024 * hd // 32, 127, np.uint8))
+    table, lens = ctx.zeros(S * (top // 1024), np.int32), ctx.from_numpy(np.full(S, top, np.uint32))
+    starts = ctx.from_numpy(np.where(np.arange(S + 1) % 2, rows, 0).astype(np.uint32))
+    q, out = ctx.zeros(rows * 16 * hd, np.float32), ctx.from_numpy(np.full(rows * 16 * hd, 7.5, np.float32))
+    mass = ctx.from_numpy(np.full(2 * 1024, 2.5, np.float32))
+    ws = ctx.alloc(ctx.attn4_workspace_bytes(p, True))
+    ctx.pagedAttn4(q, pool, pool, scale, scale, table, lens, out, p, ws, row_starts=starts, mass=mass)
+    assert np.all(out.download(np.float32) == 7.5) and np.all(mass.download(np.float32) == 2.5)
