@@ -59,46 +59,52 @@ struct Args : PagedArgs {
 
 // ---- q as digits ----
 
-// 32 neighbouring elements x of q: their digits' codes (24 bytes each, first the largest), and the scale bytes of the
-// five. Non-finite ones have a scale of NaN. Ones below 2^-106 count as 0 (the last digit's scale ends there).
-__device__ __forceinline__ void digits_of(const float* x, i6* code, uint32_t& scales, uint32_t& last) {
-  float am = 0.f;
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < BLOCK; ++i) {
-    am = fmaxf(am, fabsf(x[i]));
-    nan |= x[i] != x[i];
-  }
-  const bool bad = nan || !(am < INFINITY);
-  int e = __builtin_amdgcn_frexp_expf(am) - 1;  // 2^e <= am < 2^(e + 1)
-  const bool none = bad || am == 0.f || e < -106;
-  e = none ? 0 : e;
+// The exponent of a block of q with the largest magnitude am (its bits, so that a NaN is the largest), and the scale
+// bytes of its five digits. A block that is not finite counts as 0 under a scale of NaN, one below 2^-106 as 0 (the
+// last digit's scale ends there).
+struct QScale {
+  int e;
+  bool none;
+  uint2 bytes;  // of the first four; of the last
+};
+__device__ __forceinline__ QScale q_scale(uint32_t am) {
+  QScale z;
+  const bool bad = am >= 0x7f800000u;
+  z.e = (int)(am >> 23) - 127;  // 2^e <= am < 2^(e + 1)
+  z.none = bad || z.e < -106;
+  z.e = z.none ? 0 : z.e;
+  const uint32_t s = (uint32_t)(z.e + 127);
+  z.bytes.x = bad ? 0x7f7f7f00u | BAD : s | (s - 5) << 8 | (s - 10) << 16 | (s - 15) << 24;
+  z.bytes.y = bad ? 127u : s - 20;
+  return z;
+}
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// The digits of N neighbouring elements x of a block (the rest of it taken as 0), as their codes: to(digit, code).
+template <int N, typename F>
+__device__ __forceinline__ void digits_of(const float* x, const QScale& z, F&& to) {
   f16x a, b;  // even, odd elements (the conversion takes them in turn)
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    a[i] = none ? 0.f : __builtin_amdgcn_ldexpf(x[2 * i], -e);
-    b[i] = none ? 0.f : __builtin_amdgcn_ldexpf(x[2 * i + 1], -e);
+    a[i] = 2 * i < N && !z.none ? __builtin_amdgcn_ldexpf(x[2 * i < N ? 2 * i : 0], -z.e) : 0.f;
+    b[i] = 2 * i < N && !z.none ? __builtin_amdgcn_ldexpf(x[2 * i < N ? 2 * i + 1 : 0], -z.e) : 0.f;
   }
   static_for<DIGITS>([&](auto d) __attribute__((always_inline)) {
     constexpr int D = decltype(d)::value;
     constexpr float unit = 1.f / (float)(1u << (5 * D)), border = 1572864.f * unit;  // 1.5 * 2^20: steps of 1 / 8
     if constexpr (D == DIGITS - 1) {
-      code[D] = __builtin_bit_cast(i6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, unit));
+      to(d, __builtin_bit_cast(i6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, unit)));
     } else {
-      f16x u, v;
+      f16x u{}, v{};
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; 2 * i < N; ++i) {
         u[i] = (a[i] + border) - border;
         v[i] = (b[i] + border) - border;
         a[i] -= u[i];
         b[i] -= v[i];
       }
-      code[D] = __builtin_bit_cast(i6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(u, v, unit));
+      to(d, __builtin_bit_cast(i6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(u, v, unit)));
     }
   });
-  const uint32_t s = (uint32_t)(e + 127);
-  scales = bad ? 0x7f7f7f00u | BAD : s | (s - 5) << 8 | (s - 10) << 16 | (s - 15) << 24;
-  last = bad ? 127u : s - 20;
 }
 
 // One digit of q times 128 dims of 16 K rows, added to c. KS and QS: the bytes of ks and qs with their scales.
@@ -106,6 +112,15 @@ template <int KS, int QS>
 __device__ __forceinline__ f4 product(const i4& k, const i6& q, f4 c, uint32_t ks, uint32_t qs) {
   const i8 a{k[0], k[1], k[2], k[3], 0, 0, 0, 0}, b{q[0], q[1], q[2], q[3], q[4], q[5], 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 2, KS, (int)ks, QS, (int)qs);
+}
+
+__device__ __forceinline__ void read_digit(const uint8_t* from, i6& to) {
+#pragma unroll
+  for (int e = 0; e < 3; ++e) {
+    const uint2 y = ((const uint2*)from)[e];
+    to[2 * e] = (int)y.x;
+    to[2 * e + 1] = (int)y.y;
+  }
 }
 
 // ---- V as f16 ----
@@ -129,10 +144,11 @@ __device__ __forceinline__ void two_by_two(uint32_t x, float sx, uint32_t y, flo
 // few rows a sequence (a decode step): rows * query heads per KV head <= 16
 // ---------------------------------------------------------------------------
 //
-// HBM bounds it: every byte of K and V goes from the pool to a wave's registers
-// once, in the matrix operands' order (no LDS): a lane's 16 bytes of a K row are
-// 32 dims of its A operand, and its HD / 16 neighbouring dims of 8 V rows become
-// the B operands of HD / 16 products.
+// HBM bounds it: every byte of K and V goes from the pool to LDS once, without
+// registers in between, two steps of 32 positions ahead of each wave, and from
+// there to registers in the matrix operands' order. Rows in flight in registers
+// (72 of them at head dim 256) spilled, and a spilled value's reload waits for
+// every row asked for before it.
 //
 // The positions of all sequences, in units of 128, are dealt to the workgroups
 // in equal shares whatever the lengths (a share may end in one sequence and go
@@ -145,18 +161,50 @@ __device__ __forceinline__ void two_by_two(uint32_t x, float sx, uint32_t y, flo
 constexpr int NT = 256, UNIT = 128;
 template <int HD>
 struct StepShape {
-  static constexpr uint32_t WGS = HD == 512 ? 256 : 512;  // one or two per CU (registers)
+  static constexpr uint32_t WGS = HD == 512 ? 256 : HD == 256 ? 512 : 768;  // one to three per CU (LDS)
   static constexpr uint32_t SLOT = COLS * (HD + 2);       // floats of a partial: max, sum [16], o [16][HD]
+  // A step's rows in LDS: K of two tiles, V of two tiles, scales of K, K, V, V (256 B each). 16-byte pieces of a row
+  // are exchanged by its number, so that eight rows' same pieces are on different banks.
+  static constexpr int PRW = HD / 32, KI = HD < 128 ? 1 : HD / 128;  // pieces of a row; KB of a tile (a load each)
+  static constexpr int BYTES = 4 * KI * 1024 + 1024, LOADS = 4 * KI + 4;
+  static __device__ __forceinline__ uint32_t turn(uint32_t row) {
+    return PRW >= 8 ? row & 7u : row / (8 / PRW) & (PRW - 1u);
+  }
 };
 
+// SIZE bytes a lane from base + off to LDS at `at` (uniform), lane by lane (16 apart for 16 bytes, else 4), non-temporal
+// where NT says so. Written as the instruction itself because the compiler, which knows the builtin's LDS write, waits
+// for every such load before LDS is read; the waits are the caller's. (m0 takes the LDS address, with one wait state
+// after its write; it is a reserved register, which the compiler sets at each use of its own.)
+template <int SIZE>
+__device__ __forceinline__ void to_lds(uint32_t off, const uint8_t* base, uint32_t at) {
+  if constexpr (SIZE == 16)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(at) : "memory");
+  else if constexpr (SIZE == 4)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(at) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ushort %0, %1" ::"v"(off), "s"(base), "s"(at) : "memory");
+}
+// A barrier that waits for LDS operations alone, not for the loads to LDS on their way.
+__device__ __forceinline__ void ring_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// At most N vector memory operations in flight, and no LDS one.
+template <int N>
+__device__ __forceinline__ void wait_for_lds() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(N) : "memory");
+}
+
 template <int HD, bool MASS>
-__global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn4_step_kernel(Args a) {
+__global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_step_kernel(Args a) {
+  using S_ = StepShape<HD>;
   constexpr int VB = HD / 16, NB = HD / BLOCK, J = HD < 128 ? 1 : HD / 128, BL = HD < 256 ? 1 : HD / 256;
   constexpr int VW = VB < 8 ? 1 : VB / 8;  // words of a lane's share of a V row
-  __shared__ __align__(16) float s_o[4 * COLS * HD];
-  // (the same bytes, before the waves' sums) digits as B operands: [digit][128 dims][lane] 24 B
-  uint8_t* s_q = (uint8_t*)s_o;
-  static_assert(DIGITS * J * 64 * 24 <= sizeof(s_o));
+  constexpr int KI = S_::KI, PRW = S_::PRW;
+  __shared__ __align__(1024) uint8_t s_ring[2 * 4 * S_::BYTES];  // [step in turn][wave]
+  // (the same bytes) digits as B operands, [digit][128 dims][lane] 24 B, where the second steps go; at the end the
+  // waves' sums
+  uint8_t* s_q = s_ring + 4 * S_::BYTES;
+  float* s_o = (float*)s_ring;
+  static_assert(DIGITS * J * 64 * 24 <= 4 * S_::BYTES && 4 * COLS * HD * 4 <= sizeof(s_ring));
   __shared__ __align__(8) uint2 s_qs[J * 64];
   __shared__ float s_m[4 * COLS], s_l[4 * COLS];
   const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), qd = l >> 4, c = l & 15;
@@ -202,111 +250,84 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn4_step_kernel(Args 
     const uint32_t ncols = sq.n * a.G;
     const uint32_t rs = a.nkh * (HD / 2), ss = a.nkh * NB;  // bytes from a row to the next: codes, K scales
 
-    i4 K[2][J];
-    uint32_t V[8][VW], kw[2], vw[2];
-    // page ids of the next step and, on their way, of the one after it (vector loads, issued before the rows that
-    // go before them in use: a scalar load's wait is that of the LDS reads too)
-    int32_t pg[2], pg_far[2];
-    const uint32_t st1 = 4 * (off + take), tiles = (end - lo + 15) / 16, t0 = lo / 16;
-    const uint32_t steps = min(st1, (tiles + 1) / 2);  // (the last unit may be short)
-    const uint32_t none = 0x40000000u;  // past every tile: read as 0
-    const uint32_t k_at = HD == 64 && qd >= 2 ? none : c * rs + 16 * J * qd;
-    const uint32_t ks_at = HD == 64 && qd >= 2 ? none : c * ss + J * qd;
-    const uint32_t v_at = 4 * qd * rs + VB / 2 * c, vs_at = VB * c / BLOCK * 16 + 4 * qd;
+    // This wave's steps k are those of 32 positions st0 + 4 k; their tiles (of the pool) 32 steps at a time, a lane each:
+    // a page id is asked for once, and reaches the addresses without memory in between.
+    const uint32_t st0 = 4 * off + w, tiles = (end - lo + 15) / 16, t0 = lo / 16;
+    const uint32_t last = min(4 * (off + take), (tiles + 1) / 2);  // (the last unit may be short)
+    const uint32_t n = st0 < last ? (last - st0 + 3) / 4 : 0u;
     const int32_t* list = a.page_table + (size_t)s * a.max_pages;
-    auto pages = [&](uint32_t st, int32_t* to) {
-#pragma unroll
-      for (int p = 0; p < 2; ++p) to[p] = list[page_of(a, t0 + min(2 * st + p, tiles - 1))];
+    uint32_t ahead;
+    auto refill = [&](uint32_t k) {
+      const uint32_t t = t0 + min(2 * (st0 + 4 * (k + l / 2)) + (l & 1), tiles - 1), at = page_of(a, t);
+      ahead = clamp_page(a, list[at]) * a.page_tiles + (t - at * a.page_tiles);
     };
-    // a tile's rows as buffers; of no bytes past the last step, so that nothing is read there (a branch around the
-    // loads of the next step would spill)
-    auto tile_at = [&](uint32_t st, int p) -> size_t {
-      const uint32_t t = t0 + min(2 * st + p, tiles - 1);
-      return (size_t)clamp_page(a, uni_i(pg[p])) * a.page_tiles + (t - page_of(a, t) * a.page_tiles);
-    };
-    auto buffer = [&](const uint8_t* base, uint32_t bytes, uint32_t st) -> __amdgpu_buffer_rsrc_t {
-      return __builtin_amdgcn_make_buffer_rsrc((void*)uni((uint64_t)base), (short)0, st < steps ? (int)bytes : 0,
-                                               0x00020000);
-    };
-    auto load_k = [&](uint32_t st) {
+    // where a lane's pieces are in a tile: those of row i * 64 / PRW + l / PRW in load i (head dim 64: half a load; 512:
+    // every other load's rows are four on)
+    const uint32_t pl = HD == 64 ? l & 31 : l, prow = pl / PRW, pp = pl % PRW;
+    const uint32_t piece0 = prow * rs + 16 * (pp ^ S_::turn(prow)), piece1 = prow * rs + 16 * (pp ^ S_::turn(prow + 4));
+    const uint32_t zl = HD == 64 ? l & 15 : l % (4 * NB);
+    const uint32_t kz = HD == 64 ? zl * ss : zl / (NB / 4 > 0 ? NB / 4 : 1) * ss + 4 * (zl % (NB / 4 > 0 ? NB / 4 : 1));
+    const uint32_t vz = 4 * (l % (4 * NB));
+    const uint32_t ring = uni((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)s_ring) + w * S_::BYTES;
+    auto load = [&](uint32_t k) __attribute__((always_inline)) {
+      const uint32_t to = ring + (k & 1) * (4 * S_::BYTES);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const size_t t = tile_at(st, p);
-        const __amdgpu_buffer_rsrc_t r = buffer(a.kp + t * (16 * (size_t)rs) + kvh * (HD / 2), 15 * rs + HD / 2, st);
-        const __amdgpu_buffer_rsrc_t z = buffer(a.ks + t * (16 * (size_t)ss) + kvh * NB, 15 * ss + NB, st);
-        if constexpr (J == 4) kw[p] = __builtin_amdgcn_raw_buffer_load_b32(z, ks_at, 0, 0);
-        else if constexpr (J == 2) kw[p] = __builtin_amdgcn_raw_buffer_load_b16(z, ks_at, 0, 0);
-        else kw[p] = __builtin_amdgcn_raw_buffer_load_b8(z, ks_at, 0, 0);
+        const size_t t = pick(ahead, (2 * k + p) & 63);
+        const uint8_t *kb = a.kp + t * (16 * (size_t)rs) + kvh * (HD / 2), *vb = a.vp + t * (16 * (size_t)rs) + kvh * (HD / 2);
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-          K[p][j] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(r, k_at + 16 * j, 0, 0));
-      }
-    };
-    auto load_v = [&](uint32_t st) {
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const size_t t = tile_at(st, p);
-        const __amdgpu_buffer_rsrc_t r = buffer(a.vp + t * (16 * (size_t)rs) + kvh * (HD / 2), 15 * rs + HD / 2, st);
-        const __amdgpu_buffer_rsrc_t z = buffer(a.vs + (t * a.nkh + kvh) * (NB * 16), NB * 16, st);
-        vw[p] = __builtin_amdgcn_raw_buffer_load_b32(z, vs_at, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (VW == 4) {
-            const i4 x = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(r, v_at, i * rs, 0));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) V[4 * p + i][e] = (uint32_t)x[e];
-          } else if constexpr (VW == 2) {
-            const auto x = __builtin_amdgcn_raw_buffer_load_b64(r, v_at, i * rs, 0);
-            V[4 * p + i][0] = x[0];
-            V[4 * p + i][1] = x[1];
-          } else if constexpr (VB == 8) {
-            V[4 * p + i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, v_at, i * rs, 0);
-          } else {
-            V[4 * p + i][0] = __builtin_amdgcn_raw_buffer_load_b16(r, v_at, i * rs, 0);
-          }
+        for (int i = 0; i < KI; ++i) {
+          const uint32_t piece = HD == 512 && (i & 1) ? piece1 : piece0;
+          to_lds<16>(piece, kb + i * (64 / PRW) * (size_t)rs, to + (p * KI + i) * 1024);
+          to_lds<16>(piece, vb + i * (64 / PRW) * (size_t)rs, to + ((2 + p) * KI + i) * 1024);
         }
+        to_lds<HD == 64 ? 2 : 4>(kz, a.ks + t * (16 * (size_t)ss) + kvh * NB, to + 4 * KI * 1024 + p * 256);
+        to_lds<4>(vz, a.vs + (t * a.nkh + kvh) * (NB * 16), to + 4 * KI * 1024 + 512 + p * 256);
       }
     };
 
-    // q, a thread 32 dims of a column (asked for before the rows, whose arrival its digits then do not wait for)
-    const uint32_t col = tid / (4 * J), block = tid % (4 * J);
-    float x32[BLOCK];
-    if (tid < 64 * J) {
-      const float* qg = a.q + row_of(a, sq.first, kvh, min(col, ncols - 1)) * HD + BLOCK * (HD == 64 ? block & 1 : block);
+    // q, QE dims of a column a thread (asked for before the page ids, so that it has come when the rows are asked for)
+    constexpr int QE = 16, QT = 128 * J, QC = QT / 16;  // threads that have some; of a column
+    const uint32_t col = tid / QC, qdim = tid % QC * QE, block = qdim / BLOCK;
+    float qx[QE];
+    if (tid < QT) {
+      const float* qg = a.q + row_of(a, sq.first, kvh, min(col, ncols - 1)) * HD + (HD == 64 ? qdim % 64 : qdim);
 #pragma unroll
-      for (int e = 0; e < BLOCK; e += 4) {
+      for (int e = 0; e < QE; e += 4) {
         const f4 y = *(const f4*)(qg + e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x32[e + i] = HD == 64 && block >= 2 ? 0.f : y[i];
+        for (int i = 0; i < 4; ++i) qx[e + i] = HD == 64 && block >= 2 ? 0.f : y[i];
       }
     }
-    uint32_t st = 4 * off + w;
-    // (a wave without a step too, of no bytes: behind a branch q would be waited for together with the rows)
-    pages(st, pg);
-    pages(min(st + 4, steps - 1), pg_far);  // (before the rows: what comes after them is waited for with them)
-    load_k(st);
-    load_v(st);
-    pg[0] = pg_far[0];
-    pg[1] = pg_far[1];
+    refill(0);
+    ring_barrier();  // the previous sequence's sums are done with
+    if (n > 0) load(0);  // (uniform)
     // ---- q's digits ----
-    __syncthreads();  // the previous sequence's are done with
-    if (tid < 64 * J) {
-      i6 code[DIGITS];
-      uint2 sc;
-      digits_of(x32, code, sc.x, sc.y);
+    if (tid < QT) {
+      uint32_t am = 0;
+#pragma unroll
+      for (int e = 0; e < QE; ++e) am = max(am, magnitude(qx[e]));
+      am = max(am, (uint32_t)g4d::dppi<g4d::kDppXor1>((int)am));
+      const QScale z = q_scale(am);
       const uint32_t j = block % J, lane = block / J * 16 + col;
-      s_qs[j * 64 + lane] = sc;
+      s_qs[j * 64 + lane] = z.bytes;
+      digits_of<QE>(qx, z, [&](auto d, const i6& code) __attribute__((always_inline)) {
+        uint32_t* to = (uint32_t*)(s_q + ((decltype(d)::value * J + j) * 64 + lane) * 24 + qdim % BLOCK / 4 * 3);
 #pragma unroll
-      for (int d = 0; d < DIGITS; ++d) {
-        uint2* to = (uint2*)(s_q + ((d * J + j) * 64 + lane) * 24);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) to[i] = make_uint2(code[d][2 * i], code[d][2 * i + 1]);
-      }
+        for (int i = 0; i < QE * 3 / 16; ++i) to[i] = (uint32_t)code[i];
+      });
     }
-    __syncthreads();
+    ring_barrier();
+    i6 qb[DIGITS][J];
     uint2 qs[J];
 #pragma unroll
-    for (int j = 0; j < J; ++j) qs[j] = s_qs[j * 64 + l];
+    for (int j = 0; j < J; ++j) {
+      qs[j] = s_qs[j * 64 + l];
+#pragma unroll
+      for (int d = 0; d < DIGITS; ++d) read_digit(s_q + ((d * J + j) * 64 + l) * 24, qb[d][j]);
+    }
+    ring_barrier();  // every wave has them
+    if (n > 1) load(1);
     // this lane's column: positions clo .. clo + width - 1
     const float s_scale = a.scale * kLog2e;
     const uint32_t cpos = sq.base + div_g(a, c);
@@ -319,74 +340,83 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn4_step_kernel(Args 
     f4 O[VB];
 #pragma unroll
     for (int e = 0; e < VB; ++e) O[e] = f4{0.f, 0.f, 0.f, 0.f};
-    float m_run = kNothing, l_run = 0.f;  // of column c
-    for (; st < steps; st += 4) {
-      const uint32_t next = st + 4;
-      asm volatile("" ::: "memory");  // q's digits stay in LDS (in registers they would spill)
+    float m_run = kNothing, l_run = 0.f;  // of column c, the sum times 2^15
+    // a lane's pieces of K (row c) and V (rows 4 qd + i) of a tile
+    uint32_t k_at[J], v_at[4];
+#pragma unroll
+    for (int j = 0; j < J; ++j) k_at[j] = c * (HD / 2) + 16 * ((HD == 64 ? qd & 1 : qd * J + j) ^ S_::turn(c));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t row = 4 * qd + i, byte = VB / 2 * c;
+      v_at[i] = row * (HD / 2) + 16 * (byte / 16 ^ S_::turn(row)) + byte % 16;
+    }
+    const uint32_t kz_at = HD == 64 ? 4 * c + (qd & 1) : c * NB + J * qd, vz_at = VB * c / BLOCK * 16 + 4 * qd;
+    for (uint32_t k = 0; k < n; ++k) {
+      const uint32_t st = st0 + 4 * k;
+      const uint8_t* in = s_ring + (k & 1) * (4 * S_::BYTES) + w * S_::BYTES;
+      const uint8_t* z = in + 4 * KI * 1024;
+      // this step's rows are there once at most the next one's are on their way (a store among them: all)
+      if (k + 1 < n) wait_for_lds<S_::LOADS>();
+      else wait_for_lds<0>();
       // ---- scores ----
       f4 D[2];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) D[p] = f4{0.f, 0.f, 0.f, 0.f};
-      static_for<DIGITS * J>([&](auto k) __attribute__((always_inline)) {
-        constexpr int d = DIGITS - 1 - decltype(k)::value / J, j = decltype(k)::value % J;  // (the smallest first)
-        const uint2* from = (const uint2*)(s_q + ((d * J + j) * 64 + l) * 24);
-        i6 B;
+      for (int p = 0; p < 2; ++p) {
+        uint32_t kw = J == 4 ? *(const uint32_t*)(z + 256 * p + kz_at) : J == 2 ? *(const uint16_t*)(z + 256 * p + kz_at)
+                                                                              : z[256 * p + kz_at];
+        if (HD == 64 && qd >= 2) kw = 127;  // (no dims there)
+        i4 K[J];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          const uint2 y = from[i];
-          B[2 * i] = (int)y.x;
-          B[2 * i + 1] = (int)y.y;
-        }
-#pragma unroll
-        for (int p = 0; p < 2; ++p) D[p] = product<j, d % 4>(K[p][j], B, D[p], kw[p], d == 4 ? qs[j].y : qs[j].x);
-      });
-      pages(min(st + 8, steps - 1), pg_far);
-      load_k(next);
+        for (int j = 0; j < J; ++j) K[j] = *(const i4*)(in + p * (KI * 1024) + k_at[j]);
+        D[p] = f4{0.f, 0.f, 0.f, 0.f};
+        static_for<DIGITS * J>([&](auto i) __attribute__((always_inline)) {
+          constexpr int d = DIGITS - 1 - decltype(i)::value / J, j = decltype(i)::value % J;  // (the smallest first)
+          D[p] = product<j, d % 4>(K[j], qb[d][j], D[p], kw, d == 4 ? qs[j].y : qs[j].x);
+        });
+      }
       // ---- softmax over the step's 32 positions ----
       const uint32_t p0 = lo + 32 * st, pb = p0 + 4 * qd;
+      const uint32_t vw[2] = {*(const uint32_t*)(z + 512 + vz_at), *(const uint32_t*)(z + 768 + vz_at)};
       float x[8], vsc[8], mx = -INFINITY;
-      auto live = [&](int k) { return pb + 16 * (k / 4) + k % 4 - clo < width; };
+      auto live = [&](int i) { return pb + 16 * (i / 4) + i % 4 - clo < width; };
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = D[k / 4][k % 4] * s_scale;
-      static_for<8>([&](auto k) __attribute__((always_inline)) {
-        constexpr int n = decltype(k)::value;
+      for (int i = 0; i < 8; ++i) x[i] = D[i / 4][i % 4] * s_scale;
+      static_for<8>([&](auto i) __attribute__((always_inline)) {
+        constexpr int n = decltype(i)::value;
         vsc[n] = exponent<n % 4>(vw[n / 4]);
       });
       // (uniform) rows that no column sees may hold anything; of the others, one that is not finite makes the weight of
       // every column that sees it NaN
       if (p0 < first || p0 + 32 > end || __ballot(any_bad(vw[0]) || any_bad(vw[1]))) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t pos = pb + 16 * (k / 4) + k % 4;
-          const bool bad = vsc[k] == INFINITY;
-          if (bad) x[k] = __builtin_nanf("");
-          if (bad || pos < first || pos >= end) vsc[k] = 0.f;
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t pos = pb + 16 * (i / 4) + i % 4;
+          const bool bad = vsc[i] == INFINITY;
+          if (bad) x[i] = __builtin_nanf("");
+          if (bad || pos < first || pos >= end) vsc[i] = 0.f;
         }
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) mx = fmaxf(mx, live(k) ? x[k] : -INFINITY);
+      for (int i = 0; i < 8; ++i) {
+        x[i] = live(i) ? x[i] : -INFINITY;
+        mx = fmaxf(mx, x[i]);
+      }
+      if (MASS && (uint32_t)c < ncols) {
+        float* to = score_at + (size_t)(st / 4) * a.columns * UNIT + st % 4 * 32 + 4 * qd;
+        *(f4*)to = f4{x[0], x[1], x[2], x[3]};
+        *(f4*)(to + 16) = f4{x[4], x[5], x[6], x[7]};
+      }
       mx = g4d::xmax32(g4d::xmax16(mx));
-      const float m_new = fmaxf(m_run, ceilf(mx));
+      const float m_new = fmaxf(m_run, ceilf(mx)), up = 15.f - m_new;
       const float alpha = exp2_h(m_run - m_new);
       float ps = 0.f;
       h8 ph, pl;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float e = live(k) ? exp2_h(x[k] - m_new) : 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const float e = exp2_h(x[i] + up);
         ps += e;
-        const float es = e * kPScale;
-        ph[k] = (_Float16)es;
-        pl[k] = (_Float16)(es - (float)ph[k]);
-      }
-      if (MASS && (uint32_t)c < ncols) {
-        float* to = score_at + (size_t)(st / 4) * a.columns * UNIT + st % 4 * 32 + 4 * qd;
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          f4 y;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = live(4 * p + i) ? x[4 * p + i] : -INFINITY;
-          *(f4*)(to + 16 * p) = y;
-        }
+        ph[i] = (_Float16)e;
+        pl[i] = (_Float16)(e - (float)ph[i]);
       }
       ps = g4d::xsum32(g4d::xsum16(ps));
       l_run = l_run * alpha + ps;
@@ -401,13 +431,29 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn4_step_kernel(Args 
           for (int i = 0; i < 4; ++i) O[e][i] *= ar[i];
       }
       // ---- P V, two dims (a byte of V) at a time ----
+      uint32_t V[8][VW];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint8_t* y = in + (2 + i / 4) * (KI * 1024) + v_at[i % 4];
+        if constexpr (VW == 4) {
+          const i4 x4 = *(const i4*)y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) V[i][e] = (uint32_t)x4[e];
+        } else if constexpr (VW == 2) {
+          const uint2 x2 = *(const uint2*)y;
+          V[i][0] = x2.x;
+          V[i][1] = x2.y;
+        } else {
+          V[i][0] = VB == 8 ? *(const uint32_t*)y : *(const uint16_t*)y;
+        }
+      }
       static_for<VB / 2>([&](auto e) __attribute__((always_inline)) {
-        constexpr int b = decltype(e)::value % 4, k = decltype(e)::value / 4, n = 2 * decltype(e)::value;
+        constexpr int b = decltype(e)::value % 4, v = decltype(e)::value / 4, n = 2 * decltype(e)::value;
         h8 B[2];
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           h2 y, z;
-          two_by_two<b>(V[j][k], vsc[j], V[j + 1][k], vsc[j + 1], y, z);
+          two_by_two<b>(V[j][v], vsc[j], V[j + 1][v], vsc[j + 1], y, z);
           B[0][j] = y[0];
           B[0][j + 1] = y[1];
           B[1][j] = z[0];
@@ -419,13 +465,15 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn4_step_kernel(Args 
         for (int i = 0; i < 2; ++i) O[n + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, B[i], O[n + i], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       });
-      load_v(next);
-#pragma unroll
-      for (int p = 0; p < 2; ++p) pg[p] = pg_far[p];
+      if (k + 2 < n) {  // (uniform) into the bytes that this step has read
+        if (((k + 2) & 31) == 0) refill(k + 2);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        load(k + 2);
+      }
     }
 
     // ---- the four waves' sums, in their order ----
-    __syncthreads();  // every wave is done with q's digits
+    __syncthreads();  // every wave is done with the rows
     if (qd == 0) {
       s_m[w * COLS + c] = m_run;
       s_l[w * COLS + c] = l_run;
@@ -458,7 +506,6 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn4_step_kernel(Args 
         L += s_l[k * COLS + col] * f;
         y += *(const f4*)(s_o + (k * COLS + col) * HD + d / VB * VB + 4 * ((d % VB / 4 + d / VB) % QG)) * f;
       }
-      y *= 1.f / kPScale;
       const size_t row = row_of(a, sq.first, kvh, col);
       float* o = whole ? a.out + row * HD : part + 2 * COLS + col * HD;
       if (whole) y *= 1.0f / L;
@@ -472,7 +519,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : 2) void attn4_step_kernel(Args 
           part[col] = M;
           part[COLS + col] = L;
         } else if (MASS) {
-          a.sums[row] = make_float2(M, 1.0f / L);
+          a.sums[row] = make_float2(M, kPScale / L);
         }
       }
     }
@@ -555,7 +602,7 @@ __global__ __launch_bounds__(MT) void attn4_merge_kernel(Args a) {
   y *= 1.0f / L;
   const uint32_t row = q.first + col / a.G, head = kvh * a.G + col % a.G;
   *(f4*)(a.out + ((size_t)row * a.nqh + head) * HD + d) = y;
-  if (a.sums && d == 0) a.sums[(size_t)row * a.nqh + head] = make_float2(M, 1.0f / L);
+  if (a.sums && d == 0) a.sums[(size_t)row * a.nqh + head] = make_float2(M, kPScale / L);
   if (HD >= 256 && a.ops) write_ops(a, row, head * (HD / 256) + d / 256, threadIdx.x & 63, y);
 }
 
@@ -767,10 +814,15 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn4_ti
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[e + i] = pad ? 0.f : y[i] * sign;
       }
-      i6 code[DIGITS];
-      digits_of(x, code, qs[j].x, qs[j].y);
+      uint32_t am = 0;
 #pragma unroll
-      for (int d = 0; d < DIGITS; ++d) qb[d][j] = code[d];
+      for (int e = 0; e < BLOCK; ++e) am = max(am, magnitude(x[e]));
+      const QScale q = q_scale(am);
+      qs[j] = q.bytes;
+      digits_of<BLOCK>(x, q, [&](auto d, const i6& code) __attribute__((always_inline)) {
+        qb[decltype(d)::value][j] = code;
+      });
+      __builtin_amdgcn_sched_barrier(0);  // (the next one's elements not before these are digits)
     });
     if (MASS && st0 == 0 && ct * TC + 16 * wc < ncols) {  // (for the weights, by the one that begins the tile)
       constexpr int JT = PAIR ? 4 : J;
@@ -1114,14 +1166,8 @@ __global__ __launch_bounds__(WT, 2) void attn4_tile_weigh_kernel(Args a) {
     for (int p = 0; p < PT; ++p) D[p] = f4{0.f, 0.f, 0.f, 0.f};
     static_for<DIGITS * J>([&](auto k) __attribute__((always_inline)) {
       constexpr int d = DIGITS - 1 - decltype(k)::value / J, j = decltype(k)::value % J;  // (the smallest first)
-      const uint2* from = (const uint2*)(s_q[at] + ((d * J + j) * 64 + l) * 24);
       i6 B;
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        const uint2 y = from[i];
-        B[2 * i] = (int)y.x;
-        B[2 * i + 1] = (int)y.y;
-      }
+      read_digit(s_q[at] + ((d * J + j) * 64 + l) * 24, B);
 #pragma unroll
       for (int p = 0; p < PT; ++p) D[p] = product<j, d % 4>(A[p][j], B, D[p], z[p], d == 4 ? qs[j].y : qs[j].x);
     });
@@ -1157,7 +1203,13 @@ __global__ __launch_bounds__(WP) void attn4_mass_kernel(Args a) {
   if (t >= q.len || !*a.done) return;
   const float* from = a.weights + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * a.splits * WP + i;
   float got = 0.f;
-  for (uint32_t k = 0; k < a.splits; ++k) got += from[(size_t)k * WP];
+  for (uint32_t k0 = 0; k0 < a.splits; k0 += 16) {  // (16 on their way)
+    float x[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) x[k] = from[(size_t)min(k0 + k, a.splits - 1) * WP];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) got += k0 + k < a.splits ? x[k] : 0.f;
+  }
   const uint32_t tile = t / 16, page = page_of(a, tile);
   const int32_t id = a.page_table[(size_t)s * a.max_pages + page];
   if (id >= 0 && id < (int32_t)a.num_pages)

@@ -9,6 +9,7 @@
 // own scales: nothing is ever rounded again, whatever comes after it or moves it.
 #include <algorithm>
 
+#include "attn_paged.hpp"
 #include "kv4.hpp"
 #include "kv_rows.hpp"
 
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(VT) void kv4_values_kernel(ValArgs a) {
 //
 // kv4_select_kernel, a workgroup a sequence and KV head: the order of masses is
 // that of their bits (they are above 0, or count 0), so the bound of the largest
-// is found by four rounds of 256 bins, from the top byte down; then the rows above
+// is found by three rounds of bins, from the top 11 bits down; then the rows above
 // it and the first of those at it are listed in order. kv4_gather_kernel copies
 // the rows that move to the workspace, kv4_scatter_kernel to their places: a row
 // moves down only, so its place may be where another comes from.
@@ -201,9 +202,9 @@ struct EvictArgs {
 __device__ __forceinline__ uint32_t key_of(float x) { return x > 0.f ? __float_as_uint(x) : 0u; }
 
 __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
-  constexpr int NW = ST / 64;
+  constexpr int NW = ST / 64, BINS = 2 * ST, FAR = 8;  // FAR: masses on their way
   __shared__ uint32_t s_key[CACHED];
-  __shared__ uint32_t s_bin[256], s_above[NW], s_at[NW], s_found[2];
+  __shared__ uint32_t s_bin[BINS], s_above[NW], s_at[NW], s_found[2];
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const uint32_t s = blockIdx.x / a.sh.nkh, h = blockIdx.x % a.sh.nkh;
   const uint32_t L = a.seq_lens[s];
@@ -222,30 +223,51 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
   auto fetch = [&](uint32_t i) -> uint32_t {
     const uint32_t t = a.first + i;
     const int32_t pg = list[t / a.sh.page_size];
-    return pg >= 0 && pg < (int32_t)a.num_pages ? key_of(a.pool.mass[a.sh.row((uint32_t)pg, t % a.sh.page_size, h)])
-                                                : 0u;
+    const float x = a.pool.mass[a.sh.row(pg < 0 ? 0u : min((uint32_t)pg, a.num_pages - 1), t % a.sh.page_size, h)];
+    return pg >= 0 && pg < (int32_t)a.num_pages ? key_of(x) : 0u;
   };
-  for (uint32_t i = tid; i < min(n, CACHED); i += ST) s_key[i] = fetch(i);
+  for (uint32_t i0 = tid; i0 < min(n, CACHED); i0 += FAR * ST) {
+    uint32_t k[FAR];
+#pragma unroll
+    for (int j = 0; j < FAR; ++j) k[j] = fetch(min(i0 + j * ST, n - 1));
+#pragma unroll
+    for (int j = 0; j < FAR; ++j)
+      if (i0 + j * ST < min(n, CACHED)) s_key[i0 + j * ST] = k[j];
+  }
   auto key = [&](uint32_t i) -> uint32_t { return i < CACHED ? s_key[i] : fetch(i); };
-  uint32_t bound = 0, left = m;  // the m-th largest key so far; how many of those that share its bytes are kept
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (uint32_t i = tid; i < 256; i += ST) s_bin[i] = 0;
+  uint32_t bound = 0, left = m;  // the m-th largest key so far; how many of those that share its bits are kept
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;  // 11, 11 and 10 bits
+    s_bin[2 * tid] = s_bin[2 * tid + 1] = 0;
     __syncthreads();
-    for (uint32_t i = tid; i < n; i += ST) {
-      const uint32_t k = key(i);
-      if (shift == 24 || (k ^ bound) >> (shift + 8) == 0) atomicAdd(&s_bin[k >> shift & 255u], 1u);
+    for (uint32_t i0 = 0; i0 < n; i0 += ST) {  // (every lane: the first one's bin is counted by one of them)
+      const uint32_t i = i0 + tid, k = i < n ? key(i) : 0u;
+      const bool in = i < n && (pass == 0 || (k ^ bound) >> (pass == 1 ? 21 : 10) == 0);
+      const uint32_t b = k >> shift & (pass == 2 ? 1023u : 2047u);
+      const uint64_t some = __ballot(in);
+      if (!some) continue;
+      const int one = __ffsll((unsigned long long)some) - 1;
+      const uint32_t b1 = __builtin_amdgcn_readlane(b, one);
+      const uint64_t same = __ballot(in && b == b1);
+      if (lane == (uint32_t)one) atomicAdd(&s_bin[b1], (uint32_t)__popcll(same));
+      else if (in && b != b1) atomicAdd(&s_bin[b], 1u);
     }
     __syncthreads();
-    if (tid == 0) {
-      uint32_t b = 255, above = 0;
-      while (b > 0 && above + s_bin[b] < left) above += s_bin[b--];
-      s_found[0] = b;
-      s_found[1] = above;
+    // counts from the largest bin down: two bins a thread, summed over its wave, then over the waves
+    const uint32_t hi = s_bin[BINS - 1 - 2 * tid], lo = s_bin[BINS - 2 - 2 * tid];
+    const uint32_t upto = wave_scan(hi + lo);
+    if (lane == 63) s_above[w] = upto;
+    __syncthreads();
+    uint32_t above = upto - hi - lo;
+    for (uint32_t i = 0; i < w; ++i) above += s_above[i];
+    if (above < left && above + hi + lo >= left) {  // (one thread's)
+      const bool first = above + hi >= left;
+      s_found[0] = BINS - 1 - 2 * tid - (first ? 0 : 1);
+      s_found[1] = above + (first ? 0 : hi);
     }
     __syncthreads();
     bound |= s_found[0] << shift;
     left -= s_found[1];
-    __syncthreads();
   }
   // the rows above the bound and the first `left` at it, in order: each wave counts those of its run of candidates
   const uint32_t run = ((n + NW - 1) / NW + 63) / 64 * 64, i0 = min(w * run, n), i1 = min(i0 + run, n);
@@ -255,6 +277,7 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
     above += __popcll(__ballot(i + lane < i1 && k > bound));
     at += __popcll(__ballot(i + lane < i1 && k == bound));
   }
+  __syncthreads();  // (s_above's counts of the last pass are done with)
   if (lane == 0) {
     s_above[w] = above;
     s_at[w] = at;
