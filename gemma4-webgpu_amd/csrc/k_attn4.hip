@@ -159,6 +159,7 @@ __device__ __forceinline__ void two_by_two(uint32_t x, float sx, uint32_t y, flo
 // maxima and sums are known: 4 bytes a position and column written and read, where
 // K again would be HD / 2 * 17 / 16 bytes a position and the products once more.
 constexpr int NT = 256, UNIT = 128;
+constexpr uint32_t kSeqCost = 1;  // cost of a sequence and KV head besides its units: its q, its sums
 template <int HD>
 struct StepShape {
   static constexpr uint32_t WGS = HD == 512 ? 256 : HD == 256 ? 512 : 768;  // one to three per CU (LDS)
@@ -172,8 +173,7 @@ struct StepShape {
   }
 };
 
-// SIZE bytes a lane from base + off to LDS at `at` (uniform), lane by lane (16 apart for 16 bytes, else 4), non-temporal
-// where NT says so. Written as the instruction itself because the compiler, which knows the builtin's LDS write, waits
+// SIZE bytes a lane from base + off to LDS at `at` (uniform), lane by lane (16 apart for 16 bytes, else 4). Written as the instruction itself because the compiler, which knows the builtin's LDS write, waits
 // for every such load before LDS is read; the waits are the caller's. (m0 takes the LDS address, with one wait state
 // after its write; it is a reserved register, which the compiler sets at each use of its own.)
 template <int SIZE>
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
   auto load_chunk = [&](uint32_t first) {
     c0 = first;
     mine = first + l < S ? seq_rows(a.rows, first + l) : Seq{0, 0, 0, 0};
-    mine_units = mine.len ? (mine.len - first_seen(a, mine) + UNIT - 1) / UNIT : 0u;
+    mine_units = mine.len ? (mine.len - first_seen(a, mine) + UNIT - 1) / UNIT + kSeqCost : 0u;
     incl = wave_scan(mine_units * a.nkh);
     total = __builtin_amdgcn_readlane(incl, 63);
   };
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
     for (load_chunk(0); before + total <= ub; load_chunk(c0 + 64)) before += total;
   }
 
-  uint32_t u = ub;
+  uint32_t u = ub, used = 0;  // partials written
   while (u < ue) {
     while (before + total <= u) {  // (u < T: a later chunk holds it)
       before += total;
@@ -242,11 +242,14 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
     const int at = __ffsll((unsigned long long)__ballot(before + incl > u)) - 1;
     const uint32_t s = c0 + at;
     const Seq sq{pick(mine.first, at), pick(mine.n, at), pick(mine.base, at), pick(mine.len, at)};
-    const uint32_t units = pick(mine_units, at), seq0 = before + pick(incl, at) - units * a.nkh;
+    const uint32_t cost = pick(mine_units, at), units = cost - kSeqCost, seq0 = before + pick(incl, at) - cost * a.nkh;
     const uint32_t lo = first_seen(a, sq), end = sq.len;
-    const uint32_t kvh = a.nkh == 1 ? 0u : uni((u - seq0) / units);
-    const uint32_t seg = seq0 + kvh * units;  // its first unit
-    const uint32_t off = u - seg, take = min(units - off, ue - u);
+    const uint32_t kvh = a.nkh == 1 ? 0u : uni((u - seq0) / cost);
+    const uint32_t seg = seq0 + kvh * cost, stop = min(seg + cost, ue);  // its first unit, the last here
+    const uint32_t off = max(u, seg + kSeqCost) - (seg + kSeqCost), to = max(stop, seg + kSeqCost) - (seg + kSeqCost);
+    u = stop;
+    if (off == to) continue;  // (the share ends before its first positions)
+    const uint32_t take = to - off;
     const uint32_t ncols = sq.n * a.G;
     const uint32_t rs = a.nkh * (HD / 2), ss = a.nkh * NB;  // bytes from a row to the next: codes, K scales
 
@@ -492,7 +495,8 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
     }
     __syncthreads();
     const bool whole = take == units;
-    const uint32_t slot = 2 * wg + (u == ub ? 0u : 1u);
+    const uint32_t slot = 2 * wg + used;  // (0 for a sequence begun by another workgroup: it comes first)
+    used = 1;
     float* part = a.part + (size_t)slot * StepShape<HD>::SLOT;
     for (uint32_t i = tid; i < ncols * (HD / 4); i += NT) {
       const uint32_t col = i / (HD / 4), d = i % (HD / 4) * 4;
@@ -523,8 +527,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
         }
       }
     }
-    if (off == 0 && tid == 0) a.meta[(size_t)s * a.nkh + kvh] = make_uint2(slot, sh.owner(seg + units - 1));
-    u += take;
+    if (off == 0 && tid == 0) a.meta[(size_t)s * a.nkh + kvh] = make_uint2(slot, sh.owner(seg + cost - 1));
   }
   // rows that see nothing
   for (uint32_t i = wg; i < S * a.nkh; i += gridDim.x) {
@@ -1288,7 +1291,7 @@ int attend(g4_ctx* ctx, const g4_kv4_params& p, Args a, void* workspace) {
   a.scores = (float*)(w + z.meta + z.part + z.sums);
   if (step_fits(p)) {
     const uint64_t units = most_units(p), pairs = (uint64_t)p.num_seqs * p.num_kv_heads;
-    G4_REQUIRE(units * pairs < (1ull << 31), "g4_pagedAttn4: %u sequences of up to %u positions and %u KV heads in one "
+    G4_REQUIRE((units + kSeqCost) * pairs < (1ull << 31), "g4_pagedAttn4: %u sequences of up to %u positions and %u KV heads in one "
                "call", p.num_seqs, p.max_seq_len, p.num_kv_heads);
     G4_REQUIRE(pairs * p.max_rows * a.G < 1u << 24, "g4_pagedAttn4: %u sequences of up to %u rows of %u heads in one "
                "call", p.num_seqs, p.max_rows, p.num_q_heads);

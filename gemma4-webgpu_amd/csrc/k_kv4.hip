@@ -22,9 +22,8 @@ using g4kv4::BLOCK;
 constexpr int PT = 256;    // threads of the append
 constexpr int QH = 2;      // q heads of a wave
 constexpr int VT = 256;    // of the values kernel
-constexpr int ST = 1024;   // of the selection
-constexpr int MT = 256;    // of the moves
-constexpr uint32_t CACHED = 32768;  // candidates whose masses are held in LDS
+constexpr int ST = 1024;   // of the selection and the moves
+constexpr uint32_t PER = 32;  // masses of a thread of the selection: of more candidates they are read again for each round
 
 struct ProArgs : RowArgs {
   g4kv4::Pool pool;
@@ -183,9 +182,7 @@ __global__ __launch_bounds__(VT) void kv4_values_kernel(ValArgs a) {
 // kv4_select_kernel, a workgroup a sequence and KV head: the order of masses is
 // that of their bits (they are above 0, or count 0), so the bound of the largest
 // is found by three rounds of bins, from the top 11 bits down; then the rows above
-// it and the first of those at it are listed in order. kv4_gather_kernel copies
-// the rows that move to the workspace, kv4_scatter_kernel to their places: a row
-// moves down only, so its place may be where another comes from.
+// it and the first of those at it are listed in order. kv4_move_kernel moves them.
 struct EvictArgs {
   g4kv4::Pool pool;
   g4kv4::Shape sh;
@@ -193,18 +190,16 @@ struct EvictArgs {
   uint32_t* seq_lens;
   uint32_t num_seqs, max_pages, num_pages, max_seq_len, keep, first, recent;
   int32_t* kept;
-  uint32_t* cut;   // per sequence: whether it is cut
-  uint8_t* rows;   // what moves: codes [num_seqs][nkh][keep][hd], then scales [..][hd / 16], then masses
-  uint8_t* scales;
-  float* mass;
+  uint32_t* cut;  // per sequence: whether it is cut
+  uint32_t some;  // pieces of a row that a workgroup moves
 };
 
 __device__ __forceinline__ uint32_t key_of(float x) { return x > 0.f ? __float_as_uint(x) : 0u; }
 
 __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
-  constexpr int NW = ST / 64, BINS = 2 * ST, FAR = 8;  // FAR: masses on their way
-  __shared__ uint32_t s_key[CACHED];
-  __shared__ uint32_t s_bin[BINS], s_above[NW], s_at[NW], s_found[2];
+  constexpr uint32_t NW = ST / 64, BINS = 2 * ST, GROUP = PER * ST;
+  __shared__ uint32_t s_bin[BINS], s_sum[2 * NW], s_found[3];
+  __shared__ uint32_t s_above[PER * NW], s_at[PER * NW];
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const uint32_t s = blockIdx.x / a.sh.nkh, h = blockIdx.x % a.sh.nkh;
   const uint32_t L = a.seq_lens[s];
@@ -219,133 +214,197 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
   for (uint32_t i = tid; i < a.recent; i += ST) kept[a.keep - a.recent + i] = (int32_t)(L - a.recent + i);
   const uint32_t n = L - a.first - a.recent, m = a.keep - a.first - a.recent;  // of n candidates m are kept, m < n
   if (m == 0) return;  // (uniform)
+  const uint32_t groups = (n + GROUP - 1) / GROUP;
   const int32_t* list = a.page_table + (size_t)s * a.max_pages;
-  auto fetch = [&](uint32_t i) -> uint32_t {
-    const uint32_t t = a.first + i;
-    const int32_t pg = list[t / a.sh.page_size];
-    const float x = a.pool.mass[a.sh.row(pg < 0 ? 0u : min((uint32_t)pg, a.num_pages - 1), t % a.sh.page_size, h)];
-    return pg >= 0 && pg < (int32_t)a.num_pages ? key_of(x) : 0u;
+  uint32_t key[PER];  // of candidates g * GROUP + j * ST + tid
+  auto rows_of = [&](uint32_t g) { return min(n - g * GROUP, GROUP); };
+  auto fetch = [&](uint32_t g) {
+    const uint32_t rows = rows_of(g);
+    int32_t pg[PER];
+    // (all of the page ids on their way, then all of the masses; eight rows at a time, past the last that one again)
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) {
+      if (j % 8 == 0 && j * ST >= rows) break;  // (uniform)
+      pg[j] = list[(a.first + g * GROUP + min(j * ST + tid, rows - 1)) / a.sh.page_size];
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) {
+      if (j % 8 == 0 && j * ST >= rows) break;
+      const uint32_t t = a.first + g * GROUP + min(j * ST + tid, rows - 1);
+      const uint32_t page = pg[j] < 0 ? 0u : min((uint32_t)pg[j], a.num_pages - 1);
+      key[j] = __float_as_uint(a.pool.mass[a.sh.row(page, t % a.sh.page_size, h)]);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) {
+      if (j % 8 == 0 && j * ST >= rows) break;
+      key[j] = pg[j] >= 0 && pg[j] < (int32_t)a.num_pages ? key_of(__uint_as_float(key[j])) : 0u;
+    }
   };
-  for (uint32_t i0 = tid; i0 < min(n, CACHED); i0 += FAR * ST) {
-    uint32_t k[FAR];
-#pragma unroll
-    for (int j = 0; j < FAR; ++j) k[j] = fetch(min(i0 + j * ST, n - 1));
-#pragma unroll
-    for (int j = 0; j < FAR; ++j)
-      if (i0 + j * ST < min(n, CACHED)) s_key[i0 + j * ST] = k[j];
-  }
-  auto key = [&](uint32_t i) -> uint32_t { return i < CACHED ? s_key[i] : fetch(i); };
+  fetch(0);
   uint32_t bound = 0, left = m;  // the m-th largest key so far; how many of those that share its bits are kept
+  uint32_t share = n;            // how many share them
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;  // 11, 11 and 10 bits
     s_bin[2 * tid] = s_bin[2 * tid + 1] = 0;
     __syncthreads();
-    for (uint32_t i0 = 0; i0 < n; i0 += ST) {  // (every lane: the first one's bin is counted by one of them)
-      const uint32_t i = i0 + tid, k = i < n ? key(i) : 0u;
-      const bool in = i < n && (pass == 0 || (k ^ bound) >> (pass == 1 ? 21 : 10) == 0);
-      const uint32_t b = k >> shift & (pass == 2 ? 1023u : 2047u);
-      const uint64_t some = __ballot(in);
-      if (!some) continue;
-      const int one = __ffsll((unsigned long long)some) - 1;
-      const uint32_t b1 = __builtin_amdgcn_readlane(b, one);
-      const uint64_t same = __ballot(in && b == b1);
-      if (lane == (uint32_t)one) atomicAdd(&s_bin[b1], (uint32_t)__popcll(same));
-      else if (in && b != b1) atomicAdd(&s_bin[b], 1u);
+    for (uint32_t g = 0; g < groups; ++g) {
+      if (groups > 1 && (pass || g)) fetch(g);
+      const uint32_t rows = rows_of(g);
+#pragma unroll
+      for (uint32_t j = 0; j < PER; ++j) {
+        if (j * ST >= rows) break;
+        const uint32_t b = key[j] >> shift & (pass == 2 ? 1023u : 2047u);
+        // (the least bin has those that no other has: rows without weight, often many, are not counted one by one)
+        if (b && j * ST + tid < rows && (pass == 0 || (key[j] ^ bound) >> (pass == 1 ? 21 : 10) == 0))
+          atomicAdd(&s_bin[b], 1u);
+      }
     }
     __syncthreads();
     // counts from the largest bin down: two bins a thread, summed over its wave, then over the waves
-    const uint32_t hi = s_bin[BINS - 1 - 2 * tid], lo = s_bin[BINS - 2 - 2 * tid];
+    uint32_t hi = s_bin[BINS - 1 - 2 * tid], lo = s_bin[BINS - 2 - 2 * tid];
     const uint32_t upto = wave_scan(hi + lo);
-    if (lane == 63) s_above[w] = upto;
+    if (lane == 63) s_sum[w] = upto;
     __syncthreads();
     uint32_t above = upto - hi - lo;
-    for (uint32_t i = 0; i < w; ++i) above += s_above[i];
+    for (uint32_t i = 0; i < w; ++i) above += s_sum[i];
+    if (tid == ST - 1) lo = share - above - hi;
     if (above < left && above + hi + lo >= left) {  // (one thread's)
-      const bool first = above + hi >= left;
-      s_found[0] = BINS - 1 - 2 * tid - (first ? 0 : 1);
-      s_found[1] = above + (first ? 0 : hi);
+      const bool one = above + hi >= left;
+      s_found[0] = BINS - 1 - 2 * tid - (one ? 0 : 1);
+      s_found[1] = above + (one ? 0 : hi);
+      s_found[2] = one ? hi : lo;
     }
     __syncthreads();
     bound |= s_found[0] << shift;
     left -= s_found[1];
+    share = s_found[2];
+    __syncthreads();
   }
-  // the rows above the bound and the first `left` at it, in order: each wave counts those of its run of candidates
-  const uint32_t run = ((n + NW - 1) / NW + 63) / 64 * 64, i0 = min(w * run, n), i1 = min(i0 + run, n);
-  uint32_t above = 0, at = 0;
-  for (uint32_t i = i0; i < i1; i += 64) {
-    const uint32_t k = i + lane < i1 ? key(i + lane) : 0u;
-    above += __popcll(__ballot(i + lane < i1 && k > bound));
-    at += __popcll(__ballot(i + lane < i1 && k == bound));
-  }
-  __syncthreads();  // (s_above's counts of the last pass are done with)
-  if (lane == 0) {
-    s_above[w] = above;
-    s_at[w] = at;
-  }
-  __syncthreads();
-  above = at = 0;
-  for (uint32_t i = 0; i < w; ++i) {
-    above += s_above[i];
-    at += s_at[i];
-  }
-  const uint64_t below = (1ull << lane) - 1;
-  for (uint32_t i = i0; i < i1; i += 64) {
-    const bool in = i + lane < i1;
-    const uint32_t k = in ? key(i + lane) : 0u;
-    const uint64_t ma = __ballot(in && k > bound), me = __ballot(in && k == bound);
-    const uint32_t ra = above + __popcll(ma & below), re = at + __popcll(me & below);
-    if (in && (k > bound || (k == bound && re < left)))
-      kept[a.first + ra + min(re, left)] = (int32_t)(a.first + i + lane);
-    above += __popcll(ma);
-    at += __popcll(me);
+  // the rows above the bound and the first `left` at it, in order: how many each wave has of each ST candidates, the
+  // counts summed up, then each row's place
+  uint32_t above = 0, at = 0;  // of the groups before
+  for (uint32_t g = 0; g < groups; ++g) {
+    if (groups > 1) fetch(g);
+    const uint32_t rows = rows_of(g), chunks = (rows + ST - 1) / ST;
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) {
+      if (j * ST >= rows) break;
+      const bool in = j * ST + tid < rows;
+      const uint64_t ma = __ballot(in && key[j] > bound), me = __ballot(in && key[j] == bound);
+      if (lane == 0) {
+        s_above[j * NW + w] = __popcll(ma);
+        s_at[j * NW + w] = __popcll(me);
+      }
+    }
+    __syncthreads();
+    const uint32_t x = tid < chunks * NW ? s_above[tid] : 0u, y = tid < chunks * NW ? s_at[tid] : 0u;  // (PER * NW <= ST)
+    const uint32_t ux = wave_scan(x), uy = wave_scan(y);
+    if (lane == 63) {
+      s_sum[w] = ux;
+      s_sum[NW + w] = uy;
+    }
+    __syncthreads();
+    uint32_t bx = above + ux - x, by = at + uy - y;
+    for (uint32_t i = 0; i < NW; ++i) {
+      if (i < w) {
+        bx += s_sum[i];
+        by += s_sum[NW + i];
+      }
+      above += s_sum[i];
+      at += s_sum[NW + i];
+    }
+    if (tid < chunks * NW) {
+      s_above[tid] = bx;
+      s_at[tid] = by;
+    }
+    __syncthreads();
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) {
+      if (j * ST >= rows) break;
+      const bool in = j * ST + tid < rows;
+      const uint32_t k = key[j];
+      const uint64_t ma = __ballot(in && k > bound), me = __ballot(in && k == bound);
+      const uint32_t ra = s_above[j * NW + w] + __popcll(ma & below), re = s_at[j * NW + w] + __popcll(me & below);
+      if (in && (k > bound || (k == bound && re < left)))
+        kept[a.first + ra + min(re, left)] = (int32_t)(a.first + g * GROUP + j * ST + tid);
+    }
+    __syncthreads();
   }
 }
 
-// A thread 16 bytes of codes (K's, then V's) and one scale of a row; the row's first also its mass.
-template <bool BACK>
-__global__ __launch_bounds__(MT) void kv4_move_kernel(EvictArgs a) {
+// A workgroup the same `some` pieces of 16 bytes of every row that moves, with their scales; with K's first one also the
+// masses. A row moves down only (kept[i] >= i), so a set of rows that is read before any of it is written overwrites
+// none that a later set reads: the rows move in place, a set after the other, one barrier between.
+constexpr int SETS = 4;  // rows of a thread that move at once
+__global__ __launch_bounds__(ST) void kv4_move_kernel(EvictArgs a) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  const uint32_t pieces = a.sh.hd / 16, half = pieces / 2, per = MT / pieces;
-  const uint32_t s = blockIdx.y / a.sh.nkh, h = blockIdx.y % a.sh.nkh;
+  // (the workgroups of a sequence and KV head have numbers that differ by multiples of 8: they are on one XCD, whose L2
+  // has a row's line for all of them)
+  const uint32_t some = a.some, parts = a.sh.hd / 32 / some, pairs = a.num_seqs * a.sh.nkh;
+  const uint32_t pair = blockIdx.x / (16 * parts) * 8 + blockIdx.x % 8, part = blockIdx.x / 8 % (2 * parts);
+  if (pair >= pairs) return;
+  const uint32_t s = pair / a.sh.nkh, h = pair % a.sh.nkh;
   if (!a.cut[s]) return;
-  const uint32_t i = blockIdx.x * per + threadIdx.x / pieces, piece = threadIdx.x % pieces;
-  if (!BACK && i == 0 && threadIdx.x == 0 && h == 0) a.seq_lens[s] = a.keep;
-  if (i >= a.keep) return;
-  const size_t at = (size_t)blockIdx.y * a.keep + i;
-  const uint32_t from = (uint32_t)a.kept[at];
-  if (from == i) return;
-  const uint32_t t = BACK ? i : from;
-  const int32_t id = a.page_table[(size_t)s * a.max_pages + t / a.sh.page_size];
-  const bool in = id >= 0 && id < (int32_t)a.num_pages;
-  if (BACK && !in) return;
-  const uint32_t pg = id < 0 ? 0u : min((uint32_t)id, a.num_pages - 1), slot = t % a.sh.page_size;
-  const bool is_v = piece >= half;
-  const uint32_t b = is_v ? piece - half : piece;
-  u32x4* code = (u32x4*)((is_v ? a.pool.v : a.pool.k) + a.sh.code(pg, slot, h) + 16 * b);
-  uint8_t* scale = is_v ? a.pool.vs + a.sh.v_scale(pg, slot, h, b) : a.pool.ks + a.sh.k_scale(pg, slot, h, b);
-  u32x4* code_w = (u32x4*)(a.rows + at * a.sh.hd + 16 * piece);
-  uint8_t* scale_w = a.scales + at * pieces + piece;
-  float* mass = a.pool.mass + a.sh.row(pg, slot, h);
-  if (BACK) {
-    *code = *code_w;
-    *scale = *scale_w;
-    if (piece == 0) *mass = a.mass[at];
-  } else {
-    *code_w = *code;
-    *scale_w = *scale;
-    if (piece == 0) a.mass[at] = in ? *mass : 0.f;
+  if (h == 0 && part == 0 && threadIdx.x == 0) a.seq_lens[s] = a.keep;
+  const bool is_v = part >= parts;
+  const uint32_t b = part % parts * some + threadIdx.x % some, per = ST / some, r = threadIdx.x / some;
+  const int32_t *kept = a.kept + (size_t)pair * a.keep, *list = a.page_table + (size_t)s * a.max_pages;
+  uint8_t *codes = (is_v ? a.pool.v : a.pool.k) + 16 * b, *scales = is_v ? a.pool.vs : a.pool.ks;
+  const bool has_mass = part == 0 && threadIdx.x % some == 0;
+  // of the set at hand, the next and the one after it: where its rows are, their pages. One wait for memory a set: the
+  // rows of this one, the page ids of the next and the places of the one after it are on their way together.
+  uint32_t from[SETS], from1[SETS];
+  int32_t src[SETS], dst[SETS];
+  auto row_of_set = [&](uint32_t i0, int k) { return min(i0 + k * per + r, a.keep - 1); };  // (past the last: that one)
+  auto places = [&](uint32_t i0, uint32_t* f) {
+#pragma unroll
+    for (int k = 0; k < SETS; ++k) f[k] = (uint32_t)kept[row_of_set(i0, k)];
+  };
+  auto pages = [&](uint32_t i0, const uint32_t* f) {
+#pragma unroll
+    for (int k = 0; k < SETS; ++k) {
+      src[k] = list[f[k] / a.sh.page_size];
+      dst[k] = list[row_of_set(i0, k) / a.sh.page_size];
+    }
+  };
+  auto scale_at = [&](uint32_t page, uint32_t slot) {
+    return is_v ? a.sh.v_scale(page, slot, h, b) : a.sh.k_scale(page, slot, h, b);
+  };
+  const uint32_t rows = SETS * per;
+  places(0, from);
+  places(rows, from1);
+  pages(0, from);
+  for (uint32_t i0 = 0; i0 < a.keep; i0 += rows) {
+    u32x4 x[SETS];
+    uint8_t z[SETS];
+    float m[SETS];
+    int32_t to[SETS];  // page, or -1: it stays where it is
+#pragma unroll
+    for (int k = 0; k < SETS; ++k) {
+      const uint32_t page = src[k] < 0 ? 0u : min((uint32_t)src[k], a.num_pages - 1), slot = from[k] % a.sh.page_size;
+      x[k] = *(const u32x4*)(codes + a.sh.code(page, slot, h));
+      z[k] = scales[scale_at(page, slot)];
+      m[k] = has_mass && (uint32_t)src[k] < a.num_pages ? a.pool.mass[a.sh.row(page, slot, h)] : 0.f;
+      const uint32_t i = i0 + k * per + r;
+      to[k] = i < a.keep && from[k] != i && (uint32_t)dst[k] < a.num_pages ? dst[k] : -1;
+      from[k] = from1[k];
+    }
+    pages(i0 + rows, from);
+    places(i0 + 2 * rows, from1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (this wave's rows are here, then every wave's are)
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < SETS; ++k) {
+      if (to[k] < 0) continue;
+      const uint32_t slot = row_of_set(i0, k) % a.sh.page_size;
+      *(u32x4*)(codes + a.sh.code((uint32_t)to[k], slot, h)) = x[k];
+      scales[scale_at((uint32_t)to[k], slot)] = z[k];
+      if (has_mass) a.pool.mass[a.sh.row((uint32_t)to[k], slot, h)] = m[k];
+    }
   }
 }
 
-size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-struct EvictSizes {
-  size_t cut, rows, scales, mass;
-  size_t all() const { return cut + rows + scales + mass; }
-};
-EvictSizes evict_sizes(const g4_kv4_params& p, uint32_t keep) {
-  const size_t n = (size_t)p.num_seqs * p.num_kv_heads * keep;
-  return {up256(p.num_seqs * 4ull), up256(n * p.head_dim), up256(n * (p.head_dim / 16)), up256(n * 4)};
-}
 int evict_check(const char* fn, g4_kv4_params& p, uint32_t keep) {
   p.num_rows = p.num_seqs;
   p.max_rows = 1;
@@ -435,7 +494,7 @@ int g4_kvEvict4_workspace_size(g4_kv4_params p, uint32_t keep, size_t* bytes) {
   G4_REQUIRE(bytes, "g4_kvEvict4_workspace_size: null out");
   int rc = evict_check(__func__, p, keep);
   if (rc) return rc;
-  *bytes = evict_sizes(p, keep).all();
+  *bytes = ((size_t)p.num_seqs * sizeof(uint32_t) + 15) / 16 * 16;
   return G4_OK;
 }
 
@@ -451,22 +510,25 @@ int g4_kvEvict4(g4_ctx* ctx, uint8_t* k_pool, uint8_t* v_pool, uint8_t* k_scale,
              first, recent, keep);
   G4_REQUIRE((((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)workspace) & 15) == 0,
              "g4_kvEvict4: pools and workspace must be 16-byte aligned");
-  const EvictSizes z = evict_sizes(p, keep);
-  G4_REQUIRE(workspace_bytes >= z.all(), "g4_kvEvict4: workspace %zu bytes < %zu required", workspace_bytes, z.all());
+  size_t need = 0;
+  rc = g4_kvEvict4_workspace_size(p, keep, &need);
+  if (rc) return rc;
+  G4_REQUIRE(workspace_bytes >= need, "g4_kvEvict4: workspace %zu bytes < %zu required", workspace_bytes, need);
   const uint64_t pairs = (uint64_t)p.num_seqs * p.num_kv_heads;
   G4_REQUIRE(pairs <= 65535, "g4_kvEvict4: %u sequences of %u KV heads in one call", p.num_seqs, p.num_kv_heads);
-  uint8_t* w = (uint8_t*)workspace;
+  // As few pieces a workgroup as fill the device: one CU's address units bound a workgroup (one sequence of 2048 rows at
+  // head dim 512 in 8 workgroups 9.3 us, 8 of 4000 rows and two heads at 128 in 32 of them 19).
+  uint32_t some = std::min(p.head_dim / 32, 4u);
+  while (some > 1 && pairs * 2 * (p.head_dim / 32 / some) < 256) some /= 2;
   const EvictArgs a{{k_pool, v_pool, k_scale, v_scale, mass},
                     {p.page_size, p.num_kv_heads, p.head_dim},
                     page_table, seq_lens, p.num_seqs, p.max_pages, p.num_pages, p.max_seq_len, keep, first, recent,
-                    kept, (uint32_t*)w, w + z.cut, w + z.cut + z.rows, (float*)(w + z.cut + z.rows + z.scales)};
+                    kept, (uint32_t*)workspace, some};
   hipLaunchKernelGGL(kv4_select_kernel, dim3((unsigned)pairs), dim3(ST), 0, ctx->stream, a);
   G4_LAUNCHED(ctx, "kv4_select");
-  const dim3 grid(ceil_div(keep, MT / (p.head_dim / 16)), (unsigned)pairs);
-  hipLaunchKernelGGL(kv4_move_kernel<false>, grid, dim3(MT), 0, ctx->stream, a);
-  G4_LAUNCHED(ctx, "kv4_gather");
-  hipLaunchKernelGGL(kv4_move_kernel<true>, grid, dim3(MT), 0, ctx->stream, a);
-  G4_LAUNCHED(ctx, "kv4_scatter");
+  const dim3 moves((unsigned)((pairs + 7) / 8 * 8) * 2 * (p.head_dim / 32 / some));
+  hipLaunchKernelGGL(kv4_move_kernel, moves, dim3(ST), 0, ctx->stream, a);
+  G4_LAUNCHED(ctx, "kv4_move");
   return G4_OK;
 }
 

@@ -845,7 +845,7 @@ def test_refusals(ctx):
                  lambda: pro(p, rope=b, rows=63), lambda: pro(p, rope=b.offset(4), rows=64),
                  lambda: pro(p, rope=b, rows=0, pos=b), lambda: pro(p, qo=None), lambda: pro(p, kw=None),
                  lambda: pro(p, k=b.offset(4)), lambda: evict(p, kp=None), lambda: evict(p, mass=None),
-                 lambda: evict(p, kept=None), lambda: evict(p, wsp=ctx.zeros(16, np.uint8)),
+                 lambda: evict(p, kept=None), lambda: evict(p, wsp=ctx.zeros(8, np.uint8)),
                  lambda: evict(p, keep=0), lambda: evict(p, keep=65), lambda: evict(p, first=20, recent=13),
                  lambda: evict(p, first=33), lambda: evict(p, first=2, recent=0xffffffff),
                  lambda: evict(p, kp=b.offset(8)),
