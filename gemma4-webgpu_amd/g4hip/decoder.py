@@ -840,23 +840,39 @@ class BatchDecoder(_SyntheticModel):
     prologue, or the attention prologue), so no launch waits on another's
     workgroups and the step is deterministic.
     """
+    kv4, budget, capturing = False, None, False
 
     def __init__(self, ctx: Context, context_lens, shape: Optional[E2BShape] = None, page_size: int = 16,
                  reserve: int = 64, seed: int = 0, n_layers: Optional[int] = None, lm_head: bool = True,
                  page_seed: int = 7, shared_pages: bool = False, embed: bool = False, wtypes=None, gguf=None,
-                 kv: str = "f16", logprobs: Optional[int] = None):
+                 kv: str = "f16", logprobs: Optional[int] = None, budget: Optional[int] = None, slack: int = 256,
+                 sinks: int = 4, recent: Optional[int] = None):
         """shared_pages: every row reads and appends through one page list
         (the rows are tokens of one sequence: batched prefill). embed: an f16
         token table; each step starts from the embedding of every row's
         token in `tokens` (the previous step's sample, or the prompt). kv:
-        "f16" or "int8" pages (8-bit codes with a scale per page and KV head,
-        half the pool's bytes; page_size a multiple of 16). logprobs: a step
+        "f16", "int8" pages (8-bit codes with a scale per page and KV head,
+        half the pool's bytes; page_size a multiple of 16) or "fp4" pages
+        (4-bit floats with a scale per 32 dims, 0.27 of them). budget ("fp4"
+        pages): the layers without a window hold budget + slack rows of a
+        sequence at most, whatever its text's length. Their attention adds up
+        the weight that every row gets, and where a step or a prompt's pass
+        would not find room, evict() leaves the first `sinks` rows, the last
+        `recent` (a quarter of the budget) and the heaviest others, budget rows
+        in all. Rows keep their text's positions. Longer contexts than the
+        budget count as cut already. logprobs: a step
         that samples leaves every row's token_logprobs (of its argmax),
         entropy and this many alternatives, at most 64 (top_ids, top_logprobs
         [B][n]); a top-k 256 step, whose token the host draws, leaves
         token_logprobs as they were."""
-        if kv not in ("f16", "int8"):
-            raise ValueError(f"kv {kv!r}: f16 or int8")
+        if kv not in ("f16", "int8", "fp4"):
+            raise ValueError(f"kv {kv!r}: f16, int8 or fp4")
+        if budget is not None:
+            recent = budget // 4 if recent is None else recent
+            if kv != "fp4" or min(budget, slack) < 1 or min(sinks, recent) < 0 or sinks + recent > budget:
+                raise ValueError(f"budget {budget}: fp4 pages, and {sinks} first and {recent} last rows within it")
+            if shared_pages and slack < len(context_lens):
+                raise ValueError(f"slack {slack}: a chunk of {len(context_lens)} rows has to fit")
         if logprobs is not None and not lm_head:
             raise ValueError("logprobs need the LM head")
         if logprobs is not None and not 0 <= logprobs <= 64:
@@ -883,16 +899,40 @@ class BatchDecoder(_SyntheticModel):
                 at += n
         self.page_table_host = table
         self.lens_host = lens.astype(np.uint32)
-        rows = self.num_pages * page_size
-        self.kv8 = kv == "int8"
-        code = np.int8 if self.kv8 else np.uint16
+        self.kv8, self.kv4 = kv in ("int8", "fp4"), kv == "fp4"  # (kv8: pages of codes)
+        self.budget = budget
+        if budget is not None:
+            # the pools of the layers without a window: page lists and lengths of their own
+            self.cut = dict(keep=budget, first=sinks, recent=recent)
+            self.cut_rows = budget + slack
+            self.cut_max_pages = -(-self.cut_rows // page_size)
+            seqs = 1 if shared_pages else self.B
+            self.cut_pages = seqs * self.cut_max_pages
+            cut_order = np.random.default_rng(page_seed + 1).permutation(self.cut_pages).astype(np.int32)
+            self.cut_table_host = cut_order.reshape(seqs, self.cut_max_pages)
+        bits = {"f16": 16, "int8": 8, "fp4": 4}[kv]
         self._build_weights(ctx, shape, n_layers, seed, lm_head,
-                            lambda il: (ctx.zeros(rows * self.s.kv_dim_of(il), code),
-                                        ctx.zeros(rows * self.s.kv_dim_of(il), code)), embed=embed,
-                            wtypes=wtypes, gguf=gguf)
-        # 8-bit pools: the scales of each producer's pages (k, v), f32 [num_pages][KV heads]
-        self.kv_scales = {il: tuple(ctx.zeros(self.num_pages * self.s.n_kv_heads, np.float32) for _ in "kv")
+                            lambda il: tuple(ctx.zeros(self._pool_rows(il) * self.s.kv_dim_of(il) * bits // 8, np.uint8)
+                                             for _ in "kv"), embed=embed, wtypes=wtypes, gguf=gguf)
+        # pools of codes: the scales of each producer's pages (k, v): 8-bit f32 [num_pages][KV heads], 4-bit bytes
+        # [rows][KV heads][head dim / 32]
+        self.kv_scales = {il: tuple(ctx.zeros(self._pool_rows(il) * self.s.kv_dim_of(il) // 32, np.uint8) if self.kv4
+                                    else ctx.zeros(self.num_pages * self.s.n_kv_heads, np.float32) for _ in "kv")
                           for il in range(self.s.n_layers) if self.kv8 and self.s.is_producer(il)}
+        # with a budget: the attention weight of each cut producer's rows, and where the rows that an eviction kept were
+        cut = [il for il in range(self.s.n_layers) if self._is_cut(il) and self.s.is_producer(il)]
+        self.mass = {il: ctx.zeros(self._pool_rows(il) * self.s.n_kv_heads, np.float32) for il in cut}
+        self.kept = {}
+        if budget is not None:
+            self.cut_table = ctx.from_numpy(self.cut_table_host)
+            n = len(self.cut_table_host)
+            self.cut_lens_host = np.minimum(self.lens_host, budget)[:n]
+            self.cut_lens, self.cut_lens_next = ctx.from_numpy(self.cut_lens_host), ctx.zeros(n, np.uint32)
+            self.text = 0  # shared_pages: tokens of the sequence so far
+            self.kept = {il: ctx.zeros(n * self.s.n_kv_heads * budget, np.int32) for il in cut}
+            self.evict_params = {il: self._kv8_params(il, n, 1) for il in cut}
+            self.evict_ws = ctx.alloc(max([16] + [ctx.evict4_workspace_bytes(p, budget)
+                                                  for p in self.evict_params.values()]))
         s, B, f32 = self.s, self.B, np.float32
         self.page_table = ctx.from_numpy(table)
         self.seq_lens = ctx.from_numpy(self.lens_host)
@@ -969,6 +1009,8 @@ class BatchDecoder(_SyntheticModel):
         # many rows at a time (0: B at a time); the buffers of such a pass come
         # with the first prompt that takes one, for as many rows as it needs
         self.wide_rows = min(max(B, WIDE_ROWS // B * B), -(-self.max_seq // B) * B) if self._wide_prefill() else 0
+        if budget is not None:  # (a pass's rows have to fit)
+            self.wide_rows = min(self.wide_rows, slack // B * B)
         self.wide, self.wide_cap = None, 0
         # split-K partial sums of o and down: four chunks of a full pass, more of a short one
         self.wide_parts = 4 * max(self.wide_rows, 512) * s.hidden
@@ -980,7 +1022,18 @@ class BatchDecoder(_SyntheticModel):
         for il, L in enumerate(self.layers):
             if not self.s.is_producer(il):
                 continue
-            n = self.num_pages * self.page_size * self.s.kv_dim_of(il)
+            n = self._pool_rows(il) * self.s.kv_dim_of(il)
+            if self.kv4:  # e2m1 codes of every kind under scales of 1/4 and 1/2 (past 2^22 bytes of them, repeated)
+                rng = np.random.default_rng(splitmix64(seed, 2 * il))
+                for pool, scale in zip((L.k_cache, L.v_cache), self.kv_scales[il]):
+                    for b, lo, hi in ((pool, 0, 256), (scale, 125, 127)):
+                        m = min(b.nbytes, 1 << 22)
+                        b.upload(rng.integers(lo, hi, m).astype(np.uint8))
+                        for at in range(m, b.nbytes, m):
+                            self.ctx.copy(b.offset(at), b, min(m, b.nbytes - at))
+                if il in self.mass:
+                    self.mass[il].upload(rng.random(self._pool_rows(il) * self.s.n_kv_heads).astype(np.float32))
+                continue
             if self.kv8:  # codes ~ N(0, 32^2) under a scale of 1/32 (past 2^22 of them, repeated)
                 rng = np.random.default_rng(splitmix64(seed, 2 * il))
                 for pool, scale in zip((L.k_cache, L.v_cache), self.kv_scales[il]):
@@ -999,6 +1052,9 @@ class BatchDecoder(_SyntheticModel):
             raise ValueError("set_lengths: one length per sequence, below the reserved capacity")
         self.lens_host = lens
         self.seq_lens.upload(lens)
+        if self.budget is not None and not self.shared_pages:
+            self.cut_lens_host = np.minimum(lens, self.budget)
+            self.cut_lens.upload(self.cut_lens_host)
 
     def pool_row(self, seq: int, pos: int) -> int:
         """Pool row of sequence `seq`'s logical position `pos`."""
@@ -1013,28 +1069,48 @@ class BatchDecoder(_SyntheticModel):
                 n = int(L) + 1
                 if not s.is_global(il):
                     n = min(n, s.window)
+                if self._is_cut(il):
+                    n = min(n, self.cut_rows)
+                if self.kv4:
+                    total += n * 2 * s.kv_dim_of(il) * 17 // 32
+                    continue
                 total += n * 2 * s.kv_dim_of(il) * (1 if self.kv8 else 2)
                 if self.kv8:
                     total += -(-n // self.page_size) * 2 * s.n_kv_heads * 4
         return total
 
+    def _is_cut(self, il: int) -> bool:
+        """Layer il's cache holds a budget of rows."""
+        return self.budget is not None and self.s.is_global(il)
+
+    def _pool_rows(self, il: int) -> int:
+        return (self.cut_pages if self._is_cut(il) else self.num_pages) * self.page_size
+
     def _kv8_params(self, il: int, rows: int, valid: int, end: Optional[int] = None):
-        """Layer il's 8-bit attention over `rows` rows: of one sequence up to position `end`, of which the first
-        `valid` are its (shared_pages), or one of each sequence."""
+        """Layer il's attention over `rows` rows and pages of codes: of one sequence up to position `end`, of which the
+        first `valid` are its (shared_pages), or one of each sequence."""
         s, glob = self.s, self.s.is_global(il)
+        pages, most, count = self.max_pages, end or self.max_seq, self.num_pages
+        if self._is_cut(il):
+            pages, most, count = self.cut_max_pages, self.cut_rows, self.cut_pages
         return self.ctx.kv8_params(1 if self.shared_pages else rows, s.n_q_heads, s.n_kv_heads, s.hd(il),
-                                   self.page_size, self.max_pages, end or self.max_seq, self.num_pages, rows, valid,
+                                   self.page_size, pages, most, count, rows, valid,
                                    0 if glob else s.window, 1.0, s.eps, s.theta_global if glob else s.theta_local,
                                    int(glob))
 
+    def _attn8_bytes(self, p) -> int:
+        if self.kv4:
+            return self.ctx.attn4_workspace_bytes(p, self.budget is not None)
+        return self.ctx.attn8_workspace_bytes(p)
+
     def _attn8_workspace(self, params) -> None:
-        need = max(self.ctx.attn8_workspace_bytes(p) for p in params)
+        need = max(self._attn8_bytes(p) for p in params)
         if need > self.attn8_cap:
             self.attn8_ws, self.attn8_cap = None, 0  # (the old one is given back first)
             self.attn8_ws, self.attn8_cap = self.ctx.alloc(need), need
 
     def _attend8(self, il: int, q_parts, k_parts, v_parts, nq: int, q, out, p, ops=None) -> None:
-        """Layer il's prologue and attention over its 8-bit pages. Of a shared page list, the spare rows past
+        """Layer il's prologue and attention over its pages of codes. Of a shared page list, the spare rows past
         the sequence's get its last row's output, as if they were that row again."""
         c, s, L = self.ctx, self.s, self.layers[il]
         src = il if s.is_producer(il) else s.producer(il)
@@ -1042,14 +1118,53 @@ class BatchDecoder(_SyntheticModel):
         starts, lens = (self.span.offset(4), self.span) if self.shared_pages else (None, self.seq_lens)
         if self.shared_pages:  # (few rows take another kernel than many)
             self._attn8_workspace([p])
-        c.pagedAttnPrologue8(q_parts, k_parts if prod else None, v_parts if prod else None, nq, L.q_norm,
-                             L.k_norm if prod else None, self.rope_freqs, q, L.k_cache, L.v_cache,
-                             *self.kv_scales[src], self.page_table, lens, p, row_starts=starts,
-                             rope_cs=self.rope_cs[s.is_global(il)], rope_rows=self.rope_rows)
-        c.pagedAttn8(q, L.k_cache, L.v_cache, *self.kv_scales[src], self.page_table, lens, out, p, self.attn8_ws,
-                     row_starts=starts, ops=ops)
+        rows = (q_parts, k_parts if prod else None, v_parts if prod else None, nq, L.q_norm,
+                L.k_norm if prod else None, self.rope_freqs, q)
+        cache = (L.k_cache, L.v_cache, *self.kv_scales[src])
+        rope = dict(row_starts=starts, rope_cs=self.rope_cs[s.is_global(il)], rope_rows=self.rope_rows)
+        if self.kv4:
+            cut = self._is_cut(il)
+            where = (self.cut_table, self.cut_lens) if cut else (self.page_table, lens)
+            mass = self.mass[src] if cut else None
+            c.pagedAttnPrologue4(*rows, *cache, *where, p, positions=lens if cut else None, mass=mass, **rope)
+            c.pagedAttn4(q, *cache, *where, out, p, self.attn8_ws, row_starts=starts, mass=mass, ops=ops)
+        else:
+            c.pagedAttnPrologue8(*rows, *cache, self.page_table, lens, p, **rope)
+            c.pagedAttn8(q, *cache, self.page_table, lens, out, p, self.attn8_ws, row_starts=starts, ops=ops)
         if self.shared_pages and p.max_rows < p.num_rows:
             c.repeatRow(out, s.q_dim_of(il), p.max_rows - 1, p.max_rows, p.num_rows - p.max_rows)
+
+    def evict(self) -> None:
+        """Cuts the caches that have a budget down to it: every sequence with more rows there keeps its first, its last
+        and its heaviest (`kept[layer]` [sequences][KV heads][budget]: where they were). Steps and prompts that the
+        host enqueues call it where they need room; between the replays of a captured step, of which the host knows
+        nothing, it is the caller's, once in `slack` of them at least: a sequence without room appends nothing.
+        Waits for the device."""
+        if self.budget is None:
+            raise ValueError("evict needs a budget")
+        self._evict()
+        self.cut_lens_host = self.cut_lens.download(np.uint32)
+
+    def _evict(self) -> None:
+        c, n = self.ctx, 4 * len(self.cut_lens_host)
+        for il, p in self.evict_params.items():  # (each of the same lengths)
+            L = self.layers[il]
+            c.copy(self.cut_lens_next, self.cut_lens, n)
+            c.kvEvict4(L.k_cache, L.v_cache, *self.kv_scales[il], self.mass[il], self.cut_table, self.cut_lens_next, p,
+                       self.budget, self.cut["first"], self.cut["recent"], self.kept[il], self.evict_ws)
+        if self.evict_params:
+            c.copy(self.cut_lens, self.cut_lens_next, n)
+        self.cut_lens_host = np.minimum(self.cut_lens_host, self.budget)
+
+    def _make_room(self, rows: int) -> None:
+        """Room for `rows` more of every sequence in the caches that have a budget, and their lengths with them."""
+        if self.budget is None:
+            return
+        if not self.capturing and int(self.cut_lens_host.max()) + rows > self.cut_rows:
+            self._evict()
+        self.ctx.advanceSeqLens(self.cut_lens, len(self.cut_lens_host), rows)
+        if not self.capturing:
+            self.cut_lens_host = self.cut_lens_host + np.uint32(rows)
 
     def step(self, sample: str = "argmax", probe=None, head: bool = True,
              rows: Optional[int] = None) -> None:
@@ -1084,7 +1199,7 @@ class BatchDecoder(_SyntheticModel):
         if rows is not None and not (self.shared_pages and 1 <= rows <= self.B):
             raise ValueError(f"step: rows={rows} needs shared_pages and 1..{self.B} rows")
         if self.kv8 and self.shared_pages and not self.span_rows:
-            raise ValueError("step: 8-bit shared pages hold one sequence, whose rows prefill and score place")
+            raise ValueError("step: shared pages of codes hold one sequence, whose rows prefill and score place")
         c, s, B = self.ctx, self.s, self.B if rows is None else rows
         H = s.hidden
         if self.embedding is not None:
@@ -1095,6 +1210,8 @@ class BatchDecoder(_SyntheticModel):
             c.pleStage1Fuse(self.ple_projected, self.ple_proj_norm, self.ple_table, s.vocab, self.ple_inputs,
                             s.n_layers, s.ple_dim, s.eps, tokens_dev=self.tokens, count=B)
         c.advanceSeqLens(self.seq_lens, self.B, 1)
+        if not self.shared_pages:
+            self._make_room(1)
         nd = 0
         for il, L in enumerate(self.layers):
             Q, KV, I = s.q_dim_of(il), s.kv_dim_of(il), s.ffn_of(il)
@@ -1268,6 +1385,7 @@ class BatchDecoder(_SyntheticModel):
         T, B = int(toks.size), self.B
         if T == 0 or start < 0 or start + T > self.max_seq - 1:
             raise ValueError(f"prefill: {T} tokens from {start} do not fit {self.max_seq} positions")
+        self._begin_text(start, T)
         nch = -(-T // B)
         n = T - (nch - 1) * B
         pad = nch * B - T
@@ -1333,6 +1451,19 @@ class BatchDecoder(_SyntheticModel):
         if spans is not None:
             self.ctx.copy(self.span, spans[0].offset(12 * k), 12)
             self.span_rows = int(spans[1][k])
+            self._make_room(self.span_rows)
+
+    def _begin_text(self, start: int, tokens: int) -> None:
+        """Caches with a budget hold rows by when they came, not by position: a text begins at 0, or goes on where the
+        last one ended."""
+        if self.budget is None:
+            return
+        if start not in (0, self.text):
+            raise ValueError(f"a prompt from {start}: caches with a budget begin at 0 or go on at {self.text}")
+        if start == 0:
+            self.cut_lens.zero()
+            self.cut_lens_host = np.zeros_like(self.cut_lens_host)
+        self.text = start + tokens
 
     def score(self, tokens, start: int = 0) -> np.ndarray:
         """The log probability of each token but the first under the model, given those before it (a
@@ -1345,6 +1476,7 @@ class BatchDecoder(_SyntheticModel):
         if T < 2 or start < 0 or start + T > self.max_seq - 1:
             raise ValueError(f"score: {T} tokens from {start}: two or more within {self.max_seq} positions")
         n = T - 1  # the last token is only asked for
+        self._begin_text(start, n)
         nch = -(-n // B)
         pad = nch * B - n
         ctok = np.concatenate([toks[:n], np.repeat(toks[n - 1], pad)]).astype(np.uint32)
@@ -1539,9 +1671,11 @@ class BatchDecoder(_SyntheticModel):
         """The step as a HIP graph; each replay appends one token per sequence."""
         lens = self.lens_host.copy()
         self.ctx.graph_begin()
+        self.capturing = True
         try:
             self.step(sample)
         finally:
+            self.capturing = False
             g = self.ctx.graph_end()
         self.lens_host = lens  # capture enqueues nothing
         return g

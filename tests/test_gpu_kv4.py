@@ -565,6 +565,50 @@ def test_a_weight_far_below_the_largest_keeps_its_share(ctx, hd, rows, far):
         c.check_mass(c.mass, (a, b))
 
 
+@pytest.mark.parametrize("hd,nkh,rows,lens", [(256, 1, [1] * 5, [1, 40, 0, 300, 700]), (512, 1, [1] * 3, [9, 1000, 33]),
+                                              (256, 2, [1] * 20, [50 * s for s in range(20)]),
+                                              (512, 1, [1] * 40, [30 * s + 1 for s in range(40)]),
+                                              (256, 3, [2, 0, 1, 2], [90, 5, 1, 400])])
+def test_the_output_as_operand_blocks(ctx, hd, nkh, rows, lens):
+    """Per super-block and row: f16 hi + lo of y 2^e (22 bits of the block's largest), the sub-blocks' sums in three
+    f16 parts (33 bits, of 32 terms added in f32), and 2^-e; the blocks of the padding are not written."""
+    c = Case(ctx, lens, rows, 8 * nkh, nkh, hd, 16, 171).up()
+    R = c.p.num_rows
+    assert R == c.n.sum()
+    nblk, ntv = 8 * nkh * hd // 256, 1 if R <= 16 else 2 if R <= 32 else 4
+    size = ctx.batch_operand_bytes(8 * nkh * hd, R)
+    for mass in (False, True):
+        ops = ctx.from_numpy(np.full(size, 0x5a, np.uint8))
+        y = c.attention(ops=ops, mass=mass)
+        assert np.array_equal(y.view(np.uint32), c.attention().view(np.uint32))
+        b = ops.download(np.uint8).reshape(nblk, -1)
+        main, sums = ntv * 8 * 2 * 1024, ntv * 1024
+        assert b.shape[1] == main + sums + 64 * ntv
+        m = b[:, :main].reshape(nblk, ntv, 8, 2, 4, 16, 16).copy().view(np.float16).astype(np.float64)
+        m = m.transpose(3, 0, 1, 5, 2, 4, 6).reshape(2, nblk, 16 * ntv, 256)  # [hi, lo][block][row][32 s + 8 q + j]
+        sc = b[:, main + sums:].copy().view(np.float32).reshape(nblk, 16 * ntv).astype(np.float64)
+        p = b[:, main:main + sums].reshape(nblk, ntv, 4, 16, 16).copy().view(np.float16).astype(np.float64)
+        p = p.reshape(nblk, ntv, 4, 16, 2, 4).transpose(0, 1, 3, 2, 4, 5).reshape(nblk, 16 * ntv, 8, 4)
+        want = y.reshape(R, nblk, 256).transpose(1, 0, 2).astype(np.float64)
+        top = np.abs(want).max(-1, keepdims=True)
+        assert (np.abs((m[0] + m[1])[:, :R] * sc[:, :R, None] - want) <= 2.0 ** -22 * top).all()
+        sub = (want / sc[:, :R, None]).reshape(nblk, R, 8, 32)
+        tol = 32 * U * np.abs(sub).sum(-1) + 2.0 ** -24 * 64
+        assert (np.abs(p[:, :R].sum(-1) * 64 - sub.sum(-1)) <= tol).all() and np.all(p[:, :R, :, 3] == 0)
+        raw = b[:, :main].reshape(nblk, ntv, 8, 2, 4, 16, 16).transpose(0, 1, 5, 2, 3, 4, 6).reshape(nblk, 16 * ntv, -1)
+        assert np.all(raw[:, R:] == 0x5a)
+
+
+@pytest.mark.parametrize("change", [dict(hd=128), dict(num_seqs=65), dict(num_rows=6, max_rows=3), dict(ops=8)])
+def test_operand_blocks_that_are_refused(ctx, change):
+    b, ws = ctx.zeros(1 << 20, np.uint8), ctx.zeros(1 << 24, np.uint8)
+    ops = b.offset(change.get("ops", 0))
+    p = ctx.kv4_params(**{**dict(num_seqs=2, nqh=8, nkh=1, hd=256, page_size=16, max_pages=4, max_seq_len=64,
+                                 num_pages=9), **{k: v for k, v in change.items() if k != "ops"}})
+    with pytest.raises(g4hip.G4Error):
+        ctx.pagedAttn4(b, b, b, b, b, b, b, b, p, ws, row_starts=b if p.num_rows != p.num_seqs else None, ops=ops)
+
+
 def test_attention_of_far_pages(ctx):
     """Pools of more than 4 GiB: page offsets past 32 bits."""
     hd, ps, pages = 512, 16, (1 << 32) // (16 * 256) + 40

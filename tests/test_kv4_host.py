@@ -1,0 +1,105 @@
+"""The host's part of a budget of rows, without a device: when caches are cut, what their lengths are, and that nothing
+is decided while a step is captured."""
+import numpy as np
+import pytest
+
+from g4hip.decoder import BatchDecoder
+from test_kv8_host import Buf, Ctx, decoder
+
+
+class Lens(Buf):
+    def zero(self):
+        self.mem[:] = 0
+
+
+class CutCtx(Ctx):
+    def __init__(self):
+        super().__init__()
+        self.cuts = []
+
+    def kvEvict4(self, k, v, ks, vs, mass, table, lens, p, keep, first, recent, kept, ws):
+        self.cuts.append((p, lens.mem.view(np.uint32).tolist()))
+        x = lens.mem.view(np.uint32)
+        x[:] = np.minimum(x, keep)
+
+    def advanceSeqLens(self, lens, n, by):
+        lens.mem.view(np.uint32)[:n] += by
+
+
+def with_budget(d, lens, shared, budget=8, slack=4):
+    d.ctx.__class__ = CutCtx
+    d.ctx.cuts = []
+    d.shared_pages, d.kv4, d.budget, d.cut_rows = shared, True, budget, budget + slack
+    d.cut = dict(keep=budget, first=1, recent=2)
+    d.cut_lens_host = np.array(lens, np.uint32)
+    d.cut_lens, d.cut_lens_next = (Lens(d.ctx, np.zeros(4 * len(lens), np.uint8)) for _ in "ab")
+    d.cut_lens.upload(d.cut_lens_host)
+    d.evict_params, d.evict_ws, d.cut_table, d.text = {1: "one", 3: "three"}, None, None, 0
+    d.mass, d.kept = ({1: None, 3: None} for _ in "mk")
+    d.kv_scales = {1: (None, None), 3: (None, None)}
+    d.layers = {i: type("L", (), dict(k_cache=None, v_cache=None)) for i in (1, 3)}
+    return d
+
+
+def lens_of(d):
+    got = d.cut_lens.mem.view(np.uint32).tolist()
+    assert got == d.cut_lens_host.tolist()
+    return got
+
+
+def test_caches_are_cut_where_a_step_finds_no_room():
+    d = with_budget(decoder(), [11, 3], False)
+    d._make_room(1)
+    assert lens_of(d) == [12, 4] and not d.ctx.cuts
+    d._make_room(1)  # (13 rows do not fit): every layer of the same lengths
+    assert d.ctx.cuts == [("one", [12, 4]), ("three", [12, 4])] and lens_of(d) == [9, 5]
+    for n in (10, 11, 12):
+        d._make_room(1)
+        assert lens_of(d)[0] == n
+    assert len(d.ctx.cuts) == 2
+
+
+def test_a_captured_step_decides_nothing():
+    d = with_budget(decoder(), [12, 3], False)
+    d.capturing = True
+    d._make_room(1)
+    assert not d.ctx.cuts and d.cut_lens_host.tolist() == [12, 3] and d.cut_lens.mem.view(np.uint32).tolist() == [13, 4]
+    d.capturing = False
+    d.evict()  # what the device holds, whatever the host counted
+    assert lens_of(d) == [8, 4]
+
+
+def test_chunks_of_a_prompt_make_room_for_their_rows():
+    d = with_budget(decoder(), [0], True)
+    d.prefill(np.arange(100, 118))  # five chunks: 4, 8, 12, cut to 8, 12, cut to 8, 10
+    assert [x[1] for x in d.ctx.cuts if x[0] == "one"] == [[12], [12]] and lens_of(d) == [10] and d.text == 18
+    d.prefill([1, 2], 18)
+    assert lens_of(d) == [12] and d.text == 20
+    d.prefill([1, 2, 3])  # another text
+    assert lens_of(d) == [3] and d.text == 3
+    d.score(np.arange(6), 3)
+    assert lens_of(d) == [8] and d.text == 8
+
+
+@pytest.mark.parametrize("start", [1, 17, 19])
+def test_a_text_goes_on_where_it_ended(start):
+    d = with_budget(decoder(), [0], True)
+    d.prefill(np.arange(18))
+    before = lens_of(d), len(d.seen)
+    for call in (lambda: d.prefill([1], start), lambda: d.score([1, 2], start)):
+        with pytest.raises(ValueError, match="go on at 18"):
+            call()
+    assert (lens_of(d), len(d.seen)) == before
+
+
+def test_an_eviction_needs_a_budget():
+    with pytest.raises(ValueError, match="budget"):
+        decoder().evict()
+
+
+@pytest.mark.parametrize("kw", [dict(kv="int8", budget=4), dict(budget=4), dict(kv="fp4", budget=0),
+                                dict(kv="fp4", budget=4, sinks=3, recent=2), dict(kv="fp4", budget=4, slack=0)])
+def test_budgets_that_do_not_hold_are_refused(kw):
+    """Before anything is allocated for them."""
+    with pytest.raises(ValueError, match="budget"):
+        BatchDecoder(None, [3], **kw)
