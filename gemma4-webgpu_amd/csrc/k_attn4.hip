@@ -52,8 +52,8 @@ struct Args : PagedArgs {
   uint32_t units, columns;  // of a sequence and KV head there; many rows: 16 columns at a time, of a KV head
   uint8_t* qdigits;         // many rows, with mass: [KV head][16 columns][digit][128 dims][lane] 24 B, and the scales
   uint2* qscales;
-  float* weights;           // [sequence][KV head][256 positions][split][position]
-  uint32_t splits;
+  float* weights;           // [sequence][KV head][256 positions at a time][split][position]
+  uint32_t splits, blocks;
   uint32_t* done;           // many rows, with mass: whether the tiles were written
 };
 
@@ -653,6 +653,15 @@ __global__ __launch_bounds__(UNIT) void attn4_weigh_kernel(Args a) {
 // The work is dealt to the workgroups in equal shares (Walk), one or two
 // workgroups a CU. A tile held by one workgroup is written by it, else its
 // workgroups leave partials that attn4_tile_merge_kernel adds in order.
+//
+// A prompt of 4500 rows of 8 heads: 109 us at head dim 128, 163 at 256 and 356 at 512
+// (382, 510 and 467 TFLOP/s), of 1500 rows 33, 46 and 78, the merge included. The
+// matrix cores work 15 % of the time and the VALUs 30 (at a step of 64 positions and
+// head dim 256 a wave has 104 products and 480 VALU instructions: V's codes to f16,
+// the softmax, the masks), the rest waits: for LDS, and at the steps' barriers, since
+// registers allow two waves a SIMD. At head dim 512 a step of two barriers, with the
+// next step's rows in flight for all of it, spills and takes 82 us where this one's
+// four take 76.
 template <int HD>
 struct TileShape {
   static constexpr bool PAIR = HD == 512;
@@ -1093,8 +1102,14 @@ __global__ __launch_bounds__(HD / 4) void attn4_tile_merge_kernel(Args a) {
 // scores again, of K rows that stay in registers, with q's digits as the tiles left
 // them, 16 columns at a time through LDS; a lane adds up those of its column and
 // positions, over 16 column tiles and then over all (a sum of thousands in one chain
-// would be 2e-6 off), the lanes of a position at the end. Few blocks of positions:
-// the columns in `splits` parts, which attn4_mass_kernel adds in order.
+// would be 2e-6 off), the lanes of a position at the end. The columns of a block of
+// positions come in `splits` parts, which attn4_mass_kernel adds in order: a prompt's
+// first block is seen by all of its columns and its last by few, so twice the
+// workgroups that fit at once take 91 us where as many as fit take 101 (4500 rows of 8
+// heads, dim 128: with the tiles 161 and 183 us), and parts of 4 column tiles or more
+// (375 rows, dim 512: 53 us in all, of 8 tiles 63, of 2 51 but 68 at 750 rows for 61).
+// The products take 5.5 us of 32 at 1500 rows and dim 512: what bounds it is the way
+// to them, a row's page and digits, and one wave's exponentials beside another's products.
 constexpr int WT = 256, WP = 256;  // threads, positions of a workgroup
 template <int HD>
 __global__ __launch_bounds__(WT, 2) void attn4_tile_weigh_kernel(Args a) {
@@ -1139,10 +1154,15 @@ __global__ __launch_bounds__(WT, 2) void attn4_tile_weigh_kernel(Args a) {
 #pragma unroll
   for (int p = 0; p < PT; ++p) sum[p] = part[p] = f4{0.f, 0.f, 0.f, 0.f};
   i4 next[PER];
+  uint2 qnext[J];
+  float2 mlnext{0.f, 0.f};
   auto load = [&](uint32_t ct) __attribute__((always_inline)) {
     const i4* from = (const i4*)(a.qdigits + (first + ct) * BYTES);
 #pragma unroll
     for (int i = 0; i < PER; ++i) next[i] = from[min(i * WT + tid, PIECES - 1)];
+#pragma unroll
+    for (int j = 0; j < J; ++j) qnext[j] = a.qscales[((first + ct) * J + j) * 64 + l];
+    mlnext = a.sums[row_of(a, q.first, kvh, min(16 * ct + c, ncols - 1))];
   };
   auto store = [&](int to) __attribute__((always_inline)) {
 #pragma unroll
@@ -1155,15 +1175,15 @@ __global__ __launch_bounds__(WT, 2) void attn4_tile_weigh_kernel(Args a) {
   }
   for (uint32_t ct = ct0; ct < ct1; ++ct) {
     const int at = (ct - ct0) & 1;
+    const float2 ml = mlnext;
+    uint2 qs[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) qs[j] = qnext[j];
     __syncthreads();
     if (ct + 1 < ct1) load(ct + 1);
     const uint32_t g = 16 * ct + c, gr = min(g, ncols - 1), cpos = q.base + div_g(a, gr);
     const uint32_t clo = a.window && cpos + 1 > a.window ? cpos + 1 - a.window : 0u;
     const uint32_t width = g < ncols ? cpos + 1 - clo : 0u;
-    const float2 ml = a.sums[row_of(a, q.first, kvh, gr)];
-    uint2 qs[J];
-#pragma unroll
-    for (int j = 0; j < J; ++j) qs[j] = a.qscales[((first + ct) * J + j) * 64 + l];
     f4 D[PT];
 #pragma unroll
     for (int p = 0; p < PT; ++p) D[p] = f4{0.f, 0.f, 0.f, 0.f};
@@ -1198,21 +1218,29 @@ __global__ __launch_bounds__(WT, 2) void attn4_tile_weigh_kernel(Args a) {
       if (c == 4 * p + i) a.weights[out + 64 * w + 16 * p + 4 * qd + i] = y;
     }
 }
-// Adds the parts of each position's weight, a thread each.
-__global__ __launch_bounds__(WP) void attn4_mass_kernel(Args a) {
-  const uint32_t s = blockIdx.y / a.nkh, kvh = blockIdx.y % a.nkh, i = threadIdx.x;
+// Adds the parts of each position's weight: 64 positions a workgroup, a wave every fourth part of them.
+constexpr int SP = 64, SW = 4;
+__global__ __launch_bounds__(SP * SW) void attn4_mass_kernel(Args a) {
+  __shared__ float s_got[SW][SP];
+  const int w = threadIdx.x / SP, i = threadIdx.x % SP;
+  const uint32_t s = blockIdx.y / a.nkh, kvh = blockIdx.y % a.nkh, i0 = blockIdx.x * SP + i;  // (from the first seen)
   const Seq q = seq_rows(a.rows, s);
-  const uint32_t t = first_seen(a, q) + blockIdx.x * WP + i;
-  if (t >= q.len || !*a.done) return;
-  const float* from = a.weights + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * a.splits * WP + i;
+  const uint32_t t = first_seen(a, q) + i0;
+  if (first_seen(a, q) + blockIdx.x * SP >= q.len || !*a.done) return;  // (uniform; a length of 0 too)
+  const float* from = a.weights + ((size_t)blockIdx.y * a.blocks + i0 / WP) * a.splits * WP + i0 % WP;
   float got = 0.f;
-  for (uint32_t k0 = 0; k0 < a.splits; k0 += 16) {  // (16 on their way)
+  for (uint32_t k0 = w; k0 < a.splits; k0 += 16 * SW) {  // (16 on their way)
     float x[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) x[k] = from[(size_t)min(k0 + k, a.splits - 1) * WP];
+    for (int k = 0; k < 16; ++k) x[k] = from[(size_t)min(k0 + k * SW, a.splits - 1) * WP];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) got += k0 + k < a.splits ? x[k] : 0.f;
+    for (int k = 0; k < 16; ++k) got += k0 + k * SW < a.splits ? x[k] : 0.f;
   }
+  s_got[w][i] = got;
+  __syncthreads();
+  if (w || t >= q.len) return;
+#pragma unroll
+  for (int k = 1; k < SW; ++k) got += s_got[k][i];
   const uint32_t tile = t / 16, page = page_of(a, tile);
   const int32_t id = a.page_table[(size_t)s * a.max_pages + page];
   if (id >= 0 && id < (int32_t)a.num_pages)
@@ -1239,8 +1267,8 @@ struct Sizes {
   size_t meta, part, sums, scores, digits, scales, weights, done;
   size_t all() const { return meta + part + sums + scores + digits + scales + weights + done; }
 };
-// Many rows: 256 positions at a time of a sequence, parts of their columns (so many that the workgroups fill the device,
-// of eight column tiles or more), and how often 16 columns may begin (those of each sequence by themselves).
+// Many rows: 256 positions at a time of a sequence, parts of their columns (so many that the workgroups fill the device
+// twice over, of four column tiles or more), and how often 16 columns may begin (those of each sequence by themselves).
 uint64_t weigh_blocks(const g4_kv4_params& p) {
   uint64_t span = p.max_seq_len;
   if (p.sliding_window) span = std::min<uint64_t>(span, (uint64_t)p.sliding_window + p.max_rows - 1 + 15);
@@ -1248,7 +1276,7 @@ uint64_t weigh_blocks(const g4_kv4_params& p) {
 }
 uint32_t weigh_splits(const g4_kv4_params& p) {
   const uint64_t blocks = weigh_blocks(p) * p.num_seqs * p.num_kv_heads, tiles = tiles_of(p) * (TC / 16);
-  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / blocks, tiles / 8));
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(1024 / blocks, tiles / 4));
 }
 uint64_t weigh_columns(const g4_kv4_params& p) {
   return (uint64_t)p.num_rows * (p.num_q_heads / p.num_kv_heads) / 16 + p.num_seqs + 1;
@@ -1327,6 +1355,7 @@ int attend(g4_ctx* ctx, const g4_kv4_params& p, Args a, void* workspace) {
   if (a.mass) {
     a.columns = (uint32_t)weigh_columns(p);
     a.splits = weigh_splits(p);
+    a.blocks = (uint32_t)weigh_blocks(p);
     a.qdigits = w + z.meta + z.part + z.sums + z.scores;
     a.qscales = (uint2*)(a.qdigits + z.digits);
     a.weights = (float*)((uint8_t*)a.qscales + z.scales);
@@ -1341,10 +1370,10 @@ int attend(g4_ctx* ctx, const g4_kv4_params& p, Args a, void* workspace) {
     G4_LAUNCHED(ctx, "attn4_tile_merge");
   }
   if (!a.mass) return G4_OK;
-  const unsigned blocks = (unsigned)weigh_blocks(p), pairs = p.num_seqs * p.num_kv_heads;
-  hipLaunchKernelGGL(attn4_tile_weigh_kernel<HD>, dim3(blocks * a.splits, pairs), dim3(WT), 0, ctx->stream, a);
+  const unsigned pairs = p.num_seqs * p.num_kv_heads;
+  hipLaunchKernelGGL(attn4_tile_weigh_kernel<HD>, dim3(a.blocks * a.splits, pairs), dim3(WT), 0, ctx->stream, a);
   G4_LAUNCHED(ctx, "attn4_tile_weigh");
-  hipLaunchKernelGGL(attn4_mass_kernel, dim3(blocks, pairs), dim3(WP), 0, ctx->stream, a);
+  hipLaunchKernelGGL(attn4_mass_kernel, dim3(a.blocks * (WP / SP), pairs), dim3(SP * SW), 0, ctx->stream, a);
   G4_LAUNCHED(ctx, "attn4_mass");
   return G4_OK;
 }
@@ -1386,7 +1415,7 @@ int g4_pagedAttn4(g4_ctx* ctx, const float* q, const uint8_t* k_pool, const uint
   G4_REQUIRE(!mass || (uint64_t)p.num_seqs * p.num_kv_heads <= 65535, "g4_pagedAttn4: %u sequences of %u KV heads",
              p.num_seqs, p.num_kv_heads);
   const Args a{paged_args(p, q, page_table, seq_lens, row_starts, output, ops), k_pool, v_pool, k_scale, v_scale, mass,
-               nullptr, nullptr, 0, 0, nullptr, nullptr, nullptr, 1, nullptr};
+               nullptr, nullptr, 0, 0, nullptr, nullptr, nullptr, 1, 0, nullptr};
   switch (p.head_dim) {
     case 64: return attend<64>(ctx, p, a, workspace);
     case 128: return attend<128>(ctx, p, a, workspace);
