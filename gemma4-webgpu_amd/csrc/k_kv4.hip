@@ -182,7 +182,13 @@ __global__ __launch_bounds__(VT) void kv4_values_kernel(ValArgs a) {
 // kv4_select_kernel, a workgroup a sequence and KV head: the order of masses is
 // that of their bits (they are above 0, or count 0), so the bound of the largest
 // is found by three rounds of bins, from the top 11 bits down; then the rows above
-// it and the first of those at it are listed in order. kv4_move_kernel moves them.
+// it and the first of those at it are listed in order. The keys stay in LDS between
+// the rounds (in registers the loops over them unroll, and their conditions spill:
+// 33 us where this is 27). 2304 rows of one sequence: 8.0 us, a chain of six loads
+// (2.2), of the rounds' barriers (1 each) and of the list's; 32000 rows 27, 7 of them
+// the masses of one CU, 4 bytes of a line each, 10 the rounds and 7 the list.
+// kv4_move_kernel moves the rows: 8.6 us for one sequence of 2048 rows of head dim
+// 512, 8.0 for 64 of 1024 at 256, 14.8 for 8 of 4000 and two heads at 128.
 struct EvictArgs {
   g4kv4::Pool pool;
   g4kv4::Shape sh;
@@ -192,15 +198,19 @@ struct EvictArgs {
   int32_t* kept;
   uint32_t* cut;  // per sequence: whether it is cut
   uint32_t some;  // pieces of a row that a workgroup moves
+  uint32_t tiles, magic, same;  // of 16 rows a page, the rounded-up 2^32 / tiles (0 for one tile: `same` takes all of t)
+  // (exact as in the attention: t / 16 < 2^26, at most 64 tiles a page)
+  __device__ __forceinline__ uint32_t page_of(uint32_t t) const { return __umulhi(t / 16, magic) + (t / 16 & same); }
+  __device__ __forceinline__ uint32_t slot_of(uint32_t t) const { return t - page_of(t) * sh.page_size; }
 };
 
 __device__ __forceinline__ uint32_t key_of(float x) { return x > 0.f ? __float_as_uint(x) : 0u; }
 
 __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
   constexpr uint32_t NW = ST / 64, BINS = 2 * ST, GROUP = PER * ST;
+  __shared__ uint32_t s_key[GROUP];  // of candidates g * GROUP + .., as many in a row to each wave
   __shared__ uint32_t s_bin[BINS], s_sum[2 * NW], s_found[3];
-  __shared__ uint32_t s_above[PER * NW], s_at[PER * NW];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t s = blockIdx.x / a.sh.nkh, h = blockIdx.x % a.sh.nkh;
   const uint32_t L = a.seq_lens[s];
   int32_t* kept = a.kept + (size_t)blockIdx.x * a.keep;
@@ -216,47 +226,63 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
   if (m == 0) return;  // (uniform)
   const uint32_t groups = (n + GROUP - 1) / GROUP;
   const int32_t* list = a.page_table + (size_t)s * a.max_pages;
-  uint32_t key[PER];  // of candidates g * GROUP + j * ST + tid
+  const uint32_t page_rows = a.sh.page_size * a.sh.nkh, last_page = (L - 1) / a.sh.page_size;
+  const uint32_t pages_on = 64 / a.sh.page_size, rows_on = 64 % a.sh.page_size * a.sh.nkh;  // from a key to the next
+  // This thread's keys of a group: s_key[mine() + 64 * j], j < each().
   auto rows_of = [&](uint32_t g) { return min(n - g * GROUP, GROUP); };
+  auto each = [&](uint32_t g) { return (rows_of(g) + ST - 1) / ST; };
+  auto mine = [&](uint32_t g) { return w * 64 * each(g) + lane; };
+  // Eight at a time: their page ids, then their masses and the next eight's ids, are on their way together. Past the last
+  // candidate they are 0, which no round counts and which, behind all others in order, no place is left for.
   auto fetch = [&](uint32_t g) {
-    const uint32_t rows = rows_of(g);
-    int32_t pg[PER];
-    // (all of the page ids on their way, then all of the masses; eight rows at a time, past the last that one again)
+    const uint32_t rows = rows_of(g), count = each(g), i0 = mine(g), t0 = a.first + g * GROUP + i0;
+    uint32_t page = a.page_of(t0), row = (t0 - page * a.sh.page_size) * a.sh.nkh + h;
+    auto on = [&](uint32_t& p, uint32_t& r) {
+      r += rows_on;
+      const bool over = r >= page_rows;
+      r -= over ? page_rows : 0u;
+      p += pages_on + (over ? 1u : 0u);
+    };
+    int32_t id[8], next[8];
+    uint32_t at[8], p = page, r = row;
 #pragma unroll
-    for (uint32_t j = 0; j < PER; ++j) {
-      if (j % 8 == 0 && j * ST >= rows) break;  // (uniform)
-      pg[j] = list[(a.first + g * GROUP + min(j * ST + tid, rows - 1)) / a.sh.page_size];
-    }
+    for (uint32_t j = 0; j < 8; ++j, on(p, r)) next[j] = list[min(p, last_page)];
+    for (uint32_t j0 = 0; j0 < count; j0 += 8) {
+      float x[8];
 #pragma unroll
-    for (uint32_t j = 0; j < PER; ++j) {
-      if (j % 8 == 0 && j * ST >= rows) break;
-      const uint32_t t = a.first + g * GROUP + min(j * ST + tid, rows - 1);
-      const uint32_t page = pg[j] < 0 ? 0u : min((uint32_t)pg[j], a.num_pages - 1);
-      key[j] = __float_as_uint(a.pool.mass[a.sh.row(page, t % a.sh.page_size, h)]);
-    }
+      for (uint32_t j = 0; j < 8; ++j, on(page, row)) {
+        id[j] = next[j] < (int32_t)a.num_pages ? next[j] : -1;
+        at[j] = row;
+      }
 #pragma unroll
-    for (uint32_t j = 0; j < PER; ++j) {
-      if (j % 8 == 0 && j * ST >= rows) break;
-      key[j] = pg[j] >= 0 && pg[j] < (int32_t)a.num_pages ? key_of(__uint_as_float(key[j])) : 0u;
+      for (uint32_t j = 0; j < 8; ++j) x[j] = a.pool.mass[(size_t)(uint32_t)max(id[j], 0) * page_rows + at[j]];
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j, on(p, r)) next[j] = list[min(p, last_page)];
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const uint32_t i = i0 + (j0 + j) * 64;
+        if (j0 + j < count) s_key[i] = id[j] >= 0 && i < rows ? key_of(x[j]) : 0u;  // (uniform)
+      }
     }
   };
   fetch(0);
   uint32_t bound = 0, left = m;  // the m-th largest key so far; how many of those that share its bits are kept
   uint32_t share = n;            // how many share them
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;  // 11, 11 and 10 bits
+    // 11, 11 and 10 bits. The least bin has those that no other has: rows without weight, often many, are not counted
+    // one by one.
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t from = bound + (1u << shift), range = (pass == 0 ? 1u << 31 : pass == 1 ? 1u << 21 : 1u << 10) - (1u << shift);
     s_bin[2 * tid] = s_bin[2 * tid + 1] = 0;
     __syncthreads();
     for (uint32_t g = 0; g < groups; ++g) {
       if (groups > 1 && (pass || g)) fetch(g);
-      const uint32_t rows = rows_of(g);
-#pragma unroll
-      for (uint32_t j = 0; j < PER; ++j) {
-        if (j * ST >= rows) break;
-        const uint32_t b = key[j] >> shift & (pass == 2 ? 1023u : 2047u);
-        // (the least bin has those that no other has: rows without weight, often many, are not counted one by one)
-        if (b && j * ST + tid < rows && (pass == 0 || (key[j] ^ bound) >> (pass == 1 ? 21 : 10) == 0))
-          atomicAdd(&s_bin[b], 1u);
+      const uint32_t* key = s_key + mine(g);
+      const uint32_t count = each(g);
+#pragma unroll 8
+      for (uint32_t j = 0; j < count; ++j) {
+        const uint32_t d = key[64 * j] - from;
+        if (d < range) atomicAdd(&s_bin[(d >> shift) + 1], 1u);
       }
     }
     __syncthreads();
@@ -265,8 +291,8 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
     const uint32_t upto = wave_scan(hi + lo);
     if (lane == 63) s_sum[w] = upto;
     __syncthreads();
-    uint32_t above = upto - hi - lo;
-    for (uint32_t i = 0; i < w; ++i) above += s_sum[i];
+    const uint32_t sums = wave_scan(s_sum[lane % NW]);  // (in its first NW lanes)
+    const uint32_t above = upto - hi - lo + (w ? pick(sums, w - 1) : 0u);
     if (tid == ST - 1) lo = share - above - hi;
     if (above < left && above + hi + lo >= left) {  // (one thread's)
       const bool one = above + hi >= left;
@@ -278,58 +304,49 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
     bound |= s_found[0] << shift;
     left -= s_found[1];
     share = s_found[2];
-    __syncthreads();
   }
-  // the rows above the bound and the first `left` at it, in order: how many each wave has of each ST candidates, the
-  // counts summed up, then each row's place
+  // the rows above the bound and the first `left` at it, in order: how many each wave has, then each row's place
   uint32_t above = 0, at = 0;  // of the groups before
   for (uint32_t g = 0; g < groups; ++g) {
     if (groups > 1) fetch(g);
-    const uint32_t rows = rows_of(g), chunks = (rows + ST - 1) / ST;
-#pragma unroll
-    for (uint32_t j = 0; j < PER; ++j) {
-      if (j * ST >= rows) break;
-      const bool in = j * ST + tid < rows;
-      const uint64_t ma = __ballot(in && key[j] > bound), me = __ballot(in && key[j] == bound);
-      if (lane == 0) {
-        s_above[j * NW + w] = __popcll(ma);
-        s_at[j * NW + w] = __popcll(me);
+    const uint32_t* key = s_key + mine(g);
+    const uint32_t count = each(g);
+    uint32_t na = 0, ne = 0;
+#pragma unroll 8
+    for (uint32_t j = 0; j < count; ++j) {
+      const uint32_t k = key[64 * j];
+      na += __popcll(__ballot(k > bound));
+      ne += __popcll(__ballot(k == bound));
+    }
+    __syncthreads();  // (the last group's sums, or the last round's, are read)
+    if (lane == 0) {
+      s_sum[w] = na;
+      s_sum[NW + w] = ne;
+    }
+    __syncthreads();
+    const uint32_t sa = wave_scan(s_sum[lane % NW]), se = wave_scan(s_sum[NW + lane % NW]);
+    uint32_t wa = above + (w ? pick(sa, w - 1) : 0u), we = at + (w ? pick(se, w - 1) : 0u);
+    above += pick(sa, NW - 1);
+    at += pick(se, NW - 1);
+    auto before = [&](uint64_t lanes, uint32_t x) {  // x more than there are of them below this one
+      return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, x));
+    };
+    int32_t* to = kept + a.first;
+    const uint32_t t0 = a.first + g * GROUP + mine(g);
+#pragma unroll 8
+    for (uint32_t j = 0; j < count; ++j) {
+      const uint32_t k = key[64 * j];
+      const uint64_t ma = __ballot(k > bound), me = __ballot(k == bound);
+      if (me == 0) {  // (uniform, and the rule)
+        const uint32_t i = before(ma, wa + min(we, left));
+        if (k > bound) to[i] = (int32_t)(t0 + 64 * j);
+      } else {
+        const uint32_t ra = before(ma, wa), re = before(me, we);
+        if (k > bound || (k == bound && re < left)) to[ra + min(re, left)] = (int32_t)(t0 + 64 * j);
       }
+      wa += __popcll(ma);
+      we += __popcll(me);
     }
-    __syncthreads();
-    const uint32_t x = tid < chunks * NW ? s_above[tid] : 0u, y = tid < chunks * NW ? s_at[tid] : 0u;  // (PER * NW <= ST)
-    const uint32_t ux = wave_scan(x), uy = wave_scan(y);
-    if (lane == 63) {
-      s_sum[w] = ux;
-      s_sum[NW + w] = uy;
-    }
-    __syncthreads();
-    uint32_t bx = above + ux - x, by = at + uy - y;
-    for (uint32_t i = 0; i < NW; ++i) {
-      if (i < w) {
-        bx += s_sum[i];
-        by += s_sum[NW + i];
-      }
-      above += s_sum[i];
-      at += s_sum[NW + i];
-    }
-    if (tid < chunks * NW) {
-      s_above[tid] = bx;
-      s_at[tid] = by;
-    }
-    __syncthreads();
-    const uint64_t below = (1ull << lane) - 1;
-#pragma unroll
-    for (uint32_t j = 0; j < PER; ++j) {
-      if (j * ST >= rows) break;
-      const bool in = j * ST + tid < rows;
-      const uint32_t k = key[j];
-      const uint64_t ma = __ballot(in && k > bound), me = __ballot(in && k == bound);
-      const uint32_t ra = s_above[j * NW + w] + __popcll(ma & below), re = s_at[j * NW + w] + __popcll(me & below);
-      if (in && (k > bound || (k == bound && re < left)))
-        kept[a.first + ra + min(re, left)] = (int32_t)(a.first + g * GROUP + j * ST + tid);
-    }
-    __syncthreads();
   }
 }
 
@@ -354,7 +371,7 @@ __global__ __launch_bounds__(ST) void kv4_move_kernel(EvictArgs a) {
   const bool has_mass = part == 0 && threadIdx.x % some == 0;
   // of the set at hand, the next and the one after it: where its rows are, their pages. One wait for memory a set: the
   // rows of this one, the page ids of the next and the places of the one after it are on their way together.
-  uint32_t from[SETS], from1[SETS];
+  uint32_t from[SETS], from1[SETS] = {};
   int32_t src[SETS], dst[SETS];
   auto row_of_set = [&](uint32_t i0, int k) { return min(i0 + k * per + r, a.keep - 1); };  // (past the last: that one)
   auto places = [&](uint32_t i0, uint32_t* f) {
@@ -364,8 +381,8 @@ __global__ __launch_bounds__(ST) void kv4_move_kernel(EvictArgs a) {
   auto pages = [&](uint32_t i0, const uint32_t* f) {
 #pragma unroll
     for (int k = 0; k < SETS; ++k) {
-      src[k] = list[f[k] / a.sh.page_size];
-      dst[k] = list[row_of_set(i0, k) / a.sh.page_size];
+      src[k] = list[a.page_of(f[k])];
+      dst[k] = list[a.page_of(row_of_set(i0, k))];
     }
   };
   auto scale_at = [&](uint32_t page, uint32_t slot) {
@@ -373,7 +390,7 @@ __global__ __launch_bounds__(ST) void kv4_move_kernel(EvictArgs a) {
   };
   const uint32_t rows = SETS * per;
   places(0, from);
-  places(rows, from1);
+  if (rows < a.keep) places(rows, from1);
   pages(0, from);
   for (uint32_t i0 = 0; i0 < a.keep; i0 += rows) {
     u32x4 x[SETS];
@@ -382,7 +399,7 @@ __global__ __launch_bounds__(ST) void kv4_move_kernel(EvictArgs a) {
     int32_t to[SETS];  // page, or -1: it stays where it is
 #pragma unroll
     for (int k = 0; k < SETS; ++k) {
-      const uint32_t page = src[k] < 0 ? 0u : min((uint32_t)src[k], a.num_pages - 1), slot = from[k] % a.sh.page_size;
+      const uint32_t page = src[k] < 0 ? 0u : min((uint32_t)src[k], a.num_pages - 1), slot = a.slot_of(from[k]);
       x[k] = *(const u32x4*)(codes + a.sh.code(page, slot, h));
       z[k] = scales[scale_at(page, slot)];
       m[k] = has_mass && (uint32_t)src[k] < a.num_pages ? a.pool.mass[a.sh.row(page, slot, h)] : 0.f;
@@ -390,14 +407,16 @@ __global__ __launch_bounds__(ST) void kv4_move_kernel(EvictArgs a) {
       to[k] = i < a.keep && from[k] != i && (uint32_t)dst[k] < a.num_pages ? dst[k] : -1;
       from[k] = from1[k];
     }
-    pages(i0 + rows, from);
-    places(i0 + 2 * rows, from1);
+    if (i0 + rows < a.keep) {  // (uniform)
+      pages(i0 + rows, from);
+      places(i0 + 2 * rows, from1);
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (this wave's rows are here, then every wave's are)
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < SETS; ++k) {
       if (to[k] < 0) continue;
-      const uint32_t slot = row_of_set(i0, k) % a.sh.page_size;
+      const uint32_t slot = a.slot_of(row_of_set(i0, k));
       *(u32x4*)(codes + a.sh.code((uint32_t)to[k], slot, h)) = x[k];
       scales[scale_at((uint32_t)to[k], slot)] = z[k];
       if (has_mass) a.pool.mass[a.sh.row((uint32_t)to[k], slot, h)] = m[k];
@@ -520,10 +539,12 @@ int g4_kvEvict4(g4_ctx* ctx, uint8_t* k_pool, uint8_t* v_pool, uint8_t* k_scale,
   // head dim 512 in 8 workgroups 9.3 us, 8 of 4000 rows and two heads at 128 in 32 of them 19).
   uint32_t some = std::min(p.head_dim / 32, 4u);
   while (some > 1 && pairs * 2 * (p.head_dim / 32 / some) < 256) some /= 2;
+  const uint32_t tiles = p.page_size / 16;
   const EvictArgs a{{k_pool, v_pool, k_scale, v_scale, mass},
                     {p.page_size, p.num_kv_heads, p.head_dim},
                     page_table, seq_lens, p.num_seqs, p.max_pages, p.num_pages, p.max_seq_len, keep, first, recent,
-                    kept, (uint32_t*)workspace, some};
+                    kept, (uint32_t*)workspace, some, tiles, tiles == 1 ? 0u : (uint32_t)(((1ull << 32) + tiles - 1) / tiles),
+                    tiles == 1 ? ~0u : 0u};
   hipLaunchKernelGGL(kv4_select_kernel, dim3((unsigned)pairs), dim3(ST), 0, ctx->stream, a);
   G4_LAUNCHED(ctx, "kv4_select");
   const dim3 moves((unsigned)((pairs + 7) / 8 * 8) * 2 * (p.head_dim / 32 / some));

@@ -15,7 +15,7 @@ struct Pool {
 struct Shape {
   uint32_t page_size, nkh, hd;
   __device__ __forceinline__ size_t row(uint32_t page, uint32_t slot, uint32_t h) const {
-    return ((size_t)page * page_size + slot) * nkh + h;
+    return (size_t)page * (page_size * nkh) + (slot * nkh + h);  // (a page has 2^16 rows at most)
   }
   __device__ __forceinline__ size_t code(uint32_t page, uint32_t slot, uint32_t h) const {
     return row(page, slot, h) * (hd / 2);
