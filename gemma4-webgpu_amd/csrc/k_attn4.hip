@@ -53,7 +53,7 @@ struct Args : PagedArgs {
   uint8_t* qdigits;         // many rows, with mass: [KV head][16 columns][digit][128 dims][lane] 24 B, and the scales
   uint2* qscales;
   float* weights;           // [sequence][KV head][256 positions at a time][split][position]
-  uint32_t splits, blocks;
+  uint32_t splits, blocks;  // (few rows: the workgroups that weigh a sequence and KV head)
   uint32_t* done;           // many rows, with mass: whether the tiles were written
 };
 
@@ -155,9 +155,18 @@ __device__ __forceinline__ void two_by_two(uint32_t x, float sx, uint32_t y, flo
 // on in the next), 32 positions at a time to each of the four waves. A sequence
 // held by one workgroup is written by it; else its workgroups leave partials
 // (max, sum, o), which attn4_merge_kernel adds in order. With masses, the scores
-// go to the workspace, and attn4_weigh_kernel turns them into weights when the
-// maxima and sums are known: 4 bytes a position and column written and read, where
-// K again would be HD / 2 * 17 / 16 bytes a position and the products once more.
+// go to the workspace, and the merge's launch turns them into weights: 4 bytes a
+// position and column written and read, where K again would be HD / 2 * 17 / 16
+// bytes a position and the products once more. It adds 1 to 5 us to a step (head
+// dim 512: 64 sequences of up to 4352 positions 30.0 and 33.4, 32 of up to 32000 53
+// and 58; in a launch of its own behind the merge 1.2 more).
+//
+// In the loop the pool comes at 5.4 TB/s (head dim 512, 64 sequences: 3.3 us a step of
+// the four waves), around it stand 7.4 us until the first rows are there (lengths 0.8,
+// page ids and the first rows' requests 3, q's digits 2, the wait 1.6) and 2.7 for
+// the waves' sums. One sequence of 777 positions and a window of 512 at head dim 256
+// takes 8.2 us, 64 of up to 8192 18.7 (50 MB), 32 of up to 32000 at 512 52 (193 MB);
+// the merge 3.4 to 4.8.
 constexpr int NT = 256, UNIT = 128;
 constexpr uint32_t kSeqCost = 1;  // cost of a sequence and KV head besides its units: its q, its sums
 template <int HD>
@@ -173,9 +182,11 @@ struct StepShape {
   }
 };
 
-// SIZE bytes a lane from base + off to LDS at `at` (uniform), lane by lane (16 apart for 16 bytes, else 4). Written as the instruction itself because the compiler, which knows the builtin's LDS write, waits
-// for every such load before LDS is read; the waits are the caller's. (m0 takes the LDS address, with one wait state
-// after its write; it is a reserved register, which the compiler sets at each use of its own.)
+// SIZE bytes a lane from base + off to LDS at `at` (uniform), lane by lane (16 apart for
+// 16 bytes, else 4). Written as the instruction itself because the compiler, which knows
+// the builtin's LDS write, waits for every such load before LDS is read; the waits are the
+// caller's. (m0 takes the LDS address, with one wait state after its write; it is a
+// reserved register, which the compiler sets at each use of its own.)
 template <int SIZE>
 __device__ __forceinline__ void to_lds(uint32_t off, const uint8_t* base, uint32_t at) {
   if constexpr (SIZE == 16)
@@ -544,12 +555,55 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
 // Adds the partials of one column: those of workgroup meta.x / 2 (slot meta.x)
 // and of the ones up to meta.y (slot 0 of each), in this order over groups of
 // threads: group g takes every NG-th, then the groups are added in order.
+//
+// With masses, the workgroups behind those of the columns weigh the positions of a
+// sequence and KV head, a thread each, from their scores: they find the columns'
+// maxima and sums from the partials themselves rather than wait for the merge.
 template <int HD, int MT>
+__device__ __forceinline__ void weigh_positions(const Args& a, uint32_t b) {
+  __shared__ float2 s_sum[COLS];
+  const uint32_t sh = b / a.blocks, s = sh / a.nkh, kvh = sh % a.nkh, tid = threadIdx.x;
+  const Seq q = seq_rows(a.rows, s);
+  const uint32_t lo = first_seen(a, q), ncols = q.n * a.G;
+  uint32_t t = lo + b % a.blocks * MT + tid;
+  if (t - tid >= q.len) return;  // (uniform; a length of 0 too)
+  static_assert(MT >= COLS * 16);
+  const uint2 mt = a.meta[sh];
+  const uint32_t col = tid / 16, w0 = mt.x / 2, n = mt.y - w0 + 1;
+  if (col < ncols) {
+    if (n == 1) {  // (uniform) written by its workgroup
+      s_sum[col] = a.sums[row_of(a, q.first, kvh, col)];
+    } else {
+      auto part = [&](uint32_t k) { return a.part + (size_t)(k ? 2 * (w0 + k) : mt.x) * StepShape<HD>::SLOT + col; };
+      float m = kNothing, sum = 0.f;
+      for (uint32_t k = tid % 16; k < n; k += 16) m = fmaxf(m, *part(k));
+      m = g4d::max16(m);
+      for (uint32_t k = tid % 16; k < n; k += 16) sum += exp2_h(*part(k) - m) * part(k)[COLS];
+      sum = g4d::sum16(sum);
+      if (tid % 16 == 0) s_sum[col] = make_float2(m, kPScale / sum);
+    }
+  }
+  __syncthreads();
+  for (; t < q.len; t += a.blocks * MT) {
+    const uint32_t at = t - lo, tile = t / 16, page = page_of(a, tile);
+    const int32_t id = a.page_table[(size_t)s * a.max_pages + page];
+    const float* x = a.scores + ((size_t)sh * a.units + at / UNIT) * a.columns * UNIT + at % UNIT;
+    float got = 0.f;
+    for (uint32_t c = 0; c < ncols; ++c) got += exp2_h(x[c * UNIT] - s_sum[c].x) * s_sum[c].y;
+    if (id >= 0 && id < (int32_t)a.num_pages)
+      a.mass[((size_t)id * (a.page_tiles * 16) + (t - page * a.page_tiles * 16)) * a.nkh + kvh] += got;
+  }
+}
+template <int HD, int MT, bool MASS>
 __global__ __launch_bounds__(MT) void attn4_merge_kernel(Args a) {
   constexpr int TG = HD / 4, NG = MT / TG, MS = 4;  // threads a partial row, groups, loads in flight of each
   __shared__ float s_m[NG], s_l[NG];
   __shared__ __align__(16) float s_o[NG * HD];
   const uint32_t cols = a.rows.max_rows * a.G, col = blockIdx.x % cols;
+  if (const uint32_t merges = a.rows.num_seqs * a.nkh * cols; MASS && blockIdx.x >= merges) {
+    weigh_positions<HD, MT>(a, blockIdx.x - merges);
+    return;
+  }
   const uint32_t sh = blockIdx.x / cols, s = sh / a.nkh, kvh = sh % a.nkh;
   const Seq q = seq_rows(a.rows, s);
   if (!q.len || col >= q.n * a.G) return;
@@ -605,30 +659,7 @@ __global__ __launch_bounds__(MT) void attn4_merge_kernel(Args a) {
   y *= 1.0f / L;
   const uint32_t row = q.first + col / a.G, head = kvh * a.G + col % a.G;
   *(f4*)(a.out + ((size_t)row * a.nqh + head) * HD + d) = y;
-  if (a.sums && d == 0) a.sums[(size_t)row * a.nqh + head] = make_float2(M, kPScale / L);
   if (HD >= 256 && a.ops) write_ops(a, row, head * (HD / 256) + d / 256, threadIdx.x & 63, y);
-}
-
-// The weights of a unit's positions from their scores, a thread each, added over the columns in order.
-__global__ __launch_bounds__(UNIT) void attn4_weigh_kernel(Args a) {
-  __shared__ float2 s_sum[COLS];
-  const uint32_t sh = blockIdx.y, s = sh / a.nkh, kvh = sh % a.nkh, i = threadIdx.x;
-  const Seq q = seq_rows(a.rows, s);
-  if (!q.len) return;
-  const uint32_t ncols = q.n * a.G, lo = first_seen(a, q);
-  if (i < ncols) s_sum[i] = a.sums[row_of(a, q.first, kvh, i)];
-  __syncthreads();
-  for (uint32_t unit = blockIdx.x; lo + unit * UNIT < q.len; unit += gridDim.x) {
-    const uint32_t t = lo + unit * UNIT + i;
-    if (t >= q.len) return;
-    const float* x = a.scores + ((size_t)sh * a.units + unit) * a.columns * UNIT + i;
-    float got = 0.f;
-    for (uint32_t c = 0; c < ncols; ++c) got += exp2_h(x[c * UNIT] - s_sum[c].x) * s_sum[c].y;
-    const uint32_t tile = t / 16, page = page_of(a, tile);
-    const int32_t id = a.page_table[(size_t)s * a.max_pages + page];
-    if (id >= 0 && id < (int32_t)a.num_pages)
-      a.mass[((size_t)id * (a.page_tiles * 16) + (t - page * a.page_tiles * 16)) * a.nkh + kvh] += got;
-  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1321,7 +1352,7 @@ int attend(g4_ctx* ctx, const g4_kv4_params& p, Args a, void* workspace) {
     const uint64_t units = most_units(p), pairs = (uint64_t)p.num_seqs * p.num_kv_heads;
     G4_REQUIRE((units + kSeqCost) * pairs < (1ull << 31), "g4_pagedAttn4: %u sequences of up to %u positions and %u KV heads in one "
                "call", p.num_seqs, p.max_seq_len, p.num_kv_heads);
-    G4_REQUIRE(pairs * p.max_rows * a.G < 1u << 24, "g4_pagedAttn4: %u sequences of up to %u rows of %u heads in one "
+    G4_REQUIRE(pairs * (p.max_rows * a.G + (a.mass ? 1 : 0)) < 1u << 23, "g4_pagedAttn4: %u sequences of up to %u rows of %u heads in one "
                "call", p.num_seqs, p.max_rows, p.num_q_heads);
     a.wgs = step_wgs<HD>(p);
     a.units = (uint32_t)units;
@@ -1330,18 +1361,21 @@ int attend(g4_ctx* ctx, const g4_kv4_params& p, Args a, void* workspace) {
     if (a.mass) hipLaunchKernelGGL((attn4_step_kernel<HD, true>), grid, dim3(NT), 0, ctx->stream, a);
     else hipLaunchKernelGGL((attn4_step_kernel<HD, false>), grid, dim3(NT), 0, ctx->stream, a);
     G4_LAUNCHED(ctx, "attn4_step");
-    if (units > 1) {  // (else no sequence has partials)
-      const dim3 merges(p.num_seqs * p.num_kv_heads * p.max_rows * a.G);
-      if (std::min<uint64_t>(units, a.wgs) <= 32 || merges.x >= 1u << 22)
-        hipLaunchKernelGGL((attn4_merge_kernel<HD, 256>), merges, dim3(256), 0, ctx->stream, a);
-      else
-        hipLaunchKernelGGL((attn4_merge_kernel<HD, 1024>), merges, dim3(1024), 0, ctx->stream, a);
-      G4_LAUNCHED(ctx, "attn4_merge");
-    }
+    const uint64_t merges = pairs * p.max_rows * a.G;
+    const bool wide = std::min<uint64_t>(units, a.wgs) > 32 && merges < 1u << 20;
+    const unsigned threads = wide ? 1024 : 256;
     if (a.mass) {
-      hipLaunchKernelGGL(attn4_weigh_kernel, dim3((unsigned)std::min<uint64_t>(units, 4096), (unsigned)pairs), dim3(UNIT),
-                         0, ctx->stream, a);
-      G4_LAUNCHED(ctx, "attn4_weigh");
+      // a position a thread, in at most 2^20 workgroups
+      a.blocks = (uint32_t)std::min<uint64_t>(ceil_div(units * UNIT, threads), std::max<uint64_t>(1, (1u << 20) / pairs));
+      const dim3 grid((unsigned)(merges + pairs * a.blocks));
+      if (wide) hipLaunchKernelGGL((attn4_merge_kernel<HD, 1024, true>), grid, dim3(threads), 0, ctx->stream, a);
+      else hipLaunchKernelGGL((attn4_merge_kernel<HD, 256, true>), grid, dim3(threads), 0, ctx->stream, a);
+      G4_LAUNCHED(ctx, "attn4_merge");
+    } else if (units > 1) {  // (else no sequence has partials)
+      const dim3 grid((unsigned)merges);
+      if (wide) hipLaunchKernelGGL((attn4_merge_kernel<HD, 1024, false>), grid, dim3(threads), 0, ctx->stream, a);
+      else hipLaunchKernelGGL((attn4_merge_kernel<HD, 256, false>), grid, dim3(threads), 0, ctx->stream, a);
+      G4_LAUNCHED(ctx, "attn4_merge");
     }
     return G4_OK;
   }
