@@ -64,45 +64,42 @@ struct Args : PagedArgs {
 // last digit's scale ends there).
 struct QScale {
   int e;
-  bool none;
   uint2 bytes;  // of the first four; of the last
 };
 __device__ __forceinline__ QScale q_scale(uint32_t am) {
   QScale z;
   const bool bad = am >= 0x7f800000u;
   z.e = (int)(am >> 23) - 127;  // 2^e <= am < 2^(e + 1)
-  z.none = bad || z.e < -106;
-  z.e = z.none ? 0 : z.e;
+  z.e = bad || z.e < -106 ? 0 : z.e;  // (so small an element has digits of 0 from 2^0 on)
   const uint32_t s = (uint32_t)(z.e + 127);
   z.bytes.x = bad ? 0x7f7f7f00u | BAD : s | (s - 5) << 8 | (s - 10) << 16 | (s - 15) << 24;
   z.bytes.y = bad ? 127u : s - 20;
   return z;
 }
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-// The digits of N neighbouring elements x of a block (the rest of it taken as 0), as their codes: to(digit, code).
+// The digits of N neighbouring elements x of a block (the rest of it taken as 0), as their codes: to(digit, code). Below 2
+// units a code's steps are 1 / 8 of one, so that each conversion rounds to a digit and leaves at most half of a step, two
+// units of the next. (An element that is not finite has any digits; the block's scale is NaN then.)
 template <int N, typename F>
 __device__ __forceinline__ void digits_of(const float* x, const QScale& z, F&& to) {
   f16x a, b;  // even, odd elements (the conversion takes them in turn)
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    a[i] = 2 * i < N && !z.none ? __builtin_amdgcn_ldexpf(x[2 * i < N ? 2 * i : 0], -z.e) : 0.f;
-    b[i] = 2 * i < N && !z.none ? __builtin_amdgcn_ldexpf(x[2 * i < N ? 2 * i + 1 : 0], -z.e) : 0.f;
+    a[i] = 2 * i < N ? __builtin_amdgcn_ldexpf(x[2 * i < N ? 2 * i : 0], -z.e) : 0.f;
+    b[i] = 2 * i < N ? __builtin_amdgcn_ldexpf(x[2 * i < N ? 2 * i + 1 : 0], -z.e) : 0.f;
   }
   static_for<DIGITS>([&](auto d) __attribute__((always_inline)) {
     constexpr int D = decltype(d)::value;
-    constexpr float unit = 1.f / (float)(1u << (5 * D)), border = 1572864.f * unit;  // 1.5 * 2^20: steps of 1 / 8
-    if constexpr (D == DIGITS - 1) {
-      to(d, __builtin_bit_cast(i6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, unit)));
-    } else {
-      f16x u{}, v{};
+    constexpr float unit = 1.f / (float)(1u << (5 * D));
+    const auto code = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, unit);
+    to(d, __builtin_bit_cast(i6, code));
+    if constexpr (D < DIGITS - 1) {
+      const auto u = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(code, unit);
 #pragma unroll
       for (int i = 0; 2 * i < N; ++i) {
-        u[i] = (a[i] + border) - border;
-        v[i] = (b[i] + border) - border;
-        a[i] -= u[i];
-        b[i] -= v[i];
+        a[i] -= u[2 * i];
+        b[i] -= u[2 * i + 1];
       }
-      to(d, __builtin_bit_cast(i6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(u, v, unit)));
     }
   });
 }
