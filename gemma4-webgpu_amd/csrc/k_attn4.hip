@@ -20,6 +20,7 @@
 // Sums over steps are f32. Maxima are taken to the next power of two, so that a
 // later one rescales exactly.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "attn_paged.hpp"
@@ -39,12 +40,14 @@ typedef int i8 __attribute__((ext_vector_type(8)));
 typedef float f16x __attribute__((ext_vector_type(16)));
 
 constexpr int COLS = 16;               // columns of a matrix product
-constexpr float kLog2e = 1.44269504f;  // the softmax works in powers of two
+constexpr double kLog2e = 1.4426950408889634;  // the softmax works in powers of two
 constexpr float kPScale = 32768.f;
 constexpr float kNothing = -3e38f;     // the maximum of no positions: finite, so that differences are
 constexpr int DIGITS = 5;
 
 struct Args : PagedArgs {
+  float scale_part;  // scale * log2(e) = scale_part * 2^scale_up, its magnitude in 0.5 .. 1 (or 0)
+  int scale_up;
   const uint8_t *kp, *vp, *ks, *vs;
   float* mass;              // or null
   float2* sums;             // with mass: maximum and 1 / sum of each row and query head
@@ -60,18 +63,20 @@ struct Args : PagedArgs {
 // ---- q as digits ----
 
 // The exponent of a block of q with the largest magnitude am (its bits, so that a NaN is the largest), and the scale
-// bytes of its five digits. A block that is not finite counts as 0 under a scale of NaN, one below 2^-106 as 0 (the
-// last digit's scale ends there).
+// bytes of its five digits, with the exponent `up` of the scores' scale in them: so the sums are the scores within a
+// factor of two, whatever q's size and the scale's. A block that is not finite counts as 0 under a scale of NaN; one
+// below 2^-106 of a score as 0 (the last digit's scale ends there).
 struct QScale {
-  int e;
+  int down;     // times 2^down the largest is in 1 .. 2
   uint2 bytes;  // of the first four; of the last
 };
-__device__ __forceinline__ QScale q_scale(uint32_t am) {
+__device__ __forceinline__ QScale q_scale(uint32_t am, int up) {
   QScale z;
   const bool bad = am >= 0x7f800000u;
-  z.e = (int)(am >> 23) - 127;  // 2^e <= am < 2^(e + 1)
-  z.e = bad || z.e < -106 ? 0 : z.e;  // (so small an element has digits of 0 from 2^0 on)
-  const uint32_t s = (uint32_t)(z.e + 127);
+  const int e = max((int)(am >> 23), 1) - 127, to = min(e + up, 127);  // am < 2^(e + 1)
+  const bool none = to < -106;
+  z.down = none ? -300 : -e;
+  const uint32_t s = none ? 127u : (uint32_t)(to + 127);
   z.bytes.x = bad ? 0x7f7f7f00u | BAD : s | (s - 5) << 8 | (s - 10) << 16 | (s - 15) << 24;
   z.bytes.y = bad ? 127u : s - 20;
   return z;
@@ -85,8 +90,8 @@ __device__ __forceinline__ void digits_of(const float* x, const QScale& z, F&& t
   f16x a, b;  // even, odd elements (the conversion takes them in turn)
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    a[i] = 2 * i < N ? __builtin_amdgcn_ldexpf(x[2 * i < N ? 2 * i : 0], -z.e) : 0.f;
-    b[i] = 2 * i < N ? __builtin_amdgcn_ldexpf(x[2 * i < N ? 2 * i + 1 : 0], -z.e) : 0.f;
+    a[i] = 2 * i < N ? __builtin_amdgcn_ldexpf(x[2 * i < N ? 2 * i : 0], z.down) : 0.f;
+    b[i] = 2 * i < N ? __builtin_amdgcn_ldexpf(x[2 * i < N ? 2 * i + 1 : 0], z.down) : 0.f;
   }
   static_for<DIGITS>([&](auto d) __attribute__((always_inline)) {
     constexpr int D = decltype(d)::value;
@@ -319,7 +324,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
 #pragma unroll
       for (int e = 0; e < QE; ++e) am = max(am, magnitude(qx[e]));
       am = max(am, (uint32_t)g4d::dppi<g4d::kDppXor1>((int)am));
-      const QScale z = q_scale(am);
+      const QScale z = q_scale(am, a.scale_up);
       const uint32_t j = block % J, lane = block / J * 16 + col;
       s_qs[j * 64 + lane] = z.bytes;
       digits_of<QE>(qx, z, [&](auto d, const i6& code) __attribute__((always_inline)) {
@@ -340,7 +345,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
     ring_barrier();  // every wave has them
     if (n > 1) load(1);
     // this lane's column: positions clo .. clo + width - 1
-    const float s_scale = a.scale * kLog2e;
+    const float s_scale = a.scale_part;
     const uint32_t cpos = sq.base + div_g(a, c);
     const uint32_t clo = a.window && cpos + 1 > a.window ? cpos + 1 - a.window : 0u;
     const uint32_t width = (uint32_t)c < ncols ? cpos + 1 - clo : 0u;
@@ -841,8 +846,8 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn4_ti
     // ---- q's digits: the scale's sign goes to q; a scale of 0 leaves equal scores ----
     i6 qb[DIGITS][J];
     uint2 qs[J];
-    const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
-    const float sc = a.scale == 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);  // (0 times a masked -Inf: NaN)
+    const float sign = a.scale_part < 0.f ? -1.f : a.scale_part == 0.f ? 0.f : 1.f;
+    const float sc = a.scale_part == 0.f ? 1.f : fabsf(a.scale_part);  // (0 times a masked -Inf: NaN)
     static_for<J>([&](auto jj) __attribute__((always_inline)) {
       constexpr int j = decltype(jj)::value;
       const bool pad = HD == 64 && qd >= 2;
@@ -857,7 +862,7 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn4_ti
       uint32_t am = 0;
 #pragma unroll
       for (int e = 0; e < BLOCK; ++e) am = max(am, magnitude(x[e]));
-      const QScale q = q_scale(am);
+      const QScale q = q_scale(am, a.scale_up);
       qs[j] = q.bytes;
       digits_of<BLOCK>(x, q, [&](auto d, const i6& code) __attribute__((always_inline)) {
         qb[decltype(d)::value][j] = code;
@@ -1176,7 +1181,7 @@ __global__ __launch_bounds__(WT, 2) void attn4_tile_weigh_kernel(Args a) {
     if constexpr (J == 4) z[p] |= (uint32_t)*(const uint16_t*)(y + 8) << 16;
     if (HD == 64 && qd >= 2) z[p] = 127;  // (no dims there)
   }
-  const float sc = a.scale == 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1.2e-38f);
+  const float sc = a.scale_part == 0.f ? 1.f : fabsf(a.scale_part);
   const size_t first = (size_t)kvh * a.columns + first_columns(a, s, q);
   f4 sum[PT], part[PT];
 #pragma unroll
@@ -1445,8 +1450,11 @@ int g4_pagedAttn4(g4_ctx* ctx, const float* q, const uint8_t* k_pool, const uint
              "head and a 16-byte aligned buffer");
   G4_REQUIRE(!mass || (uint64_t)p.num_seqs * p.num_kv_heads <= 65535, "g4_pagedAttn4: %u sequences of %u KV heads",
              p.num_seqs, p.num_kv_heads);
-  const Args a{paged_args(p, q, page_table, seq_lens, row_starts, output, ops), k_pool, v_pool, k_scale, v_scale, mass,
-               nullptr, nullptr, 0, 0, nullptr, nullptr, nullptr, 1, 0, nullptr};
+  int up = 0;
+  double part = p.scale * kLog2e;
+  if (std::isfinite(part)) part = std::frexp(part, &up);
+  const Args a{paged_args(p, q, page_table, seq_lens, row_starts, output, ops), (float)part, up,
+               k_pool, v_pool, k_scale, v_scale, mass, nullptr, nullptr, 0, 0, nullptr, nullptr, nullptr, 1, 0, nullptr};
   switch (p.head_dim) {
     case 64: return attend<64>(ctx, p, a, workspace);
     case 128: return attend<128>(ctx, p, a, workspace);

@@ -687,6 +687,21 @@ def test_steps_beside_a_prompt(ctx):
     c.check_mass(c.mass)
 
 
+@pytest.mark.parametrize("up", [120, 0, -96])
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("rows", [1, 7])
+def test_queries_of_any_size(ctx, hd, rows, up):
+    """q's blocks of 32 dims have exponents of their own: large or small ones under the inverse scale, and beside each
+    other in a row."""
+    c = Case(ctx, [90, rows], [rows, rows], 8, 1, hd, 16, 191, scale=2.0 ** -up)
+    c.q *= np.float32(2.0 ** up)
+    if up <= 0:
+        c.q.reshape(-1, 32)[::2] *= np.float32(2.0 ** (-8 if up else -40))
+    before = c.mass.copy()
+    c.up().check_attention(c.attention(mass=True), what=(hd, rows, up))
+    c.check_mass(before, (hd, rows, up))
+
+
 @pytest.mark.parametrize("hd,theta,divisor", [(64, 1e4, 1), (256, 1e6, 0), (512, 1e6, 1), (128, 5e5, 1)])
 def test_prologue_by_theta_and_divisor(ctx, hd, theta, divisor):
     """Angles formed in the launch: the same bits as from a table of its theta and divisors."""
