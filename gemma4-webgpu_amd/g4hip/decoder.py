@@ -840,7 +840,7 @@ class BatchDecoder(_SyntheticModel):
     prologue, or the attention prologue), so no launch waits on another's
     workgroups and the step is deterministic.
     """
-    kv4, budget, capturing = False, None, False
+    kv4, budget, capturing, replayed = False, None, False, False
 
     def __init__(self, ctx: Context, context_lens, shape: Optional[E2BShape] = None, page_size: int = 16,
                  reserve: int = 64, seed: int = 0, n_layers: Optional[int] = None, lm_head: bool = True,
@@ -1137,9 +1137,9 @@ class BatchDecoder(_SyntheticModel):
     def evict(self) -> None:
         """Cuts the caches that have a budget down to it: every sequence with more rows there keeps its first, its last
         and its heaviest (`kept[layer]` [sequences][KV heads][budget]: where they were). Steps and prompts that the
-        host enqueues call it where they need room; between the replays of a captured step, of which the host knows
-        nothing, it is the caller's, once in `slack` of them at least: a sequence without room appends nothing.
-        Waits for the device."""
+        host enqueues call it where they need room (a step beside a captured one reads the lengths back first);
+        between the replays of a captured step it is the caller's, once in `slack` of them at least: a sequence without
+        room appends nothing. Waits for the device."""
         if self.budget is None:
             raise ValueError("evict needs a budget")
         self._evict()
@@ -1160,6 +1160,8 @@ class BatchDecoder(_SyntheticModel):
         """Room for `rows` more of every sequence in the caches that have a budget, and their lengths with them."""
         if self.budget is None:
             return
+        if self.replayed and not self.capturing:  # (how often, the host does not know)
+            self.cut_lens_host = self.cut_lens.download(np.uint32)
         if not self.capturing and int(self.cut_lens_host.max()) + rows > self.cut_rows:
             self._evict()
         self.ctx.advanceSeqLens(self.cut_lens, len(self.cut_lens_host), rows)
@@ -1675,7 +1677,7 @@ class BatchDecoder(_SyntheticModel):
         try:
             self.step(sample)
         finally:
-            self.capturing = False
+            self.capturing, self.replayed = False, True
             g = self.ctx.graph_end()
         self.lens_host = lens  # capture enqueues nothing
         return g

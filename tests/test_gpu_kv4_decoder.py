@@ -83,6 +83,30 @@ def test_steps(ctx, kind, ps):
     assert np.array_equal(d.seq_lens.download(np.uint32), np.array(LENS) + 3)
 
 
+def test_eager_steps_after_replays_find_room(ctx):
+    """The host does not count the replays of a captured step: a step of its own after them evicts where all of its own
+    would have."""
+    runs = []
+    for replays in (0, 6):
+        d = BatchDecoder(ctx, LENS, shape(), seed=53, reserve=24, embed=True, kv="fp4", budget=64, slack=8)
+        d.fill_kv(seed=54)
+        d.tokens.upload(np.arange(d.B, dtype=np.uint32))
+        g = d.capture() if replays else None
+        got = []
+        for i in range(14):
+            if i < replays:
+                ctx.graph_launch(g)
+            else:
+                d.step()
+            got.append([b.download(np.uint32) for b in (d.tokens, d.logits, d.cut_lens)])
+        runs.append(got)
+        if g is not None:
+            ctx.graph_destroy(g)
+    assert max(x[2].max() for x in runs[0]) == 72 and any(x[2].max() == 65 for x in runs[0][1:])
+    for step, (a, b) in enumerate(zip(*runs)):
+        assert all(np.array_equal(x, y) for x, y in zip(a, b)), step
+
+
 @pytest.mark.parametrize("budget", [None, 64])
 def test_a_captured_step_equals_eager_ones(ctx, budget):
     runs = []
