@@ -11,8 +11,7 @@
 //    f32 accumulator: digits in [-16, 16] / 8, q rounded to 2^-24 of its block's
 //    largest. Products and sums of one instruction are exact but for one rounding
 //    (2^-23.2 of the magnitudes' sum at most, over random blocks and scales). No
-//    conversion of K, at 16 cycles for 128 dims and a digit; three digits of 8 bits
-//    with integer products (K expanded to bytes) take 24 for the five's 40 / 2 = 20.
+//    conversion of K, and 16 cycles for 128 dims and a digit.
 //  * P V: v_mfma_f32_16x16x32_f16, P * 2^15 as f16 hi + lo in one sum: 22 bits of
 //    every P down to 2^-17 of the row's largest and 2^-40 of it below. V is exact
 //    in f16 (codes of 2 bits, scales 2^-20 .. 2^13): one conversion for two codes
@@ -167,7 +166,7 @@ __device__ __forceinline__ void two_by_two(uint32_t x, float sx, uint32_t y, flo
 // the four waves), around it stand 7.4 us until the first rows are there (lengths 0.8,
 // page ids and the first rows' requests 3, q's digits 2, the wait 1.6) and 2.7 for
 // the waves' sums. One sequence of 777 positions and a window of 512 at head dim 256
-// takes 8.2 us, 64 of up to 8192 18.7 (50 MB), 32 of up to 32000 at 512 52 (193 MB);
+// takes 7.8 us, 64 of up to 8192 18.1 (50 MB), 32 of up to 32000 at 512 52 (193 MB);
 // the merge 3.4 to 4.8.
 constexpr int NT = 256, UNIT = 128;
 constexpr uint32_t kSeqCost = 1;  // cost of a sequence and KV head besides its units: its q, its sums
@@ -687,14 +686,14 @@ __global__ __launch_bounds__(MT) void attn4_merge_kernel(Args a) {
 // workgroups a CU. A tile held by one workgroup is written by it, else its
 // workgroups leave partials that attn4_tile_merge_kernel adds in order.
 //
-// A prompt of 4500 rows of 8 heads: 109 us at head dim 128, 163 at 256 and 356 at 512
-// (382, 510 and 467 TFLOP/s), of 1500 rows 33, 46 and 78, the merge included. The
+// A prompt of 4500 rows of 8 heads: 108 us at head dim 128, 162 at 256 and 346 at 512
+// (384, 512 and 479 TFLOP/s), of 1500 rows 32, 45 and 72, the merge included. The
 // matrix cores work 15 % of the time and the VALUs 30 (at a step of 64 positions and
 // head dim 256 a wave has 104 products and 480 VALU instructions: V's codes to f16,
 // the softmax, the masks), the rest waits: for LDS, and at the steps' barriers, since
 // registers allow two waves a SIMD. At head dim 512 a step of two barriers, with the
-// next step's rows in flight for all of it, spills and takes 82 us where this one's
-// four take 76.
+// next step's rows in flight for all of it, spilled and took 82 us where this one's
+// four took 76.
 template <int HD>
 struct TileShape {
   static constexpr bool PAIR = HD == 512;
@@ -1138,9 +1137,9 @@ __global__ __launch_bounds__(HD / 4) void attn4_tile_merge_kernel(Args a) {
 // would be 2e-6 off), the lanes of a position at the end. The columns of a block of
 // positions come in `splits` parts, which attn4_mass_kernel adds in order: a prompt's
 // first block is seen by all of its columns and its last by few, so twice the
-// workgroups that fit at once take 91 us where as many as fit take 101 (4500 rows of 8
-// heads, dim 128: with the tiles 161 and 183 us), and parts of 4 column tiles or more
-// (375 rows, dim 512: 53 us in all, of 8 tiles 63, of 2 51 but 68 at 750 rows for 61).
+// workgroups that fit at once are dealt out (4500 rows of 8 heads, dim 128: 161 us with
+// the attention, as many as fit 183), in parts of 4 column tiles or more (375 rows, dim
+// 512: 53 us with the attention, of 8 tiles 63, of 2 51, but 68 at 750 rows for 66).
 // The products take 5.5 us of 32 at 1500 rows and dim 512: what bounds it is the way
 // to them, a row's page and digits, and one wave's exponentials beside another's products.
 constexpr int WT = 256, WP = 256;  // threads, positions of a workgroup

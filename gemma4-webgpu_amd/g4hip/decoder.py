@@ -20,8 +20,8 @@ decode step in either of two forms:
 ``BatchDecoder`` runs the same layers for many sequences at once (ragged
 continuous-batching decode): every matmul takes all sequences' activation
 vectors through the matrix-core kernel (each weight tile read once per
-step), and attention reads each sequence's K/V from a paged f16 pool
-through a per-sequence page table.
+step), and attention reads each sequence's K/V from a paged pool (f16, 8-bit
+or 4-bit) through a per-sequence page table.
 
 Two layer layouts (src/config/gemma4-e2b.ts:16-63):
 
@@ -824,8 +824,8 @@ class Decoder(_SyntheticModel):
 
 class BatchDecoder(_SyntheticModel):
     """Ragged multi-sequence decode: `num_seqs` sequences with their own cached
-    lengths share one set of weights and, per layer, one paged K/V pool (f16
-    or 8-bit).
+    lengths share one set of weights and, per layer, one paged K/V pool (f16,
+    8-bit or 4-bit).
 
     Pages are handed out on the host when the decoder is built: sequence i
     owns ceil((context_lens[i] + reserve) / page_size) pages, taken from a
