@@ -316,7 +316,6 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
     const uint32_t* key = s_key + mine(g);
     const uint32_t count = each(g);
     uint32_t na = 0, ne = 0;
-#pragma unroll 8
     for (uint32_t j = 0; j < count; ++j) {
       const uint32_t k = key[64 * j];
       na += __popcll(__ballot(k > bound));
@@ -337,7 +336,6 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
     };
     int32_t* to = kept + a.first;
     const uint32_t t0 = a.first + g * GROUP + mine(g);
-#pragma unroll 8
     for (uint32_t j = 0; j < count; ++j) {
       const uint32_t k = key[64 * j];
       const uint64_t ma = __ballot(k > bound), me = __ballot(k == bound);
