@@ -191,8 +191,9 @@ __global__ __launch_bounds__(VT) void kv4_values_kernel(ValArgs a) {
 // 33 us where this is 27). 2304 rows of one sequence: 8.0 us, a chain of six loads
 // (2.2), of the rounds' barriers (1 each) and of the list's; 32000 rows 27, 7 of them
 // the masses of one CU, 4 bytes of a line each, 10 the rounds and 7 the list.
-// kv4_move_kernel moves the rows: 8.6 us for one sequence of 2048 rows of head dim
-// 512, 8.0 for 64 of 1024 at 256, 14.8 for 8 of 4000 and two heads at 128.
+// kv4_move_kernel moves the rows: 8.4 us for one sequence of 2048 rows of head dim
+// 512 (places 0.6, pages 0.4, rows 3.2, stores 1.4 and the launch), 7.8 for 64 of
+// 1024 at 256, 14.9 for 8 of 4000 and two heads at 128.
 struct EvictArgs {
   g4kv4::Pool pool;
   g4kv4::Shape sh;
@@ -364,8 +365,7 @@ __global__ __launch_bounds__(ST) void kv4_move_kernel(EvictArgs a) {
   const uint32_t pair = blockIdx.x / (16 * parts) * 8 + blockIdx.x % 8, part = blockIdx.x / 8 % (2 * parts);
   if (pair >= pairs) return;
   const uint32_t s = pair / a.sh.nkh, h = pair % a.sh.nkh;
-  if (!a.cut[s]) return;
-  if (h == 0 && part == 0 && threadIdx.x == 0) a.seq_lens[s] = a.keep;
+  const uint32_t cut = a.cut[s];  // (on its way with the first places)
   const bool is_v = part >= parts;
   const uint32_t b = part % parts * some + threadIdx.x % some, per = ST / some, r = threadIdx.x / some;
   const int32_t *kept = a.kept + (size_t)pair * a.keep, *list = a.page_table + (size_t)s * a.max_pages;
@@ -393,6 +393,8 @@ __global__ __launch_bounds__(ST) void kv4_move_kernel(EvictArgs a) {
   const uint32_t rows = SETS * per;
   places(0, from);
   if (rows < a.keep) places(rows, from1);
+  if (!cut) return;
+  if (h == 0 && part == 0 && threadIdx.x == 0) a.seq_lens[s] = a.keep;
   pages(0, from);
   for (uint32_t i0 = 0; i0 < a.keep; i0 += rows) {
     u32x4 x[SETS];
