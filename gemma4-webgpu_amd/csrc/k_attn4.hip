@@ -302,10 +302,12 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
     };
 
     // q, QE dims of a column a thread (asked for before the page ids, so that it has come when the rows are asked for)
-    constexpr int QE = 16, QT = 128 * J, QC = QT / 16;  // threads that have some; of a column
-    const uint32_t col = tid / QC, qdim = tid % QC * QE, block = qdim / BLOCK;
+    constexpr int QE = 16, QC = 128 * J / QE;                // threads of a column
+    constexpr int QCOLS = COLS * QC <= NT ? COLS : NT / QC;  // columns at once (head dim 512: 8 of the 16)
+    static_assert(QCOLS == COLS || 2 * QCOLS == COLS);
+    const uint32_t qdim = tid % QC * QE, block = qdim / BLOCK;
     float qx[QE];
-    if (tid < QT) {
+    auto load_q = [&](uint32_t col) __attribute__((always_inline)) {
       const float* qg = a.q + row_of(a, sq.first, kvh, min(col, ncols - 1)) * HD + (HD == 64 ? qdim % 64 : qdim);
 #pragma unroll
       for (int e = 0; e < QE; e += 4) {
@@ -313,12 +315,13 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
 #pragma unroll
         for (int i = 0; i < 4; ++i) qx[e + i] = HD == 64 && block >= 2 ? 0.f : y[i];
       }
-    }
+    };
+    if (tid < QCOLS * QC) load_q(tid / QC);
     refill(0);
     ring_barrier();  // the previous sequence's sums are done with
     if (n > 0) load(0);  // (uniform)
     // ---- q's digits ----
-    if (tid < QT) {
+    auto store_digits = [&](uint32_t col) __attribute__((always_inline)) {
       uint32_t am = 0;
 #pragma unroll
       for (int e = 0; e < QE; ++e) am = max(am, magnitude(qx[e]));
@@ -331,6 +334,11 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
 #pragma unroll
         for (int i = 0; i < QE * 3 / 16; ++i) to[i] = (uint32_t)code[i];
       });
+    };
+    if (tid < QCOLS * QC) store_digits(tid / QC);
+    if (QCOLS < COLS && ncols > QCOLS) {  // (uniform; columns past the last one keep any digits: their weights are 0)
+      load_q(tid / QC + QCOLS);
+      store_digits(tid / QC + QCOLS);
     }
     ring_barrier();
     i6 qb[DIGITS][J];

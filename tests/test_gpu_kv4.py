@@ -368,6 +368,37 @@ def test_attention(ctx, lens, rows, nqh, nkh, hd, ps, window, mass):
         assert np.array_equal(c.dm.download(np.uint32), first)
 
 
+FULL = [  # lens, rows, query heads, K/V heads: 9 to 16 columns of a K/V head, the few-rows kernel's most
+    ([300, 33], [2, 2], 8, 1),
+    ([700], [1], 16, 1),
+    ([41, 260, 7], [1, 1, 1], 9, 1),
+    ([150, 90], [4, 3], 8, 2),
+    ([500, 9, 64], [4, 1, 3], 4, 1),
+]
+
+
+@pytest.mark.parametrize("mass", [False, True])
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("lens,rows,nqh,nkh", FULL)
+def test_attention_of_nine_to_sixteen_columns(ctx, lens, rows, nqh, nkh, hd, mass):
+    """Drafts to verify, many query heads to a K/V head: every column's output, operand blocks and weights."""
+    c = Case(ctx, lens, rows, nqh, nkh, hd, 16, 85, window=0 if nqh != 9 else 100, scale=0.8).up()
+    assert 8 < max(rows) * nqh // nkh <= 16
+    got = c.attention(mass=mass)
+    c.check_attention(got)
+    if mass:
+        c.check_mass(c.mass)
+        c.dm.upload(c.mass)
+    if hd >= 256 and nqh * hd % 256 == 0:
+        ops = ctx.zeros(ctx.batch_operand_bytes(nqh * hd, c.p.num_rows), np.uint8)
+        assert np.array_equal(c.attention(mass=mass, ops=ops).view(np.uint32), got.view(np.uint32))
+        b = ops.download(np.uint8).reshape(nqh * hd // 256, -1)  # one tile of 16 rows: hi + lo, sums, 2^-e
+        m = b[:, :16384].reshape(-1, 8, 2, 4, 16, 16).copy().view(np.float16).astype(np.float64).sum(2)
+        m = m.transpose(3, 0, 1, 2, 4).reshape(16, -1, 256) * b[:, -64:].copy().view(np.float32).T[..., None]
+        want = got.reshape(len(got), -1, 256)
+        assert (np.abs(m[:len(got)] - want) <= 2.0 ** -22 * np.abs(want).max(-1, keepdims=True)).all()
+
+
 @pytest.mark.parametrize("nkh,ragged", [(1, False), (3, True)])
 def test_attention_of_many_sequences(ctx, nkh, ragged):
     """More sequences than a wave has lanes, some without positions or rows; shares that end inside one."""
