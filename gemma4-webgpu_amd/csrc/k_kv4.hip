@@ -11,6 +11,7 @@
 
 #include "attn_paged.hpp"
 #include "kv4.hpp"
+#include "kv4_keys.hpp"
 #include "kv_rows.hpp"
 
 namespace {
@@ -18,12 +19,13 @@ namespace {
 using namespace g4kv8;
 using g4kv4::BAD;
 using g4kv4::BLOCK;
+using g4kv4::Keys;
 
 constexpr int PT = 256;    // threads of the append
 constexpr int QH = 2;      // q heads of a wave
 constexpr int VT = 256;    // of the values kernel
-constexpr int ST = 1024;   // of the selection and the moves
-constexpr uint32_t PER = 32;  // masses of a thread of the selection: of more candidates they are read again for each round
+constexpr int ST = Keys::THREADS;  // of the selection and the moves (of more than Keys::GROUP candidates the selection
+                                   // reads the masses again for each round)
 
 struct ProArgs : RowArgs {
   g4kv4::Pool pool;
@@ -212,8 +214,8 @@ struct EvictArgs {
 __device__ __forceinline__ uint32_t key_of(float x) { return x > 0.f ? __float_as_uint(x) : 0u; }
 
 __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
-  constexpr uint32_t NW = ST / 64, BINS = 2 * ST, GROUP = PER * ST;
-  __shared__ uint32_t s_key[GROUP];  // of candidates g * GROUP + .., as many in a row to each wave
+  constexpr uint32_t NW = ST / 64, BINS = 2 * ST, GROUP = Keys::GROUP;
+  __shared__ uint32_t s_key[GROUP];
   __shared__ uint32_t s_bin[BINS], s_sum[2 * NW], s_found[3];
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t s = blockIdx.x / a.sh.nkh, h = blockIdx.x % a.sh.nkh;
@@ -229,18 +231,17 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
   for (uint32_t i = tid; i < a.recent; i += ST) kept[a.keep - a.recent + i] = (int32_t)(L - a.recent + i);
   const uint32_t n = L - a.first - a.recent, m = a.keep - a.first - a.recent;  // of n candidates m are kept, m < n
   if (m == 0) return;  // (uniform)
-  const uint32_t groups = (n + GROUP - 1) / GROUP;
+  const Keys keys{n};
+  const uint32_t groups = keys.groups();
   const int32_t* list = a.page_table + (size_t)s * a.max_pages;
   const uint32_t page_rows = a.sh.page_size * a.sh.nkh, last_page = (L - 1) / a.sh.page_size;
   const uint32_t pages_on = 64 / a.sh.page_size, rows_on = 64 % a.sh.page_size * a.sh.nkh;  // from a key to the next
-  // This thread's keys of a group: s_key[mine() + 64 * j], j < each().
-  auto rows_of = [&](uint32_t g) { return min(n - g * GROUP, GROUP); };
-  auto each = [&](uint32_t g) { return (rows_of(g) + ST - 1) / ST; };
-  auto mine = [&](uint32_t g) { return w * 64 * each(g) + lane; };
+  uint32_t* const my_key = s_key + Keys::place(w) + lane;  // [64 * j]: of candidate mine(g) + 64 * j of the group
+  auto mine = [&](uint32_t g) { return keys.first(g, w) + lane; };
   // Eight at a time: their page ids, then their masses and the next eight's ids, are on their way together. Past the last
   // candidate they are 0, which no round counts and which, behind all others in order, no place is left for.
   auto fetch = [&](uint32_t g) {
-    const uint32_t rows = rows_of(g), count = each(g), i0 = mine(g), t0 = a.first + g * GROUP + i0;
+    const uint32_t rows = keys.rows(g), count = keys.each(g), i0 = mine(g), t0 = a.first + g * GROUP + i0;
     uint32_t page = a.page_of(t0), row = (t0 - page * a.sh.page_size) * a.sh.nkh + h;
     auto on = [&](uint32_t& p, uint32_t& r) {
       r += rows_on;
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) {
         const uint32_t i = i0 + (j0 + j) * 64;
-        if (j0 + j < count) s_key[i] = id[j] >= 0 && i < rows ? key_of(x[j]) : 0u;  // (uniform)
+        if (j0 + j < count) my_key[(j0 + j) * 64] = id[j] >= 0 && i < rows ? key_of(x[j]) : 0u;  // (uniform)
       }
     }
   };
@@ -282,11 +283,10 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
     __syncthreads();
     for (uint32_t g = 0; g < groups; ++g) {
       if (groups > 1 && (pass || g)) fetch(g);
-      const uint32_t* key = s_key + mine(g);
-      const uint32_t count = each(g);
+      const uint32_t count = keys.each(g);
 #pragma unroll 8
       for (uint32_t j = 0; j < count; ++j) {
-        const uint32_t d = key[64 * j] - from;
+        const uint32_t d = my_key[64 * j] - from;
         if (d < range) atomicAdd(&s_bin[(d >> shift) + 1], 1u);
       }
     }
@@ -314,11 +314,10 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
   uint32_t above = 0, at = 0;  // of the groups before
   for (uint32_t g = 0; g < groups; ++g) {
     if (groups > 1) fetch(g);
-    const uint32_t* key = s_key + mine(g);
-    const uint32_t count = each(g);
+    const uint32_t count = keys.each(g);
     uint32_t na = 0, ne = 0;
     for (uint32_t j = 0; j < count; ++j) {
-      const uint32_t k = key[64 * j];
+      const uint32_t k = my_key[64 * j];
       na += __popcll(__ballot(k > bound));
       ne += __popcll(__ballot(k == bound));
     }
@@ -338,7 +337,7 @@ __global__ __launch_bounds__(ST) void kv4_select_kernel(EvictArgs a) {
     int32_t* to = kept + a.first;
     const uint32_t t0 = a.first + g * GROUP + mine(g);
     for (uint32_t j = 0; j < count; ++j) {
-      const uint32_t k = key[64 * j];
+      const uint32_t k = my_key[64 * j];
       const uint64_t ma = __ballot(k > bound), me = __ballot(k == bound);
       if (me == 0) {  // (uniform, and the rule)
         const uint32_t i = before(ma, wa + min(we, left));

@@ -803,6 +803,16 @@ def test_eviction(ctx, lens, nkh, hd, ps, keep, first, recent, masses):
     check_evict(c, keep, first, recent)  # (nothing is left to cut)
 
 
+@pytest.mark.parametrize("lens,keep,first,recent", [([33999], 20000, 4, 0), ([60003, 32770], 32000, 0, 3),
+                                                    ([98306, 65537, 65800], 400, 1, 0)])
+def test_eviction_of_more_candidates_than_fit_in_lds(ctx, lens, keep, first, recent):
+    """The last 32768 candidates or fewer in other shares of the waves than those before."""
+    c = Case(ctx, lens, [1] * len(lens), 2, 2, 64, 512, 305)
+    c.mass *= 2.0 ** c.rng.integers(-20, 20, c.mass.shape)
+    c.mass[c.rng.random(c.mass.shape) < 0.2] = 0.25
+    check_evict(c.up(), keep, first, recent)
+
+
 def test_eviction_of_lengths_and_pages_that_do_not_hold(ctx):
     """A sequence past max_seq_len stays; rows of bad page ids count 0, are read clamped and not written."""
     c = Case(ctx, [90, 90, 95, 30], [1] * 4, 2, 2, 128, 16, 311, max_len=96)
