@@ -12,10 +12,11 @@
 //    largest. Products and sums of one instruction are exact but for one rounding
 //    (2^-23.2 of the magnitudes' sum at most, over random blocks and scales). No
 //    conversion of K, and 16 cycles for 128 dims and a digit.
-//  * P V: v_mfma_f32_16x16x32_f16, P * 2^15 as f16 hi + lo in one sum: 22 bits of
-//    every P down to 2^-17 of the row's largest and 2^-40 of it below. V is exact
-//    in f16 (codes of 2 bits, scales 2^-20 .. 2^13): one conversion for two codes
-//    with their scale, and one byte permutation for the order of the operand.
+//  * P V: v_mfma_f32_16x16x32_bf16, P * 2^15 as three bf16 of 8 bits each in one sum:
+//    all 24 bits of every P, whatever its size (two f16 hold them down to 2^-17 of
+//    the row's largest: a far key's share is then lost where the near ones' values
+//    are 0). V is exact in bf16 (codes of 2 bits): one conversion for two codes with
+//    their scale, and one byte permutation for the order of the operand.
 // Sums over steps are f32. Maxima are taken to the next power of two, so that a
 // later one rescales exactly.
 #include <algorithm>
@@ -30,9 +31,8 @@ namespace {
 using namespace g4kv8;
 using g4kv4::BAD;
 using g4kv4::BLOCK;
-using g4mm::h2;
-using g4mm::h8;
 using g4mm::static_for;
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef int i4 __attribute__((ext_vector_type(4)));
 typedef int i6 __attribute__((ext_vector_type(6)));
 typedef int i8 __attribute__((ext_vector_type(8)));
@@ -124,7 +124,27 @@ __device__ __forceinline__ void read_digit(const uint8_t* from, i6& to) {
   }
 }
 
-// ---- V as f16 ----
+// ---- P and V as bf16 ----
+
+// Eight values in three parts: 8 bits of each from the top, by cutting (the differences are exact).
+__device__ __forceinline__ void in_parts(const float* x, b8& hi, b8& mid, b8& lo) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+  auto part = [&](b8& to, bool more) __attribute__((always_inline)) {
+    i4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // (the upper halves of two)
+      y[i] = (int)__builtin_amdgcn_perm(__float_as_uint(r[2 * i + 1]), __float_as_uint(r[2 * i]), 0x07060302u);
+    to = __builtin_bit_cast(b8, y);
+    if (more)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] -= __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
+  };
+  part(hi, true);
+  part(mid, true);
+  part(lo, false);
+}
 
 // Byte I of four as the power of two that it is the exponent of (255: infinity, 0: 0).
 template <int I>
@@ -134,11 +154,11 @@ __device__ __forceinline__ float exponent(uint32_t w) {
 __device__ __forceinline__ bool any_bad(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
 // The two codes of byte B of x and of y, each times its row's scale: (first of x, first of y), (second, second).
 template <int B>
-__device__ __forceinline__ void two_by_two(uint32_t x, float sx, uint32_t y, float sy, h2& first, h2& second) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, sx, B));
-  const uint32_t v = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(y, sy, B));
-  first = __builtin_bit_cast(h2, __builtin_amdgcn_perm(v, u, 0x05040100u));
-  second = __builtin_bit_cast(h2, __builtin_amdgcn_perm(v, u, 0x07060302u));
+__device__ __forceinline__ void two_by_two(uint32_t x, float sx, uint32_t y, float sy, uint32_t& first, uint32_t& second) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, sx, B));
+  const uint32_t v = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(y, sy, B));
+  first = __builtin_amdgcn_perm(v, u, 0x05040100u);
+  second = __builtin_amdgcn_perm(v, u, 0x07060302u);
 }
 
 // ---------------------------------------------------------------------------
@@ -433,14 +453,13 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
       const float m_new = fmaxf(m_run, ceilf(mx)), up = 15.f - m_new;
       const float alpha = exp2_h(m_run - m_new);
       float ps = 0.f;
-      h8 ph, pl;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = exp2_h(x[i] + up);
-        ps += e;
-        ph[i] = (_Float16)e;
-        pl[i] = (_Float16)(e - (float)ph[i]);
+        x[i] = exp2_h(x[i] + up);
+        ps += x[i];
       }
+      b8 P[3];
+      in_parts(x, P[2], P[1], P[0]);
       ps = g4d::xsum32(g4d::xsum16(ps));
       l_run = l_run * alpha + ps;
       m_run = m_new;
@@ -472,20 +491,19 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
       }
       static_for<VB / 2>([&](auto e) __attribute__((always_inline)) {
         constexpr int b = decltype(e)::value % 4, v = decltype(e)::value / 4, n = 2 * decltype(e)::value;
-        h8 B[2];
+        i4 B[2];
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
-          h2 y, z;
+          uint32_t y, z;
           two_by_two<b>(V[j][v], vsc[j], V[j + 1][v], vsc[j + 1], y, z);
-          B[0][j] = y[0];
-          B[0][j + 1] = y[1];
-          B[1][j] = z[0];
-          B[1][j + 1] = z[1];
+          B[0][j / 2] = (int)y;
+          B[1][j / 2] = (int)z;
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) O[n + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, B[i], O[n + i], 0, 0, 0);
+        for (int k = 0; k < 3; ++k)  // (the smallest first)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) O[n + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, B[i], O[n + i], 0, 0, 0);
+          for (int i = 0; i < 2; ++i)
+            O[n + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(P[k], __builtin_bit_cast(b8, B[i]), O[n + i], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       });
       if (k + 2 < n) {  // (uniform) into the bytes that this step has read
@@ -676,7 +694,7 @@ __global__ __launch_bounds__(MT) void attn4_merge_kernel(Args a) {
 // ---------------------------------------------------------------------------
 //
 // Workgroup (64 columns of a sequence and KV head, part of their positions),
-// steps of 64 positions through LDS: K and its scales as stored, V as f16 in the
+// steps of 64 positions through LDS: K and its scales as stored, V as bf16 in the
 // order of the P V product's operand. A wave holds 16 columns: their q digits and
 // output sums in registers; two waves per SIMD, so that one's softmax runs beside
 // the other's products. The next step's rows are on their way in registers.
@@ -697,7 +715,7 @@ __global__ __launch_bounds__(MT) void attn4_merge_kernel(Args a) {
 // A prompt of 4500 rows of 8 heads: 108 us at head dim 128, 162 at 256 and 346 at 512
 // (384, 512 and 479 TFLOP/s), of 1500 rows 32, 45 and 72, the merge included. The
 // matrix cores work 15 % of the time and the VALUs 30 (at a step of 64 positions and
-// head dim 256 a wave has 104 products and 480 VALU instructions: V's codes to f16,
+// head dim 256 a wave has 104 products and 480 VALU instructions: V's codes to bf16,
 // the softmax, the masks), the rest waits: for LDS, and at the steps' barriers, since
 // registers allow two waves a SIMD. At head dim 512 a step of two barriers, with the
 // next step's rows in flight for all of it, spilled and took 82 us where this one's
@@ -733,7 +751,7 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn4_ti
   __shared__ __align__(16) uint8_t s_k[TP * S_::KS];
   __shared__ __align__(16) uint8_t s_z[TP * NB];  // K's scales
   __shared__ __align__(16) uint8_t s_v[S_::VBYTES];
-  __shared__ __align__(16) h8 s_p[PAIR ? 4 * 2 * 2 * 64 : 1];  // P: [column tile][32 positions][hi, lo][lane]
+  __shared__ __align__(16) f4 s_p[PAIR ? 4 * 2 * 2 * 64 : 1];  // P: [column tile][half][tile][lane]
   __shared__ __align__(16) f4 s_d[PAIR ? 4 * 2 * 2 * 64 : 1];  // sums: [column tile][half][tile][lane]
   __shared__ float s_mx[PAIR ? 2 * TC : 1];
   __shared__ uint32_t s_tile[4 * CH], s_bad[TP / 4];  // s_bad: rows of V that are not finite, four a word
@@ -837,13 +855,11 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn4_ti
       uint8_t* dst = s_v + (((vt >> 1) * (PAIR ? 2 : 1) + wd) * NE * 64 + vq * 16 + c) * 16 + (vt & 1) * 8;
       static_for<VD / 2>([&](auto e) __attribute__((always_inline)) {
         constexpr int k = decltype(e)::value;
-        h2 x, y, x2, y2;
+        uint32_t x, y, x2, y2;
         two_by_two<k % 4>(vr_[0][k / 4], sc[0], vr_[1][k / 4], sc[1], x, y);
         two_by_two<k % 4>(vr_[2][k / 4], sc[2], vr_[3][k / 4], sc[3], x2, y2);
-        *(g4mm::u32x2*)(dst + 2 * k * 1024) =
-            g4mm::u32x2{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x2)};
-        *(g4mm::u32x2*)(dst + (2 * k + 1) * 1024) =
-            g4mm::u32x2{__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, y2)};
+        *(g4mm::u32x2*)(dst + 2 * k * 1024) = g4mm::u32x2{x, x2};
+        *(g4mm::u32x2*)(dst + (2 * k + 1) * 1024) = g4mm::u32x2{y, y2};
       });
     };
     refill(st0);
@@ -952,45 +968,31 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn4_ti
       // P relative to a power of two (PAIR: of this wave's positions), so that a later one rescales it exactly
       const float m_own = fmaxf(m_run, ceilf(mx)), m_up = 15.f - m_own;
       float ps = 0.f;
-      h8 ph[2], pl[2];  // of 32 positions each
+      f4 P[4];  // (PAIR: this wave's two tiles, then all four)
 #pragma unroll
       for (int p = 0; p < PT; ++p) {
-        float e[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = exp2_h(fmaf(x[p][i], sc, m_up));
-        ps += (e[0] + e[1]) + (e[2] + e[3]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const _Float16 hi = (_Float16)e[i];
-          ph[p / 2][4 * (p & 1) + i] = hi;
-          pl[p / 2][4 * (p & 1) + i] = (_Float16)(e[i] - (float)hi);
-        }
+        for (int i = 0; i < 4; ++i) P[p][i] = exp2_h(fmaf(x[p][i], sc, m_up));
+        ps += (P[p][0] + P[p][1]) + (P[p][2] + P[p][3]);
       }
       ps = g4d::xsum32(g4d::xsum16(ps));
       float m_new = m_own;
       if constexpr (PAIR) {
-        h8* pp = s_p + (wc * 2 * 2) * 64 + l;
-        pp[(wd * 2) * 64] = ph[0];
-        pp[(wd * 2 + 1) * 64] = pl[0];
+        f4* pp = s_p + (wc * 2 * 2) * 64 + l;
+        pp[(wd * 2) * 64] = P[0];
+        pp[(wd * 2 + 1) * 64] = P[1];
         if (qd == 0) s_mx[wd * TC + 16 * wc + c] = m_own;
         __syncthreads();
         const float m_other = s_mx[(wd ^ 1) * TC + 16 * wc + c];
         m_new = fmaxf(m_own, m_other);
         const float f_own = exp2_h(m_own - m_new), f_other = exp2_h(m_other - m_new);
         ps *= f_own;
-        ph[0] = pp[0];
-        pl[0] = pp[64];
-        ph[1] = pp[128];
-        pl[1] = pp[192];
-        if (__ballot(f_own != f_other)) {  // (one of them is 1; f16 ends at 2^-24, so the powers of two in two halves)
-          const float d0 = (wd ? m_other : m_own) - m_new, d1 = (wd ? m_own : m_other) - m_new;
-          const float a0 = ceilf(d0 * 0.5f), a1 = ceilf(d1 * 0.5f);
-          const _Float16 f0 = (_Float16)exp2_h(a0), g0 = (_Float16)exp2_h(d0 - a0);
-          const _Float16 f1 = (_Float16)exp2_h(a1), g1 = (_Float16)exp2_h(d1 - a1);
-          ph[0] = ph[0] * f0 * g0;
-          pl[0] = pl[0] * f0 * g0;
-          ph[1] = ph[1] * f1 * g1;
-          pl[1] = pl[1] * f1 * g1;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) P[p] = pp[p * 64];
+        if (__ballot(f_own != f_other)) {  // (powers of two, one of them 1)
+          const float f0 = wd ? f_other : f_own, f1 = wd ? f_own : f_other;
+#pragma unroll
+          for (int p = 0; p < 4; ++p) P[p] *= p < 2 ? f0 : f1;
         }
       }
       const float alpha = exp2_h(m_run - m_new);
@@ -1007,29 +1009,36 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn4_ti
       }
       load_v(next);
       // ---- P V ----
-      // groups of four dims and 32 positions, the next group's operands read while one is multiplied
+      // 32 positions and groups of four dims, the next group's operands read while one is multiplied
       const uint8_t* vb = s_v + wd * NE * 1024 + l * 16;
-      h8 B[2][4];
-      auto read_b = [&](int u, h8* to) __attribute__((always_inline)) {
+      b8 B[2][4];
+      constexpr int GROUPS = NE / 4;
+      auto read_b = [&](int u, b8* to) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) to[e] = *(const h8*)(vb + ((u & 1) * (PAIR ? 2 : 1) * NE + u / 2 * 4 + e) * 1024);
+        for (int e = 0; e < 4; ++e)
+          to[e] = *(const b8*)(vb + (u / GROUPS * (PAIR ? 2 : 1) * NE + u % GROUPS * 4 + e) * 1024);
       };
       read_b(0, B[0]);
 #pragma unroll
-      for (int u = 0; u < NE / 2; ++u) {
-        if (u + 1 < NE / 2) read_b(u + 1, B[(u + 1) & 1]);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int h = 0; h < 2; ++h) {
+        float x[8];
+        b8 part[3];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          f4& o = O[u / 2 * 4 + e];
-          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[u & 1], B[u & 1][e], o, 0, 0, 0);
-        }
+        for (int i = 0; i < 8; ++i) x[i] = P[2 * h + i / 4][i % 4];
+        in_parts(x, part[2], part[1], part[0]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          f4& o = O[u / 2 * 4 + e];
-          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[u & 1], B[u & 1][e], o, 0, 0, 0);
+        for (int u = h * GROUPS; u < (h + 1) * GROUPS; ++u) {
+          if (u + 1 < 2 * GROUPS) read_b(u + 1, B[(u + 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int k = 0; k < 3; ++k)  // (the smallest first)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              f4& o = O[u % GROUPS * 4 + e];
+              o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(part[k], B[u & 1][e], o, 0, 0, 0);
+            }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
     };
     for (uint32_t st = st0; st < st1; ++st) {

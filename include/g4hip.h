@@ -878,8 +878,8 @@ int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const 
  * it; a code is the nearest, halves to the even code: |value - x| <= 2^e, a
  * quarter of the largest at most and 11 % of a normal block's deviation on the
  * average. A NaN or an infinity in a row and head makes all its scales 255, and
- * every output that sees the row NaN. V scales above 2^13 (the f16 values of the
- * products end there) are the caller's own: the weightless norm's are below 2^2.
+ * every output that sees the row NaN. (Scales that a caller writes: of V, 2^-100 to
+ * 2^100; the append's, of rows normed without weights, are 2^-20 to 2^2.)
  *
  * mass f32 [num_pages][page_size][num_kv_heads]: the attention weight that each
  * cached row has got so far, added up over query heads, rows and calls.
@@ -902,7 +902,9 @@ int g4_pagedAttnPrologue4(g4_ctx* ctx, const float* q_parts, const float* k_part
                           const uint32_t* row_starts, const uint32_t* positions, float* mass, g4_kv4_params p,
                           const float* rope_cs, uint32_t rope_rows);
 /* Attention over the pool, as g4_pagedAttn8 (a window is the last sliding_window
- * cached rows). mass (or NULL): to each cached row and KV head is added the
+ * cached rows). A weight is as exact relative to itself whatever its size: scores
+ * within 2^-19 of sum |k| (|q| + the largest |q| of its 32 dims / 32) scale, P in
+ * 24 bits. mass (or NULL): to each cached row and KV head is added the
  * softmax weight that it gets here, over the head's query heads and the
  * sequence's rows; the same sums in every run. ops (or NULL): as
  * g4_pagedAttn8Ops. workspace: g4_pagedAttn4_workspace_size bytes of these

@@ -596,6 +596,47 @@ def test_a_weight_far_below_the_largest_keeps_its_share(ctx, hd, rows, far):
         c.check_mass(c.mass, (a, b))
 
 
+@pytest.mark.parametrize("far", [1.37 * 2.0 ** -20, 1.37 * 2.0 ** -28, 1.37 * 2.0 ** -36, 2.0 ** -60, 1.37 * 2.0 ** -100])
+@pytest.mark.parametrize("hd,rows", [(64, 1), (128, 1), (256, 1), (512, 1), (64, 20), (128, 20), (256, 20), (512, 20)])
+def test_a_small_weight_is_as_exact_as_a_large_one(ctx, hd, rows, far):
+    """As above, but held to the errors of a weight relative to itself: P's size costs it no bits (f32 in three parts of 8
+    bits with its exponent), down to what f32 can hold. An output of zeros is off by 1e3 tolerances and more."""
+    for n, a, b in ((100, 3, 10), (100, 3, 40), (100, 40, 3), (100, 70, 3), (700, 5, 600), (700, 600, 5)):
+        c = Case(ctx, [n], [rows], 8, 1, hd, 16, 163)
+        pos = np.arange(n)
+        pg, slot = c.table[0, pos // 16], pos % 16
+        c.k.codes[pg, slot], c.k.scale[pg, slot] = 0, 127
+        c.k.codes[pg, slot, 0, 0] = np.where(pos == a, 7, np.where(pos == b, 6, 15))  # 6, 4, -6
+        c.v.codes[pg[a], slot[a]] = 0
+        c.q[:] = 0
+        c.q[..., 0] = -np.log(far) / 2
+        c.up()
+        got = c.attention()
+        k, v = c.k.values(), c.v.values()
+        for r in (0, rows - 1):
+            want, mag, reach, _ = K4.attend(c.q[r], k, v, c.table[0], n - rows + r, 0, 1.0)
+            tol = slack(hd, n, reach) * mag + 1e-38
+            held = mag > far / 32  # (where position b's value is not 0)
+            assert held.any() and bool((np.abs(want[held]) >= 1e3 * tol[held]).all())
+            off = (np.abs(got[r] - want) / tol).max()
+            assert off <= 1, (n, a, b, r, off)
+
+
+@pytest.mark.parametrize("hd,rows", [(64, 1), (128, 1), (256, 1), (512, 1), (64, 20), (128, 20), (256, 20), (512, 20)])
+def test_values_of_any_scale(ctx, hd, rows):
+    """V's scales from 2^-60 to 2^60, each block's by itself: what the append writes is a small part of them."""
+    c = Case(ctx, [150, 40], [rows, rows], 8, 1, hd, 16, 164)
+    c.v.scale[:] = c.rng.choice([67, 100, 127, 141, 187], c.v.scale.shape)
+    c.up()
+    got = c.attention()
+    k, v = c.k.values(), c.v.values()
+    for r in sorted({0, rows - 1, rows, 2 * rows - 1}):
+        s, pos = c.row(r)
+        want, mag, reach, _ = K4.attend(c.q[r], k, v, c.table[s], pos, 0, 1.0)
+        off = (np.abs(got[r] - want) / (slack(hd, pos + 1, reach) * mag)).max()
+        assert off <= 1, (r, off)
+
+
 @pytest.mark.parametrize("hd,nkh,rows,lens", [(256, 1, [1] * 5, [1, 40, 0, 300, 700]), (512, 1, [1] * 3, [9, 1000, 33]),
                                               (256, 2, [1] * 20, [50 * s for s in range(20)]),
                                               (512, 1, [1] * 40, [30 * s + 1 for s in range(40)]),
