@@ -325,7 +325,9 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
     constexpr int QE = 16, QC = 128 * J / QE;                // threads of a column
     constexpr int QCOLS = COLS * QC <= NT ? COLS : NT / QC;  // columns at once (head dim 512: 8 of the 16)
     static_assert(QCOLS == COLS || 2 * QCOLS == COLS);
-    const uint32_t qdim = tid % QC * QE, block = qdim / BLOCK;
+    int qt = tid;
+    asm volatile("" : "+v"(qt));  // (what follows from it is not kept over the sequences: registers would spill)
+    const uint32_t qdim = qt % QC * QE, block = qdim / BLOCK;
     float qx[QE];
     auto load_q = [&](uint32_t col) __attribute__((always_inline)) {
       const float* qg = a.q + row_of(a, sq.first, kvh, min(col, ncols - 1)) * HD + (HD == 64 ? qdim % 64 : qdim);
@@ -336,7 +338,7 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
         for (int i = 0; i < 4; ++i) qx[e + i] = HD == 64 && block >= 2 ? 0.f : y[i];
       }
     };
-    if (tid < QCOLS * QC) load_q(tid / QC);
+    if (qt < QCOLS * QC) load_q(qt / QC);
     refill(0);
     ring_barrier();  // the previous sequence's sums are done with
     if (n > 0) load(0);  // (uniform)
@@ -355,10 +357,10 @@ __global__ __launch_bounds__(NT, HD == 512 ? 1 : HD == 256 ? 2 : 3) void attn4_s
         for (int i = 0; i < QE * 3 / 16; ++i) to[i] = (uint32_t)code[i];
       });
     };
-    if (tid < QCOLS * QC) store_digits(tid / QC);
+    if (qt < QCOLS * QC) store_digits(qt / QC);
     if (QCOLS < COLS && ncols > QCOLS) {  // (uniform; columns past the last one keep any digits: their weights are 0)
-      load_q(tid / QC + QCOLS);
-      store_digits(tid / QC + QCOLS);
+      load_q(qt / QC + QCOLS);
+      store_digits(qt / QC + QCOLS);
     }
     ring_barrier();
     i6 qb[DIGITS][J];
