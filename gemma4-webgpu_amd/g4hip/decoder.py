@@ -44,6 +44,7 @@ feeds the next step without a host round trip.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from dataclasses import dataclass, field
 from typing import List, Optional
 
@@ -841,6 +842,7 @@ class BatchDecoder(_SyntheticModel):
     workgroups and the step is deterministic.
     """
     kv4, budget, capturing, replayed = False, None, False, False
+    held_mass = ()
 
     def __init__(self, ctx: Context, context_lens, shape: Optional[E2BShape] = None, page_size: int = 16,
                  reserve: int = 64, seed: int = 0, n_layers: Optional[int] = None, lm_head: bool = True,
@@ -929,6 +931,9 @@ class BatchDecoder(_SyntheticModel):
             self.cut_lens_host = np.minimum(self.lens_host, budget)[:n]
             self.cut_lens, self.cut_lens_next = ctx.from_numpy(self.cut_lens_host), ctx.zeros(n, np.uint32)
             self.text = 0  # shared_pages: tokens of the sequence so far
+            if shared_pages:
+                self.held = 0, np.zeros_like(self.cut_lens_host)
+                self.held_mass = [(ctx.zeros(self.mass[il].nbytes // 4, np.float32), self.mass[il]) for il in cut]
             self.kept = {il: ctx.zeros(n * self.s.n_kv_heads * budget, np.int32) for il in cut}
             self.evict_params = {il: self._kv8_params(il, n, 1) for il in cut}
             self.evict_ws = ctx.alloc(max([16] + [ctx.evict4_workspace_bytes(p, budget)
@@ -1163,7 +1168,11 @@ class BatchDecoder(_SyntheticModel):
         if self.replayed and not self.capturing:  # (how often, the host does not know)
             self.cut_lens_host = self.cut_lens.download(np.uint32)
         if not self.capturing and int(self.cut_lens_host.max()) + rows > self.cut_rows:
+            if self.shared_pages:  # (of an eviction that fails, nothing holds)
+                self.held = 0, np.zeros_like(self.cut_lens_host)
             self._evict()
+            if self.shared_pages:
+                self._hold()
         self.ctx.advanceSeqLens(self.cut_lens, len(self.cut_lens_host), rows)
         if not self.capturing:
             self.cut_lens_host = self.cut_lens_host + np.uint32(rows)
@@ -1379,15 +1388,17 @@ class BatchDecoder(_SyntheticModel):
         the spare rows past the 16 or 32 that hold it, whose residual rows,
         logits and samples are then copies of the last token's. Returns the row of the final
         chunk that holds the prompt's last token: its logits and `tokens`
-        entry are the first sample. probe (tests): passed to every chunk's
-        step."""
+        entry are the first sample. With a budget, a prompt that raises half
+        way leaves its caches as they were, or as an eviction on the way
+        left them: `text` says where to go on. probe (tests): passed to every
+        chunk's step."""
         if not self.shared_pages or self.embedding is None:
             raise ValueError("prefill needs a shared_pages decoder with an embedding table")
         toks = np.asarray(tokens, np.uint32)
         T, B = int(toks.size), self.B
         if T == 0 or start < 0 or start + T > self.max_seq - 1:
             raise ValueError(f"prefill: {T} tokens from {start} do not fit {self.max_seq} positions")
-        self._begin_text(start, T)
+        self._begin_text(start)
         nch = -(-T // B)
         n = T - (nch - 1) * B
         pad = nch * B - T
@@ -1409,12 +1420,11 @@ class BatchDecoder(_SyntheticModel):
         spans = self._spans(T, start, B)
         # a single chunk takes only as many rows as its matrix-core tiles need
         rows = next((r for r in (16, 32) if T <= r < B), B) if nch == 1 and probe is None else B
-        try:
+        with self._placing():
             for k in range(nch):
                 self._place_chunk(dtok, dpos, cpos, k, spans)
                 self.step(sample, probe=probe, head=k == nch - 1, rows=rows)
-        finally:
-            self.span_rows = 0
+                self._placed()
         if rows < B:  # the rows left out: the last token's again, as in a step over all B
             outs = [(self.hidden, self.s.hidden)]
             if self.lm_head is not None:
@@ -1455,7 +1465,34 @@ class BatchDecoder(_SyntheticModel):
             self.span_rows = int(spans[1][k])
             self._make_room(self.span_rows)
 
-    def _begin_text(self, start: int, tokens: int) -> None:
+    @contextmanager
+    def _placing(self):
+        """A prompt's or a text's passes, each between _place_span and _placed. One that fails leaves no rows placed, and
+        the caches that have a budget as they were before the call or, if rows were cut since, after that."""
+        try:
+            yield
+        except BaseException:
+            self.span_rows = 0
+            if self.budget is not None:
+                self.text, self.cut_lens_host = self.held
+                self.cut_lens.upload(self.cut_lens_host)
+                for saved, mass in self.held_mass:
+                    self.ctx.copy(mass, saved, mass.nbytes)
+            raise
+        self.span_rows = 0
+
+    def _placed(self) -> None:
+        if self.budget is not None:
+            self.text += self.span_rows
+
+    def _hold(self) -> None:
+        """What a pass that fails goes back to. (Rows that it appended lie behind the lengths then.)"""
+        self.held = self.text, self.cut_lens_host
+        if self.cut_lens_host.any():
+            for saved, mass in self.held_mass:
+                self.ctx.copy(saved, mass, mass.nbytes)
+
+    def _begin_text(self, start: int) -> None:
         """Caches with a budget hold rows by when they came, not by position: a text begins at 0, or goes on where the
         last one ended."""
         if self.budget is None:
@@ -1465,7 +1502,8 @@ class BatchDecoder(_SyntheticModel):
         if start == 0:
             self.cut_lens.zero()
             self.cut_lens_host = np.zeros_like(self.cut_lens_host)
-        self.text = start + tokens
+        self.text = start
+        self._hold()
 
     def score(self, tokens, start: int = 0) -> np.ndarray:
         """The log probability of each token but the first under the model, given those before it (a
@@ -1478,7 +1516,7 @@ class BatchDecoder(_SyntheticModel):
         if T < 2 or start < 0 or start + T > self.max_seq - 1:
             raise ValueError(f"score: {T} tokens from {start}: two or more within {self.max_seq} positions")
         n = T - 1  # the last token is only asked for
-        self._begin_text(start, n)
+        self._begin_text(start)
         nch = -(-n // B)
         pad = nch * B - n
         ctok = np.concatenate([toks[:n], np.repeat(toks[n - 1], pad)]).astype(np.uint32)
@@ -1487,15 +1525,14 @@ class BatchDecoder(_SyntheticModel):
         spans = self._spans(n, start, B)
         out = c.empty(n, np.float32)
         ws = c.alloc(c.logprobs_workspace_bytes(s.vocab, B, 0))
-        try:
+        with self._placing():
             for k in range(nch):
                 self._place_chunk(dtok, dpos, cpos, k, spans)
                 self.step()
                 rows = min(n - B * k, B)
                 c.logprobsBatch(self.logits, want.offset(4 * B * k), s.vocab, rows, out.offset(4 * B * k), None, 0,
                                 None, None, ws)
-        finally:
-            self.span_rows = 0
+                self._placed()
         got = out.download(np.float32)
         for b in (dtok, dpos, want, out, ws):
             b.free()
@@ -1576,21 +1613,20 @@ class BatchDecoder(_SyntheticModel):
         dtok, dlen = c.from_numpy(ctok), c.from_numpy(clen)
         spans = self._spans(T, start, self.wide_rows)
         n = 0
-        try:
+        with self._placing():
             for at in range(0, T + pad, self.wide_rows):
                 n = min(self.wide_rows, T + pad - at)
                 self._place_span(spans, at // self.wide_rows)
                 self._wide_pass(dtok.offset(4 * at), dlen.offset(4 * at), n, int(clen[at:at + n].max()))
-        finally:
-            self.span_rows = 0
-        # the last B rows are what the last chunk of B rows leaves: the residual
-        # stream, its tokens and lengths, then the head and the sample
-        c.copy(self.hidden, w["hidden"].offset(4 * H * (n - B)), 4 * H * B)
-        c.copy(self.tokens, dtok.offset(4 * (T + pad - B)), 4 * B)
-        c.copy(self.seq_lens, dlen.offset(4 * (T + pad - B)), 4 * B)
-        self.lens_host = clen[-B:].copy()
-        c.batchPrep(self.hidden, 1, self.final_norm, None, None, None, self.xn, H, B, s.eps, ops=self.xops)
-        self._head(sample, B)
+                self._placed()
+            # the last B rows are what the last chunk of B rows leaves: the residual
+            # stream, its tokens and lengths, then the head and the sample
+            c.copy(self.hidden, w["hidden"].offset(4 * H * (n - B)), 4 * H * B)
+            c.copy(self.tokens, dtok.offset(4 * (T + pad - B)), 4 * B)
+            c.copy(self.seq_lens, dlen.offset(4 * (T + pad - B)), 4 * B)
+            self.lens_host = clen[-B:].copy()
+            c.batchPrep(self.hidden, 1, self.final_norm, None, None, None, self.xn, H, B, s.eps, ops=self.xops)
+            self._head(sample, B)
         c.sync()
         dtok.free()
         dlen.free()

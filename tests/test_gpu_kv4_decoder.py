@@ -274,6 +274,41 @@ def test_a_prompt_longer_than_its_budget(ctx, B, T):
     assert d.score(rng.integers(0, s.vocab, 60)).shape == (59,) and d.text == 59
 
 
+@pytest.mark.parametrize("budget,slack,goes_on", [(200, 64, 40), (24, 24, 56)])
+def test_a_prompt_that_fails_half_way(ctx, budget, slack, goes_on):
+    """Its second chunk raises between two layers. What is made again leaves every bit as if nothing had failed: from the
+    prompt's begin, or from behind the eviction that its second chunk made."""
+    toks = np.random.default_rng(97).integers(0, 4096, 80).astype(np.uint32)
+    chunks = []
+
+    def fails(stage, il, _):
+        if stage == "prep" and il == 0:
+            chunks.append(il)
+        if stage == "attn" and il == 2 and len(chunks) == 2:
+            raise RuntimeError("half way")
+
+    runs = []
+    for broken in (False, True):
+        d = BatchDecoder(ctx, [0] * 16, shape(), seed=98, reserve=100, shared_pages=True, embed=True, kv="fp4",
+                         budget=budget, slack=slack)
+        d.prefill(toks[:40], probe=lambda *a: None)
+        at = 40
+        if broken:
+            with pytest.raises(RuntimeError, match="half way"):
+                d.prefill(toks[40:], 40, probe=fails)
+            at = d.text
+            assert at == goes_on and np.array_equal(d.cut_lens.download(np.uint32), d.cut_lens_host)
+        for a, b in ((40, goes_on), (goes_on, 80)):
+            if at <= a < b:
+                d.prefill(toks[a:b], a, probe=lambda *a: None)
+        n = int(d.cut_lens_host[0])
+        live = (d.cut_table_host[0, np.arange(n) // 16], np.arange(n) % 16)
+        runs.append([d.logits.download(np.uint32), d.cut_lens.download(np.uint32)] +
+                    [m.download(np.uint32).reshape(d.cut_pages, 16, -1)[live] for m in d.mass.values()] +
+                    [x[live] for il in d.mass for p in pools(d, il) for x in (p.codes, p.scale)])
+    assert all(np.array_equal(a, b) for a, b in zip(*runs))
+
+
 def test_refusals(ctx):
     s = shape()
     for kw in (dict(kv="int8", budget=40), dict(budget=40), dict(kv="fp4", budget=0), dict(kv="fp4", budget=40, slack=0),

@@ -103,3 +103,86 @@ def test_budgets_that_do_not_hold_are_refused(kw):
     """Before anything is allocated for them."""
     with pytest.raises(ValueError, match="budget"):
         BatchDecoder(None, [3], **kw)
+
+
+TEXTS = [(0, lambda d, n, start: d.prefill(np.arange(n), start)), (8, lambda d, n, start: d.prefill(np.arange(n), start)),
+         (0, lambda d, n, start: d.score(np.arange(n + 1), start))]
+
+
+def failing(lens, wide_rows, fail_at, **kw):
+    """A shared decoder whose step number fail_at raises, and whose steps weigh what is cached."""
+    d = with_budget(decoder(wide_rows=wide_rows, fail_at=fail_at), lens, True, **kw)
+    mass = Buf(d.ctx, np.zeros(4 * 64, np.uint8))
+    d.held_mass = [(Buf(d.ctx, np.zeros(4 * 64, np.uint8)), mass)]
+    d.masses = mass.mem.view(np.float32)
+    for name in ("step", "_wide_pass"):
+        def weighs(*a, run=getattr(d, name), **k):
+            d.masses[:int(d.cut_lens_host[0])] += 1
+            run(*a, **k)
+
+        setattr(d, name, weighs)
+    return d
+
+
+@pytest.mark.parametrize("wide_rows,call", TEXTS, ids=["chunks", "passes", "text"])
+def test_a_prompt_that_fails_leaves_the_caches_as_they_were(wide_rows, call):
+    """The rows of its passes so far are gone, what they added to others' masses too; the call can be made again."""
+    at = 5 if wide_rows else 3  # (its second pass)
+    d = failing([0], wide_rows, at, budget=100)
+    call(d, 8, 0)
+    while len(d.seen) < at - 1:
+        d.seen.append(None)
+    want = d.masses[:8].tolist()
+    with pytest.raises(RuntimeError, match="fails"):
+        call(d, 24, 8)
+    assert len(d.seen) == at and d.text == 8 and lens_of(d) == [8] and d.masses[:8].tolist() == want
+    with pytest.raises(ValueError, match="go on at 8"):
+        call(d, 1, 32)
+    d.seen.append(None)
+    call(d, 24, 8)
+    assert d.text == 32 and lens_of(d) == [32] and d.span_rows == 0
+
+
+@pytest.mark.parametrize("wide_rows,call", TEXTS, ids=["chunks", "passes", "text"])
+def test_a_first_prompt_that_fails_leaves_nothing(wide_rows, call):
+    d = failing([0], wide_rows, 1, budget=100)
+    with pytest.raises(RuntimeError, match="fails"):
+        call(d, 24, 0)
+    assert d.text == 0 and lens_of(d) == [0]
+    d.seen.append(None)
+    call(d, 24, 0)
+    assert d.text == 24 and lens_of(d) == [24]
+
+
+def test_a_prompt_that_fails_behind_an_eviction_goes_on_behind_it():
+    """What an eviction took cannot be had back: the passes before it stay."""
+    d = failing([0], 0, 4)
+    call = TEXTS[0][1]
+    call(d, 8, 0)
+    with pytest.raises(RuntimeError, match="fails"):
+        call(d, 16, 8)  # 12; cut to 8, 12; cut to 8, 12: fails
+    assert d.text == 16 and lens_of(d) == [8] and d.masses[:8].tolist() == [4, 4, 4, 4, 3, 3, 3, 3]
+    with pytest.raises(ValueError, match="go on at 16"):
+        call(d, 1, 8)
+    d.seen.append(None)
+    call(d, 8, 16)
+    assert d.text == 24 and lens_of(d) == [12]
+
+
+def test_an_eviction_that_fails_leaves_a_text_to_begin_again():
+    d = failing([0], 0, None)
+    call = TEXTS[0][1]
+    call(d, 12, 0)
+
+    def broken(*a):
+        raise MemoryError
+
+    d.ctx.kvEvict4 = broken
+    with pytest.raises(MemoryError):
+        call(d, 4, 12)
+    assert d.text == 0 and lens_of(d) == [0]
+    with pytest.raises(ValueError, match="go on at 0"):
+        call(d, 4, 12)
+    del d.ctx.kvEvict4
+    call(d, 4, 0)
+    assert d.text == 4 and lens_of(d) == [4]
