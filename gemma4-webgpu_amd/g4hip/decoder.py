@@ -44,6 +44,7 @@ feeds the next step without a host round trip.
 """
 from __future__ import annotations
 
+import warnings
 from contextlib import contextmanager
 from dataclasses import dataclass, field
 from typing import List, Optional
@@ -1144,11 +1145,23 @@ class BatchDecoder(_SyntheticModel):
         and its heaviest (`kept[layer]` [sequences][KV heads][budget]: where they were). Steps and prompts that the
         host enqueues call it where they need room (a step beside a captured one reads the lengths back first);
         between the replays of a captured step it is the caller's, once in `slack` of them at least: a sequence without
-        room appends nothing. Waits for the device."""
+        room appends nothing and its cut layers see nothing. Replays past that are warned of here (the caches go on
+        without their rows) and an error of a later step. Waits for the device."""
         if self.budget is None:
             raise ValueError("evict needs a budget")
-        self._evict()
         self.cut_lens_host = self.cut_lens.download(np.uint32)
+        over = self._overrun()
+        if over:
+            warnings.warn(over, RuntimeWarning, stacklevel=2)
+            self.cut_lens.upload(np.minimum(self.cut_lens_host, self.cut_rows).astype(np.uint32))
+        self._evict()
+
+    def _overrun(self) -> Optional[str]:
+        over = np.maximum(self.cut_lens_host.astype(np.int64) - self.cut_rows, 0)
+        if not over.any():
+            return None
+        return (f"no room for the last {over.max()} rows of sequences {np.flatnonzero(over).tolist()}: those replays' "
+                f"rows are lost and their tokens void (evict() once in {self.cut_rows - self.budget} replays at least)")
 
     def _evict(self) -> None:
         c, n = self.ctx, 4 * len(self.cut_lens_host)
@@ -1167,6 +1180,9 @@ class BatchDecoder(_SyntheticModel):
             return
         if self.replayed and not self.capturing:  # (how often, the host does not know)
             self.cut_lens_host = self.cut_lens.download(np.uint32)
+            over = self._overrun()
+            if over:
+                raise RuntimeError(over)
         if not self.capturing and int(self.cut_lens_host.max()) + rows > self.cut_rows:
             if self.shared_pages:  # (of an eviction that fails, nothing holds)
                 self.held = 0, np.zeros_like(self.cut_lens_host)
@@ -1213,6 +1229,8 @@ class BatchDecoder(_SyntheticModel):
             raise ValueError("step: shared pages of codes hold one sequence, whose rows prefill and score place")
         c, s, B = self.ctx, self.s, self.B if rows is None else rows
         H = s.hidden
+        if not self.shared_pages:
+            self._make_room(1)
         if self.embedding is not None:
             c.embeddingLookupBatch(self.embedding, s.vocab, self.hidden, H, self.tokens, B)
         if s.ple_dim:  # PLE stage 1 for every row (src/engine.ts:1516-1535)
@@ -1221,8 +1239,6 @@ class BatchDecoder(_SyntheticModel):
             c.pleStage1Fuse(self.ple_projected, self.ple_proj_norm, self.ple_table, s.vocab, self.ple_inputs,
                             s.n_layers, s.ple_dim, s.eps, tokens_dev=self.tokens, count=B)
         c.advanceSeqLens(self.seq_lens, self.B, 1)
-        if not self.shared_pages:
-            self._make_room(1)
         nd = 0
         for il, L in enumerate(self.layers):
             Q, KV, I = s.q_dim_of(il), s.kv_dim_of(il), s.ffn_of(il)

@@ -107,6 +107,37 @@ def test_eager_steps_after_replays_find_room(ctx):
         assert all(np.array_equal(x, y) for x, y in zip(a, b)), step
 
 
+def test_replays_past_the_room(ctx):
+    """One and two replays too many (63 + 10 and 64 + 10 rows for 72): a step says so and changes nothing, evict() warns and
+    cuts to the budget, and the next steps see what the caches hold."""
+    d = BatchDecoder(ctx, LENS, shape(), seed=55, reserve=24, embed=True, kv="fp4", budget=64, slack=8)
+    d.fill_kv(seed=56)
+    d.tokens.upload(np.arange(d.B, dtype=np.uint32))
+    g = d.capture()
+    for _ in range(10):
+        ctx.graph_launch(g)
+    with pytest.raises(RuntimeError, match=r"2 rows of sequences \[4, 5, 6, 7\]"):
+        d.step()
+    assert np.array_equal(d.seq_lens.download(np.uint32), np.array(LENS) + 10)
+    assert np.array_equal(d.cut_lens.download(np.uint32), np.minimum(LENS, 64) + 10)
+    with pytest.warns(RuntimeWarning, match="2 rows"):
+        d.evict()
+    want = np.minimum(np.minimum(LENS, 64) + 10, 64)
+    assert np.array_equal(d.cut_lens.download(np.uint32), want) and np.array_equal(d.cut_lens_host, want)
+    s = d.s
+
+    def probe(stage, il, _):
+        if stage == "attn":
+            at = want if d._is_cut(il) else np.array(LENS) + 10
+            check_rows(d, il, d.q.download(np.float32, d.B * s.q_dim_of(il)),
+                       d.attn.download(np.float32, d.B * s.q_dim_of(il)), [(b, b, int(at[b])) for b in range(d.B)])
+
+    d.step(probe=probe)
+    ctx.graph_launch(g)
+    assert np.array_equal(d.cut_lens.download(np.uint32), want + 2)
+    ctx.graph_destroy(g)
+
+
 @pytest.mark.parametrize("budget", [None, 64])
 def test_a_captured_step_equals_eager_ones(ctx, budget):
     runs = []

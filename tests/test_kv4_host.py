@@ -186,3 +186,43 @@ def test_an_eviction_that_fails_leaves_a_text_to_begin_again():
     del d.ctx.kvEvict4
     call(d, 4, 0)
     assert d.text == 4 and lens_of(d) == [4]
+
+
+def overrun(lens):
+    """A ragged decoder whose captured step was replayed too often; its eviction is the device's: a length past the cache's
+    rows stays."""
+    d = with_budget(decoder(), lens, False)
+    d.replayed = True
+
+    def cut(k, v, ks, vs, mass, table, now, *a):
+        x = now.mem.view(np.uint32)
+        x[:] = np.where(x > d.cut_rows, x, np.minimum(x, 8))
+
+    d.ctx.kvEvict4 = cut
+    return d
+
+
+@pytest.mark.parametrize("lens,which", [([13, 4], r"1 rows of sequences \[0\]"), ([12, 30], r"18 rows of sequences \[1\]"),
+                                        ([14, 13], r"2 rows of sequences \[0, 1\]")])
+def test_replays_past_the_room_are_not_hidden(lens, which):
+    """A step of the host's raises before it changes anything; evict() says it and leaves caches that have room again."""
+    d = overrun(lens)
+    before = d.seq_lens.mem.tolist()
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match=which):
+            BatchDecoder.step(d)
+        assert d.seq_lens.mem.tolist() == before and d.cut_lens.mem.view(np.uint32).tolist() == lens
+    with pytest.warns(RuntimeWarning, match=which):
+        d.evict()
+    assert lens_of(d) == np.minimum(lens, 8).tolist()
+    d._make_room(1)
+    assert lens_of(d) == (np.minimum(lens, 8) + 1).tolist()
+
+
+def test_replays_that_just_fit_are_no_overrun(recwarn):
+    d = overrun([12, 3])
+    d._make_room(1)
+    assert lens_of(d) == [9, 4]
+    d = overrun([12, 3])
+    d.evict()
+    assert lens_of(d) == [8, 3] and not len(recwarn)
