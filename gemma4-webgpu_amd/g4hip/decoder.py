@@ -842,7 +842,7 @@ class BatchDecoder(_SyntheticModel):
     prologue, or the attention prologue), so no launch waits on another's
     workgroups and the step is deterministic.
     """
-    kv4, budget, capturing, replayed = False, None, False, False
+    kv4, budget, capturing, launches = False, None, False, None
     held_mass = ()
 
     def __init__(self, ctx: Context, context_lens, shape: Optional[E2BShape] = None, page_size: int = 16,
@@ -1143,18 +1143,23 @@ class BatchDecoder(_SyntheticModel):
     def evict(self) -> None:
         """Cuts the caches that have a budget down to it: every sequence with more rows there keeps its first, its last
         and its heaviest (`kept[layer]` [sequences][KV heads][budget]: where they were). Steps and prompts that the
-        host enqueues call it where they need room (a step beside a captured one reads the lengths back first);
+        host enqueues call it where they need room (the first step behind replays reads the lengths back);
         between the replays of a captured step it is the caller's, once in `slack` of them at least: a sequence without
         room appends nothing and its cut layers see nothing. Replays past that are warned of here (the caches go on
         without their rows) and an error of a later step. Waits for the device."""
         if self.budget is None:
             raise ValueError("evict needs a budget")
-        self.cut_lens_host = self.cut_lens.download(np.uint32)
+        self._read_lengths()
         over = self._overrun()
         if over:
             warnings.warn(over, RuntimeWarning, stacklevel=2)
             self.cut_lens.upload(np.minimum(self.cut_lens_host, self.cut_rows).astype(np.uint32))
         self._evict()
+
+    def _read_lengths(self) -> None:
+        self.cut_lens_host = self.cut_lens.download(np.uint32)
+        if self.launches is not None:
+            self.launches = self.ctx.launches
 
     def _overrun(self) -> Optional[str]:
         over = np.maximum(self.cut_lens_host.astype(np.int64) - self.cut_rows, 0)
@@ -1178,17 +1183,18 @@ class BatchDecoder(_SyntheticModel):
         """Room for `rows` more of every sequence in the caches that have a budget, and their lengths with them."""
         if self.budget is None:
             return
-        if self.replayed and not self.capturing:  # (how often, the host does not know)
-            self.cut_lens_host = self.cut_lens.download(np.uint32)
-            over = self._overrun()
-            if over:
-                raise RuntimeError(over)
-        if not self.capturing and int(self.cut_lens_host.max()) + rows > self.cut_rows:
-            if self.shared_pages:  # (of an eviction that fails, nothing holds)
-                self.held = 0, np.zeros_like(self.cut_lens_host)
-            self._evict()
-            if self.shared_pages:
-                self._hold()
+        if not self.capturing:
+            if self.launches is not None and self.launches != self.ctx.launches:  # (how often, the host does not know)
+                self._read_lengths()
+            most = int(self.cut_lens_host.max())
+            if most > self.cut_rows:
+                raise RuntimeError(self._overrun())
+            if most + rows > self.cut_rows:
+                if self.shared_pages:  # (of an eviction that fails, nothing holds)
+                    self.held = 0, np.zeros_like(self.cut_lens_host)
+                self._evict()
+                if self.shared_pages:
+                    self._hold()
         self.ctx.advanceSeqLens(self.cut_lens, len(self.cut_lens_host), rows)
         if not self.capturing:
             self.cut_lens_host = self.cut_lens_host + np.uint32(rows)
@@ -1729,8 +1735,10 @@ class BatchDecoder(_SyntheticModel):
         try:
             self.step(sample)
         finally:
-            self.capturing, self.replayed = False, True
+            self.capturing = False
             g = self.ctx.graph_end()
+        if self.launches is None:  # of any graph, up to when the host last knew the lengths of the cut caches
+            self.launches = self.ctx.launches
         self.lens_host = lens  # capture enqueues nothing
         return g
 

@@ -110,6 +110,7 @@ class Context:
         check(lib().g4_init(device, ctypes.byref(h)))
         self.h = h
         self.device = device
+        self.launches = 0  # of graphs, through this context
 
     def close(self) -> None:
         if self.h:
@@ -200,6 +201,7 @@ class Context:
         return g
 
     def graph_launch(self, g) -> None:
+        self.launches += 1
         check(lib().g4_graph_launch(self.h, g))
 
     @staticmethod

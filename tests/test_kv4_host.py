@@ -192,7 +192,7 @@ def overrun(lens):
     """A ragged decoder whose captured step was replayed too often; its eviction is the device's: a length past the cache's
     rows stays."""
     d = with_budget(decoder(), lens, False)
-    d.replayed = True
+    d.launches, d.ctx.launches = 7, 9
 
     def cut(k, v, ks, vs, mass, table, now, *a):
         x = now.mem.view(np.uint32)
@@ -226,3 +226,36 @@ def test_replays_that_just_fit_are_no_overrun(recwarn):
     d = overrun([12, 3])
     d.evict()
     assert lens_of(d) == [8, 3] and not len(recwarn)
+
+
+def test_lengths_are_read_where_graphs_ran_since():
+    """Once after the replays, not at every step for good: a read waits for the device."""
+    d = with_budget(decoder(), [3, 2], False)
+    d.ctx.launches = 5
+    waits = []
+
+    def steps(n):
+        for _ in range(n):
+            before = d.ctx.waits
+            d._make_room(1)
+            waits.append(d.ctx.waits - before)
+
+    steps(2)  # (nothing was captured: graphs of others say nothing)
+    d.ctx.launches += 1
+    steps(1)
+    d.ctx.graph_begin = lambda: None
+    d.ctx.graph_end = lambda: "graph"
+    d.lens_host, d.step = np.zeros(2, np.uint32), lambda sample: d._make_room(1)
+    assert d.capture() == "graph"
+    d.cut_lens.mem.view(np.uint32)[:] -= np.uint32(1)  # (the capture ran nothing)
+    steps(1)
+    d.ctx.launches += 2  # two replays
+    d.cut_lens.mem.view(np.uint32)[:] += np.uint32(2)
+    steps(3)
+    assert waits == [0, 0, 0, 0, 1, 0, 0] and lens_of(d) == [12, 11] and not d.ctx.cuts
+    steps(1)
+    assert waits[-1] == 0 and lens_of(d) == [9, 9] and len(d.ctx.cuts) == 2
+    d.ctx.launches += 1
+    d.evict()
+    steps(1)
+    assert waits[-1] == 0
