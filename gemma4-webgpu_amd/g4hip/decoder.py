@@ -843,7 +843,7 @@ class BatchDecoder(_SyntheticModel):
     workgroups and the step is deterministic.
     """
     kv4, budget, capturing, launches = False, None, False, None
-    held_mass = ()
+    held_mass, gone = (), 0
 
     def __init__(self, ctx: Context, context_lens, shape: Optional[E2BShape] = None, page_size: int = 16,
                  reserve: int = 64, seed: int = 0, n_layers: Optional[int] = None, lm_head: bool = True,
@@ -930,6 +930,7 @@ class BatchDecoder(_SyntheticModel):
             self.cut_table = ctx.from_numpy(self.cut_table_host)
             n = len(self.cut_table_host)
             self.cut_lens_host = np.minimum(self.lens_host, budget)[:n]
+            self.gone = self.lens_host[:n].astype(np.int64) - self.cut_lens_host  # tokens whose rows an eviction took
             self.cut_lens, self.cut_lens_next = ctx.from_numpy(self.cut_lens_host), ctx.zeros(n, np.uint32)
             self.text = 0  # shared_pages: tokens of the sequence so far
             if shared_pages:
@@ -1053,14 +1054,25 @@ class BatchDecoder(_SyntheticModel):
             self.ctx.fill_normal_f16(L.v_cache, n, splitmix64(seed, 2 * il + 1), 0.0, 1.0)
 
     def set_lengths(self, lens) -> None:
+        """The tokens of every sequence's text. With a budget, a text that loses its last ones loses their rows in the cut
+        caches too, down to what the last eviction left (a text of 0 begins anew); a longer one counts as cut already."""
         lens = np.asarray(lens, dtype=np.uint32)
         if lens.shape != (self.B,) or int(lens.max()) >= self.max_seq:
             raise ValueError("set_lengths: one length per sequence, below the reserved capacity")
+        if self.budget is not None and not self.shared_pages:
+            self._set_cut_lengths(lens.astype(np.int64))
         self.lens_host = lens
         self.seq_lens.upload(lens)
-        if self.budget is not None and not self.shared_pages:
-            self.cut_lens_host = np.minimum(lens, self.budget)
-            self.cut_lens.upload(self.cut_lens_host)
+
+    def _set_cut_lengths(self, lens) -> None:
+        self._read_lengths()
+        longer, rows = lens > self.gone + self.cut_lens_host, lens - self.gone
+        past = ~longer & (lens > 0) & (self.gone > 0) & (rows < self.budget)
+        if past.any():
+            raise ValueError(f"set_lengths: an eviction has seen the last tokens of sequences {np.flatnonzero(past).tolist()}")
+        rows = np.where(longer, np.minimum(lens, self.budget), np.where(lens == 0, 0, rows))
+        self.gone, self.cut_lens_host = lens - rows, rows.astype(np.uint32)
+        self.cut_lens.upload(self.cut_lens_host)
 
     def pool_row(self, seq: int, pos: int) -> int:
         """Pool row of sequence `seq`'s logical position `pos`."""
@@ -1177,7 +1189,8 @@ class BatchDecoder(_SyntheticModel):
                        self.budget, self.cut["first"], self.cut["recent"], self.kept[il], self.evict_ws)
         if self.evict_params:
             c.copy(self.cut_lens, self.cut_lens_next, n)
-        self.cut_lens_host = np.minimum(self.cut_lens_host, self.budget)
+        now = np.minimum(self.cut_lens_host, self.budget)
+        self.gone, self.cut_lens_host = self.gone + self.cut_lens_host - now, now
 
     def _make_room(self, rows: int) -> None:
         """Room for `rows` more of every sequence in the caches that have a budget, and their lengths with them."""

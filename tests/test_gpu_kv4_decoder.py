@@ -107,6 +107,44 @@ def test_eager_steps_after_replays_find_room(ctx):
         assert all(np.array_equal(x, y) for x, y in zip(a, b)), step
 
 
+def test_drafts_taken_back_and_a_sequence_begun_anew(ctx):
+    """With caches that hold more than their budget: tokens taken back and decoded again leave the same bits; a sequence
+    begun anew leaves the others what they had."""
+    d = BatchDecoder(ctx, LENS, shape(), seed=57, reserve=24, embed=True, kv="fp4", budget=64, slack=12)
+    d.fill_kv(seed=58)
+    s = d.s
+    toks = np.random.default_rng(59).integers(0, s.vocab, (8, d.B)).astype(np.uint32)
+
+    def run(first, last):
+        got = []
+        for t in toks[first:last]:
+            d.tokens.upload(t)
+            d.step()
+            got.append(d.logits.download(np.uint32))
+        return got
+
+    once = run(0, 6)
+    d.set_lengths(np.array(LENS) + 2)
+    cached = np.minimum(LENS, 64) + 2
+    assert np.array_equal(d.cut_lens.download(np.uint32), cached)
+    assert np.array_equal(run(2, 6), once[2:])
+    lens = np.array(LENS) + 6
+    lens[6] = 0
+    d.set_lengths(lens)
+    cached += 4
+    cached[6] = 0
+    assert np.array_equal(d.cut_lens.download(np.uint32), cached) and np.array_equal(d.seq_lens.download(np.uint32), lens)
+
+    def probe(stage, il, _):
+        if stage == "attn":
+            at = cached if d._is_cut(il) else lens
+            check_rows(d, il, d.q.download(np.float32, d.B * s.q_dim_of(il)),
+                       d.attn.download(np.float32, d.B * s.q_dim_of(il)), [(b, b, int(at[b])) for b in range(d.B)])
+
+    d.tokens.upload(toks[6])
+    d.step(probe=probe)
+
+
 def test_replays_past_the_room(ctx):
     """One and two replays too many (63 + 10 and 64 + 10 rows for 72): a step says so and changes nothing, evict() warns and
     cuts to the budget, and the next steps see what the caches hold."""

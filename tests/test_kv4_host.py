@@ -259,3 +259,57 @@ def test_lengths_are_read_where_graphs_ran_since():
     d.evict()
     steps(1)
     assert waits[-1] == 0
+
+
+def ragged(lens, budget=8, slack=4):
+    d = with_budget(decoder(B=len(lens)), np.minimum(lens, budget), False, budget, slack)
+    d.gone = np.array(lens) - d.cut_lens_host
+    d.lens_host = np.array(lens, np.uint32)
+    return d
+
+
+def texts(d, n):
+    for _ in range(n):
+        d._make_room(1)
+        d.lens_host = d.lens_host + 1
+
+
+def test_lengths_set_back_take_the_last_rows_of_the_cut_caches():
+    """A sequence that stays keeps what it has, one that loses its last tokens loses their rows, 0 begins another text."""
+    d = ragged([5, 8, 20, 3])
+    texts(d, 3)  # 8, 11, 23 (11 cached), 6
+    d.set_lengths([8, 11, 23, 6])
+    assert lens_of(d) == [8, 11, 11, 6] and d.seq_lens.mem.view(np.uint32).tolist() == [8, 11, 23, 6]
+    d.set_lengths([6, 9, 21, 0])
+    assert lens_of(d) == [6, 9, 9, 0]
+    texts(d, 3)
+    assert lens_of(d) == [9, 12, 12, 3] and not d.ctx.cuts
+    texts(d, 2)  # (cut to 8, 8, 8, 3)
+    assert lens_of(d) == [10, 10, 10, 5] and d.ctx.cuts
+    d.set_lengths([10, 13, 25, 5])
+    assert lens_of(d) == [9, 9, 9, 5]
+    d.set_lengths([9, 12, 24, 2])
+    assert lens_of(d) == [8, 8, 8, 2]
+
+
+@pytest.mark.parametrize("lens", [[10, 11, 26, 8], [8, 14, 26, 8], [11, 14, 23, 8], [1, 14, 26, 0]])
+def test_lengths_set_back_past_an_eviction_are_refused(lens):
+    """Before anything changes: the rows that it left are not those of the shorter text."""
+    d = ragged([5, 8, 20, 2])
+    texts(d, 6)  # 11, 14, 26 and 8 tokens, of which the evictions took 1, 4, 16 and none
+    assert lens_of(d) == [10, 10, 10, 8]
+    now = lens_of(d), d.seq_lens.mem.tolist()
+    with pytest.raises(ValueError, match="eviction"):
+        d.set_lengths(lens)
+    assert (lens_of(d), d.seq_lens.mem.tolist()) == now
+
+
+def test_longer_lengths_count_as_cut():
+    d = ragged([5, 20])
+    d.set_lengths([7, 100])
+    assert lens_of(d) == [7, 8]
+    d.set_lengths([9, 0])
+    assert lens_of(d) == [8, 0]
+    texts(d, 2)
+    d.set_lengths([10, 1])
+    assert lens_of(d) == [9, 1]
