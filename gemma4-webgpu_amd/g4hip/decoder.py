@@ -1080,15 +1080,19 @@ class BatchDecoder(_SyntheticModel):
 
     def kv_bytes_per_step(self) -> int:
         """K/V bytes one step reads: every sequence's window in every layer
-        (lengths after the step's append)."""
+        (lengths after the step's append; of a cache with a budget what it
+        holds, cut first where the step finds no room)."""
         s, total = self.s, 0
+        if self.budget is not None:
+            held = self.cut_lens_host if self.cut_lens_host.max() < self.cut_rows else np.minimum(self.cut_lens_host,
+                                                                                                 self.budget)
         for il in range(s.n_layers):
-            for L in self.lens_host:
+            for i, L in enumerate(self.lens_host):
                 n = int(L) + 1
                 if not s.is_global(il):
                     n = min(n, s.window)
                 if self._is_cut(il):
-                    n = min(n, self.cut_rows)
+                    n = int(held[min(i, len(held) - 1)]) + 1
                 if self.kv4:
                     total += n * 2 * s.kv_dim_of(il) * 17 // 32
                     continue

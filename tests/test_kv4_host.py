@@ -313,3 +313,21 @@ def test_longer_lengths_count_as_cut():
     texts(d, 2)
     d.set_lengths([10, 1])
     assert lens_of(d) == [9, 1]
+
+
+def test_a_steps_bytes_are_those_of_the_rows_it_reads():
+    d = ragged([5, 8, 20])
+    d.s = type("S", (), dict(n_layers=3, window=6, is_global=lambda self, il: il != 1, kv_dim_of=lambda self, il: 64))()
+    row = 2 * 64 * 17 // 32
+
+    def rows():
+        assert d.kv_bytes_per_step() % row == 0
+        return d.kv_bytes_per_step() // row - sum(min(int(n) + 1, 6) for n in d.lens_host)
+
+    assert rows() == 2 * (6 + 9 + 9)
+    texts(d, 3)
+    assert rows() == 2 * (9 + 12 + 12)
+    texts(d, 1)  # (the next finds no room: each is cut first)
+    assert rows() == 2 * (9 + 9 + 9)
+    texts(d, 1)
+    assert lens_of(d) == [9, 9, 9] and rows() == 2 * (10 + 10 + 10)
