@@ -843,7 +843,7 @@ class BatchDecoder(_SyntheticModel):
     workgroups and the step is deterministic.
     """
     kv4, budget, capturing, launches = False, None, False, None
-    held_mass, gone = (), 0
+    held_mass, gone, evict_params = (), 0, None  # (evict_params: of the producers whose caches have a budget)
 
     def __init__(self, ctx: Context, context_lens, shape: Optional[E2BShape] = None, page_size: int = 16,
                  reserve: int = 64, seed: int = 0, n_layers: Optional[int] = None, lm_head: bool = True,
@@ -1059,7 +1059,7 @@ class BatchDecoder(_SyntheticModel):
         lens = np.asarray(lens, dtype=np.uint32)
         if lens.shape != (self.B,) or int(lens.max()) >= self.max_seq:
             raise ValueError("set_lengths: one length per sequence, below the reserved capacity")
-        if self.budget is not None and not self.shared_pages:
+        if self.evict_params and not self.shared_pages:
             self._set_cut_lengths(lens.astype(np.int64))
         self.lens_host = lens
         self.seq_lens.upload(lens)
@@ -1165,6 +1165,8 @@ class BatchDecoder(_SyntheticModel):
         without their rows) and an error of a later step. Waits for the device."""
         if self.budget is None:
             raise ValueError("evict needs a budget")
+        if not self.evict_params:  # (every layer has a window)
+            return
         self._read_lengths()
         over = self._overrun()
         if over:
@@ -1191,14 +1193,13 @@ class BatchDecoder(_SyntheticModel):
             c.copy(self.cut_lens_next, self.cut_lens, n)
             c.kvEvict4(L.k_cache, L.v_cache, *self.kv_scales[il], self.mass[il], self.cut_table, self.cut_lens_next, p,
                        self.budget, self.cut["first"], self.cut["recent"], self.kept[il], self.evict_ws)
-        if self.evict_params:
-            c.copy(self.cut_lens, self.cut_lens_next, n)
+        c.copy(self.cut_lens, self.cut_lens_next, n)
         now = np.minimum(self.cut_lens_host, self.budget)
         self.gone, self.cut_lens_host = self.gone + self.cut_lens_host - now, now
 
     def _make_room(self, rows: int) -> None:
         """Room for `rows` more of every sequence in the caches that have a budget, and their lengths with them."""
-        if self.budget is None:
+        if not self.evict_params:
             return
         if not self.capturing:
             if self.launches is not None and self.launches != self.ctx.launches:  # (how often, the host does not know)
@@ -1512,7 +1513,7 @@ class BatchDecoder(_SyntheticModel):
             yield
         except BaseException:
             self.span_rows = 0
-            if self.budget is not None:
+            if self.evict_params:
                 self.text, self.cut_lens_host = self.held
                 self.cut_lens.upload(self.cut_lens_host)
                 for saved, mass in self.held_mass:
@@ -1521,7 +1522,7 @@ class BatchDecoder(_SyntheticModel):
         self.span_rows = 0
 
     def _placed(self) -> None:
-        if self.budget is not None:
+        if self.evict_params:
             self.text += self.span_rows
 
     def _hold(self) -> None:
@@ -1534,7 +1535,7 @@ class BatchDecoder(_SyntheticModel):
     def _begin_text(self, start: int) -> None:
         """Caches with a budget hold rows by when they came, not by position: a text begins at 0, or goes on where the
         last one ended."""
-        if self.budget is None:
+        if not self.evict_params:
             return
         if start not in (0, self.text):
             raise ValueError(f"a prompt from {start}: caches with a budget begin at 0 or go on at {self.text}")

@@ -331,3 +331,19 @@ def test_a_steps_bytes_are_those_of_the_rows_it_reads():
     assert rows() == 2 * (9 + 9 + 9)
     texts(d, 1)
     assert lens_of(d) == [9, 9, 9] and rows() == 2 * (10 + 10 + 10)
+
+
+def test_a_budget_of_layers_that_all_have_a_window_limits_nothing():
+    d = ragged([5, 20])
+    d.evict_params, d.launches, d.ctx.launches = {}, 0, 0
+    texts(d, 9)
+    d.ctx.launches += 9
+    texts(d, 9)
+    d.evict()
+    d.set_lengths([21, 19])
+    assert d.seq_lens.mem.view(np.uint32).tolist() == [21, 19] and not d.ctx.cuts
+    d = with_budget(decoder(), [0], True)
+    d.evict_params = {}
+    d.prefill(np.arange(30), 5)
+    d.prefill(np.arange(30), 2)
+    assert len(d.seen) == 16 and not d.ctx.cuts
