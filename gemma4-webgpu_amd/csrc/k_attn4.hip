@@ -1441,6 +1441,8 @@ int g4_pagedAttn4_workspace_size(g4_kv4_params p, int with_mass, size_t* bytes) 
   int rc = g4_internal_kv8_check(__func__, p, p.max_rows == 1 && p.num_rows == p.num_seqs ? nullptr : &p.num_rows);
   if (rc) return rc;
   const bool mass = with_mass != 0;
+  G4_REQUIRE(!mass || step_fits(p) || weigh_blocks(p) * WP * SW < 1ull << 32,
+             "%s: weights of many rows over up to %u positions", __func__, p.max_seq_len);  // (threads of the mass kernel)
   const Sizes z = p.head_dim == 64 ? sizes_of<64>(p, mass) : p.head_dim == 128 ? sizes_of<128>(p, mass)
                   : p.head_dim == 256 ? sizes_of<256>(p, mass) : sizes_of<512>(p, mass);
   *bytes = std::max<size_t>(z.all(), 16);

@@ -904,12 +904,13 @@ int g4_pagedAttnPrologue4(g4_ctx* ctx, const float* q_parts, const float* k_part
 /* Attention over the pool, as g4_pagedAttn8 (a window is the last sliding_window
  * cached rows). A weight is as exact relative to itself whatever its size: scores
  * within 2^-19 of sum |k| (|q| + the largest |q| of its 32 dims / 32) scale, P in
- * 24 bits. mass (or NULL): to each cached row and KV head is added the
- * softmax weight that it gets here, over the head's query heads and the
- * sequence's rows; the same sums in every run. ops (or NULL): as
- * g4_pagedAttn8Ops. workspace: g4_pagedAttn4_workspace_size bytes of these
- * parameters, with or without mass (others may need more), 16-byte aligned, of
- * any content; calls sharing it must not overlap. */
+ * 24 bits. mass (or NULL): to each cached row and KV head is added the softmax
+ * weight that it gets here, over the head's query heads and the sequence's rows;
+ * the same sums in every run (of more than 16 rows x heads: over at most
+ * 2^30 - 256 positions). ops (or NULL): as g4_pagedAttn8Ops. workspace:
+ * g4_pagedAttn4_workspace_size bytes of these parameters, with or without mass
+ * (others may need more), 16-byte aligned, of any content; calls sharing it must
+ * not overlap. */
 int g4_pagedAttn4_workspace_size(g4_kv4_params p, int with_mass, size_t* bytes);
 int g4_pagedAttn4(g4_ctx* ctx, const float* q, const uint8_t* k_pool, const uint8_t* v_pool, const uint8_t* k_scale,
                   const uint8_t* v_scale, const int32_t* page_table, const uint32_t* seq_lens,

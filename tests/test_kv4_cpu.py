@@ -43,6 +43,16 @@ def test_shapes_that_are_refused(change):
     assert size(0, **change)[0] == -1 and size(1, **change)[0] == -1
 
 
+def test_weights_of_prompts_that_no_launch_numbers_are_refused():
+    """Four threads a position of the longest cache, fewer than 2^32 in all; without weights, or of few rows, 2^30
+    positions are taken. Before anything is launched."""
+    far = dict(num_seqs=1, page_size=1024, max_pages=1 << 20, num_pages=1 << 20, num_rows=40, max_rows=40)
+    assert size(1, **far, max_seq_len=1 << 30)[0] == -1
+    assert size(0, **far, max_seq_len=1 << 30)[0] == size(1, **far, max_seq_len=(1 << 30) - 256)[0] == 0
+    assert size(1, **far, max_seq_len=1 << 30, sliding_window=1 << 20)[0] == 0
+    assert size(1, **{**far, "num_rows": 2, "max_rows": 2}, max_seq_len=1 << 30)[0] == 0
+
+
 def test_eviction_workspace_sizes():
     rc, n = evict_size(64)
     assert rc == 0 and 0 < n < 1 << 20
