@@ -618,7 +618,12 @@ __device__ __forceinline__ void weigh_positions(const Args& a, uint32_t b) {
     const int32_t id = a.page_table[(size_t)s * a.max_pages + page];
     const float* x = a.scores + ((size_t)sh * a.units + at / UNIT) * a.columns * UNIT + at % UNIT;
     float got = 0.f;
-    for (uint32_t c = 0; c < ncols; ++c) got += exp2_h(x[c * UNIT] - s_sum[c].x) * s_sum[c].y;
+    for (uint32_t c = 0; c < ncols; ++c) {
+      const float y = x[c * UNIT];  // (-Inf: the column does not see the position, and its sum may be NaN)
+      const float2 sum = s_sum[c];
+      const float e = exp2_h(y - sum.x) * sum.y;
+      got += y == -INFINITY ? 0.f : e;
+    }
     if (id >= 0 && id < (int32_t)a.num_pages)
       a.mass[((size_t)id * (a.page_tiles * 16) + (t - page * a.page_tiles * 16)) * a.nkh + kvh] += got;
   }

@@ -516,6 +516,45 @@ def test_a_query_that_is_not_finite_is_alone_with_it(ctx, hd, rows, bad):
     c.check_attention(got, range(1, rows + 1))
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("window,bad", [(0, "q"), (25, "q"), (25, "k"), (25, "v")])
+def test_weights_of_a_row_that_is_not_finite_stay_with_what_it_sees(ctx, hd, rows, window, bad):
+    """One query, or a key or value that the last row alone sees: the rows that the NaN ones do not see (behind them, out of
+    their window) get what the others give them."""
+    c = Case(ctx, [101], [rows], 8, 1, hd, 16, 127, window=window)
+    if bad == "q":
+        c.q[0, 3, 5] = np.nan
+    else:
+        pool = c.k if bad == "k" else c.v
+        pool.scale[c.table[0, 100 // 16], 100 % 16] = 255
+    c.up()
+    c.attention(mass=True)
+    got = c.dm.download(np.float32).reshape(c.mass.shape)
+    more, tol = np.zeros(c.mass.shape), np.zeros(c.mass.shape)
+    nan = np.zeros(c.mass.shape, bool)
+    k, v = c.k.values(), c.v.values()
+    for r in range(rows):
+        pos = 101 - rows + r
+        t = np.arange(max(0, pos + 1 - window) if window else 0, pos + 1)
+        at = (c.table[0, t // 16], t % 16, 0)
+        if r == 0 and bad == "q" or r == rows - 1 and bad != "q":
+            nan[at] = True
+            if bad != "q":
+                continue
+        _, _, reach, p = K4.attend(c.q[r], k, v, c.table[0], pos, window, 1.0)
+        for h in range(8):
+            if np.isfinite(p[h]).all():
+                more[at] += p[h]
+                tol[at] += p[h] * slack(hd, pos + 1, reach[h, 0]) + 2.0 ** -126
+    assert 0 < nan.sum() and np.any(~nan & (more > 0))
+    assert np.array_equal(np.isnan(got), nan)
+    tol += (rows * 8 + 2) * U * more
+    want = c.mass + more
+    assert (np.abs(got - want)[~nan] <= (tol + U * want + 1e-38)[~nan]).all()
+    assert np.array_equal(got[(more == 0) & ~nan], c.mass[(more == 0) & ~nan])
+
+
 @pytest.mark.parametrize("scale", [-0.9, 0.0, 1e-30])
 @pytest.mark.parametrize("hd,rows,window", [(256, 1, 0), (512, 1, 40), (64, 50, 0), (256, 50, 60), (512, 50, 0)])
 def test_scale_of_any_sign(ctx, hd, rows, window, scale):
