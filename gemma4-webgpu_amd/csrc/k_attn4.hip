@@ -763,15 +763,17 @@ __global__ __launch_bounds__(TileShape<HD>::NTH, HD == 64 ? 3 : 2) void attn4_ti
   __shared__ float s_mx[PAIR ? 2 * TC : 1];
   __shared__ uint32_t s_tile[4 * CH], s_bad[TP / 4];  // s_bad: rows of V that are not finite, four a word
   __shared__ WalkLds<S_::NTH> s_walk;
-  const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), qd = l >> 4, c = l & 15;
-  const int wc = w & 3, wd = PAIR ? w >> 2 : 0;  // column tile; half
   Walk<S_::NTH> walk{a, s_walk};
   const bool ok = walk.begin();
-  if (MASS && blockIdx.x == 0 && tid == 0) *a.done = ok;
+  if (MASS && blockIdx.x == 0 && threadIdx.x == 0) *a.done = ok;
   if (!ok) return;
 
   Part pt;
   while (walk.next(pt)) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // (what follows from it is formed anew for each part: kept over all of them it spills)
+    const int l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), qd = l >> 4, c = l & 15;
+    const int wc = w & 3, wd = PAIR ? w >> 2 : 0;  // column tile; half
     __syncthreads();  // the previous tile's rows are done with
     const uint32_t ncols = pt.q.n * a.G, base = pt.q.base, first = pt.q.first, kvh = pt.kvh, ct = pt.ct;
     const uint32_t lo = pt.t.lo, end = pt.t.end, st0 = pt.st0, st1 = pt.st1;
