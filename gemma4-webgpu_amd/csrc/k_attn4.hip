@@ -178,15 +178,15 @@ __device__ __forceinline__ void two_by_two(uint32_t x, float sx, uint32_t y, flo
 // (max, sum, o), which attn4_merge_kernel adds in order. With masses, the scores
 // go to the workspace, and the merge's launch turns them into weights: 4 bytes a
 // position and column written and read, where K again would be HD / 2 * 17 / 16
-// bytes a position and the products once more. It adds 1 to 5 us to a step (head
-// dim 512: 64 sequences of up to 4352 positions 30.0 and 33.4, 32 of up to 32000 53
-// and 58; in a launch of its own behind the merge 1.2 more).
+// bytes a position and the products once more. It adds 3 to 6 us to a step (head
+// dim 512: 64 sequences of up to 4352 positions 31.6 and 34.5, 32 of up to 32000 57
+// and 63; in a launch of its own behind the merge 1.2 more).
 //
 // In the loop the pool comes at 5.4 TB/s (head dim 512, 64 sequences: 3.3 us a step of
-// the four waves), around it stand 7.4 us until the first rows are there (lengths 0.8,
-// page ids and the first rows' requests 3, q's digits 2, the wait 1.6) and 2.7 for
-// the waves' sums. One sequence of 777 positions and a window of 512 at head dim 256
-// takes 7.8 us, 64 of up to 8192 18.1 (50 MB), 32 of up to 32000 at 512 52 (193 MB);
+// the four waves, before P had a third part, which costs 3 % there), around it stand
+// 7.4 us until the first rows are there (lengths 0.8, page ids and the first rows'
+// requests 3, q's digits 2, the wait 1.6) and 2.7 for the waves' sums. One sequence of 777 positions and a window of 512 at head dim 256
+// takes 8.1 us, 64 of up to 8192 18.5 (50 MB), 32 of up to 32000 at 512 54 (193 MB);
 // the merge 3.4 to 4.8.
 constexpr int NT = 256, UNIT = 128;
 constexpr uint32_t kSeqCost = 1;  // cost of a sequence and KV head besides its units: its q, its sums
@@ -719,10 +719,10 @@ __global__ __launch_bounds__(MT) void attn4_merge_kernel(Args a) {
 // workgroups a CU. A tile held by one workgroup is written by it, else its
 // workgroups leave partials that attn4_tile_merge_kernel adds in order.
 //
-// A prompt of 4500 rows of 8 heads: 108 us at head dim 128, 162 at 256 and 346 at 512
-// (384, 512 and 479 TFLOP/s), of 1500 rows 32, 45 and 72, the merge included. The
-// matrix cores work 15 % of the time and the VALUs 30 (at a step of 64 positions and
-// head dim 256 a wave has 104 products and 480 VALU instructions: V's codes to bf16,
+// A prompt of 4500 rows of 8 heads: 114 us at head dim 128, 180 at 256 and 364 at 512
+// (364, 460 and 456 TFLOP/s), of 1500 rows 34, 46 and 73 to 78, the merge included. The
+// matrix cores work 18 % of the time and the VALUs 30 (at a step of 64 positions and
+// head dim 256 a wave has 136 products and 470 VALU instructions: V's codes to bf16,
 // the softmax, the masks), the rest waits: for LDS, and at the steps' barriers, since
 // registers allow two waves a SIMD. At head dim 512 a step of two barriers, with the
 // next step's rows in flight for all of it, spilled and took 82 us where this one's
@@ -1164,7 +1164,7 @@ __global__ __launch_bounds__(HD / 4) void attn4_tile_merge_kernel(Args a) {
 // positions come in `splits` parts, which attn4_mass_kernel adds in order: a prompt's
 // first block is seen by all of its columns and its last by few, so twice the
 // workgroups that fit at once are dealt out (4500 rows of 8 heads, dim 128: 161 us with
-// the attention, as many as fit 183), in parts of 4 column tiles or more (375 rows, dim
+// the attention, as many as fit 183; 168 with three parts of P), in parts of 4 column tiles or more (375 rows, dim
 // 512: 53 us with the attention, of 8 tiles 63, of 2 51, but 68 at 750 rows for 66).
 // The products take 5.5 us of 32 at 1500 rows and dim 512: what bounds it is the way
 // to them, a row's page and digits, and one wave's exponentials beside another's products.

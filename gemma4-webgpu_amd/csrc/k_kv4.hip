@@ -4,8 +4,8 @@
 // A value is an e2m1 code times 2^e, one e per 32 dims of a row and head: the
 // least with |x| <= 7 * 2^e. Between 6 and 7 the nearest of 6 and the 8 that a
 // wider code would have is 6, so every element is within 2^e of its code, and of
-// the bounds from 6 to 8 this one has the least mean square error for normal
-// values: 0.112 of their deviation, against 0.115 at 6 and at 8. Each row has its
+// the bounds from 6 to 8 this one has the least error for normal values: a root
+// mean square of 0.112 of their deviation, against 0.115 at 6 and at 8. Each row has its
 // own scales: nothing is ever rounded again, whatever comes after it or moves it.
 #include <algorithm>
 
@@ -190,11 +190,13 @@ __global__ __launch_bounds__(VT) void kv4_values_kernel(ValArgs a) {
 // is found by three rounds of bins, from the top 11 bits down; then the rows above
 // it and the first of those at it are listed in order. The keys stay in LDS between
 // the rounds (in registers the loops over them unroll, and their conditions spill:
-// 33 us where this is 27). 2304 rows of one sequence: 8.0 us, a chain of six loads
+// 33 us where this is 27). 2304 rows of one sequence: 7.7 us, a chain of six loads
 // (2.2), of the rounds' barriers (1 each) and of the list's; 32000 rows 27, 7 of them
-// the masses of one CU, 4 bytes of a line each, 10 the rounds and 7 the list.
-// kv4_move_kernel moves the rows: 8.4 us for one sequence of 2048 rows of head dim
-// 512 (places 0.6, pages 0.4, rows 3.2, stores 1.4 and the launch), 7.8 for 64 of
+// the masses of one CU, 4 bytes of a line each, 10 the rounds and 7 the list. More
+// than Keys::GROUP candidates are read again for each round and the list: 40000 rows
+// cut with their moves 71 us where 32000 are in 41.
+// kv4_move_kernel moves the rows: 8.6 us for one sequence of 2048 rows of head dim
+// 512 (places 0.6, pages 0.4, rows 3.2, stores 1.4 and the launch), 8.0 for 64 of
 // 1024 at 256, 14.9 for 8 of 4000 and two heads at 128.
 struct EvictArgs {
   g4kv4::Pool pool;

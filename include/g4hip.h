@@ -876,8 +876,8 @@ int g4_kv8Values(g4_ctx* ctx, const int8_t* k_pool, const int8_t* v_pool, const 
  *           scales of 16 neighbouring rows next to each other
  * The scale of a block is the least 2^e (e >= -20) with |x| <= 7 * 2^e for all of
  * it; a code is the nearest, halves to the even code: |value - x| <= 2^e, a
- * quarter of the largest at most and 11 % of a normal block's deviation on the
- * average. A NaN or an infinity in a row and head makes all its scales 255, and
+ * quarter of the largest at most; of normal values, a root mean square of 11 % of
+ * their deviation. A NaN or an infinity in a row and head makes all its scales 255, and
  * every output that sees the row NaN. (Scales that a caller writes: of V, 2^-100 to
  * 2^100; the append's, of rows normed without weights, are 2^-20 to 2^2.)
  *
